@@ -314,6 +314,59 @@ int mtp_vocab_shard(int V, int world_size, int rank, int *col0, int *cols);
 int mtp_lm_head_vocab_parallel(mtp_comm *c, const void *normed, int rows, int K, int ld_normed, const void *emb, int V,
                                int ld_emb, int dtype, void *out, int ld_out, void *stream);
 
+/* ---------------------------------------------------------------- operators on logits
+ * Rows of logits: [outer][inner] rows of V values, row (o, i) at logits + o * ld_outer + i * ld
+ * (elements; any alignment of the element type, overlapping rows allowed for reading), of dtype
+ * MTP_F32, MTP_BF16 or MTP_F16.  Per-row arrays hold outer * inner values in row order.  With
+ * z = x / temperature, p = softmax(z): log p_j = z_j - max z - log sum e^(z - max z).
+ * Statistics, sums and every per-row output are fp32.  A NaN or +inf in a row gives NaN; a row of
+ * -inf alone has log p = -inf, entropy 0 and gradient 0.  No device memory is allocated and
+ * nothing is kept between calls: any stream, device or graph capture.
+ *
+ * The reference has neither a log probability nor a loss; the nearest code is the full-vocabulary
+ * KL of quant_eval.py:48-68 and the greedy argmax of model.py:359. */
+
+/* logprob[r] = log p of targets[r] (0 where targets[r] < 0: no token; NaN where targets[r] >= V),
+ * entropy[r] = -sum p log p, and the top_k <= min(V, 128) most likely tokens in falling order
+ * (equal logits: the lower index first; NaN ranks first) as top_ids / top_logprobs [rows][top_k].
+ * stats [rows][2] = largest logit and log sum, for the backward call.  logprob (with targets),
+ * entropy and stats may each be NULL. */
+int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld, int V,
+                       const int64_t *targets, float temperature, float *logprob, float *entropy, float *stats,
+                       int top_k, int64_t *top_ids, float *top_logprobs, void *stream);
+/* Gradient with respect to the logits from d_logprob [rows] (g) and d_entropy [rows] (h), either
+ * may be NULL: grad_j = (g (1{j = target} - p_j) - h p_j (log p_j + entropy)) / temperature, in the
+ * logits' dtype, row (o, i) at grad + o * grad_ld_outer + i * grad_ld.  Rows with g = h = 0 (g is 0
+ * without a token) are zeroed without being read.  grad and logits must not overlap. */
+int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld,
+                           int V, const int64_t *targets, float temperature, const float *stats, const float *entropy,
+                           const float *d_logprob, const float *d_entropy, void *grad, int64_t grad_ld_outer,
+                           int64_t grad_ld, void *stream);
+/* Distillation from a teacher's k <= 128 top logits per row, ids [rows][k] and values [rows][k]
+ * (v_dtype; logits or log probabilities): q = softmax(values / temperature) over the used entries
+ * (id >= 0 and value not -inf), loss[r] = sum q_i (log q_i - log p_id_i).  A row without a used
+ * entry has loss 0; an id >= V that is used gives NaN.  Equal ids add up.  stats as above or NULL. */
+int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld, int V,
+                     const int64_t *ids, const void *values, int v_dtype, int k, float temperature, float *loss,
+                     float *stats, void *stream);
+/* Its gradient, grad_j = row_weight[r] (p_j - sum of q_i over id_i = j) / temperature (0 in a row
+ * without a used entry or of weight 0).  With stats from mtp_distill_topk this is the backward
+ * pass; with stats NULL one call computes loss (or NULL) and gradient. */
+int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld,
+                          int V, const int64_t *ids, const void *values, int v_dtype, int k, float temperature,
+                          const float *stats, const float *row_weight, float *loss, void *grad, int64_t grad_ld_outer,
+                          int64_t grad_ld, void *stream);
+/* Log probabilities from the last hidden states: logits = hidden[rows, K] . weight[V, K]^T in fp32
+ * (hidden and weight of dtype MTP_F32 or MTP_BF16), never held as a whole, then logprob, entropy
+ * and the top_k alternatives as mtp_token_logprobs.  workspace: 16-byte aligned device memory of
+ * at least the size that mtp_lm_head_logprobs_workspace gives for the same sizes; calls that
+ * overlap on the GPU need one each. */
+int mtp_lm_head_logprobs_workspace(int rows, int V, int K, int dtype, int top_k, int64_t *bytes);
+int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight, int V,
+                         int dtype, const int64_t *targets, float temperature, float *logprob, float *entropy,
+                         int top_k, int64_t *top_ids, float *top_logprobs, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+
 /* ---------------------------------------------------------------- persistent decode
  * One cooperative launch per decode step runs every layer of the model for a batch
  * of single tokens: embedding gather (tp_model.py:318), per layer the block's

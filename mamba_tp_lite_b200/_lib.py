@@ -19,7 +19,7 @@ RED_FP32, RED_FP16, RED_INT8TOK, RED_INT8TENSOR, RED_INT8SUM, RED_INT8LEGACY = 0
 EPI_STORE, EPI_BIAS_SOFTPLUS, EPI_BIAS = 0, 1, 2
 GEMM_AUTO, GEMM_TCGEN05, GEMM_SIMT, GEMM_GEMV = 0, 1, 2, 3
 
-_vp, _i, _f, _d, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_uint64
+_vp, _i, _f, _d, _u64, _l = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_uint64, C.c_int64
 
 # name -> argtypes (all return int unless listed in _RESTYPES)
 _SIGS = {
@@ -63,6 +63,12 @@ _SIGS = {
     "mtp_allreduce_noalloc": [_i, _vp, _vp, _i, _i, _vp],
     "mtp_vocab_shard": [_i, _i, _i, C.POINTER(_i), C.POINTER(_i)],
     "mtp_lm_head_vocab_parallel": [_vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp],
+    "mtp_token_logprobs": [_vp, _i, _l, _l, _l, _l, _i, _vp, _f, _vp, _vp, _vp, _i, _vp, _vp, _vp],
+    "mtp_token_logprobs_bwd": [_vp, _i, _l, _l, _l, _l, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _l, _l, _vp],
+    "mtp_distill_topk": [_vp, _i, _l, _l, _l, _l, _i, _vp, _vp, _i, _i, _f, _vp, _vp, _vp],
+    "mtp_distill_topk_grad": [_vp, _i, _l, _l, _l, _l, _i, _vp, _vp, _i, _i, _f, _vp, _vp, _vp, _vp, _l, _l, _vp],
+    "mtp_lm_head_logprobs_workspace": [_i, _i, _i, _i, _i, C.POINTER(_l)],
+    "mtp_lm_head_logprobs": [_vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _f, _vp, _vp, _i, _vp, _vp, _vp, _l, _vp],
     "mtp_decode_plan_create": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, C.POINTER(_vp)],
     "mtp_decode_bind_cache": [_vp, _vp, _vp, _i, C.POINTER(_vp)],
     "mtp_decode_step": [_vp, _vp, _vp, _vp, _vp],

@@ -311,6 +311,12 @@ class _LMKernels:
         c.set_sequence_parallel(ok)
 
     def _forward_prefill(self, input_ids: torch.Tensor, cache=None):
+        normed, new_cache = self._forward_hidden(input_ids, cache)
+        b, l = input_ids.shape
+        return self._lm_head(normed).view(b, l, -1), new_cache
+
+    def _forward_hidden(self, input_ids: torch.Tensor, cache=None):
+        """The prefill up to norm_f: (hidden states [b * l, d_model], new cache)."""
         self._sync_sequence_parallel()
         b, l = input_ids.shape
         resid = self._embed(input_ids)
@@ -319,8 +325,7 @@ class _LMKernels:
         split = self._overlap_split(b, l)
         if split is not None:
             new_layers = self._prefill_overlapped(normed, resid, b, l, cache, split)
-            logits = self._lm_head(normed)
-            return logits.view(b, l, -1), MambaCache(new_layers)
+            return normed, MambaCache(new_layers)
         eps = self.cfg.layer_norm_epsilon
         new_layers = []
         for i, layer in enumerate(self.layers):
@@ -329,8 +334,7 @@ class _LMKernels:
             si = lc.ssm_state.float().contiguous() if lc is not None else None
             cf, sf = layer.mixer._prefill_core(normed, b, l, ci, si, resid, self._next_norm_w(i), eps, normed)
             new_layers.append(LayerCache(conv_state=cf, ssm_state=sf))
-        logits = self._lm_head(normed)
-        return logits.view(b, l, -1), MambaCache(new_layers)
+        return normed, MambaCache(new_layers)
 
     def _decode_plan(self, b: int, cache):
         """(plan, binding) of the persistent decode kernel, or None for the per-layer chain."""
@@ -386,6 +390,26 @@ class _LMKernels:
             lc = cache.layers[i]
             layer.mixer._step_core(normed, lc.conv_state, lc.ssm_state, resid, self._next_norm_w(i), eps, normed)
         return self._lm_head(normed).view(b, 1, -1)
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, cache=None, targets: torch.Tensor | None = None, top_k: int = 0,
+              temperature: float = 1.0):
+        """Scores input_ids [b, l]: (TokenLogprobs of [b, l] rows, new MambaCache).  Row i holds the log
+        probability of ``targets[:, i]`` after reading positions 0..i; by default the next token,
+        input_ids[:, i + 1] (the last position has none: log probability 0).  A prefill whose
+        lm_head never holds logits (``logprobs.lm_head_logprobs``): they are not rounded to the
+        model dtype, so a bf16 model's values differ from those of its prefill logits by that
+        rounding.  At TP > 1 every rank scores all rows."""
+        from .logprobs import lm_head_logprobs
+
+        L.require_cuda(input_ids, "input_ids")
+        if targets is None:
+            targets = torch.full_like(input_ids, -1)
+            targets[:, :-1] = input_ids[:, 1:]
+        b, l = input_ids.shape
+        normed, new_cache = self._forward_hidden(input_ids, cache)
+        return lm_head_logprobs(normed.view(b, l, -1), self.embedding.weight, targets, top_k=top_k,
+                                temperature=temperature), new_cache
 
     def greedy_next(self, logits: torch.Tensor) -> torch.Tensor:
         """argmax over the vocabulary of the last position: [b, l, V] -> [b, 1] (libmtp kernel)."""
