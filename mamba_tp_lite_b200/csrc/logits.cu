@@ -3,15 +3,26 @@
 //
 // With z = x / T, m = max z and S = sum e^(z - m), a row gives
 //   log p_j = (z_j - m) - log S          H = log S - sum e^(z - m) (z - m) / S
-// All sums and statistics are fp32.  One CTA per row.
+// All sums and statistics are fp32.  Every kernel reads a row in 16-byte vectors at the row's own alignment (the elements
+// before the first and after the last whole vector one by one), a thread taking every 256th vector.  A forward pass
+// reads its row once: each thread keeps the running maximum m, S and U = sum e^y y (y in units of log2) of its elements
+// and rescales them when m grows; threads, and the CTAs of a cluster that share a row, are joined at the end.
+#include <cooperative_groups.h>
 #include "common.cuh"
 
 namespace mtp {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAX_TOP = 128;  // alternatives or teacher entries per row
-constexpr int NT = 256;
+namespace cg = cooperative_groups;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int MAX_TOP = 128;      // alternatives or teacher entries per row
+constexpr int NT = 256;           // threads per CTA
+constexpr int NW = NT / 32;
+constexpr int MAX_CLUSTER = 8;    // CTAs that share a row
+constexpr int LIST = 1024;        // candidates for the alternatives that a CTA holds
+constexpr float LOWEST = -3.402823466e38f;
+constexpr float FLOOR_Y = -1024.f;  // 2^FLOOR_Y is 0: stands for -inf where it is multiplied by a 0
 
 // Row r of a batch laid out as [outer][inner] rows: r = o * inner + i.
 struct Rows {
@@ -19,17 +30,252 @@ struct Rows {
   __device__ __forceinline__ int64_t at(int64_t r) const { return (r / inner) * ld_outer + (r % inner) * ld; }
 };
 
-// Order of the alternatives as unsigned integers: larger value first, -0 equal to +0, NaN above +inf.
-__device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  const uint32_t b = v == 0.f ? 0u : __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+// ----------------------------------------------------------------- arithmetic
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-__device__ __forceinline__ float nan_max(float a, float b) {
+// The same with subnormal results kept (a gradient is a product of one with a factor that can be large).
+__device__ __forceinline__ float ex2_sub(float x) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// Packed fp32 pairs (one instruction for two lanes' worth of arithmetic).
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(F2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// 16 bytes of logits.
+template <typename T> struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(const uint4 &r, float (&x)[N]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[N]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(x[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+__device__ __forceinline__ uint4 load16(const void *p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// The part of a row that CTA `rank` of `parts` works on: vectors [v0, v1) of those that start `head` elements into the
+// row, the first CTA also the elements before them, the last the `tail` elements from `tail0` on.
+template <typename T> struct Slice {
+  const T *row;
+  int head, v0, v1, nhead, tail0, ntail;
+  __device__ __forceinline__ Slice(const T *r, int V, int rank, int parts) : row(r) {
+    constexpr int N = Vec<T>::N;
+    head = (int)(((16u - (unsigned)(reinterpret_cast<uintptr_t>(r) & 15u)) & 15u) / sizeof(T));
+    if (head > V) head = V;
+    const int nv = (V - head) / N;
+    v0 = (int)((long long)nv * rank / parts);
+    v1 = (int)((long long)nv * (rank + 1) / parts);
+    nhead = rank == 0 ? head : 0;
+    tail0 = head + nv * N;
+    ntail = rank == parts - 1 ? V - tail0 : 0;
+  }
+  __device__ __forceinline__ const T *vec(int v) const { return row + head + (int64_t)v * Vec<T>::N; }
+  __device__ __forceinline__ int first(int v) const { return head + v * Vec<T>::N; }  // index of a vector's first element
+};
+
+// ----------------------------------------------------------------- row statistics
+// Of a set of elements: m their largest (LOWEST if they are none or all -inf: then s is 0), s = sum e^((x - m) / T),
+// u = sum e^y y with y = (x - m) / T * log2 e.  A NaN or +inf among them makes s NaN.
+struct Stat {
+  float m, s, u;
+};
+
+template <bool ENT>
+__device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  const float ya = fmaxf((a.m - r.m) * c2, FLOOR_Y), yb = fmaxf((b.m - r.m) * c2, FLOOR_Y);
+  const float ea = ex2(ya), eb = ex2(yb);
+  r.s = a.s * ea + b.s * eb;
+  r.u = ENT ? fmaf(ya, a.s, a.u) * ea + fmaf(yb, b.s, b.u) * eb : 0.f;
+  return r;
+}
+
+template <bool ENT, int N>
+__device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float c2) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+  const float m = fmaxf(st.m, mx);
+  const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
+  const float corr = ex2(dy);
+  const F2 nm = f2(-m, -m), cc = f2(c2, c2);
+  F2 s = f2(0.f, 0.f), u = f2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const F2 y = mul2(add2(f2(x[i], x[i + 1]), nm), cc);
+    float y0, y1;
+    un2(y, y0, y1);
+    const F2 e = f2(ex2(y0), ex2(y1));
+    s = add2(s, e);
+    if constexpr (ENT) u = fma2(e, f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), u);
+  }
+  float s0, s1, u0, u1;
+  un2(s, s0, s1);
+  un2(u, u0, u1);
+  if constexpr (ENT) st.u = fmaf(fmaf(dy, st.s, st.u), corr, u0 + u1);
+  st.s = fmaf(st.s, corr, s0 + s1);
+  st.m = m;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void accumulate1(Stat &st, float x, float c2) {
+  const float v[2] = {x, -INFINITY};
+  accumulate<ENT, 2>(st, v, c2);
+}
+
+// One thread's elements of a slice.  Four vectors are in flight per thread.
+template <typename T, bool ENT>
+__device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2) {
+  constexpr int N = Vec<T>::N, DEPTH = 4;
+  Stat st{LOWEST, 0.f, 0.f};
+  int v = sl.v0 + threadIdx.x;
+  for (; v + (DEPTH - 1) * NT < sl.v1; v += DEPTH * NT) {
+    uint4 raw[DEPTH];
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) raw[j] = load16(sl.vec(v + j * NT));
+#pragma unroll
+    for (int j = 0; j < DEPTH; j += 2) {
+      float x[2 * N], lo[N], hi[N];
+      Vec<T>::unpack(raw[j], lo);
+      Vec<T>::unpack(raw[j + 1], hi);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = lo[i], x[N + i] = hi[i];
+      accumulate<ENT, 2 * N>(st, x, c2);
+    }
+  }
+  {
+    uint4 raw[DEPTH - 1];
+#pragma unroll
+    for (int j = 0; j < DEPTH - 1; ++j)
+      if (v + j * NT < sl.v1) raw[j] = load16(sl.vec(v + j * NT));
+#pragma unroll
+    for (int j = 0; j < DEPTH - 1; ++j)
+      if (v + j * NT < sl.v1) {
+        float x[N];
+        Vec<T>::unpack(raw[j], x);
+        accumulate<ENT, N>(st, x, c2);
+      }
+  }
+  if (threadIdx.x < (unsigned)sl.nhead) accumulate1<ENT>(st, ldf(sl.row + threadIdx.x), c2);
+  if (threadIdx.x < (unsigned)sl.ntail) accumulate1<ENT>(st, ldf(sl.row + sl.tail0 + threadIdx.x), c2);
+  return st;
+}
+
+template <bool ENT>
+__device__ __forceinline__ Stat warp_join(Stat st, float c2) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    Stat other;
+    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    other.u = ENT ? __shfl_xor_sync(0xffffffffu, st.u, o) : 0.f;
+    st = join<ENT>(st, other, c2);
+  }
+  return st;
+}
+
+struct RowStats {
+  float m, log_s, entropy;  // m: largest logit (not divided by T), -inf for a row of -inf alone
+};
+
+__device__ __forceinline__ RowStats finish(Stat st) {
+  if (st.s == 0.f) return {-INFINITY, 0.f, 0.f};
+  const float ls = logf(st.s);
+  return {st.m, ls, ls - LN2 * (st.u / st.s)};
+}
+
+// log p of a logit of the row; a row whose logits are all -inf gives -inf.
+__device__ __forceinline__ float log_prob(float x, float m, float log_s, float inv_t) {
+  return m == -INFINITY ? -INFINITY : (x - m) * inv_t - log_s;
+}
+
+// Shared state of the CTAs of a row.  Every CTA gets every CTA's statistics (and group maxima) in its own copy.
+struct RowShared {
+  Stat warp[NW];
+  Stat cta[MAX_CLUSTER];
+};
+
+// Joins the threads of the CTA and the CTAs of the cluster; every thread of the cluster returns the row's statistics.
+// Orders the shared memory written before it (the group maxima, peers' copies included) for all threads.
+template <bool ENT>
+__device__ Stat row_join(Stat st, RowShared &sh, float c2, int rank, int parts) {
+  st = warp_join<ENT>(st, c2);
+  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
+  __syncthreads();
+  Stat all = sh.warp[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) all = join<ENT>(all, sh.warp[i], c2);  // the same order in every thread
+  if (parts > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    if (threadIdx.x < (unsigned)parts) *cl.map_shared_rank(&sh.cta[rank], threadIdx.x) = all;
+    cl.sync();
+    all = sh.cta[0];
+    for (int i = 1; i < parts; ++i) all = join<ENT>(all, sh.cta[i], c2);
+  }
+  return all;
 }
 
 template <typename F, typename T>
@@ -40,106 +286,350 @@ __device__ __forceinline__ T block_reduce(T v, T *red, F op) {
   if (l == 0) red[w] = v;
   __syncthreads();
   T s = red[0];
-  for (int i = 1; i < NT / 32; ++i) s = op(s, red[i]);  // fixed order: the same in every thread
+  for (int i = 1; i < NW; ++i) s = op(s, red[i]);  // fixed order: the same in every thread
   return s;
 }
 
-__device__ __forceinline__ float sum_op(float a, float b) { return a + b; }
+// ----------------------------------------------------------------- top alternatives
+// Order of the alternatives as unsigned integers: larger value first, -0 equal to +0, NaN above +inf.  An element's
+// key is its value's order above its complemented index, so that no two are equal and the lower index wins a tie.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  const uint32_t b = v == 0.f ? 0u : __float_as_uint(v);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k == 0xFFFFFFFFu ? 0x7fffffffu : (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ uint64_t element_key(float v, int i) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~i; }
 
-struct RowStats {
-  float m, log_s, entropy;  // m: largest logit (not divided by T)
+// The k largest of a row without a second pass over it.  The threads of all CTAs form NT groups (a group is `parts`
+// neighbouring threads of a CTA); the k-th largest of the groups' maxima is a lower bound of the row's k-th largest
+// element, since each of k groups holds an element that is not below it.  Only threads whose own maximum reaches the
+// bound look at their elements again (k = 64 of 50280: about 75 threads) and put those that reach it on the CTA's
+// list.  The lists of the cluster are joined in its first CTA, and an element's place in the result is the number of
+// elements above it.
+struct TopShared {
+  uint32_t group[NT];       // order keys of the groups' maxima, all CTAs'
+  uint64_t list[LIST];
+  uint64_t final_list[MAX_CLUSTER * MAX_TOP];
+  uint64_t red[NW];
+  uint32_t bound;
+  int n;
 };
 
-// log p of a logit of the row; a row whose logits are all -inf gives -inf.
-__device__ __forceinline__ float log_prob(float x, float m, float log_s, float inv_t) {
-  return m == -INFINITY ? -INFINITY : (x - m) * inv_t - log_s;
-}
-
-template <typename T>
-__device__ RowStats row_stats(const T *row, int V, float inv_t, float *red) {
-  auto fmx = [](float a, float b) { return nan_max(a, b); };
-  auto add = [](float a, float b) { return sum_op(a, b); };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += NT) m = nan_max(m, ldf(row + i));
-  m = block_reduce(m, red, fmx);
-  if (m == -INFINITY) return {m, 0.f, 0.f};
-  float s = 0.f, u = 0.f;
-  for (int i = threadIdx.x; i < V; i += NT) {
-    const float d = (ldf(row + i) - m) * inv_t;
-    const float e = expf(d);
-    s += e;
-    u += e * fmaxf(d, -1000.f);  // e is 0 below: a masked logit adds nothing
+// Largest b with at least k of the NT keys >= b, or a smaller one that fewer than k + k / 8 + 4 reach.  One warp.
+__device__ __forceinline__ uint32_t group_bound(const uint32_t *group, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[NW], lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    key[i] = group[lane + 32 * i];
+    lo = min(lo, key[i]);
+    hi = max(hi, key[i]);
   }
-  s = block_reduce(s, red, add);
-  u = block_reduce(u, red, add);
-  const float ls = logf(s);
-  return {m, ls, ls - u / s};
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const int enough = k + k / 8 + 4;
+  // all NT >= k keys reach lo; fewer than k, or nobody knows yet, reach more than hi
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) c += key[i] >= mid;
+    c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= enough) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
 }
 
+// Calls f(value, index) for the elements of thread t of the slice; the lanes of the calling warp share them.
+template <typename T, typename F>
+__device__ __forceinline__ void warp_elements(const Slice<T> &sl, int t, F f) {
+  constexpr int N = Vec<T>::N;
+  const int lane = threadIdx.x & 31;
+  for (int v = sl.v0 + t + lane * NT; v < sl.v1; v += 32 * NT) {
+    float x[N];
+    Vec<T>::unpack(load16(sl.vec(v)), x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f(x[i], sl.first(v) + i);
+  }
+  if (lane == 0 && t < sl.nhead) f(ldf(sl.row + t), t);
+  if (lane == 1 && t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
+}
+
+// The same for a thread's own elements.
+template <typename T, typename F>
+__device__ __forceinline__ void thread_elements(const Slice<T> &sl, F f) {
+  constexpr int N = Vec<T>::N;
+  const int t = threadIdx.x;
+  for (int v = sl.v0 + t; v < sl.v1; v += NT) {
+    float x[N];
+    Vec<T>::unpack(load16(sl.vec(v)), x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f(x[i], sl.first(v) + i);
+  }
+  if (t < sl.nhead) f(ldf(sl.row + t), t);
+  if (t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
+}
+
+__device__ __forceinline__ uint64_t count_op(uint64_t a, uint64_t b) { return a + b; }
+
+// Largest key that at least k of the counted elements reach, or a smaller one that at most `most` >= k reach.
+// count(key): how many elements of the calling thread are >= key; lo: a key that at least k reach; no key is above hi.
+template <typename F>
+__device__ uint64_t key_bound(uint64_t lo, uint64_t hi, int k, int most, uint64_t *red, F count) {
+  auto add = [](uint64_t a, uint64_t b) { return count_op(a, b); };
+  while (lo < hi) {
+    const uint64_t mid = lo + (hi - lo) / 2 + 1;
+    const uint64_t c = block_reduce((uint64_t)count(mid), red, add);
+    if (c >= (uint64_t)k) {
+      lo = mid;
+      if (c <= (uint64_t)most) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// Cuts list[0, n) down to at most `most` >= k keys, the k largest among them; n <= LIST.
+__device__ int cut_list(uint64_t *list, int n, int k, int most, TopShared &sh) {
+  if (n <= most) return n;
+  const uint64_t b = key_bound(0, ~0ull, k, most, sh.red, [&](uint64_t key) {
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += NT) c += list[i] >= key;
+    return c;
+  });
+  uint64_t mine[LIST / NT];
+#pragma unroll
+  for (int i = 0; i < LIST / NT; ++i) {
+    const int at = threadIdx.x + i * NT;
+    mine[i] = at < n ? list[at] : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < LIST / NT; ++i)
+    if (mine[i] >= b && threadIdx.x + i * NT < n) list[atomicAdd(&sh.n, 1)] = mine[i];
+  __syncthreads();
+  return sh.n;
+}
+
+// st: the calling thread's own statistics, total: the row's; group maxima are in place (row_join has ordered them).
+template <typename T>
+__device__ void top_alternatives(const Slice<T> &sl, Stat st, RowStats row, int k, float inv_t, int V, TopShared &sh,
+                                 int rank, int parts, int64_t *ids, float *logprobs) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    const uint32_t b = group_bound(sh.group, k);
+    if (lane == 0) {
+      sh.bound = b;
+      sh.n = 0;
+    }
+  }
+  __syncthreads();
+  const uint32_t bound = sh.bound;
+  // a thread whose sum is NaN may hold a NaN, which its maximum passes over
+  unsigned todo = __ballot_sync(0xffffffffu, order_key(st.s == 0.f ? -INFINITY : st.m) >= bound || st.s != st.s);
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    warp_elements(sl, warp * 32 + src, [&](float x, int i) {
+      if (order_key(x) >= bound) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < LIST) sh.list[at] = element_key(x, i);
+      }
+    });
+  }
+  __syncthreads();
+  int n = sh.n;
+  if (n > LIST) {
+    // more elements reach the bound than the list holds (a row of equal logits): find the key of this CTA's k-th
+    // largest element by bisection, one scan of the slice a step, and collect again
+    const uint64_t lo = ((uint64_t)bound << 32) | (uint32_t)~(V - 1);
+    const uint64_t hi = row.log_s != row.log_s ? ~0ull : ((uint64_t)order_key(row.m) << 32) | 0xFFFFFFFFu;
+    const uint64_t b = key_bound(lo, hi, k, MAX_TOP, sh.red, [&](uint64_t key) {
+      int c = 0;
+      thread_elements(sl, [&](float x, int i) { c += element_key(x, i) >= key; });
+      return c;
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    thread_elements(sl, [&](float x, int i) {
+      const uint64_t key = element_key(x, i);
+      if (key >= b) sh.list[atomicAdd(&sh.n, 1)] = key;
+    });
+    __syncthreads();
+    n = sh.n;
+  }
+  const uint64_t *list = sh.list;
+  if (parts > 1) {
+    n = cut_list(sh.list, n, k, MAX_TOP, sh);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = n;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    if (rank == 0) {
+      int at = 0;
+      for (int c = 0; c < parts; ++c) {
+        const int nc = *cl.map_shared_rank(&sh.n, c);
+        const uint64_t *from = cl.map_shared_rank(sh.list, c);
+        if (threadIdx.x < (unsigned)nc) sh.final_list[at + threadIdx.x] = from[threadIdx.x];
+        at += nc;
+      }
+      n = at;
+    }
+    cl.sync();  // the peers' lists have been read
+    if (rank != 0) return;
+    list = sh.final_list;
+  }
+  n = cut_list(const_cast<uint64_t *>(list), n, k, NT, sh);
+  if (threadIdx.x < (unsigned)n) {
+    const uint64_t key = list[threadIdx.x];
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += list[i] > key;
+    if (place < k) {
+      ids[place] = (int64_t)(int)~(uint32_t)key;
+      logprobs[place] = log_prob(key_value((uint32_t)(key >> 32)), row.m, row.log_s, inv_t);
+    }
+  }
+}
+
+// ----------------------------------------------------------------- log probabilities
 struct FwdArgs {
   const int64_t *targets;
   float *logprob, *entropy, *stats;
   int top_k;
   int64_t *top_ids;
   float *top_logprobs;
-  float inv_t;
-  int V;
+  float inv_t, c2;  // 1 / T, log2 e / T
+  int V, parts;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(NT) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
+template <typename T, bool ENT, bool TOP>
+__global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  __shared__ float red[NT / 32];
-  __shared__ unsigned long long redk[NT / 32];
-  const int64_t r = blockIdx.x;
+  __shared__ RowShared sh;
+  __shared__ TopShared top;
+  const int parts = a.parts;
+  const int64_t r = blockIdx.x / parts;
+  const int rank = (int)(blockIdx.x % parts);
   const T *row = logits + rows.at(r);
-  const RowStats st = row_stats(row, a.V, a.inv_t, red);
-  if (threadIdx.x == 0) {
+  const Slice<T> sl(row, a.V, rank, parts);
+  if (parts > 1) cg::this_cluster().sync();  // every CTA of the cluster runs: its shared memory may be written
+  const Stat st = thread_stats<T, ENT>(sl, a.c2);
+  if constexpr (TOP) {
+    // maxima of groups of `parts` threads to every CTA of the cluster
+    uint32_t g = sl.v0 + (int)threadIdx.x < sl.v1 || threadIdx.x < (unsigned)sl.nhead || threadIdx.x < (unsigned)sl.ntail
+                     ? order_key(st.s == 0.f ? -INFINITY : st.m)
+                     : 0u;
+    for (int o = 1; o < parts; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    const int slot = rank * (NT / parts) + threadIdx.x / parts;
+    const int to = threadIdx.x % parts;
+    if (parts > 1) *cg::this_cluster().map_shared_rank(&top.group[slot], to) = g;
+    else top.group[slot] = g;
+  }
+  const RowStats s = finish(row_join<ENT>(st, sh, a.c2, rank, parts));
+  if (rank == 0 && threadIdx.x == 0) {
     if (a.logprob) {
       const int64_t t = a.targets[r];
-      a.logprob[r] = t < 0 ? 0.f : t >= a.V ? NAN : log_prob(ldf(row + t), st.m, st.log_s, a.inv_t);
+      a.logprob[r] = t < 0 ? 0.f : t >= a.V ? NAN : log_prob(ldf(row + t), s.m, s.log_s, a.inv_t);
     }
-    if (a.entropy) a.entropy[r] = st.entropy;
+    if (a.entropy) a.entropy[r] = s.entropy;
     if (a.stats) {
-      a.stats[2 * r] = st.m;
-      a.stats[2 * r + 1] = st.log_s;
+      a.stats[2 * r] = s.m;
+      a.stats[2 * r + 1] = s.log_s;
     }
   }
-  // one scan per alternative: the largest (value, lowest index) key below the last one taken
-  unsigned long long last = ~0ull;
-  auto kmax = [](unsigned long long x, unsigned long long y) { return x > y ? x : y; };
-  for (int k = 0; k < a.top_k; ++k) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < a.V; i += NT) {
-      const unsigned long long key = ((unsigned long long)order_key(ldf(row + i)) << 32) | (uint32_t)~i;
-      if ((k == 0 || key < last) && key > best) best = key;
-    }
-    last = block_reduce(best, redk, kmax);
-    if (threadIdx.x == 0) {
-      const int i = (int)~(uint32_t)last;
-      a.top_ids[r * a.top_k + k] = i;
-      a.top_logprobs[r * a.top_k + k] = log_prob(ldf(row + i), st.m, st.log_s, a.inv_t);
-    }
+  if constexpr (TOP)
+    top_alternatives(sl, st, s, a.top_k, a.inv_t, a.V, top, rank, parts, a.top_ids + r * a.top_k,
+                     a.top_logprobs + r * a.top_k);
+}
+
+// ----------------------------------------------------------------- gradients
+// out_j = p_j (a + b y_j) with p_j = 2^y_j, y = log2 p; the element `hit` gets `extra` on top.
+struct Dense {
+  float m, l2, c2;  // largest logit, log2 S, log2 e / T
+  float a, b;
+  __device__ __forceinline__ float one(float x) const {
+    const float y = (x - m) * c2 - l2;
+    return ex2_sub(y) * fmaf(b, fmaxf(y, FLOOR_Y), a);
   }
+};
+
+// Writes the slice's gradient.  16-byte stores where the gradient row is aligned as the logits row is.
+template <typename T>
+__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense &d, bool zero, int64_t hit, float extra) {
+  constexpr int N = Vec<T>::N, DEPTH = 4;
+  const bool same = ((reinterpret_cast<uintptr_t>(sl.row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  auto one = [&](int i) {
+    float v = 0.f;
+    if (!zero) {
+      v = d.one(ldf(sl.row + i));
+      if (i == hit) v += extra;
+    }
+    stf(out + i, v);
+  };
+  if (same) {
+    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += DEPTH * NT) {
+      uint4 raw[DEPTH];
+      if (!zero) {
+#pragma unroll
+        for (int j = 0; j < DEPTH; ++j)
+          if (v + j * NT < sl.v1) raw[j] = load16(sl.vec(v + j * NT));
+      }
+#pragma unroll
+      for (int j = 0; j < DEPTH; ++j) {
+        if (v + j * NT < sl.v1) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (!zero) {
+            float x[N];
+            Vec<T>::unpack(raw[j], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = d.one(x[i]);
+            const int64_t at = hit - sl.first(v + j * NT);
+            if (at >= 0 && at < N) {
+#pragma unroll
+              for (int i = 0; i < N; ++i)
+                if (i == at) x[i] += extra;
+            }
+            w = Vec<T>::pack(x);
+          }
+          __stcs(reinterpret_cast<uint4 *>(out + sl.first(v + j * NT)), w);
+        }
+      }
+    }
+  } else {
+    for (int64_t i = sl.first(sl.v0) + (int)threadIdx.x; i < sl.first(sl.v1); i += NT) one((int)i);
+  }
+  if (threadIdx.x < (unsigned)sl.nhead) one(threadIdx.x);
+  if (threadIdx.x < (unsigned)sl.ntail) one(sl.tail0 + threadIdx.x);
 }
 
 struct BwdArgs {
   const int64_t *targets;
   const float *stats, *entropy, *d_logprob, *d_entropy;
-  float inv_t;
-  int V;
+  float inv_t, c2;
+  int V, parts;
 };
 
 // dx_j = (g (1{j = t} - p_j) - h p_j (log p_j + H)) / T
 template <typename T>
-__global__ void __launch_bounds__(NT) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
-                                                                T *__restrict__ grad, Rows grows) {
+__global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
+                                                                   T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  const int64_t r = blockIdx.x;
-  const T *row = logits + rows.at(r);
-  T *out = grad + grows.at(r);
+  const int64_t r = blockIdx.x / a.parts;
+  const Slice<T> sl(logits + rows.at(r), a.V, (int)(blockIdx.x % a.parts), a.parts);
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1];
   const float h = a.d_entropy ? a.d_entropy[r] : 0.f;
   int64_t t = -1;
@@ -149,20 +639,12 @@ __global__ void __launch_bounds__(NT) token_logprobs_bwd_kernel(const T *__restr
     g = t < 0 ? 0.f : t >= a.V ? NAN : a.d_logprob[r];
   }
   const float ent = a.entropy ? a.entropy[r] : 0.f;
-  const bool none = (g == 0.f && h == 0.f) || m == -INFINITY;
-  for (int i = threadIdx.x; i < a.V; i += NT) {
-    float v = 0.f;
-    if (!none) {
-      const float lp = (ldf(row + i) - m) * a.inv_t - log_s;
-      const float p = expf(lp);
-      v = -p * (g + h * (fmaxf(lp, -1000.f) + ent));
-      if (i == t) v += g;
-      v *= a.inv_t;
-    }
-    stf(out + i, v);
-  }
+  const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
+  const Dense d{m, log_s * LOG2E, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t};
+  write_grad(sl, grad + grows.at(r), d, zero, t, g * a.inv_t);
 }
 
+// ----------------------------------------------------------------- distillation
 struct DistillArgs {
   const int64_t *ids;
   const void *values;
@@ -170,8 +652,8 @@ struct DistillArgs {
   const float *row_weight;
   float *loss, *stats;
   const float *stats_in;
-  float inv_t;
-  int V;
+  float inv_t, c2;
+  int V, parts;
 };
 
 __device__ __forceinline__ float load_value(const void *p, int64_t i, int dtype) {
@@ -180,21 +662,31 @@ __device__ __forceinline__ float load_value(const void *p, int64_t i, int dtype)
                              : __half2float(((const __half *)p)[i]);
 }
 
-// loss = sum q_i (log q_i - log p_id_i), dx_j = w (sum q p_j - sum_{id_i = j} q_i) / T; q: softmax over the used
-// entries of the teacher's logits / T.  GRAD: the gradient is written too.
+__device__ __forceinline__ float nan_max(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// loss = sum q_i (log q_i - log p_id_i), dx_j = w (p_j - sum_{id_i = j} q_i) / T; q: softmax over the used entries of
+// the teacher's logits / T, thread i holding entry i.  GRAD: the gradient is written too.
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(NT) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
-                                                     T *__restrict__ grad, Rows grows) {
+__global__ void __launch_bounds__(NT, 4) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
+                                                        T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  __shared__ float red[NT / 32];
+  __shared__ RowShared sh;
+  __shared__ float red[NW];
   __shared__ int64_t sid[MAX_TOP];
   __shared__ float sq[MAX_TOP];
-  const int64_t r = blockIdx.x;
+  const int parts = a.parts;
+  const int64_t r = blockIdx.x / parts;
+  const int rank = (int)(blockIdx.x % parts);
   const T *row = logits + rows.at(r);
+  const Slice<T> sl(row, a.V, rank, parts);
+  if (parts > 1 && !a.stats_in) cg::this_cluster().sync();  // peers' shared memory may be written
   auto fmx = [](float x, float y) { return nan_max(x, y); };
-  auto add = [](float x, float y) { return sum_op(x, y); };
-  // teacher: thread i holds entry i
+  auto add = [](float x, float y) { return x + y; };
   float tv = -INFINITY;
   int64_t id = -1;
   if (threadIdx.x < (unsigned)a.k) {
@@ -209,17 +701,17 @@ __global__ void __launch_bounds__(NT) distill_kernel(const T *__restrict__ logit
   const float q = used ? te / ts : 0.f;
   const bool bad = q != 0.f && id >= a.V;
   const RowStats st = a.stats_in ? RowStats{a.stats_in[2 * r], a.stats_in[2 * r + 1], 0.f}
-                                 : row_stats(row, a.V, a.inv_t, red);
-  float term = 0.f;
-  if (bad) term = NAN;
-  else if (q != 0.f) term = q * ((td - logf(ts)) - log_prob(ldf(row + id), st.m, st.log_s, a.inv_t));
-  const float loss = block_reduce(term, red, add);
-  if (threadIdx.x == 0) {
-    if (a.loss) a.loss[r] = loss;
-    if (a.stats) {
-      a.stats[2 * r] = st.m;
-      a.stats[2 * r + 1] = st.log_s;
-    }
+                                 : finish(row_join<false>(thread_stats<T, false>(sl, a.c2), sh, a.c2, rank, parts));
+  float lp = 0.f;
+  if (q != 0.f && !bad) lp = log_prob(ldf(row + id), st.m, st.log_s, a.inv_t);
+  if (a.loss && rank == 0) {
+    const float term = bad ? NAN : q != 0.f ? q * ((td - logf(ts)) - lp) : 0.f;
+    const float loss = block_reduce(term, red, add);
+    if (threadIdx.x == 0) a.loss[r] = loss;
+  }
+  if (a.stats && rank == 0 && threadIdx.x == 0) {
+    a.stats[2 * r] = st.m;
+    a.stats[2 * r + 1] = st.log_s;
   }
   if constexpr (GRAD) {
     if (threadIdx.x < (unsigned)a.k) {
@@ -228,19 +720,51 @@ __global__ void __launch_bounds__(NT) distill_kernel(const T *__restrict__ logit
     }
     const bool any_bad = block_reduce(bad ? 1.f : 0.f, red, add) != 0.f;  // also orders sid / sq
     const float w = a.row_weight[r] * a.inv_t;
-    const bool none = !used || w == 0.f || st.m == -INFINITY;
+    const bool zero = !used || w == 0.f || st.m == -INFINITY;
     T *out = grad + grows.at(r);
-    for (int i = threadIdx.x; i < a.V; i += NT) {
-      float v = 0.f;
-      if (!none) {
-        v = expf((ldf(row + i) - st.m) * a.inv_t - st.log_s);
-        float qs = 0.f;
-        for (int j = 0; j < a.k; ++j) qs += sid[j] == i ? sq[j] : 0.f;
-        v = any_bad ? NAN : w * (v - qs);
+    const Dense d{st.m, st.log_s * LOG2E, a.c2, any_bad ? NAN : w, 0.f};
+    write_grad(sl, out, d, zero, -1, 0.f);
+    __syncthreads();  // the teacher's elements are written again, after the pass over all of them
+    const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
+    if (!zero && !any_bad && q != 0.f && mine) {
+      float qs = 0.f;
+      bool first = true;
+      for (int j = 0; j < a.k; ++j) {
+        if (sid[j] == id) {
+          qs += sq[j];
+          first = first && j >= (int)threadIdx.x;
+        }
       }
-      stf(out + i, v);
+      if (first) stf(out + id, w * (ex2_sub(lp * LOG2E) - qs));
     }
   }
+}
+
+// CTAs that share a row: rows alone fill the GPU from about four CTAs per SM on; a CTA takes no fewer than NT vectors.
+inline int row_parts(int64_t rows, int V, int elem) {
+  const int64_t want = 4ll * num_sms();
+  const int64_t vecs = (int64_t)V * elem / 16;
+  int parts = 1;
+  while (parts < MAX_CLUSTER && rows * parts < want && vecs / (2 * parts) >= NT) parts *= 2;
+  return parts;
+}
+
+// Launch with the CTAs of a row as a cluster.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int parts, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)parts;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
 #define MTP_DISPATCH_LOGITS(code, T, ...)                                    \
@@ -275,9 +799,15 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   MTP_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "top_k needs top_ids and top_logprobs");
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows{inner, ld_outer, ld};
-  const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature, V};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(token_logprobs_kernel<T>, dim3((unsigned)(outer * inner)), dim3(NT), 0, s,
-                                           (const T *)logits, rows, a));
+  const int64_t n = outer * inner;
+  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
+                  (float)(1.4426950408889634 / temperature), V, parts};
+  MTP_DISPATCH_LOGITS(dtype, T, {
+    auto kern = top_k ? (entropy ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, false, true>)
+                      : (entropy ? token_logprobs_kernel<T, true, false> : token_logprobs_kernel<T, false, false>);
+    launch_rows(kern, n, parts, s, (const T *)logits, rows, a);
+  });
   return check_launch("token_logprobs");
 }
 
@@ -291,8 +821,11 @@ int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t
   MTP_REQUIRE(!d_entropy || entropy, "d_entropy needs entropy");
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows{inner, ld_outer, ld}, grows{inner, grad_ld_outer, grad_ld};
-  const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature, V};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(token_logprobs_bwd_kernel<T>, dim3((unsigned)(outer * inner)), dim3(NT), 0, s,
+  const int64_t n = outer * inner;
+  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature,
+                  (float)(1.4426950408889634 / temperature), V, parts};
+  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(token_logprobs_bwd_kernel<T>, dim3((unsigned)(n * parts)), dim3(NT), 0, s,
                                            (const T *)logits, rows, a, (T *)grad, grows));
   return check_launch("token_logprobs_bwd");
 }
@@ -306,9 +839,12 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
   MTP_REQUIRE(v_dtype == MTP_F32 || v_dtype == MTP_BF16 || v_dtype == MTP_F16, "values must be F32, BF16 or F16");
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows{inner, ld_outer, ld};
-  const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature, V};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(distill_kernel<T, false>, dim3((unsigned)(outer * inner)), dim3(NT), 0, s,
-                                           (const T *)logits, rows, a, (T *)nullptr, rows));
+  const int64_t n = outer * inner;
+  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature,
+                      (float)(1.4426950408889634 / temperature), V, parts};
+  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false>, n, parts, s, (const T *)logits, rows, a,
+                                            (T *)nullptr, rows));
   return check_launch("distill_topk");
 }
 
@@ -322,9 +858,12 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   MTP_REQUIRE(v_dtype == MTP_F32 || v_dtype == MTP_BF16 || v_dtype == MTP_F16, "values must be F32, BF16 or F16");
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows{inner, ld_outer, ld}, grows{inner, grad_ld_outer, grad_ld};
-  const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature, V};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(distill_kernel<T, true>, dim3((unsigned)(outer * inner)), dim3(NT), 0, s,
-                                           (const T *)logits, rows, a, (T *)grad, grows));
+  const int64_t n = outer * inner;
+  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature,
+                      (float)(1.4426950408889634 / temperature), V, parts};
+  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, true>, n, parts, s, (const T *)logits, rows, a,
+                                            (T *)grad, grows));
   return check_launch("distill_topk_grad");
 }
 
