@@ -359,9 +359,10 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
 /* Log probabilities from the last hidden states: logits = hidden[rows, K] . weight[V, K]^T in fp32
  * (hidden and weight of dtype MTP_F32 or MTP_BF16), never held as a whole, then logprob, entropy
  * and the top_k alternatives as mtp_token_logprobs.  workspace: 16-byte aligned device memory of
- * at least the size that mtp_lm_head_logprobs_workspace gives for the same sizes; calls that
- * overlap on the GPU need one each. */
-int mtp_lm_head_logprobs_workspace(int rows, int V, int K, int dtype, int top_k, int64_t *bytes);
+ * at least the size that mtp_lm_head_logprobs_workspace gives for the same arguments, with
+ * nothing in it to start with; calls that overlap on the GPU need one each. */
+int mtp_lm_head_logprobs_workspace(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight,
+                                   int V, int dtype, int top_k, int64_t *bytes);
 int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight, int V,
                          int dtype, const int64_t *targets, float temperature, float *logprob, float *entropy,
                          int top_k, int64_t *top_ids, float *top_logprobs, void *workspace, int64_t workspace_bytes,

@@ -67,7 +67,7 @@ _SIGS = {
     "mtp_token_logprobs_bwd": [_vp, _i, _l, _l, _l, _l, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _l, _l, _vp],
     "mtp_distill_topk": [_vp, _i, _l, _l, _l, _l, _i, _vp, _vp, _i, _i, _f, _vp, _vp, _vp],
     "mtp_distill_topk_grad": [_vp, _i, _l, _l, _l, _l, _i, _vp, _vp, _i, _i, _f, _vp, _vp, _vp, _vp, _l, _l, _vp],
-    "mtp_lm_head_logprobs_workspace": [_i, _i, _i, _i, _i, C.POINTER(_l)],
+    "mtp_lm_head_logprobs_workspace": [_vp, _i, _i, _i, _vp, _i, _i, _i, _i, C.POINTER(_l)],
     "mtp_lm_head_logprobs": [_vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _f, _vp, _vp, _i, _vp, _vp, _vp, _l, _vp],
     "mtp_decode_plan_create": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, C.POINTER(_vp)],
     "mtp_decode_bind_cache": [_vp, _vp, _vp, _i, C.POINTER(_vp)],

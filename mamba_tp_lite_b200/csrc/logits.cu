@@ -9,20 +9,19 @@
 // and rescales them when m grows; threads, and the CTAs of a cluster that share a row, are joined at the end.
 #include <cooperative_groups.h>
 #include "common.cuh"
+#include "logits.cuh"
 
 namespace mtp {
 namespace {
 
 namespace cg = cooperative_groups;
+using namespace lg;
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int MAX_TOP = 128;      // alternatives or teacher entries per row
 constexpr int NT = 256;           // threads per CTA
 constexpr int NW = NT / 32;
 constexpr int MAX_CLUSTER = 8;    // CTAs that share a row
 constexpr int LIST = 1024;        // candidates for the alternatives that a CTA holds
-constexpr float LOWEST = -3.402823466e38f;
-constexpr float FLOOR_Y = -1024.f;  // 2^FLOOR_Y is 0: stands for -inf where it is multiplied by a 0
 
 // Row r of a batch laid out as [outer][inner] rows: r = o * inner + i.
 struct Rows {
@@ -30,46 +29,7 @@ struct Rows {
   __device__ __forceinline__ int64_t at(int64_t r) const { return (r / inner) * ld_outer + (r % inner) * ld; }
 };
 
-// ----------------------------------------------------------------- arithmetic
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// The same with subnormal results kept (a gradient is a product of one with a factor that can be large).
-__device__ __forceinline__ float ex2_sub(float x) {
-  float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Packed fp32 pairs (one instruction for two lanes' worth of arithmetic).
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void un2(F2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
+// ----------------------------------------------------------------- rows in vectors
 // 16 bytes of logits.
 template <typename T> struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -136,56 +96,6 @@ template <typename T> struct Slice {
 };
 
 // ----------------------------------------------------------------- row statistics
-// Of a set of elements: m their largest (LOWEST if they are none or all -inf: then s is 0), s = sum e^((x - m) / T),
-// u = sum e^y y with y = (x - m) / T * log2 e.  A NaN or +inf among them makes s NaN.
-struct Stat {
-  float m, s, u;
-};
-
-template <bool ENT>
-__device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  const float ya = fmaxf((a.m - r.m) * c2, FLOOR_Y), yb = fmaxf((b.m - r.m) * c2, FLOOR_Y);
-  const float ea = ex2(ya), eb = ex2(yb);
-  r.s = a.s * ea + b.s * eb;
-  r.u = ENT ? fmaf(ya, a.s, a.u) * ea + fmaf(yb, b.s, b.u) * eb : 0.f;
-  return r;
-}
-
-template <bool ENT, int N>
-__device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float c2) {
-  float mx = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  const float m = fmaxf(st.m, mx);
-  const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
-  const float corr = ex2(dy);
-  const F2 nm = f2(-m, -m), cc = f2(c2, c2);
-  F2 s = f2(0.f, 0.f), u = f2(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const F2 y = mul2(add2(f2(x[i], x[i + 1]), nm), cc);
-    float y0, y1;
-    un2(y, y0, y1);
-    const F2 e = f2(ex2(y0), ex2(y1));
-    s = add2(s, e);
-    if constexpr (ENT) u = fma2(e, f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), u);
-  }
-  float s0, s1, u0, u1;
-  un2(s, s0, s1);
-  un2(u, u0, u1);
-  if constexpr (ENT) st.u = fmaf(fmaf(dy, st.s, st.u), corr, u0 + u1);
-  st.s = fmaf(st.s, corr, s0 + s1);
-  st.m = m;
-}
-
-template <bool ENT>
-__device__ __forceinline__ void accumulate1(Stat &st, float x, float c2) {
-  const float v[2] = {x, -INFINITY};
-  accumulate<ENT, 2>(st, v, c2);
-}
-
 // One thread's elements of a slice.  Four vectors are in flight per thread.
 template <typename T, bool ENT>
 __device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2) {
@@ -235,21 +145,6 @@ __device__ __forceinline__ Stat warp_join(Stat st, float c2) {
     st = join<ENT>(st, other, c2);
   }
   return st;
-}
-
-struct RowStats {
-  float m, log_s, entropy;  // m: largest logit (not divided by T), -inf for a row of -inf alone
-};
-
-__device__ __forceinline__ RowStats finish(Stat st) {
-  if (st.s == 0.f) return {-INFINITY, 0.f, 0.f};
-  const float ls = logf(st.s);
-  return {st.m, ls, ls - LN2 * (st.u / st.s)};
-}
-
-// log p of a logit of the row; a row whose logits are all -inf gives -inf.
-__device__ __forceinline__ float log_prob(float x, float m, float log_s, float inv_t) {
-  return m == -INFINITY ? -INFINITY : (x - m) * inv_t - log_s;
 }
 
 // Shared state of the CTAs of a row.  Every CTA gets every CTA's statistics (and group maxima) in its own copy.
@@ -865,52 +760,6 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, true>, n, parts, s, (const T *)logits, rows, a,
                                             (T *)grad, grows));
   return check_launch("distill_topk_grad");
-}
-
-// Rows of fp32 logits that one pass of mtp_lm_head_logprobs holds: about 256 MB of them.
-static int64_t score_block(int64_t rows, int V) {
-  int64_t b = (256ll << 20) / (4ll * V);
-  b = b < 128 ? 128 : b / 128 * 128;
-  return rows < b ? rows : b;
-}
-static int64_t score_ld(int V) { return ((int64_t)V + 7) / 8 * 8; }
-
-int mtp_lm_head_logprobs_workspace(int rows, int V, int K, int dtype, int top_k, int64_t *bytes) {
-  MTP_REQUIRE(rows >= 0 && V > 0 && V <= (1 << 30) && K > 0 && top_k >= 0 && bytes, "bad arguments");
-  MTP_REQUIRE(dtype == MTP_F32 || dtype == MTP_BF16, "dtype must be F32 or BF16");
-  *bytes = score_block(rows, V) * score_ld(V) * 4;
-  return MTP_OK;
-}
-
-int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight, int V,
-                         int dtype, const int64_t *targets, float temperature, float *logprob, float *entropy,
-                         int top_k, int64_t *top_ids, float *top_logprobs, void *workspace, int64_t workspace_bytes,
-                         void *stream) {
-  MTP_REQUIRE(rows >= 0 && V > 0 && V <= (1 << 30) && K > 0 && ld_hidden >= K && ld_weight >= K, "bad sizes");
-  MTP_REQUIRE(dtype == MTP_F32 || dtype == MTP_BF16, "dtype must be F32 or BF16");
-  MTP_REQUIRE(temperature > 0.f && temperature < INFINITY, "temperature must be positive and finite");
-  MTP_REQUIRE(top_k >= 0 && top_k <= MAX_TOP && top_k <= V, "top_k must be between 0 and min(V, 128)");
-  if (rows == 0) return MTP_OK;
-  MTP_REQUIRE(hidden && weight && workspace, "null pointer");
-  MTP_REQUIRE(!logprob || targets, "logprob needs targets");
-  MTP_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "top_k needs top_ids and top_logprobs");
-  int64_t need = 0;
-  mtp_lm_head_logprobs_workspace(rows, V, K, dtype, top_k, &need);
-  MTP_REQUIRE(workspace_bytes >= need && aligned16(workspace), "workspace too small or not 16-byte aligned");
-  const int64_t blk = score_block(rows, V), ld = score_ld(V);
-  const size_t es = dtype == MTP_F32 ? 4 : 2;
-  for (int64_t r0 = 0; r0 < rows; r0 += blk) {
-    const int n = (int)(rows - r0 < blk ? rows - r0 : blk);
-    int rc = mtp_gemm((const char *)hidden + (size_t)r0 * ld_hidden * es, weight, workspace, n, V, K, ld_hidden, ld_weight,
-                      (int)ld, dtype, MTP_F32, MTP_EPI_STORE, nullptr, 0, stream);
-    if (rc) return rc;
-    rc = mtp_token_logprobs(workspace, MTP_F32, 1, n, 0, ld, V, targets ? targets + r0 : nullptr, temperature,
-                            logprob ? logprob + r0 : nullptr, entropy ? entropy + r0 : nullptr, nullptr, top_k,
-                            top_ids ? top_ids + r0 * top_k : nullptr, top_logprobs ? top_logprobs + r0 * top_k : nullptr,
-                            stream);
-    if (rc) return rc;
-  }
-  return MTP_OK;
 }
 
 }  // extern "C"

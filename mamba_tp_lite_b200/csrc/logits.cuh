@@ -1,0 +1,119 @@
+// Softmax statistics shared by the kernels over logits rows and the lm_head kernel that never writes logits.
+#pragma once
+#include "common.cuh"
+
+namespace mtp {
+namespace lg {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOWEST = -3.402823466e38f;
+constexpr float FLOOR_Y = -1024.f;  // 2^FLOOR_Y is 0: stands for -inf where it is multiplied by a 0
+
+// ----------------------------------------------------------------- arithmetic
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The same with subnormal results kept (a gradient is a product of one with a factor that can be large).
+__device__ __forceinline__ float ex2_sub(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Packed fp32 pairs (one instruction for two lanes' worth of arithmetic).
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(F2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// ----------------------------------------------------------------- row statistics
+// Of a set of elements: m their largest (LOWEST if they are none or all -inf: then s is 0), s = sum e^((x - m) / T),
+// u = sum e^y y with y = (x - m) / T * log2 e.  A NaN or +inf among them makes s NaN.
+struct Stat {
+  float m, s, u;
+};
+
+template <bool ENT>
+__device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  const float ya = fmaxf((a.m - r.m) * c2, FLOOR_Y), yb = fmaxf((b.m - r.m) * c2, FLOOR_Y);
+  const float ea = ex2(ya), eb = ex2(yb);
+  r.s = a.s * ea + b.s * eb;
+  r.u = ENT ? fmaf(ya, a.s, a.u) * ea + fmaf(yb, b.s, b.u) * eb : 0.f;
+  return r;
+}
+
+template <bool ENT, int N>
+__device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float c2) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+  const float m = fmaxf(st.m, mx);
+  const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
+  const float corr = ex2(dy);
+  const F2 nm = f2(-m, -m), cc = f2(c2, c2);
+  F2 s = f2(0.f, 0.f), u = f2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const F2 y = mul2(add2(f2(x[i], x[i + 1]), nm), cc);
+    float y0, y1;
+    un2(y, y0, y1);
+    const F2 e = f2(ex2(y0), ex2(y1));
+    s = add2(s, e);
+    if constexpr (ENT) u = fma2(e, f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), u);
+  }
+  float s0, s1, u0, u1;
+  un2(s, s0, s1);
+  un2(u, u0, u1);
+  if constexpr (ENT) st.u = fmaf(fmaf(dy, st.s, st.u), corr, u0 + u1);
+  st.s = fmaf(st.s, corr, s0 + s1);
+  st.m = m;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void accumulate1(Stat &st, float x, float c2) {
+  const float v[2] = {x, -INFINITY};
+  accumulate<ENT, 2>(st, v, c2);
+}
+
+struct RowStats {
+  float m, log_s, entropy;  // m: largest logit (not divided by T), -inf for a row of -inf alone
+};
+
+__device__ __forceinline__ RowStats finish(Stat st) {
+  if (st.s == 0.f) return {-INFINITY, 0.f, 0.f};
+  const float ls = logf(st.s);
+  return {st.m, ls, ls - LN2 * (st.u / st.s)};
+}
+
+// log p of a logit of the row; a row whose logits are all -inf gives -inf.
+__device__ __forceinline__ float log_prob(float x, float m, float log_s, float inv_t) {
+  return m == -INFINITY ? -INFINITY : (x - m) * inv_t - log_s;
+}
+
+}  // namespace lg
+}  // namespace mtp

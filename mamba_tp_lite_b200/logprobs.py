@@ -326,16 +326,17 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.
         x = x.contiguous()
     if weight.stride(1) != 1 or not k <= weight.stride(0) <= MAX_VOCAB:
         weight = weight.contiguous()
-    rows, dt = x.shape[0], L.dtype_code(x.dtype)
+    rows = x.shape[0]
+    args = (L.ptr(x), x.stride(0) if rows > 1 else k, rows, k, L.ptr(weight), weight.stride(0) if v > 1 else k, v,
+            L.dtype_code(x.dtype))
     new = lambda *tail, dtype=torch.float32: torch.empty((*lead, *tail), device=x.device, dtype=dtype)
     lp = None if targets is None else new()
     ent = new() if entropy else None
     ids, tlp = (new(top_k, dtype=torch.int64), new(top_k)) if top_k else (None, None)
     need = C.c_int64(0)
-    L.call("mtp_lm_head_logprobs_workspace", rows, v, k, dt, top_k, C.byref(need))
-    work = torch.empty(need.value, device=x.device, dtype=torch.uint8)
     with _on(x):
-        L.call("mtp_lm_head_logprobs", L.ptr(x), x.stride(0) if rows > 1 else k, rows, k, L.ptr(weight),
-               weight.stride(0) if v > 1 else k, v, dt, L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), top_k,
-               L.ptr(ids), L.ptr(tlp), L.ptr(work), need.value, L.stream_ptr())
+        L.call("mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need))
+        work = torch.empty(need.value, device=x.device, dtype=torch.uint8)
+        L.call("mtp_lm_head_logprobs", *args, L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), top_k, L.ptr(ids),
+               L.ptr(tlp), L.ptr(work), need.value, L.stream_ptr())
     return TokenLogprobs(lp, ent, ids, tlp)

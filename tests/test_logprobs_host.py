@@ -209,9 +209,9 @@ def test_c_entry_points_refuse_bad_arguments():
     _refused(*dg(w=None))
     _refused(*dg(gld=1))
     n = C.c_int64(0)
-    _refused("mtp_lm_head_logprobs_workspace", 4, 64, 32, L.F16, 0, C.byref(n), text="dtype")
-    _refused("mtp_lm_head_logprobs_workspace", -1, 64, 32, L.BF16, 0, C.byref(n))
-    assert L.load().mtp_lm_head_logprobs_workspace(4, 64, 32, L.BF16, 0, C.byref(n)) == L.MTP_OK and n.value > 0
+    _refused("mtp_lm_head_logprobs_workspace", p, 32, 4, 32, p, 32, 64, L.F16, 0, C.byref(n), text="dtype")
+    _refused("mtp_lm_head_logprobs_workspace", p, 32, -1, 32, p, 32, 64, L.BF16, 0, C.byref(n))
+    assert L.load().mtp_lm_head_logprobs_workspace(p, 32, 4, 32, p, 32, 64, L.BF16, 0, C.byref(n)) == L.MTP_OK and n.value > 0
     lm = lambda ws=p, nb=n.value, ldh=32, dt=L.BF16, tgt=p, k=0: (
         "mtp_lm_head_logprobs", p, ldh, 4, 32, p, 32, 64, dt, tgt, 1.0, p, p, k, None, None, ws, nb, None)
     _refused(*lm(ws=None), text="null")
