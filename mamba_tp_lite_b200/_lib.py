@@ -148,8 +148,9 @@ def vocab_shard(V: int, ws: int, rank: int) -> tuple[int, int]:
 
 
 def stream_ptr(stream=None) -> int:
-    s = torch.cuda.current_stream() if stream is None else stream
-    return s.cuda_stream
+    if stream is None:  # the current stream's handle without building a Stream object (3 us)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream.cuda_stream
 
 
 def ptr(t) -> int | None:

@@ -241,28 +241,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
 }
 
-// Joins the tiles of a row: 32 rows per CTA (a lane each), the warps share the tiles, eight of them in flight per lane.
-constexpr int JOIN_WARPS = 8;
+// Joins the tiles of a row: 8 rows per CTA, 32 threads a row (4 lanes of each warp, so that a warp reads four 32-byte
+// sectors), eight tiles in flight per thread: one round of loads up to 256 tiles.
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = 8;
 template <bool ENT>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) lm_score_join_kernel(const ScoreParams p, int ctas, float inv_t,
                                                                         float *__restrict__ logprob,
                                                                         float *__restrict__ entropy) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  __shared__ Stat sh[JOIN_WARPS][32];
+  constexpr int STRIDE = 4 * JOIN_WARPS;
+  __shared__ Stat sh[JOIN_WARPS][JOIN_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 32 + lane;
+  const int row = blockIdx.x * JOIN_ROWS + (lane & 7);
   int gave_up = 0;
   for (int i = threadIdx.x; i < ctas; i += 32 * JOIN_WARPS) gave_up |= p.status[i];
-  gave_up = __syncthreads_or(gave_up);
   Stat st{LOWEST, 0.f, 0.f};
   if (row < p.M) {
     const int64_t plane = (int64_t)p.tiles_n * p.M;
-    for (int t = warp; t < p.tiles_n; t += 8 * JOIN_WARPS) {
+    for (int t = warp * 4 + (lane >> 3); t < p.tiles_n; t += 8 * STRIDE) {
       Stat s[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int tj = t + j * JOIN_WARPS;
+        const int tj = t + j * STRIDE;
         s[j] = Stat{LOWEST, 0.f, 0.f};
         if (tj < p.tiles_n) {
           const int64_t at = (int64_t)tj * p.M + row;
@@ -273,9 +274,17 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) lm_score_join_kernel(const Sc
       for (int j = 0; j < 8; ++j) st = join<ENT>(st, s[j], p.c2);
     }
   }
-  sh[warp][lane] = st;
-  __syncthreads();
-  if (warp != 0 || row >= p.M) return;
+#pragma unroll
+  for (int o = 8; o < 32; o *= 2) {
+    Stat other;
+    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    other.u = ENT ? __shfl_xor_sync(0xffffffffu, st.u, o) : 0.f;
+    st = join<ENT>(st, other, p.c2);
+  }
+  if (lane < JOIN_ROWS) sh[warp][lane] = st;
+  gave_up = __syncthreads_or(gave_up);
+  if (threadIdx.x >= JOIN_ROWS || row >= p.M) return;
   for (int w = 1; w < JOIN_WARPS; ++w) st = join<ENT>(st, sh[w][lane], p.c2);
   RowStats r = finish(st);
   if (gave_up) r.log_s = r.entropy = NAN;
@@ -362,7 +371,7 @@ int launch_score(const void *hidden, int ld_hidden, int rows, int K, const void 
   rc = check_launch("lm_score");
   if (rc) return rc;
   auto join = entropy ? lm_score_join_kernel<true> : lm_score_join_kernel<false>;
-  launch_pdl(join, dim3(ceil_div(rows, 32)), dim3(32 * JOIN_WARPS), 0, stream, p, plan.grid, 1.f / temperature, logprob,
+  launch_pdl(join, dim3(ceil_div(rows, JOIN_ROWS)), dim3(32 * JOIN_WARPS), 0, stream, p, plan.grid, 1.f / temperature, logprob,
              entropy);
   return check_launch("lm_score_join");
 }

@@ -96,41 +96,108 @@ template <typename T> struct Slice {
 };
 
 // ----------------------------------------------------------------- row statistics
-// One thread's elements of a slice.  Four vectors are in flight per thread.
+// Asynchronous 16-byte copies into the calling thread's own places of shared memory: no thread reads another's, so that
+// waiting for one's own copies is all the ordering that is needed.
+__device__ __forceinline__ void copy16(uint4 *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// Vectors of the slice that thread t takes: v0 + t, v0 + t + NT, ...
+template <typename T> __device__ __forceinline__ int thread_vectors(const Slice<T> &sl) {
+  const int left = sl.v1 - sl.v0 - (int)threadIdx.x;
+  return left > 0 ? (left + NT - 1) / NT : 0;
+}
+
 template <typename T, bool ENT>
-__device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2) {
-  constexpr int N = Vec<T>::N, DEPTH = 4;
-  Stat st{LOWEST, 0.f, 0.f};
-  int v = sl.v0 + threadIdx.x;
-  for (; v + (DEPTH - 1) * NT < sl.v1; v += DEPTH * NT) {
-    uint4 raw[DEPTH];
+__device__ __forceinline__ void accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
+  constexpr int N = Vec<T>::N;
+  float x[2 * N], lo[N], hi[N];
+  Vec<T>::unpack(a, lo);
+  Vec<T>::unpack(b, hi);
 #pragma unroll
-    for (int j = 0; j < DEPTH; ++j) raw[j] = load16(sl.vec(v + j * NT));
-#pragma unroll
-    for (int j = 0; j < DEPTH; j += 2) {
-      float x[2 * N], lo[N], hi[N];
-      Vec<T>::unpack(raw[j], lo);
-      Vec<T>::unpack(raw[j + 1], hi);
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = lo[i], x[N + i] = hi[i];
-      accumulate<ENT, 2 * N>(st, x, c2);
-    }
-  }
-  {
-    uint4 raw[DEPTH - 1];
-#pragma unroll
-    for (int j = 0; j < DEPTH - 1; ++j)
-      if (v + j * NT < sl.v1) raw[j] = load16(sl.vec(v + j * NT));
-#pragma unroll
-    for (int j = 0; j < DEPTH - 1; ++j)
-      if (v + j * NT < sl.v1) {
-        float x[N];
-        Vec<T>::unpack(raw[j], x);
-        accumulate<ENT, N>(st, x, c2);
-      }
-  }
+  for (int i = 0; i < N; ++i) x[i] = lo[i], x[N + i] = hi[i];
+  accumulate<ENT, 2 * N>(st, x, c2);
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ void accumulate_vec(Stat &st, const uint4 &a, float c2) {
+  constexpr int N = Vec<T>::N;
+  float x[N];
+  Vec<T>::unpack(a, x);
+  accumulate<ENT, N>(st, x, c2);
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ void accumulate_ends(Stat &st, const Slice<T> &sl, float c2) {
   if (threadIdx.x < (unsigned)sl.nhead) accumulate1<ENT>(st, ldf(sl.row + threadIdx.x), c2);
   if (threadIdx.x < (unsigned)sl.ntail) accumulate1<ENT>(st, ldf(sl.row + sl.tail0 + threadIdx.x), c2);
+}
+
+// One thread's statistics of its elements, streamed through a ring of RING pairs of vectors per thread (32 KB a CTA, so
+// that five CTAs keep 160 KB in flight on an SM whatever they compute).
+constexpr int RING = 4, RING_BYTES = 2 * RING * NT * 16;
+template <typename T, bool ENT>
+__device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2, uint4 *ring) {
+  Stat st{LOWEST, 0.f, 0.f};
+  const int n = thread_vectors(sl);
+  const T *src = sl.vec(sl.v0 + (int)threadIdx.x);
+  constexpr int STEP = NT * Vec<T>::N;  // elements between a thread's vectors
+  uint4 *mine = ring + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < RING; ++j) {
+    if (2 * j < n) copy16(mine + (2 * j) * NT, src + (int64_t)(2 * j) * STEP);
+    if (2 * j + 1 < n) copy16(mine + (2 * j + 1) * NT, src + (int64_t)(2 * j + 1) * STEP);
+    copy_commit();
+  }
+  src += (int64_t)2 * RING * STEP;
+  int slot = 0;
+  for (int i = 0; i < n; i += 2) {
+    copy_wait<RING - 1>();
+    uint4 *at = mine + slot * 2 * NT;
+    if (i + 1 < n) accumulate_pair<T, ENT>(st, at[0], at[NT], c2);
+    else accumulate_vec<T, ENT>(st, at[0], c2);
+    if (i + 2 * RING < n) copy16(at, src);
+    if (i + 2 * RING + 1 < n) copy16(at + NT, src + STEP);
+    copy_commit();
+    src += 2 * STEP;
+    slot = (slot + 1) & (RING - 1);
+  }
+  accumulate_ends<T, ENT>(st, sl, c2);
+  return st;
+}
+
+// The same with the whole slice kept in shared memory, at most RESIDENT vectors per thread, all of them in flight at once.
+constexpr int RESIDENT = 13, RESIDENT_BYTES = RESIDENT * NT * 16;
+template <typename T, bool ENT>
+__device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, uint4 *keep) {
+  Stat st{LOWEST, 0.f, 0.f};
+  const int n = thread_vectors(sl);
+  const T *src = sl.vec(sl.v0 + (int)threadIdx.x);
+  constexpr int STEP = NT * Vec<T>::N, PAIRS = (RESIDENT + 1) / 2;
+  uint4 *mine = keep + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) {
+    if (2 * j < n) copy16(mine + (2 * j) * NT, src + (int64_t)(2 * j) * STEP);
+    if (2 * j + 1 < n) copy16(mine + (2 * j + 1) * NT, src + (int64_t)(2 * j + 1) * STEP);
+    copy_commit();
+  }
+  auto step = [&](int j) {
+    if (2 * j + 1 < n) accumulate_pair<T, ENT>(st, mine[2 * j * NT], mine[(2 * j + 1) * NT], c2);
+    else if (2 * j < n) accumulate_vec<T, ENT>(st, mine[2 * j * NT], c2);
+  };
+  static_assert(PAIRS == 7, "one wait per pair below");
+  copy_wait<6>(); step(0);
+  copy_wait<5>(); step(1);
+  copy_wait<4>(); step(2);
+  copy_wait<3>(); step(3);
+  copy_wait<2>(); step(4);
+  copy_wait<1>(); step(5);
+  copy_wait<0>(); step(6);
+  accumulate_ends<T, ENT>(st, sl, c2);
   return st;
 }
 
@@ -205,9 +272,9 @@ __device__ __forceinline__ uint64_t element_key(float v, int i) { return ((uint6
 // list.  The lists of the cluster are joined in its first CTA, and an element's place in the result is the number of
 // elements above it.
 struct TopShared {
-  uint32_t group[NT];       // order keys of the groups' maxima, all CTAs'
-  uint64_t list[LIST];
-  uint64_t final_list[MAX_CLUSTER * MAX_TOP];
+  uint32_t group[NT];   // order keys of the groups' maxima, all CTAs'
+  uint64_t *list;       // [LIST] this CTA's candidates, [MAX_CLUSTER * MAX_TOP] the cluster's after them: both lie in
+                        // the ring, which has been read when the first candidate is written
   uint64_t red[NW];
   uint32_t bound;
   int n;
@@ -377,14 +444,14 @@ __device__ void top_alternatives(const Slice<T> &sl, Stat st, RowStats row, int 
       for (int c = 0; c < parts; ++c) {
         const int nc = *cl.map_shared_rank(&sh.n, c);
         const uint64_t *from = cl.map_shared_rank(sh.list, c);
-        if (threadIdx.x < (unsigned)nc) sh.final_list[at + threadIdx.x] = from[threadIdx.x];
+        if (threadIdx.x < (unsigned)nc) sh.list[LIST + at + threadIdx.x] = from[threadIdx.x];
         at += nc;
       }
       n = at;
     }
     cl.sync();  // the peers' lists have been read
     if (rank != 0) return;
-    list = sh.final_list;
+    list = sh.list + LIST;
   }
   n = cut_list(const_cast<uint64_t *>(list), n, k, NT, sh);
   if (threadIdx.x < (unsigned)n) {
@@ -410,19 +477,22 @@ struct FwdArgs {
 };
 
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
+__global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
   __shared__ RowShared sh;
   __shared__ TopShared top;
+  __shared__ uint4 ring[2 * RING * NT];
+  static_assert(sizeof(ring) >= 8 * (LIST + MAX_CLUSTER * MAX_TOP), "the ring holds the lists");
   const int parts = a.parts;
   const int64_t r = blockIdx.x / parts;
   const int rank = (int)(blockIdx.x % parts);
   const T *row = logits + rows.at(r);
   const Slice<T> sl(row, a.V, rank, parts);
   if (parts > 1) cg::this_cluster().sync();  // every CTA of the cluster runs: its shared memory may be written
-  const Stat st = thread_stats<T, ENT>(sl, a.c2);
+  const Stat st = thread_stats<T, ENT>(sl, a.c2, ring);
   if constexpr (TOP) {
+    if (threadIdx.x == 0) top.list = reinterpret_cast<uint64_t *>(ring);
     // maxima of groups of `parts` threads to every CTA of the cluster
     uint32_t g = sl.v0 + (int)threadIdx.x < sl.v1 || threadIdx.x < (unsigned)sl.nhead || threadIdx.x < (unsigned)sl.ntail
                      ? order_key(st.s == 0.f ? -INFINITY : st.m)
@@ -461,9 +531,11 @@ struct Dense {
   }
 };
 
-// Writes the slice's gradient.  16-byte stores where the gradient row is aligned as the logits row is.
-template <typename T>
-__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense &d, bool zero, int64_t hit, float extra) {
+// Writes the slice's gradient.  16-byte stores where the gradient row is aligned as the logits row is.  KEPT: the vectors
+// are where resident_stats left them in shared memory.
+template <typename T, bool KEPT>
+__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense &d, bool zero, int64_t hit, float extra,
+                                           const uint4 *kept) {
   constexpr int N = Vec<T>::N, DEPTH = 4;
   const bool same = ((reinterpret_cast<uintptr_t>(sl.row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   auto one = [&](int i) {
@@ -475,12 +547,13 @@ __device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Den
     stf(out + i, v);
   };
   if (same) {
-    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += DEPTH * NT) {
+    kept += threadIdx.x;
+    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += DEPTH * NT, kept += DEPTH * NT) {
       uint4 raw[DEPTH];
       if (!zero) {
 #pragma unroll
         for (int j = 0; j < DEPTH; ++j)
-          if (v + j * NT < sl.v1) raw[j] = load16(sl.vec(v + j * NT));
+          if (v + j * NT < sl.v1) raw[j] = KEPT ? kept[j * NT] : load16(sl.vec(v + j * NT));
       }
 #pragma unroll
       for (int j = 0; j < DEPTH; ++j) {
@@ -536,7 +609,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__re
   const float ent = a.entropy ? a.entropy[r] : 0.f;
   const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
   const Dense d{m, log_s * LOG2E, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t};
-  write_grad(sl, grad + grows.at(r), d, zero, t, g * a.inv_t);
+  write_grad<T, false>(sl, grad + grows.at(r), d, zero, t, g * a.inv_t, nullptr);
 }
 
 // ----------------------------------------------------------------- distillation
@@ -564,12 +637,14 @@ __device__ __forceinline__ float nan_max(float a, float b) {
 }
 
 // loss = sum q_i (log q_i - log p_id_i), dx_j = w (p_j - sum_{id_i = j} q_i) / T; q: softmax over the used entries of
-// the teacher's logits / T, thread i holding entry i.  GRAD: the gradient is written too.
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(NT, 4) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
+// the teacher's logits / T, thread i holding entry i.  GRAD: the gradient is written too.  RES: the slice stays in shared
+// memory between the statistics and the gradient, so that the logits are read from memory once.
+template <typename T, bool GRAD, bool RES>
+__global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
                                                         T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
+  extern __shared__ uint4 buffer[];  // the ring, or with RES the slice
   __shared__ RowShared sh;
   __shared__ float red[NW];
   __shared__ int64_t sid[MAX_TOP];
@@ -596,7 +671,9 @@ __global__ void __launch_bounds__(NT, 4) distill_kernel(const T *__restrict__ lo
   const float q = used ? te / ts : 0.f;
   const bool bad = q != 0.f && id >= a.V;
   const RowStats st = a.stats_in ? RowStats{a.stats_in[2 * r], a.stats_in[2 * r + 1], 0.f}
-                                 : finish(row_join<false>(thread_stats<T, false>(sl, a.c2), sh, a.c2, rank, parts));
+                                 : finish(row_join<false>(RES ? resident_stats<T, false>(sl, a.c2, buffer)
+                                                              : thread_stats<T, false>(sl, a.c2, buffer),
+                                                          sh, a.c2, rank, parts));
   float lp = 0.f;
   if (q != 0.f && !bad) lp = log_prob(ldf(row + id), st.m, st.log_s, a.inv_t);
   if (a.loss && rank == 0) {
@@ -618,7 +695,7 @@ __global__ void __launch_bounds__(NT, 4) distill_kernel(const T *__restrict__ lo
     const bool zero = !used || w == 0.f || st.m == -INFINITY;
     T *out = grad + grows.at(r);
     const Dense d{st.m, st.log_s * LOG2E, a.c2, any_bad ? NAN : w, 0.f};
-    write_grad(sl, out, d, zero, -1, 0.f);
+    write_grad<T, RES>(sl, out, d, zero, -1, 0.f, buffer);
     __syncthreads();  // the teacher's elements are written again, after the pass over all of them
     const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
     if (!zero && !any_bad && q != 0.f && mine) {
@@ -646,10 +723,12 @@ inline int row_parts(int64_t rows, int V, int elem) {
 
 // Launch with the CTAs of a row as a cluster.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int parts, cudaStream_t stream, Args... args) {
+inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int parts, size_t smem, cudaStream_t stream,
+                               Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * parts));
   cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -701,7 +780,7 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   MTP_DISPATCH_LOGITS(dtype, T, {
     auto kern = top_k ? (entropy ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, false, true>)
                       : (entropy ? token_logprobs_kernel<T, true, false> : token_logprobs_kernel<T, false, false>);
-    launch_rows(kern, n, parts, s, (const T *)logits, rows, a);
+    launch_rows(kern, n, parts, 0, s, (const T *)logits, rows, a);
   });
   return check_launch("token_logprobs");
 }
@@ -738,8 +817,8 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
   const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
   const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature,
                       (float)(1.4426950408889634 / temperature), V, parts};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false>, n, parts, s, (const T *)logits, rows, a,
-                                            (T *)nullptr, rows));
+  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false, false>, n, parts, RING_BYTES, s,
+                                            (const T *)logits, rows, a, (T *)nullptr, rows));
   return check_launch("distill_topk");
 }
 
@@ -754,11 +833,30 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows{inner, ld_outer, ld}, grows{inner, grad_ld_outer, grad_ld};
   const int64_t n = outer * inner;
-  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const int elem = dtype == MTP_F32 ? 4 : 2;
+  int parts = row_parts(n, V, elem);
+  // keep the slices resident: CTAs per row until a slice fits (a head of up to 15 bytes may leave one vector less)
+  auto fits = [&](int c) { return ((int64_t)V * elem / 16 + c - 1) / c <= RESIDENT * NT; };
+  bool res = stats == nullptr;
+  if (res) {
+    int c = parts;
+    while (c < MAX_CLUSTER && !fits(c)) c *= 2;
+    res = fits(c);
+    if (res) parts = c;
+  }
   const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature,
                       (float)(1.4426950408889634 / temperature), V, parts};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, true>, n, parts, s, (const T *)logits, rows, a,
-                                            (T *)grad, grows));
+  MTP_DISPATCH_LOGITS(dtype, T, {
+    if (res) {
+      // set at every call: the attribute belongs to the current device
+      if (cudaFuncSetAttribute(distill_kernel<T, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               RESIDENT_BYTES) != cudaSuccess)
+        return fail(MTP_ERR_CUDA, "distill_topk_grad: shared memory");
+      launch_rows(distill_kernel<T, true, true>, n, parts, RESIDENT_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
+    } else {
+      launch_rows(distill_kernel<T, true, false>, n, parts, RING_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
+    }
+  });
   return check_launch("distill_topk_grad");
 }
 

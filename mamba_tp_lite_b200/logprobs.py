@@ -51,17 +51,19 @@ def _check_logits(x: torch.Tensor, what: str) -> None:
 def _check_ids(ids: torch.Tensor, shape, device, what: str, name: str) -> torch.Tensor:
     if ids.dtype not in _INT_TYPES:
         raise TypeError(f"{what}: {name} must be integers, got {ids.dtype}")
-    if tuple(ids.shape) != tuple(shape):
+    if ids.shape != shape:
         raise ValueError(f"{what}: {name} have shape {tuple(ids.shape)}, expected {tuple(shape)}")
     if ids.device != device:
         raise ValueError(f"{what}: {name} are on {ids.device}, the logits on {device}")
-    return ids.to(torch.int64).contiguous()
+    if ids.dtype != torch.int64:
+        ids = ids.to(torch.int64)
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def _check_rows(v: torch.Tensor, shape, device, what: str, name: str) -> torch.Tensor:
     if not v.dtype.is_floating_point:
         raise TypeError(f"{what}: {name} must be floating point, got {v.dtype}")
-    if tuple(v.shape) != tuple(shape):
+    if v.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(v.shape)}, expected {tuple(shape)}")
     if v.device != device:
         raise ValueError(f"{what}: {name} is on {v.device}, the logits on {device}")
@@ -123,34 +125,34 @@ def _grad_like(x: torch.Tensor, inner: int, ld_outer: int, ld: int):
     return buf.as_strided(x.shape, x.stride(), off), ld_outer, ld
 
 
-class _on:
-    """The logits' device as the current one for a launch (no cost where it already is)."""
+def _call(x: torch.Tensor, name: str, *args) -> None:
+    """The entry point ``name`` on the current stream of x's device, as the current device."""
+    if x.device.index == torch.cuda.current_device():
+        L.call(name, *args, L.stream_ptr())
+    else:
+        with torch.cuda.device(x.device):
+            L.call(name, *args, L.stream_ptr())
 
-    def __init__(self, x: torch.Tensor):
-        self.guard = None if x.device.index == torch.cuda.current_device() else torch.cuda.device(x.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _row_like(x: torch.Tensor, ids: torch.Tensor | None) -> torch.Tensor:
+    """An uninitialised fp32 value per row of x; ids [...] or None has x's leading shape."""
+    if ids is not None:  # the cheapest of torch's allocating calls
+        return torch.empty_like(ids, dtype=torch.float32)
+    return x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
 # ------------------------------------------------------------------ log probabilities
 def _logprobs_fwd(x, targets, top_k, temperature, entropy, want_stats):
-    lead = x.shape[:-1]
+    lp = None if targets is None else _row_like(x, targets)
+    ent = _row_like(x, targets) if entropy else None
+    stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32) if want_stats else None
+    ids = tlp = None
+    if top_k:
+        ids = x.new_empty((*x.shape[:-1], top_k), dtype=torch.int64)
+        tlp = torch.empty_like(ids, dtype=torch.float32)
     x, outer, inner, ld_outer, ld = _row_layout(x)
-    new = lambda *tail, dtype=torch.float32: torch.empty((*lead, *tail), device=x.device, dtype=dtype)
-    lp = None if targets is None else new()
-    ent = new() if entropy else None
-    stats = new(2) if want_stats else None
-    ids, tlp = (new(top_k, dtype=torch.int64), new(top_k)) if top_k else (None, None)
-    with _on(x):
-        L.call("mtp_token_logprobs", L.ptr(x), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
-               L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), L.ptr(stats), top_k, L.ptr(ids), L.ptr(tlp),
-               L.stream_ptr())
+    _call(x, "mtp_token_logprobs", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
+          L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), L.ptr(stats), top_k, L.ptr(ids), L.ptr(tlp))
     return lp, ent, stats, ids, tlp
 
 
@@ -179,10 +181,9 @@ def _logprobs_bwd(x, targets, temperature, stats, ent, g, h):
     h = None if h is None else h.float().contiguous()
     x, outer, inner, ld_outer, ld = _row_layout(x)
     grad, g_ld_outer, g_ld = _grad_like(x, inner, ld_outer, ld)
-    with _on(x):
-        L.call("mtp_token_logprobs_bwd", L.ptr(x), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
-               L.ptr(targets), temperature, L.ptr(stats), L.ptr(ent), L.ptr(g), L.ptr(h), L.ptr(grad), g_ld_outer, g_ld,
-               L.stream_ptr())
+    _call(x, "mtp_token_logprobs_bwd", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
+          L.ptr(targets), temperature, stats.data_ptr(), ent.data_ptr(), L.ptr(g), L.ptr(h), grad.data_ptr(), g_ld_outer,
+          g_ld)
     return grad
 
 
@@ -214,10 +215,10 @@ def _teacher(logits, ids, values, what):
     if ids.dim() != logits.dim() or not 1 <= ids.shape[-1] <= MAX_TOP:
         raise ValueError(f"{what}: teacher ids have shape {tuple(ids.shape)}, expected {tuple(logits.shape[:-1])} and "
                          f"1 to {MAX_TOP} entries")
-    shape = (*logits.shape[:-1], ids.shape[-1])
+    shape = torch.Size((*logits.shape[:-1], ids.shape[-1]))
     ids = _check_ids(ids, shape, logits.device, what, "teacher ids")
-    if tuple(values.shape) != shape:
-        raise ValueError(f"{what}: teacher logits have shape {tuple(values.shape)}, expected {shape}")
+    if values.shape != shape:
+        raise ValueError(f"{what}: teacher logits have shape {tuple(values.shape)}, expected {tuple(shape)}")
     if values.device != logits.device:
         raise ValueError(f"{what}: teacher logits are on {values.device}, the logits on {logits.device}")
     L.dtype_code(values.dtype)
@@ -225,26 +226,22 @@ def _teacher(logits, ids, values, what):
 
 
 def _distill_fwd(x, ids, values, temperature, want_stats):
-    lead = x.shape[:-1]
+    loss = _row_like(x, None)
+    stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32) if want_stats else None
     x, outer, inner, ld_outer, ld = _row_layout(x)
-    loss = torch.empty(lead, device=x.device, dtype=torch.float32)
-    stats = torch.empty((*lead, 2), device=x.device, dtype=torch.float32) if want_stats else None
-    with _on(x):
-        L.call("mtp_distill_topk", L.ptr(x), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1], L.ptr(ids),
-               L.ptr(values), L.dtype_code(values.dtype), ids.shape[-1], temperature, L.ptr(loss), L.ptr(stats),
-               L.stream_ptr())
+    _call(x, "mtp_distill_topk", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
+          ids.data_ptr(), values.data_ptr(), L.dtype_code(values.dtype), ids.shape[-1], temperature, loss.data_ptr(),
+          L.ptr(stats))
     return loss, stats
 
 
 def _distill_grad(x, ids, values, temperature, stats, weight, want_loss):
-    lead = x.shape[:-1]
+    loss = _row_like(x, None) if want_loss else None
     x, outer, inner, ld_outer, ld = _row_layout(x)
-    loss = torch.empty(lead, device=x.device, dtype=torch.float32) if want_loss else None
     grad, g_ld_outer, g_ld = _grad_like(x, inner, ld_outer, ld)
-    with _on(x):
-        L.call("mtp_distill_topk_grad", L.ptr(x), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
-               L.ptr(ids), L.ptr(values), L.dtype_code(values.dtype), ids.shape[-1], temperature, L.ptr(stats),
-               L.ptr(weight), L.ptr(loss), L.ptr(grad), g_ld_outer, g_ld, L.stream_ptr())
+    _call(x, "mtp_distill_topk_grad", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
+          ids.data_ptr(), values.data_ptr(), L.dtype_code(values.dtype), ids.shape[-1], temperature, L.ptr(stats),
+          weight.data_ptr(), L.ptr(loss), grad.data_ptr(), g_ld_outer, g_ld)
     return loss, grad
 
 
@@ -329,14 +326,15 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.
     rows = x.shape[0]
     args = (L.ptr(x), x.stride(0) if rows > 1 else k, rows, k, L.ptr(weight), weight.stride(0) if v > 1 else k, v,
             L.dtype_code(x.dtype))
-    new = lambda *tail, dtype=torch.float32: torch.empty((*lead, *tail), device=x.device, dtype=dtype)
-    lp = None if targets is None else new()
-    ent = new() if entropy else None
-    ids, tlp = (new(top_k, dtype=torch.int64), new(top_k)) if top_k else (None, None)
+    lp = None if targets is None else _row_like(hidden, targets)
+    ent = _row_like(hidden, targets) if entropy else None
+    ids = tlp = None
+    if top_k:
+        ids = x.new_empty((*lead, top_k), dtype=torch.int64)
+        tlp = torch.empty_like(ids, dtype=torch.float32)
     need = C.c_int64(0)
-    with _on(x):
-        L.call("mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need))
-        work = torch.empty(need.value, device=x.device, dtype=torch.uint8)
-        L.call("mtp_lm_head_logprobs", *args, L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), top_k, L.ptr(ids),
-               L.ptr(tlp), L.ptr(work), need.value, L.stream_ptr())
+    L.call("mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need))
+    work = x.new_empty(need.value, dtype=torch.uint8)
+    _call(x, "mtp_lm_head_logprobs", *args, L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), top_k, L.ptr(ids),
+          L.ptr(tlp), work.data_ptr(), need.value)
     return TokenLogprobs(lp, ent, ids, tlp)

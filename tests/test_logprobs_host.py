@@ -140,7 +140,7 @@ def test_argument_checks():
     x = torch.randn(2, 3, 8)
     ids = torch.zeros(2, 3, dtype=torch.int64)
     with pytest.raises(TypeError, match="integers"):
-        P._check_ids(ids.float(), (2, 3), x.device, "f", "targets")
+        P._check_ids(ids.float(), x.shape[:-1], x.device, "f", "targets")
     with pytest.raises(TypeError, match="integers"):
         P._check_ids(ids.bool(), (2, 3), x.device, "f", "targets")
     with pytest.raises(ValueError, match="shape"):
