@@ -201,35 +201,42 @@ __device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, uin
   return st;
 }
 
-template <bool ENT>
-__device__ __forceinline__ Stat warp_join(Stat st, float c2) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Stat other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.u = ENT ? __shfl_xor_sync(0xffffffffu, st.u, o) : 0.f;
-    st = join<ENT>(st, other, c2);
-  }
-  return st;
-}
-
 // Shared state of the CTAs of a row.  Every CTA gets every CTA's statistics (and group maxima) in its own copy.
 struct RowShared {
-  Stat warp[NW];
+  float m[NW];
+  float2 su[NW];
   Stat cta[MAX_CLUSTER];
 };
 
 // Joins the threads of the CTA and the CTAs of the cluster; every thread of the cluster returns the row's statistics.
-// Orders the shared memory written before it (the group maxima, peers' copies included) for all threads.
+// The CTA's maximum comes first, so that each thread rescales its sums once and the rest are additions, in an order
+// that is the same in every thread.  Orders the shared memory written before it (the group maxima, peers' copies
+// included) for all threads.
 template <bool ENT>
-__device__ Stat row_join(Stat st, RowShared &sh, float c2, int rank, int parts) {
-  st = warp_join<ENT>(st, c2);
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
-  __syncthreads();
-  Stat all = sh.warp[0];
+__device__ __forceinline__ Stat row_join(Stat st, RowShared &sh, float c2, int rank, int parts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = st.m;
 #pragma unroll
-  for (int i = 1; i < NW; ++i) all = join<ENT>(all, sh.warp[i], c2);  // the same order in every thread
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) sh.m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) m = fmaxf(m, sh.m[i]);
+  const float y = fmaxf((st.m - m) * c2, FLOOR_Y), e = ex2(y);
+  float u = ENT ? fmaf(y, st.s, st.u) * e : 0.f, s = st.s * e;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (ENT) u += __shfl_xor_sync(0xffffffffu, u, o);
+  }
+  if (lane == 0) sh.su[warp] = make_float2(s, u);
+  __syncthreads();
+  Stat all{m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    all.s += sh.su[i].x;
+    all.u += sh.su[i].y;
+  }
   if (parts > 1) {
     cg::cluster_group cl = cg::this_cluster();
     if (threadIdx.x < (unsigned)parts) *cl.map_shared_rank(&sh.cta[rank], threadIdx.x) = all;

@@ -84,12 +84,24 @@ __device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float 
     un2(y, y0, y1);
     const F2 e = f2(ex2(y0), ex2(y1));
     s = add2(s, e);
-    if constexpr (ENT) u = fma2(e, f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), u);
+    if constexpr (ENT) u = fma2(e, y, u);
   }
-  float s0, s1, u0, u1;
+  float s0, s1;
   un2(s, s0, s1);
-  un2(u, u0, u1);
-  if constexpr (ENT) st.u = fmaf(fmaf(dy, st.s, st.u), corr, u0 + u1);
+  if constexpr (ENT) {
+    float u0, u1;
+    un2(u, u0, u1);
+    u0 += u1;
+    if (u0 != u0) {  // 0 * -inf of a masked logit (or a NaN among x): the same with y no lower than FLOOR_Y
+      u0 = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = (x[i] - m) * c2;
+        u0 = fmaf(ex2(y), fmaxf(y, FLOOR_Y), u0);
+      }
+    }
+    st.u = fmaf(fmaf(dy, st.s, st.u), corr, u0);
+  }
   st.s = fmaf(st.s, corr, s0 + s1);
   st.m = m;
 }
