@@ -528,21 +528,42 @@ __global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restri
 }
 
 // ----------------------------------------------------------------- gradients
-// out_j = p_j (a + b y_j) with p_j = 2^y_j, y = log2 p; the element `hit` gets `extra` on top.
-struct Dense {
+// out_j = p_j (a + b y_j) with p_j = 2^y_j, y = log2 p; the element `hit` gets `extra` on top.  ENT: b is not 0.
+// A p below 2^-126 still counts where its factor is large: 2^(y + 32) is taken, which is flushed to zero only where p
+// is below the smallest subnormal, and 2^-32 goes into the factor.
+template <bool ENT> struct Dense {
   float m, l2, c2;  // largest logit, log2 S, log2 e / T
-  float a, b;
+  float a, b;       // times 2^-32
+  static constexpr float LIFT = 32.f;
+  __device__ __forceinline__ Dense(float m_, float log_s, float c2_, float a_, float b_)
+      : m(m_), l2(log_s * LOG2E), c2(c2_), a(a_ * 0x1p-32f), b(b_ * 0x1p-32f) {
+    if (!ENT) l2 -= LIFT;
+  }
+  __device__ __forceinline__ F2 two(F2 x) const {
+    const F2 y = fma2(add2(x, f2(-m, -m)), f2(c2, c2), f2(-l2, -l2));
+    float y0, y1;
+    if constexpr (!ENT) {
+      un2(y, y0, y1);
+      return mul2(f2(ex2(y0), ex2(y1)), f2(a, a));
+    } else {
+      un2(y, y0, y1);
+      const F2 f = fma2(f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), f2(b, b), f2(a, a));
+      un2(add2(y, f2(LIFT, LIFT)), y0, y1);
+      return mul2(f2(ex2(y0), ex2(y1)), f);
+    }
+  }
   __device__ __forceinline__ float one(float x) const {
-    const float y = (x - m) * c2 - l2;
-    return ex2_sub(y) * fmaf(b, fmaxf(y, FLOOR_Y), a);
+    float v, w;
+    un2(two(f2(x, x)), v, w);
+    return v;
   }
 };
 
 // Writes the slice's gradient.  16-byte stores where the gradient row is aligned as the logits row is.  KEPT: the vectors
 // are where resident_stats left them in shared memory.
-template <typename T, bool KEPT>
-__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense &d, bool zero, int64_t hit, float extra,
-                                           const uint4 *kept) {
+template <typename T, bool KEPT, bool ENT>
+__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense<ENT> &d, bool zero, int64_t hit,
+                                           float extra, const uint4 *kept) {
   constexpr int N = Vec<T>::N, DEPTH = 4;
   const bool same = ((reinterpret_cast<uintptr_t>(sl.row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   auto one = [&](int i) {
@@ -553,38 +574,42 @@ __device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Den
     }
     stf(out + i, v);
   };
-  if (same) {
-    kept += threadIdx.x;
-    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += DEPTH * NT, kept += DEPTH * NT) {
+  if (!same) {
+    for (int64_t i = sl.first(sl.v0) + (int)threadIdx.x; i < sl.first(sl.v1); i += NT) one((int)i);
+  } else if (zero) {
+    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += NT)
+      __stcs(reinterpret_cast<uint4 *>(out + sl.first(v)), make_uint4(0, 0, 0, 0));
+  } else {
+    const int n = thread_vectors(sl), v0 = sl.v0 + (int)threadIdx.x;
+    const int hv = hit >= sl.first(sl.v0) && hit < sl.first(sl.v1) ? (int)((hit - sl.head) / N) : -1;
+    const T *src = sl.vec(v0);
+    T *dst = out + sl.first(v0);
+    const uint4 *keep = kept + threadIdx.x;
+    constexpr int STEP = NT * N;
+    for (int i = 0; i < n; i += DEPTH) {
       uint4 raw[DEPTH];
-      if (!zero) {
 #pragma unroll
-        for (int j = 0; j < DEPTH; ++j)
-          if (v + j * NT < sl.v1) raw[j] = KEPT ? kept[j * NT] : load16(sl.vec(v + j * NT));
-      }
+      for (int j = 0; j < DEPTH; ++j)
+        if (i + j < n) raw[j] = KEPT ? keep[(i + j) * NT] : load16(src + j * STEP);
 #pragma unroll
       for (int j = 0; j < DEPTH; ++j) {
-        if (v + j * NT < sl.v1) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (!zero) {
-            float x[N];
-            Vec<T>::unpack(raw[j], x);
+        if (i + j < n) {
+          float x[N];
+          Vec<T>::unpack(raw[j], x);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = d.one(x[i]);
-            const int64_t at = hit - sl.first(v + j * NT);
-            if (at >= 0 && at < N) {
+          for (int k = 0; k < N; k += 2) un2(d.two(f2(x[k], x[k + 1])), x[k], x[k + 1]);
+          if (v0 + (i + j) * NT == hv) {
+            const int at = (int)(hit - sl.first(hv));
 #pragma unroll
-              for (int i = 0; i < N; ++i)
-                if (i == at) x[i] += extra;
-            }
-            w = Vec<T>::pack(x);
+            for (int k = 0; k < N; ++k)
+              if (k == at) x[k] += extra;
           }
-          __stcs(reinterpret_cast<uint4 *>(out + sl.first(v + j * NT)), w);
+          __stcs(reinterpret_cast<uint4 *>(dst + j * STEP), Vec<T>::pack(x));
         }
       }
+      src += DEPTH * STEP;
+      dst += DEPTH * STEP;
     }
-  } else {
-    for (int64_t i = sl.first(sl.v0) + (int)threadIdx.x; i < sl.first(sl.v1); i += NT) one((int)i);
   }
   if (threadIdx.x < (unsigned)sl.nhead) one(threadIdx.x);
   if (threadIdx.x < (unsigned)sl.ntail) one(sl.tail0 + threadIdx.x);
@@ -598,7 +623,7 @@ struct BwdArgs {
 };
 
 // dx_j = (g (1{j = t} - p_j) - h p_j (log p_j + H)) / T
-template <typename T>
+template <typename T, bool ENT>
 __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
                                                                    T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
@@ -606,17 +631,17 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__re
   const int64_t r = blockIdx.x / a.parts;
   const Slice<T> sl(logits + rows.at(r), a.V, (int)(blockIdx.x % a.parts), a.parts);
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1];
-  const float h = a.d_entropy ? a.d_entropy[r] : 0.f;
+  const float h = ENT ? a.d_entropy[r] : 0.f;
   int64_t t = -1;
   float g = 0.f;
   if (a.d_logprob) {
     t = a.targets[r];
     g = t < 0 ? 0.f : t >= a.V ? NAN : a.d_logprob[r];
   }
-  const float ent = a.entropy ? a.entropy[r] : 0.f;
+  const float ent = ENT ? a.entropy[r] : 0.f;
   const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
-  const Dense d{m, log_s * LOG2E, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t};
-  write_grad<T, false>(sl, grad + grows.at(r), d, zero, t, g * a.inv_t, nullptr);
+  const Dense<ENT> d(m, log_s, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t);
+  write_grad<T, false, ENT>(sl, grad + grows.at(r), d, zero, t, g * a.inv_t, nullptr);
 }
 
 // ----------------------------------------------------------------- distillation
@@ -701,8 +726,8 @@ __global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__re
     const float w = a.row_weight[r] * a.inv_t;
     const bool zero = !used || w == 0.f || st.m == -INFINITY;
     T *out = grad + grows.at(r);
-    const Dense d{st.m, st.log_s * LOG2E, a.c2, any_bad ? NAN : w, 0.f};
-    write_grad<T, RES>(sl, out, d, zero, -1, 0.f, buffer);
+    const Dense<false> d(st.m, st.log_s, a.c2, any_bad ? NAN : w, 0.f);
+    write_grad<T, RES, false>(sl, out, d, zero, -1, 0.f, buffer);
     __syncthreads();  // the teacher's elements are written again, after the pass over all of them
     const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
     if (!zero && !any_bad && q != 0.f && mine) {
@@ -714,7 +739,7 @@ __global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__re
           first = first && j >= (int)threadIdx.x;
         }
       }
-      if (first) stf(out + id, w * (ex2_sub(lp * LOG2E) - qs));
+      if (first) stf(out + id, w * (ex2(lp * LOG2E) - qs));
     }
   }
 }
@@ -806,8 +831,10 @@ int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t
   const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
   const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature,
                   (float)(1.4426950408889634 / temperature), V, parts};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_pdl(token_logprobs_bwd_kernel<T>, dim3((unsigned)(n * parts)), dim3(NT), 0, s,
-                                           (const T *)logits, rows, a, (T *)grad, grows));
+  MTP_DISPATCH_LOGITS(dtype, T, {
+    auto kern = d_entropy ? token_logprobs_bwd_kernel<T, true> : token_logprobs_bwd_kernel<T, false>;
+    launch_pdl(kern, dim3((unsigned)(n * parts)), dim3(NT), 0, s, (const T *)logits, rows, a, (T *)grad, grows);
+  });
   return check_launch("token_logprobs_bwd");
 }
 

@@ -16,10 +16,9 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// The same with subnormal results kept (a gradient is a product of one with a factor that can be large).
-__device__ __forceinline__ float ex2_sub(float x) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -69,10 +68,9 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
 
 template <bool ENT, int N>
 __device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float c2) {
-  float mx = x[0];
+  float m = st.m;
 #pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  const float m = fmaxf(st.m, mx);
+  for (int i = 0; i < N; i += 2) m = max3(m, x[i], x[i + 1]);
   const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
   const float corr = ex2(dy);
   const F2 nm = f2(-m, -m), cc = f2(c2, c2);
