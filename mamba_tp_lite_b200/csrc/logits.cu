@@ -23,10 +23,28 @@ constexpr int NW = NT / 32;
 constexpr int MAX_CLUSTER = 8;    // CTAs that share a row
 constexpr int LIST = 1024;        // candidates for the alternatives that a CTA holds
 
-// Row r of a batch laid out as [outer][inner] rows: r = o * inner + i.
+// Row r of a batch laid out as [outer][inner] rows: r = o * inner + i; inner 0: one level, r = i.  (Integer divisions are
+// what a thread's fixed cost per row consists of, so they are few and of 32 bits.)
 struct Rows {
-  int64_t inner, ld_outer, ld;
-  __device__ __forceinline__ int64_t at(int64_t r) const { return (r / inner) * ld_outer + (r % inner) * ld; }
+  uint32_t inner;
+  int64_t ld_outer, ld;
+  __device__ __forceinline__ int64_t at(uint32_t r) const {
+    if (inner == 0) return r * ld;
+    const uint32_t o = r / inner;
+    return o * ld_outer + (r - o * inner) * ld;
+  }
+};
+inline Rows make_rows(int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld) {
+  if (outer == 1) return Rows{0, 0, ld};
+  if (inner == 1) return Rows{0, 0, ld_outer};
+  return Rows{(uint32_t)inner, ld_outer, ld};
+}
+
+// CTA of a row: 2^shift of them share it.
+struct Part {
+  uint32_t row;
+  int rank, shift;
+  __device__ __forceinline__ explicit Part(int s) : row(blockIdx.x >> s), rank((int)(blockIdx.x & ((1u << s) - 1))), shift(s) {}
 };
 
 // ----------------------------------------------------------------- rows in vectors
@@ -75,21 +93,21 @@ __device__ __forceinline__ uint4 load16(const void *p) {
   return r;
 }
 
-// The part of a row that CTA `rank` of `parts` works on: vectors [v0, v1) of those that start `head` elements into the
+// The part of a row that CTA `rank` of 2^shift works on: vectors [v0, v1) of those that start `head` elements into the
 // row, the first CTA also the elements before them, the last the `tail` elements from `tail0` on.
 template <typename T> struct Slice {
   const T *row;
   int head, v0, v1, nhead, tail0, ntail;
-  __device__ __forceinline__ Slice(const T *r, int V, int rank, int parts) : row(r) {
+  __device__ __forceinline__ Slice(const T *r, int V, int rank, int shift) : row(r) {
     constexpr int N = Vec<T>::N;
     head = (int)(((16u - (unsigned)(reinterpret_cast<uintptr_t>(r) & 15u)) & 15u) / sizeof(T));
     if (head > V) head = V;
     const int nv = (V - head) / N;
-    v0 = (int)((long long)nv * rank / parts);
-    v1 = (int)((long long)nv * (rank + 1) / parts);
+    v0 = (int)((int64_t)nv * rank >> shift);
+    v1 = (int)((int64_t)nv * (rank + 1) >> shift);
     nhead = rank == 0 ? head : 0;
     tail0 = head + nv * N;
-    ntail = rank == parts - 1 ? V - tail0 : 0;
+    ntail = rank + 1 == 1 << shift ? V - tail0 : 0;
   }
   __device__ __forceinline__ const T *vec(int v) const { return row + head + (int64_t)v * Vec<T>::N; }
   __device__ __forceinline__ int first(int v) const { return head + v * Vec<T>::N; }  // index of a vector's first element
@@ -172,9 +190,7 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2, uint4
 
 // The same with the whole slice kept in shared memory, at most RESIDENT vectors per thread, all of them in flight at once.
 constexpr int RESIDENT = 13, RESIDENT_BYTES = RESIDENT * NT * 16;
-template <typename T, bool ENT>
-__device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, uint4 *keep) {
-  Stat st{LOWEST, 0.f, 0.f};
+template <typename T> __device__ __forceinline__ void resident_fetch(const Slice<T> &sl, uint4 *keep) {
   const int n = thread_vectors(sl);
   const T *src = sl.vec(sl.v0 + (int)threadIdx.x);
   constexpr int STEP = NT * Vec<T>::N, PAIRS = (RESIDENT + 1) / 2;
@@ -185,6 +201,14 @@ __device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, uin
     if (2 * j + 1 < n) copy16(mine + (2 * j + 1) * NT, src + (int64_t)(2 * j + 1) * STEP);
     copy_commit();
   }
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, const uint4 *keep) {
+  Stat st{LOWEST, 0.f, 0.f};
+  const int n = thread_vectors(sl);
+  const uint4 *mine = keep + threadIdx.x;
+  constexpr int PAIRS = (RESIDENT + 1) / 2;
   auto step = [&](int j) {
     if (2 * j + 1 < n) accumulate_pair<T, ENT>(st, mine[2 * j * NT], mine[(2 * j + 1) * NT], c2);
     else if (2 * j < n) accumulate_vec<T, ENT>(st, mine[2 * j * NT], c2);
@@ -212,12 +236,19 @@ struct RowShared {
 // The CTA's maximum comes first, so that each thread rescales its sums once and the rest are additions, in an order
 // that is the same in every thread.  Orders the shared memory written before it (the group maxima, peers' copies
 // included) for all threads.
+// cluster_begin, called once before: a CTA of the cluster says that it runs and its shared memory may be written.
+__device__ __forceinline__ void cluster_begin(int parts) {
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_ready(int parts) {
+  if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
 template <bool ENT>
 __device__ __forceinline__ Stat row_join(Stat st, RowShared &sh, float c2, int rank, int parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m = st.m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(st.m));
   if (lane == 0) sh.m[warp] = m;
   __syncthreads();
 #pragma unroll
@@ -283,6 +314,7 @@ struct TopShared {
   uint64_t *list;       // [LIST] this CTA's candidates, [MAX_CLUSTER * MAX_TOP] the cluster's after them: both lie in
                         // the ring, which has been read when the first candidate is written
   uint64_t red[NW];
+  unsigned char lanes[NW][32];
   uint32_t bound;
   int n;
 };
@@ -317,19 +349,45 @@ __device__ __forceinline__ uint32_t group_bound(const uint32_t *group, int k) {
   return lo;
 }
 
-// Calls f(value, index) for the elements of thread t of the slice; the lanes of the calling warp share them.
+// Calls f(value, index) for the elements of those threads of the calling warp whose bit in `todo` is set.  The lanes
+// share all of their vectors, four loads in flight each.  lanes: 32 bytes of shared memory of the warp.
 template <typename T, typename F>
-__device__ __forceinline__ void warp_elements(const Slice<T> &sl, int t, F f) {
-  constexpr int N = Vec<T>::N;
-  const int lane = threadIdx.x & 31;
-  for (int v = sl.v0 + t + lane * NT; v < sl.v1; v += 32 * NT) {
-    float x[N];
-    Vec<T>::unpack(load16(sl.vec(v)), x);
+__device__ __forceinline__ void warp_elements(const Slice<T> &sl, unsigned todo, unsigned char *lanes, F f) {
+  constexpr int N = Vec<T>::N, DEPTH = 4;
+  const int lane = threadIdx.x & 31, warp0 = threadIdx.x & ~31;
+  if (todo >> lane & 1) lanes[__popc(todo & ((1u << lane) - 1))] = (unsigned char)lane;
+  __syncwarp();
+  const int each = (sl.v1 - sl.v0 + NT - 1) / NT, items = __popc(todo) * each;
+  for (int base = 0; base < items; base += 32 * DEPTH) {
+    uint4 raw[DEPTH];
+    int at[DEPTH];
 #pragma unroll
-    for (int i = 0; i < N; ++i) f(x[i], sl.first(v) + i);
+    for (int j = 0; j < DEPTH; ++j) {
+      const int item = base + 32 * j + lane;
+      at[j] = -1;
+      if (item < items) {
+        const int v = sl.v0 + warp0 + lanes[item / each] + (item % each) * NT;
+        if (v < sl.v1) {
+          at[j] = sl.first(v);
+          raw[j] = load16(sl.vec(v));
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) {
+      if (at[j] >= 0) {
+        float x[N];
+        Vec<T>::unpack(raw[j], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(x[i], at[j] + i);
+      }
+    }
   }
-  if (lane == 0 && t < sl.nhead) f(ldf(sl.row + t), t);
-  if (lane == 1 && t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
+  if (todo >> lane & 1) {
+    const int t = threadIdx.x;
+    if (t < sl.nhead) f(ldf(sl.row + t), t);
+    if (t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
+  }
 }
 
 // The same for a thread's own elements.
@@ -406,17 +464,15 @@ __device__ void top_alternatives(const Slice<T> &sl, Stat st, RowStats row, int 
   __syncthreads();
   const uint32_t bound = sh.bound;
   // a thread whose sum is NaN may hold a NaN, which its maximum passes over
-  unsigned todo = __ballot_sync(0xffffffffu, order_key(st.s == 0.f ? -INFINITY : st.m) >= bound || st.s != st.s);
-  while (todo) {
-    const int src = __ffs(todo) - 1;
-    todo &= todo - 1;
-    warp_elements(sl, warp * 32 + src, [&](float x, int i) {
-      if (order_key(x) >= bound) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < LIST) sh.list[at] = element_key(x, i);
-      }
-    });
-  }
+  const unsigned todo =
+      __ballot_sync(0xffffffffu, order_key(st.s == 0.f ? -INFINITY : st.m) >= bound || st.s != st.s);
+  const float least = key_value(bound);  // bound 0 (a group without an element) gives NaN, which everything passes
+  warp_elements(sl, todo, sh.lanes[warp], [&](float x, int i) {
+    if (!(x < least)) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < LIST) sh.list[at] = element_key(x, i);
+    }
+  });
   __syncthreads();
   int n = sh.n;
   if (n > LIST) {
@@ -480,7 +536,7 @@ struct FwdArgs {
   int64_t *top_ids;
   float *top_logprobs;
   float inv_t, c2;  // 1 / T, log2 e / T
-  int V, parts;
+  int V, shift;
 };
 
 template <typename T, bool ENT, bool TOP>
@@ -491,13 +547,14 @@ __global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restri
   __shared__ TopShared top;
   __shared__ uint4 ring[2 * RING * NT];
   static_assert(sizeof(ring) >= 8 * (LIST + MAX_CLUSTER * MAX_TOP), "the ring holds the lists");
-  const int parts = a.parts;
-  const int64_t r = blockIdx.x / parts;
-  const int rank = (int)(blockIdx.x % parts);
-  const T *row = logits + rows.at(r);
-  const Slice<T> sl(row, a.V, rank, parts);
-  if (parts > 1) cg::this_cluster().sync();  // every CTA of the cluster runs: its shared memory may be written
+  const Part part(a.shift);
+  const int parts = 1 << a.shift, rank = part.rank;
+  const int64_t r = part.row;
+  const T *row = logits + rows.at(part.row);
+  const Slice<T> sl(row, a.V, rank, a.shift);
+  cluster_begin(parts);
   const Stat st = thread_stats<T, ENT>(sl, a.c2, ring);
+  cluster_ready(parts);
   if constexpr (TOP) {
     if (threadIdx.x == 0) top.list = reinterpret_cast<uint64_t *>(ring);
     // maxima of groups of `parts` threads to every CTA of the cluster
@@ -505,12 +562,14 @@ __global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restri
                      ? order_key(st.s == 0.f ? -INFINITY : st.m)
                      : 0u;
     for (int o = 1; o < parts; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    const int slot = rank * (NT / parts) + threadIdx.x / parts;
-    const int to = threadIdx.x % parts;
+    const int slot = rank * (NT >> a.shift) + ((int)threadIdx.x >> a.shift);
+    const int to = threadIdx.x & (parts - 1);
     if (parts > 1) *cg::this_cluster().map_shared_rank(&top.group[slot], to) = g;
     else top.group[slot] = g;
   }
-  const RowStats s = finish(row_join<ENT>(st, sh, a.c2, rank, parts));
+  const Stat all = row_join<ENT>(st, sh, a.c2, rank, parts);
+  if (!TOP && threadIdx.x >= 32) return;
+  const RowStats s = finish(all);
   if (rank == 0 && threadIdx.x == 0) {
     if (a.logprob) {
       const int64_t t = a.targets[r];
@@ -619,7 +678,7 @@ struct BwdArgs {
   const int64_t *targets;
   const float *stats, *entropy, *d_logprob, *d_entropy;
   float inv_t, c2;
-  int V, parts;
+  int V, shift;
 };
 
 // dx_j = (g (1{j = t} - p_j) - h p_j (log p_j + H)) / T
@@ -628,8 +687,9 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__re
                                                                    T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  const int64_t r = blockIdx.x / a.parts;
-  const Slice<T> sl(logits + rows.at(r), a.V, (int)(blockIdx.x % a.parts), a.parts);
+  const Part part(a.shift);
+  const int64_t r = part.row;
+  const Slice<T> sl(logits + rows.at(part.row), a.V, part.rank, a.shift);
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1];
   const float h = ENT ? a.d_entropy[r] : 0.f;
   int64_t t = -1;
@@ -641,7 +701,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__re
   const float ent = ENT ? a.entropy[r] : 0.f;
   const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
   const Dense<ENT> d(m, log_s, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t);
-  write_grad<T, false, ENT>(sl, grad + grows.at(r), d, zero, t, g * a.inv_t, nullptr);
+  write_grad<T, false, ENT>(sl, grad + grows.at(part.row), d, zero, t, g * a.inv_t, nullptr);
 }
 
 // ----------------------------------------------------------------- distillation
@@ -653,7 +713,7 @@ struct DistillArgs {
   float *loss, *stats;
   const float *stats_in;
   float inv_t, c2;
-  int V, parts;
+  int V, shift;
 };
 
 __device__ __forceinline__ float load_value(const void *p, int64_t i, int dtype) {
@@ -668,6 +728,67 @@ __device__ __forceinline__ float nan_max(float a, float b) {
   return r;
 }
 
+// A row's teacher: token, probability, its log, and the student's logit of entry i; entries that are not used have q = 0.
+struct TeacherShared {
+  int64_t id[MAX_TOP];
+  float q[MAX_TOP], log_q[MAX_TOP], x[MAX_TOP];
+  bool used, bad;  // any entry is used; a used one lies outside the vocabulary, or the probabilities are NaN
+};
+
+// By one warp, four entries a lane.
+template <typename T>
+__device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a, int64_t r, TeacherShared &te) {
+  constexpr int PER = MAX_TOP / 32;
+  const int lane = threadIdx.x;
+  int64_t id[PER];
+  float t[PER], x[PER], m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = lane + 32 * j;
+    id[j] = -1;
+    t[j] = -INFINITY;
+    if (i < a.k) {
+      id[j] = a.ids[r * a.k + i];
+      t[j] = load_value(a.values, r * a.k + i, a.v_dtype);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (id[j] < 0) t[j] = -INFINITY;
+    x[j] = id[j] >= 0 && id[j] < a.V ? ldf(row + id[j]) : 0.f;
+    m = nan_max(m, t[j]);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = nan_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float e[PER], s = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    e[j] = t[j] == -INFINITY ? 0.f : expf((t[j] - m) * a.inv_t);
+    s += e[j];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float ls = logf(s);
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = lane + 32 * j;
+    const float q = s != 0.f ? e[j] / s : 0.f;
+    bad = bad || q != q || (q != 0.f && id[j] >= a.V);
+    if (i < a.k) {
+      te.id[i] = id[j];
+      te.q[i] = q;
+      te.log_q[i] = (t[j] - m) * a.inv_t - ls;
+      te.x[i] = x[j];
+    }
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    te.used = s != 0.f;
+    te.bad = bad;
+  }
+}
+
 // loss = sum q_i (log q_i - log p_id_i), dx_j = w (p_j - sum_{id_i = j} q_i) / T; q: softmax over the used entries of
 // the teacher's logits / T, thread i holding entry i.  GRAD: the gradient is written too.  RES: the slice stays in shared
 // memory between the statistics and the gradient, so that the logits are read from memory once.
@@ -678,87 +799,79 @@ __global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__re
   MTP_PDL_TRIGGER();
   extern __shared__ uint4 buffer[];  // the ring, or with RES the slice
   __shared__ RowShared sh;
-  __shared__ float red[NW];
-  __shared__ int64_t sid[MAX_TOP];
-  __shared__ float sq[MAX_TOP];
-  const int parts = a.parts;
-  const int64_t r = blockIdx.x / parts;
-  const int rank = (int)(blockIdx.x % parts);
-  const T *row = logits + rows.at(r);
-  const Slice<T> sl(row, a.V, rank, parts);
-  if (parts > 1 && !a.stats_in) cg::this_cluster().sync();  // peers' shared memory may be written
-  auto fmx = [](float x, float y) { return nan_max(x, y); };
-  auto add = [](float x, float y) { return x + y; };
-  float tv = -INFINITY;
-  int64_t id = -1;
-  if (threadIdx.x < (unsigned)a.k) {
-    id = a.ids[r * a.k + threadIdx.x];
-    if (id >= 0) tv = load_value(a.values, r * a.k + threadIdx.x, a.v_dtype);
+  __shared__ TeacherShared te;
+  const Part part(a.shift);
+  const int parts = 1 << a.shift, rank = part.rank;
+  const int64_t r = part.row;
+  const T *row = logits + rows.at(part.row);
+  const Slice<T> sl(row, a.V, rank, a.shift);
+  const float w = GRAD ? a.row_weight[r] * a.inv_t : 0.f;
+  if (!a.stats_in) cluster_begin(parts);
+  if (RES) resident_fetch(sl, buffer);
+  if (threadIdx.x < 32) read_teacher(row, a, r, te);  // while the slice is on its way
+  RowStats st;
+  if (a.stats_in) {
+    st = RowStats{a.stats_in[2 * r], a.stats_in[2 * r + 1], 0.f};
+    __syncthreads();
+  } else {
+    const Stat own = RES ? resident_stats<T, false>(sl, a.c2, buffer) : thread_stats<T, false>(sl, a.c2, buffer);
+    cluster_ready(parts);
+    st = finish(row_join<false>(own, sh, a.c2, rank, parts));
   }
-  const float tm = block_reduce(tv, red, fmx);
-  const float td = (tv - tm) * a.inv_t;
-  const float te = tv == -INFINITY ? 0.f : expf(td);
-  const float ts = block_reduce(te, red, add);
-  const bool used = ts != 0.f;
-  const float q = used ? te / ts : 0.f;
-  const bool bad = q != 0.f && id >= a.V;
-  const RowStats st = a.stats_in ? RowStats{a.stats_in[2 * r], a.stats_in[2 * r + 1], 0.f}
-                                 : finish(row_join<false>(RES ? resident_stats<T, false>(sl, a.c2, buffer)
-                                                              : thread_stats<T, false>(sl, a.c2, buffer),
-                                                          sh, a.c2, rank, parts));
-  float lp = 0.f;
-  if (q != 0.f && !bad) lp = log_prob(ldf(row + id), st.m, st.log_s, a.inv_t);
-  if (a.loss && rank == 0) {
-    const float term = bad ? NAN : q != 0.f ? q * ((td - logf(ts)) - lp) : 0.f;
-    const float loss = block_reduce(term, red, add);
-    if (threadIdx.x == 0) a.loss[r] = loss;
-  }
-  if (a.stats && rank == 0 && threadIdx.x == 0) {
-    a.stats[2 * r] = st.m;
-    a.stats[2 * r + 1] = st.log_s;
+  if (rank == 0 && threadIdx.x < 32) {
+    float loss = 0.f;
+    for (int i = threadIdx.x; i < a.k; i += 32)
+      if (te.q[i] != 0.f) loss += te.q[i] * (te.log_q[i] - log_prob(te.x[i], st.m, st.log_s, a.inv_t));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    if (threadIdx.x == 0) {
+      if (a.loss) a.loss[r] = te.bad ? NAN : loss;
+      if (a.stats) {
+        a.stats[2 * r] = st.m;
+        a.stats[2 * r + 1] = st.log_s;
+      }
+    }
   }
   if constexpr (GRAD) {
-    if (threadIdx.x < (unsigned)a.k) {
-      sid[threadIdx.x] = q != 0.f ? id : -1;
-      sq[threadIdx.x] = q;
-    }
-    const bool any_bad = block_reduce(bad ? 1.f : 0.f, red, add) != 0.f;  // also orders sid / sq
-    const float w = a.row_weight[r] * a.inv_t;
-    const bool zero = !used || w == 0.f || st.m == -INFINITY;
-    T *out = grad + grows.at(r);
-    const Dense<false> d(st.m, st.log_s, a.c2, any_bad ? NAN : w, 0.f);
+    const bool zero = !te.used || w == 0.f || st.m == -INFINITY;
+    T *out = grad + grows.at(part.row);
+    const Dense<false> d(st.m, st.log_s, a.c2, te.bad ? NAN : w, 0.f);
     write_grad<T, RES, false>(sl, out, d, zero, -1, 0.f, buffer);
     __syncthreads();  // the teacher's elements are written again, after the pass over all of them
+    if (threadIdx.x >= (unsigned)a.k || zero || te.bad) return;
+    const int64_t id = te.id[threadIdx.x];
     const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
-    if (!zero && !any_bad && q != 0.f && mine) {
+    if (te.q[threadIdx.x] != 0.f && mine) {
       float qs = 0.f;
       bool first = true;
       for (int j = 0; j < a.k; ++j) {
-        if (sid[j] == id) {
-          qs += sq[j];
-          first = first && j >= (int)threadIdx.x;
+        if (te.id[j] == id) {
+          qs += te.q[j];
+          first = first && (j >= (int)threadIdx.x || te.q[j] == 0.f);
         }
       }
+      const float lp = log_prob(te.x[threadIdx.x], st.m, st.log_s, a.inv_t);
       if (first) stf(out + id, w * (ex2(lp * LOG2E) - qs));
     }
   }
 }
 
-// CTAs that share a row: rows alone fill the GPU from about four CTAs per SM on; a CTA takes no fewer than NT vectors.
-inline int row_parts(int64_t rows, int V, int elem) {
+// log2 of the CTAs that share a row: rows alone fill the GPU from about four CTAs per SM on; a CTA takes no fewer than NT
+// vectors.
+inline int row_shift(int64_t rows, int V, int elem) {
   const int64_t want = 4ll * num_sms();
   const int64_t vecs = (int64_t)V * elem / 16;
-  int parts = 1;
-  while (parts < MAX_CLUSTER && rows * parts < want && vecs / (2 * parts) >= NT) parts *= 2;
-  return parts;
+  int shift = 0;
+  while (2 << shift <= MAX_CLUSTER && rows << shift < want && vecs >> (shift + 1) >= NT) ++shift;
+  return shift;
 }
 
 // Launch with the CTAs of a row as a cluster.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int parts, size_t smem, cudaStream_t stream,
+inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int shift, size_t smem, cudaStream_t stream,
                                Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.gridDim = dim3((unsigned)(rows << shift));
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -766,10 +879,10 @@ inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int parts, 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)parts;
+  attr[1].val.clusterDim.x = 1u << shift;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = parts > 1 ? 2 : 1;
+  cfg.numAttrs = shift > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
@@ -804,15 +917,15 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   MTP_REQUIRE(top_k >= 0 && top_k <= MAX_TOP && top_k <= V, "top_k must be between 0 and min(V, 128)");
   MTP_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "top_k needs top_ids and top_logprobs");
   cudaStream_t s = (cudaStream_t)stream;
-  const Rows rows{inner, ld_outer, ld};
+  const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
   const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
-                  (float)(1.4426950408889634 / temperature), V, parts};
+                  (float)(1.4426950408889634 / temperature), V, shift};
   MTP_DISPATCH_LOGITS(dtype, T, {
     auto kern = top_k ? (entropy ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, false, true>)
                       : (entropy ? token_logprobs_kernel<T, true, false> : token_logprobs_kernel<T, false, false>);
-    launch_rows(kern, n, parts, 0, s, (const T *)logits, rows, a);
+    launch_rows(kern, n, shift, 0, s, (const T *)logits, rows, a);
   });
   return check_launch("token_logprobs");
 }
@@ -826,14 +939,14 @@ int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t
   MTP_REQUIRE(!d_logprob || targets, "d_logprob needs targets");
   MTP_REQUIRE(!d_entropy || entropy, "d_entropy needs entropy");
   cudaStream_t s = (cudaStream_t)stream;
-  const Rows rows{inner, ld_outer, ld}, grows{inner, grad_ld_outer, grad_ld};
+  const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
-  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
   const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature,
-                  (float)(1.4426950408889634 / temperature), V, parts};
+                  (float)(1.4426950408889634 / temperature), V, shift};
   MTP_DISPATCH_LOGITS(dtype, T, {
     auto kern = d_entropy ? token_logprobs_bwd_kernel<T, true> : token_logprobs_bwd_kernel<T, false>;
-    launch_pdl(kern, dim3((unsigned)(n * parts)), dim3(NT), 0, s, (const T *)logits, rows, a, (T *)grad, grows);
+    launch_pdl(kern, dim3((unsigned)(n << shift)), dim3(NT), 0, s, (const T *)logits, rows, a, (T *)grad, grows);
   });
   return check_launch("token_logprobs_bwd");
 }
@@ -846,12 +959,12 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
   MTP_REQUIRE(k > 0 && k <= MAX_TOP, "k must be between 1 and 128");
   MTP_REQUIRE(v_dtype == MTP_F32 || v_dtype == MTP_BF16 || v_dtype == MTP_F16, "values must be F32, BF16 or F16");
   cudaStream_t s = (cudaStream_t)stream;
-  const Rows rows{inner, ld_outer, ld};
+  const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const int parts = row_parts(n, V, dtype == MTP_F32 ? 4 : 2);
+  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
   const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature,
-                      (float)(1.4426950408889634 / temperature), V, parts};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false, false>, n, parts, RING_BYTES, s,
+                      (float)(1.4426950408889634 / temperature), V, shift};
+  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false, false>, n, shift, RING_BYTES, s,
                                             (const T *)logits, rows, a, (T *)nullptr, rows));
   return check_launch("distill_topk");
 }
@@ -865,30 +978,30 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   MTP_REQUIRE(k > 0 && k <= MAX_TOP, "k must be between 1 and 128");
   MTP_REQUIRE(v_dtype == MTP_F32 || v_dtype == MTP_BF16 || v_dtype == MTP_F16, "values must be F32, BF16 or F16");
   cudaStream_t s = (cudaStream_t)stream;
-  const Rows rows{inner, ld_outer, ld}, grows{inner, grad_ld_outer, grad_ld};
+  const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
   const int elem = dtype == MTP_F32 ? 4 : 2;
-  int parts = row_parts(n, V, elem);
-  // keep the slices resident: CTAs per row until a slice fits (a head of up to 15 bytes may leave one vector less)
-  auto fits = [&](int c) { return ((int64_t)V * elem / 16 + c - 1) / c <= RESIDENT * NT; };
+  int shift = row_shift(n, V, elem);
+  // keep the slices resident: more CTAs per row until a slice fits
+  auto fits = [&](int c) { return (((int64_t)V * elem / 16 - 1) >> c) + 1 <= RESIDENT * NT; };
   bool res = stats == nullptr;
   if (res) {
-    int c = parts;
-    while (c < MAX_CLUSTER && !fits(c)) c *= 2;
+    int c = shift;
+    while (2 << c <= MAX_CLUSTER && !fits(c)) ++c;
     res = fits(c);
-    if (res) parts = c;
+    if (res) shift = c;
   }
   const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature,
-                      (float)(1.4426950408889634 / temperature), V, parts};
+                      (float)(1.4426950408889634 / temperature), V, shift};
   MTP_DISPATCH_LOGITS(dtype, T, {
     if (res) {
       // set at every call: the attribute belongs to the current device
       if (cudaFuncSetAttribute(distill_kernel<T, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                RESIDENT_BYTES) != cudaSuccess)
         return fail(MTP_ERR_CUDA, "distill_topk_grad: shared memory");
-      launch_rows(distill_kernel<T, true, true>, n, parts, RESIDENT_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
+      launch_rows(distill_kernel<T, true, true>, n, shift, RESIDENT_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
     } else {
-      launch_rows(distill_kernel<T, true, false>, n, parts, RING_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
+      launch_rows(distill_kernel<T, true, false>, n, shift, RING_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
     }
   });
   return check_launch("distill_topk_grad");
