@@ -3,10 +3,13 @@
 //
 // With z = x / T, m = max z and S = sum e^(z - m), a row gives
 //   log p_j = (z_j - m) - log S          H = log S - sum e^(z - m) (z - m) / S
-// All sums and statistics are fp32.  Every kernel reads a row in 16-byte vectors at the row's own alignment (the elements
-// before the first and after the last whole vector one by one), a thread taking every 256th vector.  A forward pass
-// reads its row once: each thread keeps the running maximum m, S and U = sum e^y y (y in units of log2) of its elements
-// and rescales them when m grows; threads, and the CTAs of a cluster that share a row, are joined at the end.
+// All sums and statistics are fp32.  A row belongs to a group of threads: a warp (short rows, eight to a CTA), a CTA, or
+// a cluster of up to 8 CTAs (few rows).  A row is read in 16-byte vectors at its own alignment (the elements before the
+// first and after the last whole vector one by one), through a ring in shared memory that asynchronous copies fill: a
+// thread reads only what it copied itself, so that nothing waits for another thread.  A forward pass reads its row once:
+// each thread keeps the running maximum m, S and U = sum e^y y (y in units of log2) of its elements and rescales them
+// when m grows; threads and CTAs are joined at the end.  A pass that needs the row a second time takes it in the opposite
+// order: first what is still in the ring, then the part of the row that L2 saw last.
 #include <cooperative_groups.h>
 #include "common.cuh"
 #include "logits.cuh"
@@ -18,10 +21,22 @@ namespace cg = cooperative_groups;
 using namespace lg;
 
 constexpr int MAX_TOP = 128;      // alternatives or teacher entries per row
-constexpr int NT = 256;           // threads per CTA
-constexpr int NW = NT / 32;
+constexpr int CTA = 256;          // threads per CTA
 constexpr int MAX_CLUSTER = 8;    // CTAs that share a row
-constexpr int LIST = 1024;        // candidates for the alternatives that a CTA holds
+constexpr int RING = 4;           // pairs of vectors per thread in flight: 32 KB a CTA
+constexpr int RING_BYTES = 2 * RING * CTA * 16;
+
+// The threads that share a row within a CTA: GW warps.
+template <int GW> struct Group {
+  static_assert(GW == 1 || GW == CTA / 32, "a warp or the CTA");
+  static constexpr int NT = 32 * GW, ROWS = CTA / NT;  // threads of the group, groups of the CTA
+  static __device__ __forceinline__ int tid() { return threadIdx.x & (NT - 1); }
+  static __device__ __forceinline__ int index() { return threadIdx.x / NT; }
+  static __device__ __forceinline__ void sync() {
+    if (GW == 1) __syncwarp();
+    else __syncthreads();
+  }
+};
 
 // Row r of a batch laid out as [outer][inner] rows: r = o * inner + i; inner 0: one level, r = i.  (Integer divisions are
 // what a thread's fixed cost per row consists of, so they are few and of 32 bits.)
@@ -40,11 +55,13 @@ inline Rows make_rows(int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld
   return Rows{(uint32_t)inner, ld_outer, ld};
 }
 
-// CTA of a row: 2^shift of them share it.
-struct Part {
+// The calling thread's row, and which of the 2^shift CTAs that share it this one is.
+template <int GW> struct Part {
   uint32_t row;
   int rank, shift;
-  __device__ __forceinline__ explicit Part(int s) : row(blockIdx.x >> s), rank((int)(blockIdx.x & ((1u << s) - 1))), shift(s) {}
+  __device__ __forceinline__ explicit Part(int s)
+      : row(GW == 1 ? blockIdx.x * Group<1>::ROWS + Group<1>::index() : blockIdx.x >> s),
+        rank(GW == 1 ? 0 : (int)(blockIdx.x & ((1u << s) - 1))), shift(GW == 1 ? 0 : s) {}
 };
 
 // ----------------------------------------------------------------- rows in vectors
@@ -94,12 +111,13 @@ __device__ __forceinline__ uint4 load16(const void *p) {
 }
 
 // The part of a row that CTA `rank` of 2^shift works on: vectors [v0, v1) of those that start `head` elements into the
-// row, the first CTA also the elements before them, the last the `tail` elements from `tail0` on.
-template <typename T> struct Slice {
+// row, the first CTA also the elements before them, the last the `tail` elements from `tail0` on.  Thread t of the group
+// takes the vectors v0 + t, v0 + t + NT, ... (n of them), and one of the elements at each end.
+template <typename T, int GW> struct Slice {
+  static constexpr int N = Vec<T>::N, NT = Group<GW>::NT, STEP = NT * N;  // STEP: elements between a thread's vectors
   const T *row;
-  int head, v0, v1, nhead, tail0, ntail;
+  int head, v0, v1, nhead, tail0, ntail, n;
   __device__ __forceinline__ Slice(const T *r, int V, int rank, int shift) : row(r) {
-    constexpr int N = Vec<T>::N;
     head = (int)(((16u - (unsigned)(reinterpret_cast<uintptr_t>(r) & 15u)) & 15u) / sizeof(T));
     if (head > V) head = V;
     const int nv = (V - head) / N;
@@ -108,14 +126,16 @@ template <typename T> struct Slice {
     nhead = rank == 0 ? head : 0;
     tail0 = head + nv * N;
     ntail = rank + 1 == 1 << shift ? V - tail0 : 0;
+    const int left = v1 - v0 - Group<GW>::tid();
+    n = left > 0 ? (left + NT - 1) / NT : 0;
   }
-  __device__ __forceinline__ const T *vec(int v) const { return row + head + (int64_t)v * Vec<T>::N; }
-  __device__ __forceinline__ int first(int v) const { return head + v * Vec<T>::N; }  // index of a vector's first element
+  __device__ __forceinline__ const T *vec(int v) const { return row + head + (int64_t)v * N; }
+  __device__ __forceinline__ int first(int v) const { return head + v * N; }  // index of a vector's first element
+  __device__ __forceinline__ const T *mine() const { return vec(v0 + Group<GW>::tid()); }
+  __device__ __forceinline__ int pairs() const { return ((v1 - v0 + NT - 1) / NT + 1) >> 1; }  // of the group's first thread
 };
 
-// ----------------------------------------------------------------- row statistics
-// Asynchronous 16-byte copies into the calling thread's own places of shared memory: no thread reads another's, so that
-// waiting for one's own copies is all the ordering that is needed.
+// Asynchronous 16-byte copies into the calling thread's own places of shared memory.
 __device__ __forceinline__ void copy16(uint4 *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
@@ -124,119 +144,99 @@ template <int PENDING> __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// Vectors of the slice that thread t takes: v0 + t, v0 + t + NT, ...
-template <typename T> __device__ __forceinline__ int thread_vectors(const Slice<T> &sl) {
-  const int left = sl.v1 - sl.v0 - (int)threadIdx.x;
-  return left > 0 ? (left + NT - 1) / NT : 0;
+// A thread's places: pair p of its vectors is at [(p % RING) * 2 * NT] and NT further.  A group's part is contiguous.
+template <int GW> __device__ __forceinline__ uint4 *ring_of(uint4 *ring) {
+  constexpr int NT = Group<GW>::NT;
+  return ring + Group<GW>::index() * 2 * RING * NT + Group<GW>::tid();
+}
+template <typename T, int GW>
+__device__ __forceinline__ void fetch_pair(const Slice<T, GW> &sl, uint4 *mine, int p) {
+  constexpr int NT = Group<GW>::NT;
+  if (p >= 0 && 2 * p < sl.n) {
+    uint4 *at = mine + (p % RING) * 2 * NT;
+    const T *src = sl.mine() + (int64_t)(2 * p) * sl.STEP;
+    copy16(at, src);
+    if (2 * p + 1 < sl.n) copy16(at + NT, src + sl.STEP);
+  }
+  copy_commit();
 }
 
+// ----------------------------------------------------------------- row statistics
 template <typename T, bool ENT>
-__device__ __forceinline__ void accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
+__device__ __forceinline__ float accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
   constexpr int N = Vec<T>::N;
   float x[2 * N], lo[N], hi[N];
   Vec<T>::unpack(a, lo);
   Vec<T>::unpack(b, hi);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = lo[i], x[N + i] = hi[i];
-  accumulate<ENT, 2 * N>(st, x, c2);
+  return accumulate<ENT, 2 * N>(st, x, c2);
 }
-
 template <typename T, bool ENT>
-__device__ __forceinline__ void accumulate_vec(Stat &st, const uint4 &a, float c2) {
-  constexpr int N = Vec<T>::N;
-  float x[N];
+__device__ __forceinline__ float accumulate_vec(Stat &st, const uint4 &a, float c2) {
+  float x[Vec<T>::N];
   Vec<T>::unpack(a, x);
-  accumulate<ENT, N>(st, x, c2);
+  return accumulate<ENT, Vec<T>::N>(st, x, c2);
 }
 
-template <typename T, bool ENT>
-__device__ __forceinline__ void accumulate_ends(Stat &st, const Slice<T> &sl, float c2) {
-  if (threadIdx.x < (unsigned)sl.nhead) accumulate1<ENT>(st, ldf(sl.row + threadIdx.x), c2);
-  if (threadIdx.x < (unsigned)sl.ntail) accumulate1<ENT>(st, ldf(sl.row + sl.tail0 + threadIdx.x), c2);
+// Maxima of a thread's chunks of 2 * `per` vectors, for the alternatives: bf16, rounded up, at [chunk][thread].
+constexpr int CHUNKS = 16;
+struct ChunkMaxima {
+  __nv_bfloat16 *at;
+  int per;
+};
+template <typename T> __device__ __forceinline__ __nv_bfloat16 upper(float x) {
+  return std::is_same<T, __nv_bfloat16>::value ? __float2bfloat16_rn(x) : __float2bfloat16_ru(x);
 }
 
-// One thread's statistics of its elements, streamed through a ring of RING pairs of vectors per thread (32 KB a CTA, so
-// that five CTAs keep 160 KB in flight on an SM whatever they compute).
-constexpr int RING = 4, RING_BYTES = 2 * RING * NT * 16;
-template <typename T, bool ENT>
-__device__ __forceinline__ Stat thread_stats(const Slice<T> &sl, float c2, uint4 *ring) {
+// One thread's statistics of its elements.  Afterwards the ring holds the thread's last RING pairs.
+template <typename T, int GW, bool ENT, bool TOP>
+__device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, uint4 *ring, ChunkMaxima cm) {
+  constexpr int NT = Group<GW>::NT;
   Stat st{LOWEST, 0.f, 0.f};
-  const int n = thread_vectors(sl);
-  const T *src = sl.vec(sl.v0 + (int)threadIdx.x);
-  constexpr int STEP = NT * Vec<T>::N;  // elements between a thread's vectors
-  uint4 *mine = ring + threadIdx.x;
+  uint4 *mine = ring_of<GW>(ring);
 #pragma unroll
-  for (int j = 0; j < RING; ++j) {
-    if (2 * j < n) copy16(mine + (2 * j) * NT, src + (int64_t)(2 * j) * STEP);
-    if (2 * j + 1 < n) copy16(mine + (2 * j + 1) * NT, src + (int64_t)(2 * j + 1) * STEP);
-    copy_commit();
-  }
-  src += (int64_t)2 * RING * STEP;
-  int slot = 0;
+  for (int p = 0; p < RING; ++p) fetch_pair(sl, mine, p);
+  const int n = sl.n;
+  const T *src = sl.mine() + (int64_t)2 * RING * sl.STEP;
+  int slot = 0, in_chunk = 0;
+  float chunk = -INFINITY;
   for (int i = 0; i < n; i += 2) {
     copy_wait<RING - 1>();
     uint4 *at = mine + slot * 2 * NT;
-    if (i + 1 < n) accumulate_pair<T, ENT>(st, at[0], at[NT], c2);
-    else accumulate_vec<T, ENT>(st, at[0], c2);
+    const float mx = i + 1 < n ? accumulate_pair<T, ENT>(st, at[0], at[NT], c2) : accumulate_vec<T, ENT>(st, at[0], c2);
+    if constexpr (TOP) {
+      chunk = fmaxf(chunk, mx);
+      if (++in_chunk == cm.per) {
+        *cm.at = upper<T>(chunk);
+        cm.at += CTA;
+        chunk = -INFINITY;
+        in_chunk = 0;
+      }
+    }
     if (i + 2 * RING < n) copy16(at, src);
-    if (i + 2 * RING + 1 < n) copy16(at + NT, src + STEP);
+    if (i + 2 * RING + 1 < n) copy16(at + NT, src + sl.STEP);
     copy_commit();
-    src += 2 * STEP;
+    src += 2 * sl.STEP;
     slot = (slot + 1) & (RING - 1);
   }
-  accumulate_ends<T, ENT>(st, sl, c2);
-  return st;
-}
-
-// The same with the whole slice kept in shared memory, at most RESIDENT vectors per thread, all of them in flight at once.
-constexpr int RESIDENT = 13, RESIDENT_BYTES = RESIDENT * NT * 16;
-template <typename T> __device__ __forceinline__ void resident_fetch(const Slice<T> &sl, uint4 *keep) {
-  const int n = thread_vectors(sl);
-  const T *src = sl.vec(sl.v0 + (int)threadIdx.x);
-  constexpr int STEP = NT * Vec<T>::N, PAIRS = (RESIDENT + 1) / 2;
-  uint4 *mine = keep + threadIdx.x;
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-    if (2 * j < n) copy16(mine + (2 * j) * NT, src + (int64_t)(2 * j) * STEP);
-    if (2 * j + 1 < n) copy16(mine + (2 * j + 1) * NT, src + (int64_t)(2 * j + 1) * STEP);
-    copy_commit();
+  if constexpr (TOP) {
+    if (in_chunk) *cm.at = upper<T>(chunk);
   }
-}
-
-template <typename T, bool ENT>
-__device__ __forceinline__ Stat resident_stats(const Slice<T> &sl, float c2, const uint4 *keep) {
-  Stat st{LOWEST, 0.f, 0.f};
-  const int n = thread_vectors(sl);
-  const uint4 *mine = keep + threadIdx.x;
-  constexpr int PAIRS = (RESIDENT + 1) / 2;
-  auto step = [&](int j) {
-    if (2 * j + 1 < n) accumulate_pair<T, ENT>(st, mine[2 * j * NT], mine[(2 * j + 1) * NT], c2);
-    else if (2 * j < n) accumulate_vec<T, ENT>(st, mine[2 * j * NT], c2);
-  };
-  static_assert(PAIRS == 7, "one wait per pair below");
-  copy_wait<6>(); step(0);
-  copy_wait<5>(); step(1);
-  copy_wait<4>(); step(2);
-  copy_wait<3>(); step(3);
-  copy_wait<2>(); step(4);
-  copy_wait<1>(); step(5);
-  copy_wait<0>(); step(6);
-  accumulate_ends<T, ENT>(st, sl, c2);
+  const int t = Group<GW>::tid();
+  if (t < sl.nhead) accumulate1<ENT>(st, ldf(sl.row + t), c2);
+  if (t < sl.ntail) accumulate1<ENT>(st, ldf(sl.row + sl.tail0 + t), c2);
   return st;
 }
 
 // Shared state of the CTAs of a row.  Every CTA gets every CTA's statistics (and group maxima) in its own copy.
 struct RowShared {
-  float m[NW];
-  float2 su[NW];
+  float m[CTA / 32];
+  float2 su[CTA / 32];
   Stat cta[MAX_CLUSTER];
 };
 
-// Joins the threads of the CTA and the CTAs of the cluster; every thread of the cluster returns the row's statistics.
-// The CTA's maximum comes first, so that each thread rescales its sums once and the rest are additions, in an order
-// that is the same in every thread.  Orders the shared memory written before it (the group maxima, peers' copies
-// included) for all threads.
-// cluster_begin, called once before: a CTA of the cluster says that it runs and its shared memory may be written.
+// A CTA of a cluster says that it runs and its shared memory may be written; the peers wait for that before they do.
 __device__ __forceinline__ void cluster_begin(int parts) {
   if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
@@ -244,15 +244,25 @@ __device__ __forceinline__ void cluster_ready(int parts) {
   if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <bool ENT>
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
+// Joins the threads of the group and the CTAs of the cluster; every thread returns the row's statistics.  The maximum
+// comes first, so that each thread rescales its sums once and the rest are additions, in an order that is the same in
+// every thread.  Orders the shared memory written before it (the group maxima, peers' copies included) for all threads.
+template <int GW, bool ENT>
 __device__ __forceinline__ Stat row_join(Stat st, RowShared &sh, float c2, int rank, int parts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(st.m));
-  if (lane == 0) sh.m[warp] = m;
-  __syncthreads();
+  float m = warp_max(st.m);
+  if constexpr (GW > 1) {
+    if (lane == 0) sh.m[warp] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NW; ++i) m = fmaxf(m, sh.m[i]);
+    for (int i = 0; i < GW; ++i) m = fmaxf(m, sh.m[i]);
+  }
   const float y = fmaxf((st.m - m) * c2, FLOOR_Y), e = ex2(y);
   float u = ENT ? fmaf(y, st.s, st.u) * e : 0.f, s = st.s * e;
 #pragma unroll
@@ -260,34 +270,25 @@ __device__ __forceinline__ Stat row_join(Stat st, RowShared &sh, float c2, int r
     s += __shfl_xor_sync(0xffffffffu, s, o);
     if (ENT) u += __shfl_xor_sync(0xffffffffu, u, o);
   }
-  if (lane == 0) sh.su[warp] = make_float2(s, u);
-  __syncthreads();
-  Stat all{m, 0.f, 0.f};
+  Stat all{m, s, u};
+  if constexpr (GW > 1) {
+    if (lane == 0) sh.su[warp] = make_float2(s, u);
+    __syncthreads();
+    all.s = all.u = 0.f;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    all.s += sh.su[i].x;
-    all.u += sh.su[i].y;
-  }
-  if (parts > 1) {
-    cg::cluster_group cl = cg::this_cluster();
-    if (threadIdx.x < (unsigned)parts) *cl.map_shared_rank(&sh.cta[rank], threadIdx.x) = all;
-    cl.sync();
-    all = sh.cta[0];
-    for (int i = 1; i < parts; ++i) all = join<ENT>(all, sh.cta[i], c2);
+    for (int i = 0; i < GW; ++i) {
+      all.s += sh.su[i].x;
+      all.u += sh.su[i].y;
+    }
+    if (parts > 1) {
+      cg::cluster_group cl = cg::this_cluster();
+      if (threadIdx.x < (unsigned)parts) *cl.map_shared_rank(&sh.cta[rank], threadIdx.x) = all;
+      cl.sync();
+      all = sh.cta[0];
+      for (int i = 1; i < parts; ++i) all = join<ENT>(all, sh.cta[i], c2);
+    }
   }
   return all;
-}
-
-template <typename F, typename T>
-__device__ __forceinline__ T block_reduce(T v, T *red, F op) {
-  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  __syncthreads();
-  if (l == 0) red[w] = v;
-  __syncthreads();
-  T s = red[0];
-  for (int i = 1; i < NW; ++i) s = op(s, red[i]);  // fixed order: the same in every thread
-  return s;
 }
 
 // ----------------------------------------------------------------- top alternatives
@@ -303,41 +304,40 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t element_key(float v, int i) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~i; }
 
-// The k largest of a row without a second pass over it.  The threads of all CTAs form NT groups (a group is `parts`
-// neighbouring threads of a CTA); the k-th largest of the groups' maxima is a lower bound of the row's k-th largest
-// element, since each of k groups holds an element that is not below it.  Only threads whose own maximum reaches the
-// bound look at their elements again (k = 64 of 50280: about 75 threads) and put those that reach it on the CTA's
-// list.  The lists of the cluster are joined in its first CTA, and an element's place in the result is the number of
-// elements above it.
-struct TopShared {
-  uint32_t group[NT];   // order keys of the groups' maxima, all CTAs'
-  uint64_t *list;       // [LIST] this CTA's candidates, [MAX_CLUSTER * MAX_TOP] the cluster's after them: both lie in
-                        // the ring, which has been read when the first candidate is written
-  uint64_t red[NW];
-  unsigned char lanes[NW][32];
+
+// The k largest of a row without a second pass over it.  A lower bound of the k-th largest element is the k-th largest of
+// the maxima of disjoint sets of elements: the threads of all CTAs in 256 sets (a set is `parts` neighbouring threads of
+// a CTA), or for a warp's row the lanes' chunks.  Only chunks whose maximum reaches the bound are read again (k = 64 of
+// 50280: about 75 of 4000); their elements that reach it go on the group's list.  The lists of a cluster are joined in its
+// first CTA, and an element's place in the result is the number of elements above it.
+template <int GW> struct TopShared {
+  static constexpr int LIST = GW == 1 ? 384 : 1024;  // candidates
+  static constexpr int JOINED = GW == 1 ? 0 : MAX_CLUSTER * MAX_TOP;  // the cluster's candidates
+  static constexpr int WORK = GW == 1 ? 256 : 1024;  // chunks to be read again
+  static_assert(8 * (LIST + JOINED) + 4 * WORK <= 2 * RING * Group<GW>::NT * 16, "they lie in the group's part of the ring");
+  uint32_t set[GW == 1 ? 1 : CTA];  // order keys of the maxima of the sets, all CTAs'
+  uint64_t red[GW];
   uint32_t bound;
-  int n;
+  int n, work;
 };
 
-// Largest b with at least k of the NT keys >= b, or a smaller one that fewer than k + k / 8 + 4 reach.  One warp.
-__device__ __forceinline__ uint32_t group_bound(const uint32_t *group, int k) {
-  const int lane = threadIdx.x & 31;
-  uint32_t key[NW], lo = 0xFFFFFFFFu, hi = 0;
+// Largest b with at least k of the warp's 32 * NK keys >= b, or a smaller one that at most k + k / 8 + 4 reach; the
+// lowest key where all of them are fewer than k.
+template <int NK> __device__ __forceinline__ uint32_t key_quantile(const uint32_t (&key)[NK], int k) {
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    key[i] = group[lane + 32 * i];
+  for (int i = 0; i < NK; ++i) {
     lo = min(lo, key[i]);
     hi = max(hi, key[i]);
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   const int enough = k + k / 8 + 4;
-  // all NT >= k keys reach lo; fewer than k, or nobody knows yet, reach more than hi
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo) / 2 + 1;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) c += key[i] >= mid;
+    for (int i = 0; i < NK; ++i) c += key[i] >= mid;
     c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
     if (c >= k) {
       lo = mid;
@@ -349,53 +349,12 @@ __device__ __forceinline__ uint32_t group_bound(const uint32_t *group, int k) {
   return lo;
 }
 
-// Calls f(value, index) for the elements of those threads of the calling warp whose bit in `todo` is set.  The lanes
-// share all of their vectors, four loads in flight each.  lanes: 32 bytes of shared memory of the warp.
-template <typename T, typename F>
-__device__ __forceinline__ void warp_elements(const Slice<T> &sl, unsigned todo, unsigned char *lanes, F f) {
-  constexpr int N = Vec<T>::N, DEPTH = 4;
-  const int lane = threadIdx.x & 31, warp0 = threadIdx.x & ~31;
-  if (todo >> lane & 1) lanes[__popc(todo & ((1u << lane) - 1))] = (unsigned char)lane;
-  __syncwarp();
-  const int each = (sl.v1 - sl.v0 + NT - 1) / NT, items = __popc(todo) * each;
-  for (int base = 0; base < items; base += 32 * DEPTH) {
-    uint4 raw[DEPTH];
-    int at[DEPTH];
-#pragma unroll
-    for (int j = 0; j < DEPTH; ++j) {
-      const int item = base + 32 * j + lane;
-      at[j] = -1;
-      if (item < items) {
-        const int v = sl.v0 + warp0 + lanes[item / each] + (item % each) * NT;
-        if (v < sl.v1) {
-          at[j] = sl.first(v);
-          raw[j] = load16(sl.vec(v));
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < DEPTH; ++j) {
-      if (at[j] >= 0) {
-        float x[N];
-        Vec<T>::unpack(raw[j], x);
-#pragma unroll
-        for (int i = 0; i < N; ++i) f(x[i], at[j] + i);
-      }
-    }
-  }
-  if (todo >> lane & 1) {
-    const int t = threadIdx.x;
-    if (t < sl.nhead) f(ldf(sl.row + t), t);
-    if (t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
-  }
-}
-
-// The same for a thread's own elements.
-template <typename T, typename F>
-__device__ __forceinline__ void thread_elements(const Slice<T> &sl, F f) {
+// Calls f(value, index) for the calling thread's elements.
+template <typename T, int GW, typename F>
+__device__ __forceinline__ void thread_elements(const Slice<T, GW> &sl, F f) {
   constexpr int N = Vec<T>::N;
-  const int t = threadIdx.x;
-  for (int v = sl.v0 + t; v < sl.v1; v += NT) {
+  const int t = Group<GW>::tid();
+  for (int v = sl.v0 + t; v < sl.v1; v += Group<GW>::NT) {
     float x[N];
     Vec<T>::unpack(load16(sl.vec(v)), x);
 #pragma unroll
@@ -405,19 +364,23 @@ __device__ __forceinline__ void thread_elements(const Slice<T> &sl, F f) {
   if (t < sl.ntail) f(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
 }
 
-__device__ __forceinline__ uint64_t count_op(uint64_t a, uint64_t b) { return a + b; }
-
-// Largest key that at least k of the counted elements reach, or a smaller one that at most `most` >= k reach.
+// Largest key that at least k of the group's counted elements reach, or a smaller one that at most `most` >= k reach.
 // count(key): how many elements of the calling thread are >= key; lo: a key that at least k reach; no key is above hi.
-template <typename F>
+template <int GW, typename F>
 __device__ uint64_t key_bound(uint64_t lo, uint64_t hi, int k, int most, uint64_t *red, F count) {
-  auto add = [](uint64_t a, uint64_t b) { return count_op(a, b); };
   while (lo < hi) {
     const uint64_t mid = lo + (hi - lo) / 2 + 1;
-    const uint64_t c = block_reduce((uint64_t)count(mid), red, add);
-    if (c >= (uint64_t)k) {
+    int c = (int)__reduce_add_sync(0xffffffffu, (unsigned)count(mid));
+    if constexpr (GW > 1) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = (uint64_t)c;
+      __syncthreads();
+      c = 0;
+      for (int i = 0; i < GW; ++i) c += (int)red[i];
+    }
+    if (c >= k) {
       lo = mid;
-      if (c <= (uint64_t)most) break;
+      if (c <= most) break;
     } else {
       hi = mid - 1;
     }
@@ -426,99 +389,156 @@ __device__ uint64_t key_bound(uint64_t lo, uint64_t hi, int k, int most, uint64_
 }
 
 // Cuts list[0, n) down to at most `most` >= k keys, the k largest among them; n <= LIST.
-__device__ int cut_list(uint64_t *list, int n, int k, int most, TopShared &sh) {
+template <int GW> __device__ int cut_list(uint64_t *list, int n, int k, int most, TopShared<GW> &sh) {
+  using G = Group<GW>;
+  constexpr int EACH = (TopShared<GW>::LIST + G::NT - 1) / G::NT;
   if (n <= most) return n;
-  const uint64_t b = key_bound(0, ~0ull, k, most, sh.red, [&](uint64_t key) {
+  const uint64_t b = key_bound<GW>(0, ~0ull, k, most, sh.red, [&](uint64_t key) {
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += NT) c += list[i] >= key;
+    for (int i = G::tid(); i < n; i += G::NT) c += list[i] >= key;
     return c;
   });
-  uint64_t mine[LIST / NT];
+  uint64_t mine[EACH];
 #pragma unroll
-  for (int i = 0; i < LIST / NT; ++i) {
-    const int at = threadIdx.x + i * NT;
+  for (int i = 0; i < EACH; ++i) {
+    const int at = G::tid() + i * G::NT;
     mine[i] = at < n ? list[at] : 0;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
+  G::sync();
+  if (G::tid() == 0) sh.n = 0;
+  G::sync();
 #pragma unroll
-  for (int i = 0; i < LIST / NT; ++i)
-    if (mine[i] >= b && threadIdx.x + i * NT < n) list[atomicAdd(&sh.n, 1)] = mine[i];
-  __syncthreads();
+  for (int i = 0; i < EACH; ++i)
+    if (mine[i] >= b && G::tid() + i * G::NT < n) list[atomicAdd(&sh.n, 1)] = mine[i];
+  G::sync();
   return sh.n;
 }
 
-// st: the calling thread's own statistics, total: the row's; group maxima are in place (row_join has ordered them).
-template <typename T>
-__device__ void top_alternatives(const Slice<T> &sl, Stat st, RowStats row, int k, float inv_t, int V, TopShared &sh,
-                                 int rank, int parts, int64_t *ids, float *logprobs) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    const uint32_t b = group_bound(sh.group, k);
-    if (lane == 0) {
-      sh.bound = b;
-      sh.n = 0;
+// st: the calling thread's own statistics, row: the row's; the maxima of the sets are in place (row_join has ordered
+// them), and the ring has been read.
+template <typename T, int GW>
+__device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st, RowStats row, int k, float inv_t, int V,
+                                                 TopShared<GW> &sh, uint4 *ring, ChunkMaxima cm, int rank, int parts,
+                                                 int64_t *ids, float *logprobs) {
+  using G = Group<GW>;
+  using S = TopShared<GW>;
+  constexpr int NT = G::NT, N = Vec<T>::N;
+  const int t = G::tid(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t *list = reinterpret_cast<uint64_t *>(ring + G::index() * 2 * RING * NT);
+  int *work = reinterpret_cast<int *>(list + S::LIST + S::JOINED);
+  const int chunks = (((sl.n + 1) >> 1) + cm.per - 1) / cm.per;  // the calling thread's
+  uint32_t bound;
+  if constexpr (GW == 1) {
+    // a maximum that was rounded up is at least the next lower bf16
+    constexpr uint32_t down = std::is_same<T, __nv_bfloat16>::value ? 0u : 0x10000u;
+    uint32_t key[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) key[c] = c < chunks ? order_key(__bfloat162float(cm.at[c * CTA])) - down : 0u;
+    bound = key_quantile<CHUNKS>(key, k);
+    if (lane == 0) sh.n = sh.work = 0;
+  } else {
+    if (warp == 0) {
+      uint32_t key[CTA / 32];
+#pragma unroll
+      for (int i = 0; i < CTA / 32; ++i) key[i] = sh.set[lane + 32 * i];
+      const uint32_t b = key_quantile<CTA / 32>(key, k);
+      if (lane == 0) {
+        sh.bound = b;
+        sh.n = sh.work = 0;
+      }
     }
+    __syncthreads();
+    bound = sh.bound;
   }
-  __syncthreads();
-  const uint32_t bound = sh.bound;
-  // a thread whose sum is NaN may hold a NaN, which its maximum passes over
-  const unsigned todo =
-      __ballot_sync(0xffffffffu, order_key(st.s == 0.f ? -INFINITY : st.m) >= bound || st.s != st.s);
-  const float least = key_value(bound);  // bound 0 (a group without an element) gives NaN, which everything passes
-  warp_elements(sl, todo, sh.lanes[warp], [&](float x, int i) {
+  const float least = key_value(bound);  // below every order (a set without an element) it is NaN, which all pass
+  auto take = [&](float x, int i) {
     if (!(x < least)) {
       const int at = atomicAdd(&sh.n, 1);
-      if (at < LIST) sh.list[at] = element_key(x, i);
+      if (at < S::LIST) list[at] = element_key(x, i);
     }
-  });
-  __syncthreads();
+  };
+  G::sync();
+  // a thread whose sum is NaN may hold a NaN, which maxima pass over
+  const bool nan = st.s != st.s;
+  if (nan || !(st.m < least) || st.s == 0.f) {
+    for (int c = 0; c < chunks; ++c) {
+      if (nan || !(__bfloat162float(cm.at[c * CTA]) < least)) {
+        const int at = atomicAdd(&sh.work, 1);
+        if (at < S::WORK) work[at] = t * CHUNKS + c;
+      }
+    }
+    if (t < sl.nhead) take(ldf(sl.row + t), t);
+    if (t < sl.ntail) take(ldf(sl.row + sl.tail0 + t), sl.tail0 + t);
+  }
+  G::sync();
+  const int items = sh.work;
+  if (items <= S::WORK) {
+    for (int e = t; e < items; e += NT) {
+      const int of = work[e] / CHUNKS, first = sl.v0 + of + 2 * cm.per * (work[e] % CHUNKS) * NT;
+      for (int j = 0; j < cm.per; ++j) {
+        const int v = first + 2 * j * NT;
+        if (v >= sl.v1) break;
+        const bool two = v + NT < sl.v1;
+        const uint4 a = load16(sl.vec(v)), b = two ? load16(sl.vec(v + NT)) : make_uint4(0, 0, 0, 0);
+        float x[N];
+        Vec<T>::unpack(a, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) take(x[i], sl.first(v) + i);
+        if (two) {
+          Vec<T>::unpack(b, x);
+#pragma unroll
+          for (int i = 0; i < N; ++i) take(x[i], sl.first(v + NT) + i);
+        }
+      }
+    }
+  }
+  G::sync();
   int n = sh.n;
-  if (n > LIST) {
+  if (n > S::LIST || items > S::WORK) {
     // more elements reach the bound than the list holds (a row of equal logits): find the key of this CTA's k-th
     // largest element by bisection, one scan of the slice a step, and collect again
     const uint64_t lo = ((uint64_t)bound << 32) | (uint32_t)~(V - 1);
     const uint64_t hi = row.log_s != row.log_s ? ~0ull : ((uint64_t)order_key(row.m) << 32) | 0xFFFFFFFFu;
-    const uint64_t b = key_bound(lo, hi, k, MAX_TOP, sh.red, [&](uint64_t key) {
+    const uint64_t b = key_bound<GW>(lo, hi, k, MAX_TOP, sh.red, [&](uint64_t key) {
       int c = 0;
       thread_elements(sl, [&](float x, int i) { c += element_key(x, i) >= key; });
       return c;
     });
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
+    G::sync();
+    if (t == 0) sh.n = 0;
+    G::sync();
     thread_elements(sl, [&](float x, int i) {
       const uint64_t key = element_key(x, i);
-      if (key >= b) sh.list[atomicAdd(&sh.n, 1)] = key;
+      if (key >= b) list[atomicAdd(&sh.n, 1)] = key;
     });
-    __syncthreads();
+    G::sync();
     n = sh.n;
   }
-  const uint64_t *list = sh.list;
-  if (parts > 1) {
-    n = cut_list(sh.list, n, k, MAX_TOP, sh);
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n = n;
-    cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-    if (rank == 0) {
-      int at = 0;
-      for (int c = 0; c < parts; ++c) {
-        const int nc = *cl.map_shared_rank(&sh.n, c);
-        const uint64_t *from = cl.map_shared_rank(sh.list, c);
-        if (threadIdx.x < (unsigned)nc) sh.list[LIST + at + threadIdx.x] = from[threadIdx.x];
-        at += nc;
+  if constexpr (GW > 1) {
+    if (parts > 1) {
+      n = cut_list<GW>(list, n, k, MAX_TOP, sh);
+      __syncthreads();
+      if (t == 0) sh.n = n;
+      cg::cluster_group cl = cg::this_cluster();
+      cl.sync();
+      if (rank == 0) {
+        int at = 0;
+        for (int c = 0; c < parts; ++c) {
+          const int nc = *cl.map_shared_rank(&sh.n, c);
+          const uint64_t *from = cl.map_shared_rank(list, c);
+          if (t < nc) list[S::LIST + at + t] = from[t];
+          at += nc;
+        }
+        n = at;
       }
-      n = at;
+      cl.sync();  // the peers' lists have been read
+      if (rank != 0) return;
+      list += S::LIST;
     }
-    cl.sync();  // the peers' lists have been read
-    if (rank != 0) return;
-    list = sh.list + LIST;
+    n = cut_list<GW>(list, n, k, 2 * MAX_TOP, sh);
   }
-  n = cut_list(const_cast<uint64_t *>(list), n, k, NT, sh);
-  if (threadIdx.x < (unsigned)n) {
-    const uint64_t key = list[threadIdx.x];
+  for (int e = t; e < n; e += NT) {
+    const uint64_t key = list[e];
     int place = 0;
     for (int i = 0; i < n; ++i) place += list[i] > key;
     if (place < k) {
@@ -537,40 +557,40 @@ struct FwdArgs {
   float *top_logprobs;
   float inv_t, c2;  // 1 / T, log2 e / T
   int V, shift;
+  uint32_t rows;
 };
 
-template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
+template <typename T, int GW, bool ENT, bool TOP>
+__global__ void __launch_bounds__(CTA, 5) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
+  using G = Group<GW>;
+  extern __shared__ uint4 ring[];
   __shared__ RowShared sh;
-  __shared__ TopShared top;
-  __shared__ uint4 ring[2 * RING * NT];
-  static_assert(sizeof(ring) >= 8 * (LIST + MAX_CLUSTER * MAX_TOP), "the ring holds the lists");
-  const Part part(a.shift);
-  const int parts = 1 << a.shift, rank = part.rank;
+  __shared__ TopShared<GW> top[G::ROWS];
+  __shared__ __nv_bfloat16 maxima[TOP ? CHUNKS * CTA : 1];
+  const Part<GW> part(a.shift);
+  if (GW == 1 && part.row >= a.rows) return;
+  const int parts = 1 << part.shift, rank = part.rank;
   const int64_t r = part.row;
   const T *row = logits + rows.at(part.row);
-  const Slice<T> sl(row, a.V, rank, a.shift);
+  const Slice<T, GW> sl(row, a.V, rank, part.shift);
+  const ChunkMaxima cm{maxima + (TOP ? threadIdx.x : 0), TOP ? max(1, (sl.pairs() + CHUNKS - 1) / CHUNKS) : 1};
   cluster_begin(parts);
-  const Stat st = thread_stats<T, ENT>(sl, a.c2, ring);
+  const Stat st = thread_stats<T, GW, ENT, TOP>(sl, a.c2, ring, cm);
   cluster_ready(parts);
-  if constexpr (TOP) {
-    if (threadIdx.x == 0) top.list = reinterpret_cast<uint64_t *>(ring);
-    // maxima of groups of `parts` threads to every CTA of the cluster
-    uint32_t g = sl.v0 + (int)threadIdx.x < sl.v1 || threadIdx.x < (unsigned)sl.nhead || threadIdx.x < (unsigned)sl.ntail
-                     ? order_key(st.s == 0.f ? -INFINITY : st.m)
-                     : 0u;
+  if constexpr (TOP && GW > 1) {
+    // maxima of the sets of `parts` threads to every CTA of the cluster
+    uint32_t g = sl.n > 0 || G::tid() < sl.nhead || G::tid() < sl.ntail ? order_key(st.s == 0.f ? -INFINITY : st.m) : 0u;
     for (int o = 1; o < parts; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    const int slot = rank * (NT >> a.shift) + ((int)threadIdx.x >> a.shift);
-    const int to = threadIdx.x & (parts - 1);
-    if (parts > 1) *cg::this_cluster().map_shared_rank(&top.group[slot], to) = g;
-    else top.group[slot] = g;
+    const int slot = rank * (CTA >> part.shift) + ((int)threadIdx.x >> part.shift);
+    if (parts > 1) *cg::this_cluster().map_shared_rank(&top[0].set[slot], threadIdx.x & (parts - 1)) = g;
+    else top[0].set[slot] = g;
   }
-  const Stat all = row_join<ENT>(st, sh, a.c2, rank, parts);
-  if (!TOP && threadIdx.x >= 32) return;
+  const Stat all = row_join<GW, ENT>(st, sh, a.c2, rank, parts);
+  if (!TOP && threadIdx.x >= 32 && GW > 1) return;
   const RowStats s = finish(all);
-  if (rank == 0 && threadIdx.x == 0) {
+  if (rank == 0 && G::tid() == 0) {
     if (a.logprob) {
       const int64_t t = a.targets[r];
       a.logprob[r] = t < 0 ? 0.f : t >= a.V ? NAN : log_prob(ldf(row + t), s.m, s.log_s, a.inv_t);
@@ -582,8 +602,8 @@ __global__ void __launch_bounds__(NT, 5) token_logprobs_kernel(const T *__restri
     }
   }
   if constexpr (TOP)
-    top_alternatives(sl, st, s, a.top_k, a.inv_t, a.V, top, rank, parts, a.top_ids + r * a.top_k,
-                     a.top_logprobs + r * a.top_k);
+    top_alternatives<T, GW>(sl, st, s, a.top_k, a.inv_t, a.V, top[G::index()], ring, cm, rank, parts,
+                            a.top_ids + r * a.top_k, a.top_logprobs + r * a.top_k);
 }
 
 // ----------------------------------------------------------------- gradients
@@ -618,13 +638,14 @@ template <bool ENT> struct Dense {
   }
 };
 
-// Writes the slice's gradient.  16-byte stores where the gradient row is aligned as the logits row is.  KEPT: the vectors
-// are where resident_stats left them in shared memory.
-template <typename T, bool KEPT, bool ENT>
-__device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Dense<ENT> &d, bool zero, int64_t hit,
-                                           float extra, const uint4 *kept) {
-  constexpr int N = Vec<T>::N, DEPTH = 4;
+// Writes the slice's gradient, last pair first.  KEPT: thread_stats has just read the slice, so the ring holds the
+// thread's last RING pairs.  16-byte stores where the gradient row is aligned as the logits row is.
+template <typename T, int GW, bool KEPT, bool ENT>
+__device__ __forceinline__ void write_grad(const Slice<T, GW> &sl, T *out, const Dense<ENT> &d, bool zero, int64_t hit,
+                                           float extra, uint4 *ring) {
+  constexpr int N = Vec<T>::N, NT = Group<GW>::NT;
   const bool same = ((reinterpret_cast<uintptr_t>(sl.row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int t = Group<GW>::tid();
   auto one = [&](int i) {
     float v = 0.f;
     if (!zero) {
@@ -634,44 +655,48 @@ __device__ __forceinline__ void write_grad(const Slice<T> &sl, T *out, const Den
     stf(out + i, v);
   };
   if (!same) {
-    for (int64_t i = sl.first(sl.v0) + (int)threadIdx.x; i < sl.first(sl.v1); i += NT) one((int)i);
+    for (int64_t i = sl.first(sl.v0) + t; i < sl.first(sl.v1); i += NT) one((int)i);
   } else if (zero) {
-    for (int v = sl.v0 + threadIdx.x; v < sl.v1; v += NT)
+    for (int v = sl.v0 + t; v < sl.v1; v += NT)
       __stcs(reinterpret_cast<uint4 *>(out + sl.first(v)), make_uint4(0, 0, 0, 0));
   } else {
-    const int n = thread_vectors(sl), v0 = sl.v0 + (int)threadIdx.x;
-    const int hv = hit >= sl.first(sl.v0) && hit < sl.first(sl.v1) ? (int)((hit - sl.head) / N) : -1;
-    const T *src = sl.vec(v0);
-    T *dst = out + sl.first(v0);
-    const uint4 *keep = kept + threadIdx.x;
-    constexpr int STEP = NT * N;
-    for (int i = 0; i < n; i += DEPTH) {
-      uint4 raw[DEPTH];
+    // the vector of the element `hit`, counted in the calling thread's vectors, or -1
+    int hv = -1;
+    if (hit >= sl.first(sl.v0) && hit < sl.first(sl.v1)) {
+      const int v = (int)(hit - sl.head) / N - sl.v0;
+      if (v % NT == t) hv = v / NT;
+    }
+    uint4 *mine = ring_of<GW>(ring);
+    const int last = ((sl.n + 1) >> 1) - 1;  // pair
+    if (!KEPT) {
 #pragma unroll
-      for (int j = 0; j < DEPTH; ++j)
-        if (i + j < n) raw[j] = KEPT ? keep[(i + j) * NT] : load16(src + j * STEP);
+      for (int p = 0; p < RING; ++p) fetch_pair(sl, mine, last - p);
+    }
+    T *dst = out + sl.first(sl.v0 + t) + (int64_t)(2 * last) * sl.STEP;
+    auto store = [&](const uint4 &raw, T *to, int i) {
+      float x[N];
+      Vec<T>::unpack(raw, x);
 #pragma unroll
-      for (int j = 0; j < DEPTH; ++j) {
-        if (i + j < n) {
-          float x[N];
-          Vec<T>::unpack(raw[j], x);
+      for (int k = 0; k < N; k += 2) un2(d.two(f2(x[k], x[k + 1])), x[k], x[k + 1]);
+      if (i == hv) {
+        const int at = (int)(hit - sl.head) % N;
 #pragma unroll
-          for (int k = 0; k < N; k += 2) un2(d.two(f2(x[k], x[k + 1])), x[k], x[k + 1]);
-          if (v0 + (i + j) * NT == hv) {
-            const int at = (int)(hit - sl.first(hv));
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-              if (k == at) x[k] += extra;
-          }
-          __stcs(reinterpret_cast<uint4 *>(dst + j * STEP), Vec<T>::pack(x));
-        }
+        for (int k = 0; k < N; ++k)
+          if (k == at) x[k] += extra;
       }
-      src += DEPTH * STEP;
-      dst += DEPTH * STEP;
+      __stcs(reinterpret_cast<uint4 *>(to), Vec<T>::pack(x));
+    };
+    for (int p = last; p >= 0; --p) {
+      copy_wait<RING - 1>();
+      const uint4 *at = mine + (p % RING) * 2 * NT;
+      store(at[0], dst, 2 * p);
+      if (2 * p + 1 < sl.n) store(at[NT], dst + sl.STEP, 2 * p + 1);
+      fetch_pair(sl, mine, p - RING);
+      dst -= 2 * sl.STEP;
     }
   }
-  if (threadIdx.x < (unsigned)sl.nhead) one(threadIdx.x);
-  if (threadIdx.x < (unsigned)sl.ntail) one(sl.tail0 + threadIdx.x);
+  if (t < sl.nhead) one(t);
+  if (t < sl.ntail) one(sl.tail0 + t);
 }
 
 struct BwdArgs {
@@ -679,17 +704,20 @@ struct BwdArgs {
   const float *stats, *entropy, *d_logprob, *d_entropy;
   float inv_t, c2;
   int V, shift;
+  uint32_t rows;
 };
 
 // dx_j = (g (1{j = t} - p_j) - h p_j (log p_j + H)) / T
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
-                                                                   T *__restrict__ grad, Rows grows) {
+template <typename T, int GW, bool ENT>
+__global__ void __launch_bounds__(CTA, 5) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
+                                                                    T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  const Part part(a.shift);
+  extern __shared__ uint4 ring[];
+  const Part<GW> part(a.shift);
+  if (GW == 1 && part.row >= a.rows) return;
   const int64_t r = part.row;
-  const Slice<T> sl(logits + rows.at(part.row), a.V, part.rank, a.shift);
+  const Slice<T, GW> sl(logits + rows.at(part.row), a.V, part.rank, part.shift);
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1];
   const float h = ENT ? a.d_entropy[r] : 0.f;
   int64_t t = -1;
@@ -701,7 +729,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_bwd_kernel(const T *__re
   const float ent = ENT ? a.entropy[r] : 0.f;
   const bool zero = (g == 0.f && h == 0.f) || m == -INFINITY;
   const Dense<ENT> d(m, log_s, a.c2, -(g + h * ent) * a.inv_t, -h * LN2 * a.inv_t);
-  write_grad<T, false, ENT>(sl, grad + grows.at(part.row), d, zero, t, g * a.inv_t, nullptr);
+  write_grad<T, GW, false, ENT>(sl, grad + grows.at(part.row), d, zero, t, g * a.inv_t, ring);
 }
 
 // ----------------------------------------------------------------- distillation
@@ -714,6 +742,7 @@ struct DistillArgs {
   const float *stats_in;
   float inv_t, c2;
   int V, shift;
+  uint32_t rows;
 };
 
 __device__ __forceinline__ float load_value(const void *p, int64_t i, int dtype) {
@@ -728,18 +757,19 @@ __device__ __forceinline__ float nan_max(float a, float b) {
   return r;
 }
 
-// A row's teacher: token, probability, its log, and the student's logit of entry i; entries that are not used have q = 0.
+// A row's teacher: token (-1: not used), probability, and the student's logit of entry i.
 struct TeacherShared {
-  int64_t id[MAX_TOP];
-  float q[MAX_TOP], log_q[MAX_TOP], x[MAX_TOP];
-  bool used, bad;  // any entry is used; a used one lies outside the vocabulary, or the probabilities are NaN
+  alignas(16) int id[MAX_TOP];
+  float q[MAX_TOP], x[MAX_TOP];
+  float neg_entropy;  // sum q log q
+  bool used, bad;     // any entry is used; a used one lies outside the vocabulary, or the probabilities are NaN
 };
 
 // By one warp, four entries a lane.
 template <typename T>
 __device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a, int64_t r, TeacherShared &te) {
   constexpr int PER = MAX_TOP / 32;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 31;
   int64_t id[PER];
   float t[PER], x[PER], m = -INFINITY;
 #pragma unroll
@@ -770,62 +800,66 @@ __device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a,
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   const float ls = logf(s);
   bool bad = false;
+  float neg = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = lane + 32 * j;
     const float q = s != 0.f ? e[j] / s : 0.f;
     bad = bad || q != q || (q != 0.f && id[j] >= a.V);
-    if (i < a.k) {
-      te.id[i] = id[j];
-      te.q[i] = q;
-      te.log_q[i] = (t[j] - m) * a.inv_t - ls;
-      te.x[i] = x[j];
-    }
+    if (q != 0.f) neg += q * ((t[j] - m) * a.inv_t - ls);
+    te.id[i] = q != 0.f && id[j] < a.V ? (int)id[j] : -1;
+    te.q[i] = q;
+    te.x[i] = x[j];
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) neg += __shfl_xor_sync(0xffffffffu, neg, o);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
+    te.neg_entropy = neg;
     te.used = s != 0.f;
     te.bad = bad;
   }
 }
 
 // loss = sum q_i (log q_i - log p_id_i), dx_j = w (p_j - sum_{id_i = j} q_i) / T; q: softmax over the used entries of
-// the teacher's logits / T, thread i holding entry i.  GRAD: the gradient is written too.  RES: the slice stays in shared
-// memory between the statistics and the gradient, so that the logits are read from memory once.
-template <typename T, bool GRAD, bool RES>
-__global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
-                                                        T *__restrict__ grad, Rows grows) {
+// the teacher's logits / T.  GRAD: the gradient is written too.
+template <typename T, int GW, bool GRAD>
+__global__ void __launch_bounds__(CTA, 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
+                                                         T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
-  extern __shared__ uint4 buffer[];  // the ring, or with RES the slice
+  using G = Group<GW>;
+  extern __shared__ uint4 ring[];
   __shared__ RowShared sh;
-  __shared__ TeacherShared te;
-  const Part part(a.shift);
-  const int parts = 1 << a.shift, rank = part.rank;
+  __shared__ TeacherShared teachers[G::ROWS];
+  const Part<GW> part(a.shift);
+  if (GW == 1 && part.row >= a.rows) return;
+  TeacherShared &te = teachers[G::index()];
+  const int parts = 1 << part.shift, rank = part.rank, t = G::tid();
   const int64_t r = part.row;
   const T *row = logits + rows.at(part.row);
-  const Slice<T> sl(row, a.V, rank, a.shift);
+  const Slice<T, GW> sl(row, a.V, rank, part.shift);
   const float w = GRAD ? a.row_weight[r] * a.inv_t : 0.f;
-  if (!a.stats_in) cluster_begin(parts);
-  if (RES) resident_fetch(sl, buffer);
-  if (threadIdx.x < 32) read_teacher(row, a, r, te);  // while the slice is on its way
   RowStats st;
   if (a.stats_in) {
+    if (t < 32) read_teacher(row, a, r, te);
     st = RowStats{a.stats_in[2 * r], a.stats_in[2 * r + 1], 0.f};
-    __syncthreads();
   } else {
-    const Stat own = RES ? resident_stats<T, false>(sl, a.c2, buffer) : thread_stats<T, false>(sl, a.c2, buffer);
+    cluster_begin(parts);
+    if (t < 32) read_teacher(row, a, r, te);
+    const Stat own = thread_stats<T, GW, false, false>(sl, a.c2, ring, ChunkMaxima{});
     cluster_ready(parts);
-    st = finish(row_join<false>(own, sh, a.c2, rank, parts));
+    st = finish(row_join<GW, false>(own, sh, a.c2, rank, parts));
   }
-  if (rank == 0 && threadIdx.x < 32) {
+  G::sync();
+  if (rank == 0 && t < 32) {
     float loss = 0.f;
-    for (int i = threadIdx.x; i < a.k; i += 32)
-      if (te.q[i] != 0.f) loss += te.q[i] * (te.log_q[i] - log_prob(te.x[i], st.m, st.log_s, a.inv_t));
+    for (int i = t; i < a.k; i += 32)
+      if (te.q[i] != 0.f) loss -= te.q[i] * log_prob(te.x[i], st.m, st.log_s, a.inv_t);
 #pragma unroll
     for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-    if (threadIdx.x == 0) {
-      if (a.loss) a.loss[r] = te.bad ? NAN : loss;
+    if (t == 0) {
+      if (a.loss) a.loss[r] = te.bad ? NAN : loss + te.neg_entropy;
       if (a.stats) {
         a.stats[2 * r] = st.m;
         a.stats[2 * r + 1] = st.log_s;
@@ -836,54 +870,76 @@ __global__ void __launch_bounds__(NT, GRAD ? 4 : 5) distill_kernel(const T *__re
     const bool zero = !te.used || w == 0.f || st.m == -INFINITY;
     T *out = grad + grows.at(part.row);
     const Dense<false> d(st.m, st.log_s, a.c2, te.bad ? NAN : w, 0.f);
-    write_grad<T, RES, false>(sl, out, d, zero, -1, 0.f, buffer);
-    __syncthreads();  // the teacher's elements are written again, after the pass over all of them
-    if (threadIdx.x >= (unsigned)a.k || zero || te.bad) return;
-    const int64_t id = te.id[threadIdx.x];
-    const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
-    if (te.q[threadIdx.x] != 0.f && mine) {
-      float qs = 0.f;
+    if (a.stats_in) write_grad<T, GW, false, false>(sl, out, d, zero, -1, 0.f, ring);
+    else write_grad<T, GW, true, false>(sl, out, d, zero, -1, 0.f, ring);
+    G::sync();  // the teacher's elements are written again, after the pass over all of them
+    if (zero || te.bad) return;
+    for (int i = t; i < a.k; i += G::NT) {
+      const int id = te.id[i];
+      const bool mine = id >= (rank == 0 ? 0 : sl.first(sl.v0)) && id < (rank == parts - 1 ? a.V : sl.first(sl.v1));
+      if (!mine) continue;
+      int same = 0;
+      for (int j = 0; j < a.k; j += 4) {
+        const int4 o = *reinterpret_cast<const int4 *>(te.id + j);
+        same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+      }
+      float qs = te.q[i];
       bool first = true;
-      for (int j = 0; j < a.k; ++j) {
-        if (te.id[j] == id) {
+      if (same > 1) {  // a token given more than once: the first entry of it writes the sum
+        qs = 0.f;
+        for (int j = 0; j < a.k; ++j) {
+          if (te.id[j] != id) continue;
+          first = first && j >= i;
           qs += te.q[j];
-          first = first && (j >= (int)threadIdx.x || te.q[j] == 0.f);
         }
       }
-      const float lp = log_prob(te.x[threadIdx.x], st.m, st.log_s, a.inv_t);
+      const float lp = log_prob(te.x[i], st.m, st.log_s, a.inv_t);
       if (first) stf(out + id, w * (ex2(lp * LOG2E) - qs));
     }
   }
 }
 
-// log2 of the CTAs that share a row: rows alone fill the GPU from about four CTAs per SM on; a CTA takes no fewer than NT
-// vectors.
-inline int row_shift(int64_t rows, int V, int elem) {
-  const int64_t want = 4ll * num_sms();
-  const int64_t vecs = (int64_t)V * elem / 16;
+// How rows are shared out.  A warp takes a row of up to WARP_ROW bytes where there are rows enough for every warp;
+// else 2^shift CTAs share one: rows alone fill the GPU from about four CTAs per SM on, and a CTA takes no fewer vectors
+// than it has threads.
+constexpr int64_t WARP_ROW = 16384;
+struct Share {
+  bool warp;
+  int shift;
+  unsigned grid;
+};
+inline Share share_rows(int64_t rows, int V, int elem, int top_k) {
+  const int64_t sms = num_sms(), bytes = (int64_t)V * elem;
+  // alternatives: the lanes' chunks must be clearly more than k
+  if (bytes <= WARP_ROW && rows >= 16 * sms && (top_k == 0 || bytes / 32 >= 2 * top_k))
+    return {true, 0, (unsigned)((rows + Group<1>::ROWS - 1) / Group<1>::ROWS)};
   int shift = 0;
-  while (2 << shift <= MAX_CLUSTER && rows << shift < want && vecs >> (shift + 1) >= NT) ++shift;
-  return shift;
+  while (2 << shift <= MAX_CLUSTER && rows << shift < 4 * sms && bytes / 16 >> (shift + 1) >= CTA) ++shift;
+  return {false, shift, (unsigned)(rows << shift)};
 }
 
 // Launch with the CTAs of a row as a cluster.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_rows(void (*kern)(KArgs...), int64_t rows, int shift, size_t smem, cudaStream_t stream,
-                               Args... args) {
+inline cudaError_t launch_rows(void (*kern)(KArgs...), const Share &sh, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows << shift));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(sh.grid);
+  cfg.blockDim = dim3(CTA);
+  cfg.dynamicSmemBytes = RING_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1u << shift;
+  attr[1].val.clusterDim.x = 1u << sh.shift;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = shift > 0 ? 2 : 1;
+  cfg.numAttrs = sh.shift > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+template <typename T, int GW> auto fwd_kernel(bool ent, bool top) {
+  return top ? (ent ? token_logprobs_kernel<T, GW, true, true> : token_logprobs_kernel<T, GW, false, true>)
+             : (ent ? token_logprobs_kernel<T, GW, true, false> : token_logprobs_kernel<T, GW, false, false>);
 }
 
 #define MTP_DISPATCH_LOGITS(code, T, ...)                                    \
@@ -919,13 +975,12 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, top_k);
   const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
-                  (float)(1.4426950408889634 / temperature), V, shift};
+                  (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
-    auto kern = top_k ? (entropy ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, false, true>)
-                      : (entropy ? token_logprobs_kernel<T, true, false> : token_logprobs_kernel<T, false, false>);
-    launch_rows(kern, n, shift, 0, s, (const T *)logits, rows, a);
+    auto kern = sh.warp ? fwd_kernel<T, 1>(entropy, top_k > 0) : fwd_kernel<T, 8>(entropy, top_k > 0);
+    launch_rows(kern, sh, s, (const T *)logits, rows, a);
   });
   return check_launch("token_logprobs");
 }
@@ -941,12 +996,13 @@ int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
-  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
   const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature,
-                  (float)(1.4426950408889634 / temperature), V, shift};
+                  (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
-    auto kern = d_entropy ? token_logprobs_bwd_kernel<T, true> : token_logprobs_bwd_kernel<T, false>;
-    launch_pdl(kern, dim3((unsigned)(n << shift)), dim3(NT), 0, s, (const T *)logits, rows, a, (T *)grad, grows);
+    auto kern = sh.warp ? (d_entropy ? token_logprobs_bwd_kernel<T, 1, true> : token_logprobs_bwd_kernel<T, 1, false>)
+                        : (d_entropy ? token_logprobs_bwd_kernel<T, 8, true> : token_logprobs_bwd_kernel<T, 8, false>);
+    launch_rows(kern, sh, s, (const T *)logits, rows, a, (T *)grad, grows);
   });
   return check_launch("token_logprobs_bwd");
 }
@@ -961,11 +1017,13 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const int shift = row_shift(n, V, dtype == MTP_F32 ? 4 : 2);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
   const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature,
-                      (float)(1.4426950408889634 / temperature), V, shift};
-  MTP_DISPATCH_LOGITS(dtype, T, launch_rows(distill_kernel<T, false, false>, n, shift, RING_BYTES, s,
-                                            (const T *)logits, rows, a, (T *)nullptr, rows));
+                      (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
+  MTP_DISPATCH_LOGITS(dtype, T, {
+    auto kern = sh.warp ? distill_kernel<T, 1, false> : distill_kernel<T, 8, false>;
+    launch_rows(kern, sh, s, (const T *)logits, rows, a, (T *)nullptr, rows);
+  });
   return check_launch("distill_topk");
 }
 
@@ -980,29 +1038,12 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
-  const int elem = dtype == MTP_F32 ? 4 : 2;
-  int shift = row_shift(n, V, elem);
-  // keep the slices resident: more CTAs per row until a slice fits
-  auto fits = [&](int c) { return (((int64_t)V * elem / 16 - 1) >> c) + 1 <= RESIDENT * NT; };
-  bool res = stats == nullptr;
-  if (res) {
-    int c = shift;
-    while (2 << c <= MAX_CLUSTER && !fits(c)) ++c;
-    res = fits(c);
-    if (res) shift = c;
-  }
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
   const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature,
-                      (float)(1.4426950408889634 / temperature), V, shift};
+                      (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
-    if (res) {
-      // set at every call: the attribute belongs to the current device
-      if (cudaFuncSetAttribute(distill_kernel<T, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               RESIDENT_BYTES) != cudaSuccess)
-        return fail(MTP_ERR_CUDA, "distill_topk_grad: shared memory");
-      launch_rows(distill_kernel<T, true, true>, n, shift, RESIDENT_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
-    } else {
-      launch_rows(distill_kernel<T, true, false>, n, shift, RING_BYTES, s, (const T *)logits, rows, a, (T *)grad, grows);
-    }
+    auto kern = sh.warp ? distill_kernel<T, 1, true> : distill_kernel<T, 8, true>;
+    launch_rows(kern, sh, s, (const T *)logits, rows, a, (T *)grad, grows);
   });
   return check_launch("distill_topk_grad");
 }

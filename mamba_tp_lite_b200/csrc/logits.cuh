@@ -66,11 +66,13 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
   return r;
 }
 
+// Adds N elements; returns the largest of them (NaN passed over).
 template <bool ENT, int N>
-__device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float c2) {
-  float m = st.m;
+__device__ __forceinline__ float accumulate(Stat &st, const float (&x)[N], float c2) {
+  float mx = fmaxf(x[0], x[1]);
 #pragma unroll
-  for (int i = 0; i < N; i += 2) m = max3(m, x[i], x[i + 1]);
+  for (int i = 2; i < N; i += 2) mx = max3(mx, x[i], x[i + 1]);
+  const float m = fmaxf(st.m, mx);
   const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
   const float corr = ex2(dy);
   const F2 nm = f2(-m, -m), cc = f2(c2, c2);
@@ -102,6 +104,7 @@ __device__ __forceinline__ void accumulate(Stat &st, const float (&x)[N], float 
   }
   st.s = fmaf(st.s, corr, s0 + s1);
   st.m = m;
+  return mx;
 }
 
 template <bool ENT>
