@@ -132,7 +132,7 @@ template <typename T, int GW> struct Slice {
   __device__ __forceinline__ const T *vec(int v) const { return row + head + (int64_t)v * N; }
   __device__ __forceinline__ int first(int v) const { return head + v * N; }  // index of a vector's first element
   __device__ __forceinline__ const T *mine() const { return vec(v0 + Group<GW>::tid()); }
-  __device__ __forceinline__ int pairs() const { return ((v1 - v0 + NT - 1) / NT + 1) >> 1; }  // of the group's first thread
+  __device__ __forceinline__ int most() const { return (v1 - v0 + NT - 1) / NT; }  // n of the group's first thread
 };
 
 // Asynchronous 16-byte copies into the calling thread's own places of shared memory.
@@ -163,7 +163,7 @@ __device__ __forceinline__ void fetch_pair(const Slice<T, GW> &sl, uint4 *mine, 
 
 // ----------------------------------------------------------------- row statistics
 template <typename T, bool ENT>
-__device__ __forceinline__ float accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
+__device__ __forceinline__ float2 accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
   constexpr int N = Vec<T>::N;
   float x[2 * N], lo[N], hi[N];
   Vec<T>::unpack(a, lo);
@@ -173,13 +173,15 @@ __device__ __forceinline__ float accumulate_pair(Stat &st, const uint4 &a, const
   return accumulate<ENT, 2 * N>(st, x, c2);
 }
 template <typename T, bool ENT>
-__device__ __forceinline__ float accumulate_vec(Stat &st, const uint4 &a, float c2) {
+__device__ __forceinline__ float2 accumulate_vec(Stat &st, const uint4 &a, float c2) {
   float x[Vec<T>::N];
   Vec<T>::unpack(a, x);
-  return accumulate<ENT, Vec<T>::N>(st, x, c2);
+  const float2 mx = accumulate<ENT, Vec<T>::N>(st, x, c2);
+  return make_float2(fmaxf(mx.x, mx.y), -INFINITY);
 }
 
-// Maxima of a thread's chunks of 2 * `per` vectors, for the alternatives: bf16, rounded up, at [chunk][thread].
+// Maxima of a thread's chunks of `per` vectors (1, or a multiple of 2), for the alternatives: bf16, rounded up, at
+// [chunk][thread].
 constexpr int CHUNKS = 16;
 struct ChunkMaxima {
   __nv_bfloat16 *at;
@@ -204,14 +206,21 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, u
   for (int i = 0; i < n; i += 2) {
     copy_wait<RING - 1>();
     uint4 *at = mine + slot * 2 * NT;
-    const float mx = i + 1 < n ? accumulate_pair<T, ENT>(st, at[0], at[NT], c2) : accumulate_vec<T, ENT>(st, at[0], c2);
+    const float2 mx = i + 1 < n ? accumulate_pair<T, ENT>(st, at[0], at[NT], c2) : accumulate_vec<T, ENT>(st, at[0], c2);
     if constexpr (TOP) {
-      chunk = fmaxf(chunk, mx);
-      if (++in_chunk == cm.per) {
-        *cm.at = upper<T>(chunk);
-        cm.at += CTA;
-        chunk = -INFINITY;
-        in_chunk = 0;
+      if (cm.per == 1) {
+        cm.at[0] = upper<T>(mx.x);
+        if (i + 1 < n) cm.at[CTA] = upper<T>(mx.y);
+        cm.at += 2 * CTA;
+      } else {
+        chunk = max3(chunk, mx.x, mx.y);
+        in_chunk += 2;
+        if (in_chunk == cm.per) {
+          *cm.at = upper<T>(chunk);
+          cm.at += CTA;
+          chunk = -INFINITY;
+          in_chunk = 0;
+        }
       }
     }
     if (i + 2 * RING < n) copy16(at, src);
@@ -426,7 +435,7 @@ __device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st
   const int t = G::tid(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t *list = reinterpret_cast<uint64_t *>(ring + G::index() * 2 * RING * NT);
   int *work = reinterpret_cast<int *>(list + S::LIST + S::JOINED);
-  const int chunks = (((sl.n + 1) >> 1) + cm.per - 1) / cm.per;  // the calling thread's
+  const int chunks = (sl.n + cm.per - 1) / cm.per;  // the calling thread's
   uint32_t bound;
   if constexpr (GW == 1) {
     // a maximum that was rounded up is at least the next lower bf16
@@ -474,11 +483,11 @@ __device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st
   const int items = sh.work;
   if (items <= S::WORK) {
     for (int e = t; e < items; e += NT) {
-      const int of = work[e] / CHUNKS, first = sl.v0 + of + 2 * cm.per * (work[e] % CHUNKS) * NT;
-      for (int j = 0; j < cm.per; ++j) {
-        const int v = first + 2 * j * NT;
+      const int of = work[e] / CHUNKS, first = sl.v0 + of + cm.per * (work[e] % CHUNKS) * NT;
+      for (int j = 0; j < cm.per; j += 2) {
+        const int v = first + j * NT;
         if (v >= sl.v1) break;
-        const bool two = v + NT < sl.v1;
+        const bool two = cm.per > 1 && v + NT < sl.v1;
         const uint4 a = load16(sl.vec(v)), b = two ? load16(sl.vec(v + NT)) : make_uint4(0, 0, 0, 0);
         float x[N];
         Vec<T>::unpack(a, x);
@@ -575,7 +584,8 @@ __global__ void __launch_bounds__(CTA, 5) token_logprobs_kernel(const T *__restr
   const int64_t r = part.row;
   const T *row = logits + rows.at(part.row);
   const Slice<T, GW> sl(row, a.V, rank, part.shift);
-  const ChunkMaxima cm{maxima + (TOP ? threadIdx.x : 0), TOP ? max(1, (sl.pairs() + CHUNKS - 1) / CHUNKS) : 1};
+  const ChunkMaxima cm{maxima + (TOP ? threadIdx.x : 0),
+                       !TOP || sl.most() <= CHUNKS ? 1 : (sl.most() + 2 * CHUNKS - 1) / (2 * CHUNKS) * 2};
   cluster_begin(parts);
   const Stat st = thread_stats<T, GW, ENT, TOP>(sl, a.c2, ring, cm);
   cluster_ready(parts);
@@ -899,22 +909,31 @@ __global__ void __launch_bounds__(CTA, 5) distill_kernel(const T *__restrict__ l
   }
 }
 
-// How rows are shared out.  A warp takes a row of up to WARP_ROW bytes where there are rows enough for every warp;
-// else 2^shift CTAs share one: rows alone fill the GPU from about four CTAs per SM on, and a CTA takes no fewer vectors
-// than it has threads.
-constexpr int64_t WARP_ROW = 16384;
+// How rows are shared out.  A warp takes a row of up to 16 KB where there are rows enough for 16 warps per SM: a CTA's
+// fixed cost a row (its barriers and joins) is several times the work of such a row.  60000 rows of 1000 bf16 logits, loss
+// and gradient: 188 us by warps, 853 us by CTAs.  Else 2^shift CTAs share a row:
+//   - until there is one for every SM, each with no fewer vectors than threads: a cluster adds about 2 us of barriers, so
+//     more pays off only where SMs idle (64 rows of 50280 bf16 logits: 10.3 us by 4 CTAs, 12.3 by one; 300 rows: 18.4 by
+//     2, 16.6 by one);
+//   - where the row is read twice, until a CTA's part is at most TWICE bytes, so that what the CTAs at work read stays in
+//     L2 (5 per SM x 104 KB = 77 MB of 126): 4096 rows of 50280 fp32 logits 338 us by 2 CTAs, 395 by one; 1024 of
+//     131072 235 us by 8, 288 by one; 8192 of 50280 bf16 329 by one, 350 by two.
+constexpr int64_t WARP_ROW = 16384, TWICE = 104 * 1024;
 struct Share {
   bool warp;
   int shift;
   unsigned grid;
 };
-inline Share share_rows(int64_t rows, int V, int elem, int top_k) {
+inline Share share_rows(int64_t rows, int V, int elem, bool twice, int top_k = 0) {
   const int64_t sms = num_sms(), bytes = (int64_t)V * elem;
-  // alternatives: the lanes' chunks must be clearly more than k
-  if (bytes <= WARP_ROW && rows >= 16 * sms && (top_k == 0 || bytes / 32 >= 2 * top_k))
+  // for its alternatives a warp needs clearly more vectors than alternatives (60000 rows of 1000 bf16 logits, 125 vectors,
+  // 128 alternatives: 1043 us by CTAs, 1948 by warps; 64 alternatives 262 by warps, 574 by CTAs)
+  if (bytes <= WARP_ROW && rows >= 16 * sms && bytes / 16 >= top_k + top_k / 4)
     return {true, 0, (unsigned)((rows + Group<1>::ROWS - 1) / Group<1>::ROWS)};
   int shift = 0;
-  while (2 << shift <= MAX_CLUSTER && rows << shift < 4 * sms && bytes / 16 >> (shift + 1) >= CTA) ++shift;
+  while (2 << shift <= MAX_CLUSTER && bytes / 16 >> (shift + 1) >= CTA &&
+         (rows << shift < sms || (twice && bytes >> shift > TWICE)))
+    ++shift;
   return {false, shift, (unsigned)(rows << shift)};
 }
 
@@ -975,7 +994,7 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, top_k);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, false, top_k);
   const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
                   (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
@@ -996,7 +1015,7 @@ int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
-  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, false);
   const BwdArgs a{targets, stats, entropy, d_logprob, d_entropy, 1.f / temperature,
                   (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
@@ -1017,7 +1036,7 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld);
   const int64_t n = outer * inner;
-  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, false);
   const DistillArgs a{ids, values, v_dtype, k, nullptr, loss, stats, nullptr, 1.f / temperature,
                       (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {
@@ -1038,7 +1057,7 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
   cudaStream_t s = (cudaStream_t)stream;
   const Rows rows = make_rows(outer, inner, ld_outer, ld), grows = make_rows(outer, inner, grad_ld_outer, grad_ld);
   const int64_t n = outer * inner;
-  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, 0);
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, stats == nullptr);
   const DistillArgs a{ids, values, v_dtype, k, row_weight, loss, nullptr, stats, 1.f / temperature,
                       (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
   MTP_DISPATCH_LOGITS(dtype, T, {

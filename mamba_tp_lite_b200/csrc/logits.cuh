@@ -66,13 +66,20 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
   return r;
 }
 
-// Adds N elements; returns the largest of them (NaN passed over).
+// Adds N elements; returns the largest of each half of them (NaN passed over).
 template <bool ENT, int N>
-__device__ __forceinline__ float accumulate(Stat &st, const float (&x)[N], float c2) {
-  float mx = fmaxf(x[0], x[1]);
+__device__ __forceinline__ float2 accumulate(Stat &st, const float (&x)[N], float c2) {
+  float2 mx = make_float2(x[0], x[N / 2]);
 #pragma unroll
-  for (int i = 2; i < N; i += 2) mx = max3(mx, x[i], x[i + 1]);
-  const float m = fmaxf(st.m, mx);
+  for (int i = 1; i + 1 < N / 2; i += 2) {
+    mx.x = max3(mx.x, x[i], x[i + 1]);
+    mx.y = max3(mx.y, x[N / 2 + i], x[N / 2 + i + 1]);
+  }
+  if (N / 2 % 2 == 0) {
+    mx.x = fmaxf(mx.x, x[N / 2 - 1]);
+    mx.y = fmaxf(mx.y, x[N - 1]);
+  }
+  const float m = max3(st.m, mx.x, mx.y);
   const float dy = fmaxf((st.m - m) * c2, FLOOR_Y);
   const float corr = ex2(dy);
   const F2 nm = f2(-m, -m), cc = f2(c2, c2);

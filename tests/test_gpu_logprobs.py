@@ -29,8 +29,11 @@ def f64(x):
 
 
 def close(got, want, bound, what=""):
-    """|got - want| <= bound where want is finite; the same infinities and NaN elsewhere."""
+    """|got - want| <= bound where want is finite; the same infinities and NaN elsewhere.  Results are fp32 (or
+    smaller): from 2^128 - 2^103 on, half a step past the largest fp32, a value rounds to infinity (the lowest fp32
+    logit divided by a temperature below 1 is one)."""
     got = f64(got) if isinstance(got, torch.Tensor) else got
+    want = np.where(np.abs(want) >= 2.0 ** 128 - 2.0 ** 103, np.copysign(np.inf, want), want)
     bound = np.broadcast_to(bound, want.shape)
     fin = np.isfinite(want)
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=what)
@@ -98,6 +101,52 @@ def test_token_logprobs_without_targets():
 @pytest.mark.parametrize("v", [24, 1003])
 def test_token_logprobs_many_rows(rows, v):
     check_forward(make(rows, v, BF, rows), targets_for(rows, v), 4)
+
+
+WARP_ROWS = 2500  # short rows in such numbers go a warp each
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("v", [1, 9, 130, 1003, 3000])
+def test_short_rows_in_large_numbers(dtype, v):
+    """Forward, gradient and distillation of rows that a warp takes each, with rows where a softmax goes
+    wrong easily among them."""
+    x = make(WARP_ROWS, v, dtype, v)
+    if v >= 40:
+        x[:16] = special_rows(v, dtype)
+        x[-16:] = x[:16]
+    t = targets_for(WARP_ROWS, v)
+    for k in sorted({0, 1, min(7, v), min(64, v), min(128, v)}):
+        check_forward(x, t, k, 0.8)
+    g = torch.linspace(0.5, 1.5, WARP_ROWS, device=dev())
+    h = torch.linspace(-1, 0.9, WARP_ROWS, device=dev())
+    for heads in (2, 1):
+        leaf = x.detach().requires_grad_()
+        r = P.token_logprobs(leaf, t)
+        outs, grads = [r.logprob, r.entropy][:heads], [g, h][:heads]
+        (grad,) = torch.autograd.grad(outs, [leaf], grads)
+        check_grad(x, t, g, h if heads == 2 else torch.zeros_like(h), grad)
+    x = make(WARP_ROWS, v, dtype, v)
+    ids, vals = teacher_for(x, min(20, v))
+    ids[3] = -1
+    ids[4] = ids[4, 0].clone()
+    loss, grad = P.distill_topk_loss_and_grad(x, ids, vals, g)
+    check_distill(x, ids, vals, g, loss, grad)
+    leaf = x.detach().requires_grad_()
+    loss = P.distill_topk_loss(leaf, ids, vals)
+    (grad,) = torch.autograd.grad([loss], [leaf], [g])
+    check_distill(x, ids, vals, g, loss, grad)
+
+
+@pytest.mark.parametrize("rows,v,dtype", [(160, 60000, F32), (150, 131071, BF), (20, 131072, F32), (149, 30001, F32)])
+def test_long_rows_shared_by_clusters(rows, v, dtype):
+    x = make(rows, v, dtype, 4)
+    t = targets_for(rows, v)
+    check_forward(x, t, 33)
+    ids, vals = teacher_for(x, 40)
+    w = torch.linspace(0.5, 1.5, rows, device=dev())
+    loss, grad = P.distill_topk_loss_and_grad(x, ids, vals, w)
+    check_distill(x, ids, vals, w, loss, grad)
 
 
 LAYOUTS = {
