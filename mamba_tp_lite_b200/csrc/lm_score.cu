@@ -38,6 +38,7 @@ struct ScoreParams {
   int *status;    // [gridDim.x]
   int M, N, K;
   int bn, tiles_m, tiles_n, num_tiles, group_m;
+  int a_rows;  // rows of a hidden-state box
   uint32_t idesc;
   float c2;
 };
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   MTP_PDL_TRIGGER();
   const uint32_t tmem_base = *tmem_holder;
   const int num_kb = (p.K + BK - 1) / BK;
-  const uint32_t tx_bytes = (uint32_t)(A_BYTES + p.bn * BK * 2);
+  const uint32_t tx_bytes = (uint32_t)((p.a_rows + p.bn) * BK * 2);
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -356,10 +357,13 @@ int launch_score(const void *hidden, int ld_hidden, int rows, int K, const void 
   p.tiles_n = plan.tiles_n;
   p.num_tiles = plan.tiles_m * plan.tiles_n;
   p.group_m = 32;
+  // one row block: only the 8-row groups that hold rows are loaded; the MMA's other rows are whatever the ring held, and
+  // their accumulators are not read
+  p.a_rows = rows < BM ? (rows + 7) / 8 * 8 : BM;
   p.idesc = idesc_bf16(BM, plan.bn);
   p.c2 = (float)(1.4426950408889634 / temperature);
   CUtensorMap ta, tb;
-  int rc = make_tmap(&ta, hidden, rows, K, ld_hidden, BM);
+  int rc = make_tmap(&ta, hidden, rows, K, ld_hidden, p.a_rows);
   if (rc) return rc;
   rc = make_tmap(&tb, weight, V, K, ld_weight, plan.bn);
   if (rc) return rc;

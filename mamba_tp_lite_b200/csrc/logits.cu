@@ -570,7 +570,7 @@ struct FwdArgs {
 };
 
 template <typename T, int GW, bool ENT, bool TOP>
-__global__ void __launch_bounds__(CTA, 5) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
+__global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) token_logprobs_kernel(const T *__restrict__ logits, Rows rows, FwdArgs a) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
   using G = Group<GW>;
@@ -719,7 +719,7 @@ struct BwdArgs {
 
 // dx_j = (g (1{j = t} - p_j) - h p_j (log p_j + H)) / T
 template <typename T, int GW, bool ENT>
-__global__ void __launch_bounds__(CTA, 5) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
+__global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) token_logprobs_bwd_kernel(const T *__restrict__ logits, Rows rows, BwdArgs a,
                                                                     T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
@@ -834,7 +834,7 @@ __device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a,
 // loss = sum q_i (log q_i - log p_id_i), dx_j = w (p_j - sum_{id_i = j} q_i) / T; q: softmax over the used entries of
 // the teacher's logits / T.  GRAD: the gradient is written too.
 template <typename T, int GW, bool GRAD>
-__global__ void __launch_bounds__(CTA, 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
+__global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
                                                          T *__restrict__ grad, Rows grows) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
