@@ -5,12 +5,17 @@
 //   warp 0     one lane issues TMA tile loads (hidden 128x64, weight bn x 64, 128-byte swizzle) into a 4-stage ring;
 //   warp 1     allocates 512 TMEM columns (two 128 x bn fp32 accumulators), one lane issues tcgen05.mma;
 //   warps 2-9  epilogue: two warps per TMEM lane quarter, each on half of the tile's columns, a lane holding one row.
-//              A lane keeps the running (m, S, U) of its columns, the second warp hands its own to the first through
-//              shared memory, and one (m, S, U) per row and tile goes to the workspace, the given token's logit beside it.
-// A second kernel joins a row's tiles.  The epilogue costs about 6 instructions a logit (2,000 cycles a tile for the
-// 8 warps) against 8 K cycles of tensor work a tile, so that it hides from K = 256 on.
+//              A lane adds the accumulators of the splits of K in registers, then keeps the running (m, S, U) of its
+//              columns; the second warp hands its own to the first through shared memory, and one (m, S, U) per row and
+//              tile goes to the workspace, the given token's logit beside it.
+// A second kernel joins a row's tiles.  K is split because the tensor core truncates at every step of its sum: measured
+// against 64 bits, a sum over K is 8.6e-10 K of its value too small (1.8e-6 at K = 2048, which an entropy shows).  Every
+// further split costs 600 cycles a tile, in which the accumulator is read (8192 rows of K = 2048, V = 50280: 1060 us
+// unsplit, 1100 with two splits, 1180 with four, 1364 with eight), so that one sums up to 1024.
+// The epilogue works on a tile while the tensor core fills the next one's accumulators.
 // Every mbarrier wait is bounded; a CTA that gives up marks its status slot, frees its TMEM and returns, and the second
 // kernel then writes NaN.
+#include <type_traits>
 #include "common.cuh"
 #include "logits.cuh"
 #include "tc_common.cuh"
@@ -24,6 +29,7 @@ using namespace lg;
 using namespace tc;
 
 constexpr int BM = 128, BK = 64, BN_MAX = 256, STAGES = 4;
+constexpr int SPLIT = 16;  // K blocks that one accumulator sums, at most
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN_MAX * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int EPI_WARPS = 8, NUM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 512;
@@ -39,6 +45,7 @@ struct ScoreParams {
   int M, N, K;
   int bn, tiles_m, tiles_n, num_tiles, group_m;
   int a_rows;  // rows of a hidden-state box
+  int split;   // K blocks that one accumulator sums
   uint32_t idesc;
   float c2;
 };
@@ -53,6 +60,11 @@ __device__ __forceinline__ void tile_coords(const ScoreParams &p, int t, int &mt
   const int r = t - g * gsize;
   mt = first_m + r % gm;
   nt = r / gm;
+}
+
+// h = v where at == i.  (Written out, so that a row of them is not turned into an indexed array in local memory.)
+__device__ __forceinline__ void pick(float &h, float v, int at, int i) {
+  asm("{\n.reg .pred p;\nsetp.eq.s32 p, %2, %3;\nselp.f32 %0, %1, %0, p;\n}" : "+f"(h) : "f"(v), "r"(at), "r"(i));
 }
 
 template <bool ENT>
@@ -134,27 +146,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int s = 0, local = 0;
       uint32_t ph = 0;
       bool any = false;
-      for (int t = blockIdx.x; t < p.num_tiles && !*abort; t += gridDim.x, ++local) {
-        const int a = local & 1;
-        const uint32_t use = (uint32_t)(local >> 1);
-        if (!mbar_wait(tempty_bar(a), (use & 1u) ^ 1u, abort, TIMEOUT_NS)) break;
-        tc_fence_after();
-        const uint32_t d = tmem_base + (uint32_t)(a * BN_MAX);
-        bool ok = true;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) { ok = false; break; }
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < p.num_tiles && !*abort; t += gridDim.x) {
+        for (int kb0 = 0; ok && kb0 < num_kb; kb0 += p.split, ++local) {
+          const int a = local & 1;
+          const uint32_t use = (uint32_t)(local >> 1);
+          if (!mbar_wait(tempty_bar(a), (use & 1u) ^ 1u, abort, TIMEOUT_NS)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = base + s * STAGE_BYTES;
-          const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + A_BYTES);
+          const uint32_t d = tmem_base + (uint32_t)(a * BN_MAX);
+          const int nkb = min(p.split, num_kb - kb0);
+          for (int kb = 0; kb < nkb; ++kb) {
+            if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = base + s * STAGE_BYTES;
+            const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + A_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)  // +32 bytes along K per instruction
-            umma_bf16(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), p.idesc, (kb | k) != 0);
-          any = true;
-          umma_commit(empty_bar(s));
-          if (++s == STAGES) { s = 0; ph ^= 1u; }
+            for (int k = 0; k < BK / 16; ++k)  // +32 bytes along K per instruction
+              umma_bf16(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), p.idesc, (kb | k) != 0);
+            any = true;
+            umma_commit(empty_bar(s));
+            if (++s == STAGES) { s = 0; ph ^= 1u; }
+          }
+          if (ok) umma_commit(tfull_bar(a));
         }
-        if (!ok) break;
-        umma_commit(tfull_bar(a));
       }
       if (*abort && any) {
         umma_commit(drain_bar);
@@ -169,11 +183,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int half = (warp - 2) >> 2;  // its half of the tile's 16-column chunks
     const int chunks = p.bn / 16, cut = (chunks + 1) / 2;
     const int c_lo = half ? cut : 0, c_hi = half ? chunks : cut;
-    int local = 0;
+    const int nch = c_hi - c_lo;
+    int local = 0, tile = 0;
     bool alive = true;
-    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++local) {
-      const int a = local & 1;
-      const uint32_t use = (uint32_t)(local >> 1);
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++tile) {
       int mt, nt;
       tile_coords(p, t, mt, nt);
       const int row = mt * BM + q * 32 + lane;
@@ -181,45 +194,63 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (p.targets && row < p.M) tgt = p.targets[row];
       const int64_t rel = tgt - (int64_t)nt * p.bn;  // the given token's column of this tile, if it is in it
       const int at = rel >= 0 && rel < p.bn && tgt < p.N ? (int)rel : -16;
-      // a warp that gives up still meets its partner at the barrier below
-      alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, TIMEOUT_NS));
-      tc_fence_after();
+      F2 acc[BN_MAX / 32][8];  // this lane's sums so far: half a tile
       Stat st{LOWEST, 0.f, 0.f};
-      if (alive) {
-        const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN_MAX);
-        auto chunk = [&](int c, float (&v)[16]) {
-          const int n0 = nt * p.bn + 16 * c;
-          if (n0 + 16 > p.N) {  // tokens past the vocabulary
+      auto chunk = [&](int c, const F2 (&x)[8]) {
+        const int n0 = nt * p.bn + 16 * (c_lo + c);
+        float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n0 + i >= p.N) v[i] = -INFINITY;
-          }
-          if ((at >> 4) == c) {
-            float x = v[0];
+        for (int i = 0; i < 8; ++i) un2(x[i], v[2 * i], v[2 * i + 1]);
+        if (n0 + 16 > p.N) {  // tokens past the vocabulary
 #pragma unroll
-            for (int i = 1; i < 16; ++i) x = (at & 15) == i ? v[i] : x;
-            p.hit[row] = x;
-          }
-          accumulate<ENT, 16>(st, v, p.c2);
-        };
-        int c = c_lo;
-        for (; c + 1 < c_hi; c += 2) {  // two chunks per TMEM wait
-          float v[16], w[16];
-          tmem_ld16x2(tbase + 16u * c, tbase + 16u * (c + 1), v, w);
-          chunk(c, v);
-          chunk(c + 1, w);
+          for (int i = 0; i < 16; ++i)
+            if (n0 + i >= p.N) v[i] = -INFINITY;
         }
-        if (c < c_hi) {
-          float v[16];
-          tmem_ld16(tbase + 16u * c, v);
-          chunk(c, v);
+        if ((at >> 4) == c_lo + c) {
+          float h = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pick(h, v[i], at & 15, i);
+          p.hit[row] = h;
         }
+        accumulate<ENT, 16>(st, v, p.c2);
+      };
+      for (int kb0 = 0; kb0 < num_kb; kb0 += p.split, ++local) {
+        const int a = local & 1;
+        const uint32_t use = (uint32_t)(local >> 1);
+        // a warp that gives up still meets its partner at the barrier below
+        alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, TIMEOUT_NS));
+        tc_fence_after();
+        if (alive) {
+          const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN_MAX + 16 * c_lo);
+          auto take = [&](auto first) {
+#pragma unroll
+            for (int c = 0; c < BN_MAX / 32; ++c) {
+              if (c < nch) {
+                float v[16];
+                tmem_ld16(tbase + 16u * c, v);
+                F2 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  x[i] = f2(v[2 * i], v[2 * i + 1]);
+                  acc[c][i] = first ? x[i] : add2(acc[c][i], x[i]);
+                }
+              }
+            }
+          };
+          if (kb0 == 0) take(std::true_type{});
+          else take(std::false_type{});
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(a));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar(a));
+      if (alive) {
+#pragma unroll
+        for (int c = 0; c < BN_MAX / 32; ++c)
+          if (c < nch) chunk(c, acc[c]);
+      }
       // the second half's statistics to the first; the buffer alternates by tile, so one barrier a tile orders both uses
-      float *h = hand + ((a * 4 + q) * 32 + lane) * 3;
+      float *h = hand + (((tile & 1) * 4 + q) * 32 + lane) * 3;
       if (half) {
         h[0] = st.m;
         h[1] = st.s;
@@ -360,6 +391,8 @@ int launch_score(const void *hidden, int ld_hidden, int rows, int K, const void 
   // one row block: only the 8-row groups that hold rows are loaded; the MMA's other rows are whatever the ring held, and
   // their accumulators are not read
   p.a_rows = rows < BM ? (rows + 7) / 8 * 8 : BM;
+  const int num_kb = (K + BK - 1) / BK, splits = (num_kb + SPLIT - 1) / SPLIT;
+  p.split = (num_kb + splits - 1) / splits;
   p.idesc = idesc_bf16(BM, plan.bn);
   p.c2 = (float)(1.4426950408889634 / temperature);
   CUtensorMap ta, tb;
@@ -369,8 +402,10 @@ int launch_score(const void *hidden, int ld_hidden, int rows, int K, const void 
   if (rc) return rc;
   auto kern = entropy ? lm_score_kernel<true> : lm_score_kernel<false>;
   // set at every call: the attribute belongs to the current device
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+    cudaGetLastError();
     return fail(MTP_ERR_CUDA, "lm_score: shared memory");
+  }
   launch_pdl(kern, dim3(plan.grid), dim3(NUM_THREADS), SMEM_BYTES, stream, ta, tb, p);
   rc = check_launch("lm_score");
   if (rc) return rc;

@@ -141,6 +141,13 @@ def _row_like(x: torch.Tensor, ids: torch.Tensor | None) -> torch.Tensor:
     return x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
+def _f32(g: torch.Tensor | None) -> torch.Tensor | None:
+    """A row gradient as the kernels read it: dense fp32 (autograd may hand on an expanded scalar)."""
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.float().contiguous()
+
+
 # ------------------------------------------------------------------ log probabilities
 def _logprobs_fwd(x, targets, top_k, temperature, entropy, want_stats):
     lp = None if targets is None else _row_like(x, targets)
@@ -177,8 +184,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
 
 
 def _logprobs_bwd(x, targets, temperature, stats, ent, g, h):
-    g = None if g is None else g.float().contiguous()
-    h = None if h is None else h.float().contiguous()
+    g, h = _f32(g), _f32(h)
     x, outer, inner, ld_outer, ld = _row_layout(x)
     grad, g_ld_outer, g_ld = _grad_like(x, inner, ld_outer, ld)
     _call(x, "mtp_token_logprobs_bwd", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
@@ -257,7 +263,7 @@ class _DistillFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         x, ids, values, stats = ctx.saved_tensors
-        _, grad = _distill_grad(x, ids, values, ctx.temperature, stats, g.float().contiguous(), False)
+        _, grad = _distill_grad(x, ids, values, ctx.temperature, stats, _f32(g), False)
         return grad, None, None, None
 
 
