@@ -17,8 +17,9 @@
  * here; the Python package binds this header with ctypes.
  *
  * Devices: the library serves one device per process (one rank per process), except
- * the allocation-free reduction scratch, the reductions' row scratch and the chunked
- * scan's state scratch, which are kept per device; the status words of the GEMM and of the fused scan are per process.
+ * the operators on logits (any device; mtp_lm_head_logprobs only where it needs no mtp_gemm: bf16
+ * operands that TMA can read and no alternatives), the allocation-free reduction scratch, the
+ * reductions' row scratch and the chunked scan's state scratch, which are kept per device; the status words of the GEMM and of the fused scan are per process.
  *
  * Layout conventions: matrices are row-major; a "token row" is one position
  * of one sequence, tokens ordered (batch, position).  Element type codes are
@@ -350,7 +351,8 @@ int mtp_distill_topk(const void *logits, int dtype, int64_t outer, int64_t inner
                      const int64_t *ids, const void *values, int v_dtype, int k, float temperature, float *loss,
                      float *stats, void *stream);
 /* Its gradient, grad_j = row_weight[r] (p_j - sum of q_i over id_i = j) / temperature (0 in a row
- * without a used entry or of weight 0).  With stats from mtp_distill_topk this is the backward
+ * without a used entry or of weight 0; NaN where a teacher value that is used is NaN or +inf).
+ * grad and logits must not overlap.  With stats from mtp_distill_topk this is the backward
  * pass; with stats NULL one call computes loss (or NULL) and gradient. */
 int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld,
                           int V, const int64_t *ids, const void *values, int v_dtype, int k, float temperature,
@@ -358,7 +360,9 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
                           int64_t grad_ld, void *stream);
 /* Log probabilities from the last hidden states: logits = hidden[rows, K] . weight[V, K]^T in fp32
  * (hidden and weight of dtype MTP_F32 or MTP_BF16), never held as a whole, then logprob, entropy
- * and the top_k alternatives as mtp_token_logprobs.  workspace: 16-byte aligned device memory of
+ * and the top_k alternatives as mtp_token_logprobs.  bf16 operands on 16-byte boundaries with
+ * top_k 0 take one tensor-core pass that keeps no logits at all (a device wait that expires there
+ * gives NaN); everything else goes through blocks of about 256 MB of fp32 logits in the workspace.  workspace: 16-byte aligned device memory of
  * at least the size that mtp_lm_head_logprobs_workspace gives for the same arguments, with
  * nothing in it to start with; calls that overlap on the GPU need one each. */
 int mtp_lm_head_logprobs_workspace(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight,
