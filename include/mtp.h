@@ -319,7 +319,7 @@ int mtp_lm_head_vocab_parallel(mtp_comm *c, const void *normed, int rows, int K,
  * Rows of logits: [outer][inner] rows of V values, row (o, i) at logits + o * ld_outer + i * ld
  * (elements; any alignment of the element type, overlapping rows allowed for reading), of dtype
  * MTP_F32, MTP_BF16 or MTP_F16.  Per-row arrays hold outer * inner values in row order.  With
- * z = x / temperature, p = softmax(z): log p_j = z_j - max z - log sum e^(z - max z).
+ * z = x / temperature (between 1e-6 and 1e6), p = softmax(z): log p_j = z_j - max z - log sum e^(z - max z).
  * Statistics, sums and every per-row output are fp32.  A NaN or +inf in a row gives NaN; a row of
  * -inf alone has log p = -inf, entropy 0 and gradient 0.  No device memory is allocated and
  * nothing is kept between calls: any stream, device or graph capture.

@@ -439,7 +439,7 @@ int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, con
                          void *stream) {
   MTP_REQUIRE(rows >= 0 && V > 0 && V <= (1 << 30) && K > 0 && ld_hidden >= K && ld_weight >= K, "bad sizes");
   MTP_REQUIRE(dtype == MTP_F32 || dtype == MTP_BF16, "dtype must be F32 or BF16");
-  MTP_REQUIRE(temperature > 0.f && temperature < INFINITY, "temperature must be positive and finite");
+  MTP_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, "temperature must be between 1e-6 and 1e6");
   MTP_REQUIRE(top_k >= 0 && top_k <= 128 && top_k <= V, "top_k must be between 0 and min(V, 128)");
   if (rows == 0) return MTP_OK;
   MTP_REQUIRE(hidden && weight && workspace, "null pointer");

@@ -558,7 +558,7 @@ __device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st
 }
 
 // ----------------------------------------------------------------- log probabilities
-// Bound by the exponentials at the clocks of a long run under the power cap (16 per cycle and SM, 1.06 a logit: 470 us of
+// Bound by the exponentials at the clocks of a long run under the power cap (16 per cycle and SM, 1.06 a logit: 480 us of
 // the 655 us that 32 x 1023 rows of 50280 bf16 logits take at 1.53 GHz, their issue slots 75% used), by HBM otherwise: the
 // same rows 556 us in isolation, 5.92 TB/s or 0.92 of the measured copy rate.  fp32 rows are HBM-bound: 4096 of 50280
 // 139 us, 0.92.  A ring of 32 KB per CTA and five CTAs per SM were taken: 6 CTAs (spills) 575 us, a ring twice as deep
@@ -985,7 +985,7 @@ template <typename T, int GW> auto fwd_kernel(bool ent, bool top) {
   MTP_REQUIRE(outer >= 0 && inner >= 0 && ld_outer >= 0 && ld >= 0, "bad sizes");                                 \
   MTP_REQUIRE(V > 0 && V <= (1 << 30), "the vocabulary must have 1 to 2^30 tokens");                              \
   MTP_REQUIRE(inner == 0 || outer <= 0x7fffffffll / inner, "more than 2^31 - 1 rows");                            \
-  MTP_REQUIRE(temperature > 0.f && temperature < INFINITY, "temperature must be positive and finite");            \
+  MTP_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, "temperature must be between 1e-6 and 1e6");           \
   if (outer == 0 || inner == 0) return MTP_OK;                                                                    \
   MTP_REQUIRE(logits, "null pointer")
 

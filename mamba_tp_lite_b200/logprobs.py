@@ -12,7 +12,6 @@ a CUDA graph.  The reference has no counterpart; the nearest is the full-vocabul
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import NamedTuple
 
 import torch
@@ -78,8 +77,8 @@ def _check_top_k(top_k: int, vocab: int, what: str) -> int:
 
 def _check_temperature(t: float, what: str) -> float:
     t = float(t)
-    if not (t > 0.0 and math.isfinite(t)):
-        raise ValueError(f"{what}: temperature must be positive and finite, got {t}")
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{what}: temperature must be between 1e-6 and 1e6, got {t}")
     return t
 
 

@@ -816,3 +816,44 @@ def test_step_alternatives_in_a_decode_loop():
         out.append(nxt)
         logits = m.step(nxt, cache)
     assert torch.equal(torch.cat(out, 1), want)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e6])
+@pytest.mark.parametrize("rows", [3, WARP_ROWS])
+def test_extreme_temperatures(temperature, rows):
+    """The ends of the allowed range: one token of probability 1, and all nearly equal; masked logits stay out."""
+    x = make(rows, 700, F32, 12)
+    x[:, 5::7] = float("-inf")
+    check_forward(x, targets_for(rows, 700), 9, temperature)
+    g = torch.ones(rows, device=dev())
+    leaf = x.detach().requires_grad_()
+    r = P.token_logprobs(leaf, targets_for(rows, 700), temperature=temperature)
+    (grad,) = torch.autograd.grad([r.logprob], [leaf], [g])
+    check_grad(x, targets_for(rows, 700), g, torch.zeros_like(g), grad, temperature)
+
+
+def test_a_backward_pass_on_another_stream_than_the_forward():
+    """autograd runs the backward pass on the forward's stream; the caller's stream waits for it."""
+    x = make(200, 5001, BF, 13)
+    t = targets_for(200, 5001)
+    g = torch.ones(200, device=dev())
+    leaf = x.detach().requires_grad_()
+    (want,) = torch.autograd.grad([P.token_logprobs(leaf, t).logprob], [leaf], [g])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf2 = x.detach().requires_grad_()
+        lp = P.token_logprobs(leaf2, t).logprob
+    torch.cuda.current_stream().wait_stream(side)
+    (got,) = torch.autograd.grad([lp], [leaf2], [g])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_teacher_values_that_are_no_numbers():
+    x = make(3, 90, F32, 14)
+    ids = torch.tensor([[1, 2, 3]] * 3, device=dev())
+    vals = torch.tensor([[0.0, float("nan"), 1.0], [0.0, float("inf"), 1.0], [0.0, 0.5, 1.0]], device=dev())
+    loss, grad = P.distill_topk_loss_and_grad(x, ids, vals, torch.ones(3, device=dev()))
+    assert torch.isnan(loss[:2]).all() and torch.isfinite(loss[2])
+    assert torch.isnan(grad[:2]).all() and torch.isfinite(grad[2]).all()

@@ -150,7 +150,7 @@ def test_argument_checks():
     for k in (-1, 9, 129):
         with pytest.raises(ValueError, match="top_k"):
             P._check_top_k(k, 8 if k < 100 else 1000, "f")
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1e-40, 1e30, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="temperature"):
             P._check_temperature(t, "f")
     with pytest.raises(ValueError, match="shape"):
