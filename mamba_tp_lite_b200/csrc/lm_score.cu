@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (int i = 0; i < 16; ++i) pick(h, v[i], at & 15, i);
           p.hit[row] = h;
         }
-        accumulate<ENT, 16>(st, v, p.c2);
+        bool masked;
+        accumulate<ENT, 16>(st, v, p.c2, masked);
       };
       for (int kb0 = 0; kb0 < num_kb; kb0 += p.split, ++local) {
         const int a = local & 1;

@@ -162,21 +162,22 @@ __device__ __forceinline__ void fetch_pair(const Slice<T, GW> &sl, uint4 *mine, 
 }
 
 // ----------------------------------------------------------------- row statistics
-template <typename T, bool ENT>
-__device__ __forceinline__ float2 accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2) {
+template <typename T, bool ENT, bool MASKED>
+__device__ __forceinline__ float2 accumulate_pair(Stat &st, const uint4 &a, const uint4 &b, float c2, bool &masked) {
   constexpr int N = Vec<T>::N;
   float x[2 * N], lo[N], hi[N];
   Vec<T>::unpack(a, lo);
   Vec<T>::unpack(b, hi);
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = lo[i], x[N + i] = hi[i];
-  return accumulate<ENT, 2 * N>(st, x, c2);
+  return accumulate<ENT, 2 * N, MASKED>(st, x, c2, masked);
 }
 template <typename T, bool ENT>
 __device__ __forceinline__ float2 accumulate_vec(Stat &st, const uint4 &a, float c2) {
   float x[Vec<T>::N];
   Vec<T>::unpack(a, x);
-  const float2 mx = accumulate<ENT, Vec<T>::N>(st, x, c2);
+  bool masked;
+  const float2 mx = accumulate<ENT, Vec<T>::N, true>(st, x, c2, masked);
   return make_float2(fmaxf(mx.x, mx.y), -INFINITY);
 }
 
@@ -202,11 +203,15 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, u
   const int n = sl.n;
   const T *src = sl.mine() + (int64_t)2 * RING * sl.STEP;
   int slot = 0, in_chunk = 0;
+  bool masked = false;
   float chunk = -INFINITY;
   for (int i = 0; i < n; i += 2) {
     copy_wait<RING - 1>();
     uint4 *at = mine + slot * 2 * NT;
-    const float2 mx = i + 1 < n ? accumulate_pair<T, ENT>(st, at[0], at[NT], c2) : accumulate_vec<T, ENT>(st, at[0], c2);
+    float2 mx;
+    if (i + 1 == n) mx = accumulate_vec<T, ENT>(st, at[0], c2);
+    else if (ENT && masked) mx = accumulate_pair<T, ENT, true>(st, at[0], at[NT], c2, masked);
+    else mx = accumulate_pair<T, ENT, false>(st, at[0], at[NT], c2, masked);
     if constexpr (TOP) {
       if (cm.per == 1) {
         cm.at[0] = upper<T>(mx.x);
@@ -559,8 +564,8 @@ __device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st
 
 // ----------------------------------------------------------------- log probabilities
 // Bound by the exponentials at the clocks of a long run under the power cap (16 per cycle and SM, 1.06 a logit: 480 us of
-// the 655 us that 32 x 1023 rows of 50280 bf16 logits take at 1.53 GHz, their issue slots 75% used), by HBM otherwise: the
-// same rows 556 us in isolation, 5.92 TB/s or 0.92 of the measured copy rate.  fp32 rows are HBM-bound: 4096 of 50280
+// the 677 us that 32 x 1023 rows of 50280 bf16 logits take at 1.53 GHz, their issue slots 75% used), by HBM otherwise: the
+// same rows 559 us in isolation, 5.89 TB/s or 0.92 of the measured copy rate.  fp32 rows are HBM-bound: 4096 of 50280
 // 139 us, 0.92.  A ring of 32 KB per CTA and five CTAs per SM were taken: 6 CTAs (spills) 575 us, a ring twice as deep
 // (three CTAs) 11% slower.  Alternatives cost a row its joins and the second look: 2048 fp32 rows 98 us with 64 of them.
 struct FwdArgs {
