@@ -319,8 +319,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) lm_score_join_kernel(const Sc
   gave_up = __syncthreads_or(gave_up);
   if (threadIdx.x >= JOIN_ROWS || row >= p.M) return;
   for (int w = 1; w < JOIN_WARPS; ++w) st = join<ENT>(st, sh[w][lane], p.c2);
-  RowStats r = finish(st);
-  if (gave_up) r.log_s = r.entropy = NAN;
+  const RowStats r = gave_up ? expired() : finish(st);
   if (logprob) {
     const int64_t t = p.targets[row];
     logprob[row] = t < 0 ? 0.f : t >= p.N ? NAN : log_prob(p.hit[row], r.m, r.log_s, inv_t);

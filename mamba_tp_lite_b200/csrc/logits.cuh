@@ -135,6 +135,10 @@ __device__ __forceinline__ RowStats finish(Stat st) {
   return {st.m, ls, ls - LN2 * (st.u / st.s)};
 }
 
+// Of a row whose logits are not to be trusted, because a device wait of the pass that made them expired: everything that
+// is derived from it is NaN (a largest logit of -inf would give log probabilities of -inf, as of a row of -inf alone).
+__device__ __forceinline__ RowStats expired() { return {NAN, NAN, NAN}; }
+
 // log p of a logit of the row; a row whose logits are all -inf gives -inf.
 __device__ __forceinline__ float log_prob(float x, float m, float log_s, float inv_t) {
   return m == -INFINITY ? -INFINITY : (x - m) * inv_t - log_s;
