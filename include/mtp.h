@@ -6,20 +6,21 @@
  * (passed as void*), returns an int status (0 = ok, see MTP_ERR_*) and launches
  * only on the given stream.  Device memory is allocated by the create / bind
  * calls (mtp_comm_create, mtp_decode_plan_create, mtp_decode_bind_cache) and,
- * on first use, for four internal buffers kept until exit: a status word of
- * the tensor-core GEMM, one of the fused dt_proj scan, the row scratch of
+ * on first use, for three internal buffers kept until exit: a status word of
+ * the fused dt_proj scan, the row scratch of
  * the reductions that do not hold a row in registers (rows wider than 3072
  * values or not a multiple of 4, a grid capped by mtp_comm_set_max_ctas, or a
  * per-tensor-scale mode), and the state scratch of the sequence-chunked scan;
  * the last two grow to the largest size used.  A call that is to be recorded in a
  * CUDA graph therefore needs one call of the same kind before the capture (the
- * package's GraphedStepper runs warm-up steps first).  No torch types appear
- * here; the Python package binds this header with ctypes.
+ * package's GraphedStepper runs warm-up steps first); mtp_gemm and the operators on
+ * logits do not.  No torch types appear here; the Python package binds this header with
+ * ctypes.
  *
  * Devices: the library serves one device per process (one rank per process), except
- * the operators on logits (any device; mtp_lm_head_logprobs only where it needs no mtp_gemm: bf16
- * operands that TMA can read and no alternatives), the allocation-free reduction scratch, the
- * reductions' row scratch and the chunked scan's state scratch, which are kept per device; the status words of the GEMM and of the fused scan are per process.
+ * mtp_gemm and the operators on logits (any device), the allocation-free reduction scratch, the
+ * reductions' row scratch and the chunked scan's state scratch, which are kept per device; the
+ * status word of the fused scan is per process.
  *
  * Layout conventions: matrices are row-major; a "token row" is one position
  * of one sequence, tokens ordered (batch, position).  Element type codes are

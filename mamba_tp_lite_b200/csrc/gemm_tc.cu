@@ -10,8 +10,8 @@
 //               tcgen05.ld 32 lanes x 16 columns, fused epilogue op, then the 32 x 16 chunk is
 //               staged in shared memory and written by a TMA store (or, with unaligned C,
 //               stored directly); overlaps the next tile's MMAs thanks to the second accumulator.
-// Every mbarrier wait is bounded (globaltimer); on expiry the CTA records MTP_ERR_TIMEOUT in a
-// device word, drains its in-flight copies and MMAs with bounded waits, frees TMEM and returns.
+// Every mbarrier wait is bounded (globaltimer); on expiry the CTA records MTP_ERR_TIMEOUT in
+// expired_wait, drains its in-flight copies and MMAs with bounded waits, frees TMEM and returns.
 #include <cuda.h>
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -37,7 +37,6 @@ constexpr int SMEM_BYTES_TMA_STORE = SMEM_BYTES + NUM_EPI_WARPS * STAGE_C_BYTES;
 struct Params {
   void *C;
   const void *bias;
-  int *err;
   unsigned long long timeout_ns;
   int M, N, K, ldc;
   int c_dtype, epi, bias_dtype;
@@ -48,6 +47,10 @@ struct Params {
   int wire;       // x_proj reduction epilogue (one N tile holds whole rows; C is not written)
   XprojWire x;
 };
+
+// Set once a wait of the kernel has expired.  A variable of the module: every device has its own, and nothing has to be
+// allocated (a first call may be one that is being captured).
+__device__ int expired_wait;
 
 __device__ __forceinline__ void tile_coords(const Params &p, int t, int &mt, int &nt) {
   const int gsize = p.group_m * p.tiles_n;
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (threadIdx.x == 0 && *abort) atomicExch(p.err, MTP_ERR_TIMEOUT);
+  if (threadIdx.x == 0 && *abort) atomicExch(&expired_wait, MTP_ERR_TIMEOUT);
   // x_proj reduction over peer memory: every epilogue store of this CTA is ordered before
   // the flags by the barrier above, then one system fence and release store per rank
   if (p.wire && p.x.ws > 1 && threadIdx.x < (unsigned)p.x.ws && !*abort) {
@@ -492,13 +495,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 }
 
 // ------------------------------------------------------------------ host side
-static int *device_err_word() {
-  static int *w = nullptr;  // one word per process (single device per process)
-  if (!w) {
-    if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) return nullptr;
-    cudaMemset(w, 0, sizeof(int));
+// The kernel's limit of shared memory, which belongs to the current device.
+static int allow_smem() {
+  static std::atomic<uint64_t> done{0};  // a bit for each device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load() & bit) return MTP_OK;
+  if (cudaFuncSetAttribute(gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES_TMA_STORE) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(MTP_ERR_CUDA, "gemm_tc: shared memory");
   }
-  return w;
+  done.fetch_or(bit);
+  return MTP_OK;
 }
 
 }  // namespace tc
@@ -538,8 +547,6 @@ int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda,
   const size_t cb = c_dtype == MTP_F32 ? 4 : 2;
   p.vec_ok = aligned16(C) && ((size_t)ldc * cb) % 16 == 0;
   p.timeout_ns = 2000000000ull;
-  p.err = device_err_word();
-  if (!p.err) return fail(MTP_ERR_CUDA, "could not allocate the GEMM status word");
   CUtensorMap ta, tb, tcm;
   int rc = make_tmap(&ta, A, M, K, lda, BM);
   if (rc) return rc;
@@ -556,11 +563,8 @@ int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda,
     rc = make_tmap_c(&tcm, C, M, N, ldc, c_dtype);
     if (rc) return rc;
   }
-  static bool attr = false;
-  if (!attr) {
-    cudaFuncSetAttribute(gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES_TMA_STORE);
-    attr = true;
-  }
+  rc = allow_smem();
+  if (rc) return rc;
   const int grid = p.num_tiles < num_sms() ? p.num_tiles : num_sms();
   launch_pdl(gemm_tc_kernel, dim3(grid), dim3(NUM_THREADS), p.tma_store ? SMEM_BYTES_TMA_STORE : SMEM_BYTES, stream,
              ta, tb, tcm, p);
@@ -597,19 +601,14 @@ int gemm_tc_xproj_wire(const void *A, const void *B, int M, int N, int K, int ld
   p.vec_ok = 0;
   p.tma_store = 0;
   p.timeout_ns = 2000000000ull;
-  p.err = device_err_word();
-  if (!p.err) return fail(MTP_ERR_CUDA, "could not allocate the GEMM status word");
   CUtensorMap ta, tb, tcm;
   int rc = make_tmap(&ta, A, M, K, lda, BM);
   if (rc) return rc;
   rc = make_tmap(&tb, B, N, K, ldb, p.bn);
   if (rc) return rc;
   memset(&tcm, 0, sizeof(tcm));
-  static bool attr = false;
-  if (!attr) {
-    cudaFuncSetAttribute(gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES_TMA_STORE);
-    attr = true;
-  }
+  rc = allow_smem();
+  if (rc) return rc;
   const int grid = p.num_tiles < num_sms() ? p.num_tiles : num_sms();
   *grid_out = grid;
   // the peer path stages int8 row blocks in the TMA-store staging area (4 x 6 KB)
@@ -619,9 +618,7 @@ int gemm_tc_xproj_wire(const void *A, const void *B, int M, int N, int K, int ld
 }
 
 int gemm_tc_status(int *status) {
-  int *w = tc::device_err_word();
-  if (!w) return fail(MTP_ERR_CUDA, "no status word");
-  if (cudaMemcpy(status, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return fail(MTP_ERR_CUDA, "read status");
+  if (cudaMemcpyFromSymbol(status, tc::expired_wait, sizeof(int)) != cudaSuccess) return fail(MTP_ERR_CUDA, "read status");
   return MTP_OK;
 }
 
