@@ -9,7 +9,7 @@ namespace mtp {
 
 bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda, int ldb);
 int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype,
-            int epi, const void *bias, int bias_dtype, cudaStream_t stream);
+            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired = nullptr);
 
 struct EpiArgs {
   void *C;
@@ -255,6 +255,11 @@ static int launch_gemv(const T *X, int ldx, const T *W, int ldw, int M, int N, i
   return check_launch("gemv");
 }
 
+// Whether mtp_gemm takes the tensor-core kernel, the only one of its kernels that has waits in it.
+bool gemm_on_tensor_cores(const void *A, const void *B, int M, int N, int K, int lda, int ldb, int ab_dtype) {
+  return ab_dtype == MTP_BF16 && M > 16 && gemm_tc_eligible(A, B, M, N, K, lda, ldb);
+}
+
 // Columns [col0, col0 + cols) of C = A x B^T for a B of N_full rows, computed by the
 // kernel (and so with the per-element summation order) that mtp_gemm picks for the whole
 // [M, N_full] product: the vocabulary-parallel lm_head gives the same bits as the
@@ -268,7 +273,7 @@ int gemm_cols_as_full(const void *A, const void *B, void *C, int M, int N_full, 
   const void *Bs = (const char *)B + (size_t)col0 * ldb * es;
   void *Cs = (char *)C + (size_t)col0 * es;
   EpiArgs e{Cs, ldc, dtype, MTP_EPI_STORE, nullptr, 0};
-  if (dtype == MTP_BF16 && M > 16 && gemm_tc_eligible(A, B, M, N_full, K, lda, ldb)) {
+  if (gemm_on_tensor_cores(A, B, M, N_full, K, lda, ldb, dtype)) {
     MTP_REQUIRE(aligned16(Bs), "vocabulary shard of B not 16-byte aligned");
     return gemm_tc(A, Bs, Cs, M, cols, K, lda, ldb, ldc, dtype, MTP_EPI_STORE, nullptr, 0, s);
   }
@@ -306,7 +311,7 @@ int mtp_gemm_ex(const void *A, const void *B, void *C, int M, int N, int K, int 
   if (M == 0) return MTP_OK;
   cudaStream_t s = (cudaStream_t)stream;
   if (algo == MTP_GEMM_AUTO) {
-    if (ab_dtype == MTP_BF16 && M > 16 && gemm_tc_eligible(A, B, M, N, K, lda, ldb)) algo = MTP_GEMM_TCGEN05;
+    if (gemm_on_tensor_cores(A, B, M, N, K, lda, ldb, ab_dtype)) algo = MTP_GEMM_TCGEN05;
     else if (M <= 64) algo = MTP_GEMM_GEMV;
     else algo = MTP_GEMM_SIMT;
   }

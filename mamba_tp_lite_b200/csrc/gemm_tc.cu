@@ -37,6 +37,7 @@ constexpr int SMEM_BYTES_TMA_STORE = SMEM_BYTES + NUM_EPI_WARPS * STAGE_C_BYTES;
 struct Params {
   void *C;
   const void *bias;
+  int *expired;  // set when a wait of this call has expired, or null
   unsigned long long timeout_ns;
   int M, N, K, ldc;
   int c_dtype, epi, bias_dtype;
@@ -484,7 +485,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (threadIdx.x == 0 && *abort) atomicExch(&expired_wait, MTP_ERR_TIMEOUT);
+  if (threadIdx.x == 0 && *abort) {
+    atomicExch(&expired_wait, MTP_ERR_TIMEOUT);
+    if (p.expired) atomicExch(p.expired, MTP_ERR_TIMEOUT);
+  }
   // x_proj reduction over peer memory: every epilogue store of this CTA is ordered before
   // the flags by the barrier above, then one system fence and release store per rank
   if (p.wire && p.x.ws > 1 && threadIdx.x < (unsigned)p.x.ws && !*abort) {
@@ -519,13 +523,14 @@ bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda
 }
 
 int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype,
-            int epi, const void *bias, int bias_dtype, cudaStream_t stream) {
+            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired) {
   using namespace tc;
   MTP_REQUIRE(gemm_tc_eligible(A, B, M, N, K, lda, ldb),
               "tcgen05 GEMM needs 16-byte aligned A/B, K >= 8 and lda, ldb multiples of 8");
   MTP_REQUIRE(c_dtype == MTP_F32 || c_dtype == MTP_BF16, "C must be F32 or BF16");
   MTP_REQUIRE(epi == MTP_EPI_STORE || ((epi == MTP_EPI_BIAS_SOFTPLUS || epi == MTP_EPI_BIAS) && bias), "bad epilogue");
   Params p{};
+  p.expired = expired;
   p.C = C;
   p.bias = bias;
   p.bias_dtype = bias_dtype;

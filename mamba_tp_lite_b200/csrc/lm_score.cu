@@ -22,6 +22,12 @@
 
 namespace mtp {
 bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda, int ldb);
+bool gemm_on_tensor_cores(const void *A, const void *B, int M, int N, int K, int lda, int ldb, int ab_dtype);
+int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype, int epi,
+            const void *bias, int bias_dtype, cudaStream_t stream, int *expired);
+int launch_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld, int V,
+                          const int64_t *targets, float temperature, float *logprob, float *entropy, float *stats, int top_k,
+                          int64_t *top_ids, float *top_logprobs, const int *expired, cudaStream_t stream);
 
 namespace {
 
@@ -364,6 +370,8 @@ int64_t score_block(int64_t rows, int V) {
   return rows < b ? rows : b;
 }
 int64_t score_ld(int V) { return ((int64_t)V + 7) / 8 * 8; }
+// Behind them 16 bytes for a word that says whether a wait of one of the products has expired.
+int64_t score_block_bytes(int64_t rows, int V) { return score_block(rows, V) * score_ld(V) * 4; }
 
 // The fused kernel takes bf16 operands that TMA can read, and gives no alternatives.
 bool score_fused(const void *hidden, int ld_hidden, int rows, int K, const void *weight, int ld_weight, int V, int dtype,
@@ -429,7 +437,7 @@ int mtp_lm_head_logprobs_workspace(const void *hidden, int ld_hidden, int rows, 
   if (score_fused(hidden, ld_hidden, rows, K, weight, ld_weight, V, dtype, top_k))
     *bytes = score_plan(rows, V).bytes;
   else
-    *bytes = score_block(rows, V) * score_ld(V) * 4;
+    *bytes = score_block_bytes(rows, V) + 16;
   return MTP_OK;
 }
 
@@ -453,15 +461,28 @@ int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, con
                         (char *)workspace, (cudaStream_t)stream);
   const int64_t blk = score_block(rows, V), ld = score_ld(V);
   const size_t es = dtype == MTP_F32 ? 4 : 2;
+  cudaStream_t st = (cudaStream_t)stream;
+  int *expired = nullptr;
+  if (gemm_on_tensor_cores(hidden, weight, rows, V, K, ld_hidden, ld_weight, dtype)) {
+    expired = (int *)((char *)workspace + score_block_bytes(rows, V));
+    if (cudaMemsetAsync(expired, 0, sizeof(int), st) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(MTP_ERR_CUDA, "mtp_lm_head_logprobs: could not clear the status word");
+    }
+  }
   for (int64_t r0 = 0; r0 < rows; r0 += blk) {
     const int n = (int)(rows - r0 < blk ? rows - r0 : blk);
-    int rc = mtp_gemm((const char *)hidden + (size_t)r0 * ld_hidden * es, weight, workspace, n, V, K, ld_hidden, ld_weight,
-                      (int)ld, dtype, MTP_F32, MTP_EPI_STORE, nullptr, 0, stream);
+    const char *h = (const char *)hidden + (size_t)r0 * ld_hidden * es;
+    int rc = gemm_on_tensor_cores(h, weight, n, V, K, ld_hidden, ld_weight, dtype)
+                 ? gemm_tc(h, weight, workspace, n, V, K, ld_hidden, ld_weight, (int)ld, MTP_F32, MTP_EPI_STORE, nullptr, 0,
+                           st, expired)
+                 : mtp_gemm(h, weight, workspace, n, V, K, ld_hidden, ld_weight, (int)ld, dtype, MTP_F32, MTP_EPI_STORE,
+                            nullptr, 0, stream);
     if (rc) return rc;
-    rc = mtp_token_logprobs(workspace, MTP_F32, 1, n, 0, ld, V, targets ? targets + r0 : nullptr, temperature,
-                            logprob ? logprob + r0 : nullptr, entropy ? entropy + r0 : nullptr, nullptr, top_k,
-                            top_ids ? top_ids + r0 * top_k : nullptr, top_logprobs ? top_logprobs + r0 * top_k : nullptr,
-                            stream);
+    rc = launch_token_logprobs(workspace, MTP_F32, 1, n, 0, ld, V, targets ? targets + r0 : nullptr, temperature,
+                               logprob ? logprob + r0 : nullptr, entropy ? entropy + r0 : nullptr, nullptr, top_k,
+                               top_ids ? top_ids + r0 * top_k : nullptr,
+                               top_logprobs ? top_logprobs + r0 * top_k : nullptr, expired, st);
     if (rc) return rc;
   }
   return MTP_OK;

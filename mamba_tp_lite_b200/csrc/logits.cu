@@ -577,6 +577,7 @@ struct FwdArgs {
   float inv_t, c2;  // 1 / T, log2 e / T
   int V, shift;
   uint32_t rows;
+  const int *expired;  // of fp32 logits: a word that is set if a wait of the pass that made them has expired, or null
 };
 
 template <typename T, int GW, bool ENT, bool TOP>
@@ -609,7 +610,8 @@ __global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) token_logprobs_kernel(co
   }
   const Stat all = row_join<GW, ENT>(st, sh, a.c2, rank, parts);
   if (!TOP && threadIdx.x >= 32 && GW > 1) return;
-  const RowStats s = finish(all);
+  RowStats s = finish(all);
+  if (std::is_same<T, float>::value && a.expired && *a.expired) s = expired();
   if (rank == 0 && G::tid() == 0) {
     if (a.logprob) {
       const int64_t t = a.targets[r];
@@ -995,6 +997,24 @@ template <typename T, int GW> auto fwd_kernel(bool ent, bool top) {
   MTP_REQUIRE(logits, "null pointer")
 
 }  // namespace
+
+// mtp_token_logprobs of arguments that have been checked.  expired: of fp32 logits, a word in device memory that is not 0 if
+// they are not to be trusted (every log probability and entropy is then NaN); or null.
+int launch_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld, int V,
+                          const int64_t *targets, float temperature, float *logprob, float *entropy, float *stats, int top_k,
+                          int64_t *top_ids, float *top_logprobs, const int *expired, cudaStream_t stream) {
+  const Rows rows = make_rows(outer, inner, ld_outer, ld);
+  const int64_t n = outer * inner;
+  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, false, top_k);
+  const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
+                  (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n, expired};
+  MTP_DISPATCH_LOGITS(dtype, T, {
+    auto kern = sh.warp ? fwd_kernel<T, 1>(entropy, top_k > 0) : fwd_kernel<T, 8>(entropy, top_k > 0);
+    launch_rows(kern, sh, stream, (const T *)logits, rows, a);
+  });
+  return check_launch("token_logprobs");
+}
+
 }  // namespace mtp
 
 using namespace mtp;
@@ -1008,17 +1028,8 @@ int mtp_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inn
   MTP_REQUIRE(!logprob || targets, "logprob needs targets");
   MTP_REQUIRE(top_k >= 0 && top_k <= MAX_TOP && top_k <= V, "top_k must be between 0 and min(V, 128)");
   MTP_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "top_k needs top_ids and top_logprobs");
-  cudaStream_t s = (cudaStream_t)stream;
-  const Rows rows = make_rows(outer, inner, ld_outer, ld);
-  const int64_t n = outer * inner;
-  const Share sh = share_rows(n, V, dtype == MTP_F32 ? 4 : 2, false, top_k);
-  const FwdArgs a{targets, logprob, entropy, stats, top_k, top_ids, top_logprobs, 1.f / temperature,
-                  (float)(1.4426950408889634 / temperature), V, sh.shift, (uint32_t)n};
-  MTP_DISPATCH_LOGITS(dtype, T, {
-    auto kern = sh.warp ? fwd_kernel<T, 1>(entropy, top_k > 0) : fwd_kernel<T, 8>(entropy, top_k > 0);
-    launch_rows(kern, sh, s, (const T *)logits, rows, a);
-  });
-  return check_launch("token_logprobs");
+  return launch_token_logprobs(logits, dtype, outer, inner, ld_outer, ld, V, targets, temperature, logprob, entropy, stats,
+                               top_k, top_ids, top_logprobs, nullptr, (cudaStream_t)stream);
 }
 
 int mtp_token_logprobs_bwd(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld,

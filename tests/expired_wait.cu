@@ -18,3 +18,11 @@ extern "C" int test_score_join(const int64_t *targets, float *part, float *hit, 
              ctas, 1.f, logprob, entropy);
   return check_launch("test_score_join");
 }
+
+// mtp_token_logprobs on fp32 logits [rows][V] that a product whose status word is `expired` has made.
+extern "C" int test_rows_after_a_product(const float *logits, int64_t rows, int V, const int64_t *targets, float *logprob,
+                                         float *entropy, int top_k, int64_t *top_ids, float *top_logprobs,
+                                         const int *expired, void *stream) {
+  return launch_token_logprobs(logits, MTP_F32, 1, rows, 0, V, V, targets, 1.f, logprob, entropy, nullptr, top_k, top_ids,
+                               top_logprobs, expired, (cudaStream_t)stream);
+}

@@ -10,6 +10,7 @@ import torch
 
 from mamba_tp_lite_b200 import _lib as L
 from mamba_tp_lite_b200 import build as B
+from mamba_tp_lite_b200 import logprobs as P
 from tests.gpu_util import dev
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,51 @@ def test_scores_of_a_pass_that_came_through(kernels):
     # ten terms of at most 2^-22 relative error each, a logarithm of at most 2^3: below 1e-5
     assert (lp[ok] - want[ok, 0]).abs().max() < 1e-5 and (ent[ok] + (p * want).sum(-1)[ok]).abs().max() < 1e-5
     assert lp[4] == float("-inf") and ent[4] == 0
+
+
+@pytest.mark.parametrize("rows,v", [(1, 9), (1, 50280), (200, 3001), (2500, 200)])
+@pytest.mark.parametrize("top_k", [0, 5])
+def test_rows_of_a_product_whose_wait_expired_are_nan(kernels, rows, v, top_k):
+    """Scoring in blocks: the product's logits are whatever the workspace held, so nothing that comes from them may look
+    like a value.  With the word clear the results are those of the plain call."""
+    x = (torch.randn(rows, v, generator=torch.Generator().manual_seed(rows)) * 3).to(dev())
+    targets = (torch.arange(rows) % v).to(dev())
+    if rows > 2:
+        targets[1], targets[2] = -1, v
+    want = P.token_logprobs(x, targets, top_k=top_k)
+    fn = kernels.test_rows_after_a_product
+    fn.argtypes = [C.c_void_p, C.c_int64, C.c_int] + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 4
+    for status in (0, 1):
+        word = torch.tensor([status], dtype=torch.int32, device=dev())
+        lp, ent = torch.full((rows,), 7.0, device=dev()), torch.full((rows,), 7.0, device=dev())
+        ids = torch.zeros(rows, max(top_k, 1), dtype=torch.int64, device=dev())
+        tlp = torch.full((rows, max(top_k, 1)), 7.0, device=dev())
+        assert fn(L.ptr(x), rows, v, L.ptr(targets), L.ptr(lp), L.ptr(ent), top_k, L.ptr(ids), L.ptr(tlp), L.ptr(word),
+                  L.stream_ptr()) == 0
+        torch.cuda.synchronize()
+        if status:
+            assert torch.isnan(lp[targets >= 0]).all() and (lp[targets < 0] == 0).all() and torch.isnan(ent).all()
+            assert top_k == 0 or (torch.isnan(tlp).all() and (ids >= 0).all() and (ids < v).all())
+        else:
+            for got, ref in ((lp, want.logprob), (ent, want.entropy)):
+                assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(ref))
+            assert top_k == 0 or (torch.equal(ids, want.top_ids) and torch.equal(tlp, want.top_logprobs))
+
+
+@pytest.mark.parametrize("rows,dtype", [(300, torch.bfloat16), (16, torch.bfloat16), (300, torch.float32)])
+def test_scoring_in_blocks_clears_its_status_word(rows, dtype):
+    """The word lies in the workspace, which holds anything to start with: all ones here."""
+    v, k, top_k = 700, 64, 3
+    g = torch.Generator().manual_seed(rows)
+    h = torch.randn(rows, k, generator=g).to(dtype).to(dev())
+    w = torch.randn(v, k, generator=g).to(dtype).to(dev())
+    args = (L.ptr(h), k, rows, k, L.ptr(w), k, v, L.dtype_code(dtype))
+    need = C.c_int64(0)
+    L.call("mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need))
+    ws = torch.full((need.value,), 255, dtype=torch.uint8, device=dev())
+    ent = torch.empty(rows, device=dev())
+    ids, tlp = torch.empty(rows, top_k, dtype=torch.int64, device=dev()), torch.empty(rows, top_k, device=dev())
+    L.call("mtp_lm_head_logprobs", *args, None, 1.0, None, L.ptr(ent), top_k, L.ptr(ids), L.ptr(tlp), L.ptr(ws), need.value,
+           L.stream_ptr())
+    want = P.lm_head_logprobs(h, w, top_k=top_k)
+    assert torch.equal(ent, want.entropy) and torch.equal(tlp, want.top_logprobs) and torch.isfinite(ent).all()
