@@ -124,13 +124,13 @@ def _grad_like(x: torch.Tensor, inner: int, ld_outer: int, ld: int):
     return buf.as_strided(x.shape, x.stride(), off), ld_outer, ld
 
 
-def _call(x: torch.Tensor, name: str, *args) -> None:
-    """The entry point ``name`` on the current stream of x's device, as the current device."""
+def _call(x: torch.Tensor, name: str, *args, stream: bool = True) -> None:
+    """The entry point ``name`` with x's device as the current one, on its current stream."""
     if x.device.index == torch.cuda.current_device():
-        L.call(name, *args, L.stream_ptr())
+        L.call(name, *args, *((L.stream_ptr(),) if stream else ()))
     else:
         with torch.cuda.device(x.device):
-            L.call(name, *args, L.stream_ptr())
+            L.call(name, *args, *((L.stream_ptr(),) if stream else ()))
 
 
 def _row_like(x: torch.Tensor, ids: torch.Tensor | None) -> torch.Tensor:
@@ -338,7 +338,7 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.
         ids = x.new_empty((*lead, top_k), dtype=torch.int64)
         tlp = torch.empty_like(ids, dtype=torch.float32)
     need = C.c_int64(0)
-    L.call("mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need))
+    _call(x, "mtp_lm_head_logprobs_workspace", *args, top_k, C.byref(need), stream=False)
     work = x.new_empty(need.value, dtype=torch.uint8)
     _call(x, "mtp_lm_head_logprobs", *args, L.ptr(targets), temperature, L.ptr(lp), L.ptr(ent), top_k, L.ptr(ids),
           L.ptr(tlp), work.data_ptr(), need.value)

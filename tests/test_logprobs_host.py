@@ -221,3 +221,43 @@ def test_c_entry_points_refuse_bad_arguments():
     _refused(*lm(dt=L.F16), text="dtype")
     _refused(*lm(tgt=None), text="targets")
     _refused(*lm(k=3), text="top_ids")
+
+
+# ------------------------------------------------------------------ calls, on a library that only records them
+class Recorder:
+    """In place of the library: the calls' names and arguments, and whether the device was set around each."""
+
+    def __init__(self, monkeypatch):
+        self.calls, self.depth = [], 0
+        monkeypatch.setattr(L, "require_cuda", lambda t, what: None)
+        monkeypatch.setattr(L, "stream_ptr", lambda stream=None: 0)
+        monkeypatch.setattr(L, "call", self.call)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)  # a CPU tensor's device has no index: another one
+        monkeypatch.setattr(torch.cuda, "device", self.device)
+
+    def call(self, name, *args):
+        self.calls.append((name, args, self.depth))
+
+    def device(self, dev):
+        rec = self
+
+        class Guard:
+            def __enter__(self):
+                rec.depth += 1
+
+            def __exit__(self, *exc):
+                rec.depth -= 1
+
+        return Guard()
+
+
+def test_every_call_is_made_on_the_device_of_its_tensors(monkeypatch):
+    """The workspace depends on the number of SMs, so its size is asked for on that device too."""
+    rec = Recorder(monkeypatch)
+    x, t = torch.randn(4, 16), torch.zeros(4, dtype=torch.int64)
+    P.token_logprobs(x, t)
+    P.distill_topk_loss(x, t[:, None], torch.zeros(4, 1))
+    P.lm_head_logprobs(x, torch.randn(9, 16), t, top_k=2)
+    assert [c[0] for c in rec.calls] == ["mtp_token_logprobs", "mtp_distill_topk", "mtp_lm_head_logprobs_workspace",
+                                         "mtp_lm_head_logprobs"]
+    assert all(depth == 1 for _, _, depth in rec.calls)
