@@ -5,7 +5,7 @@ taken straight from hidden states and the (tied) lm_head matrix.
 Logits are [..., V] CUDA tensors (float32, bfloat16 or float16) whose rows may be strided
 (``logits[:, :-1]``, a vocabulary whose padding columns are cut off); every statistic and
 per-row result is float32.  ``token_logprobs`` and ``distill_topk_loss`` are
-differentiable with respect to the logits.  Calls run on the current stream of the
+differentiable with respect to the logits (reverse mode, once).  Calls run on the current stream of the
 logits' device, allocate through torch only and keep nothing, so they can be captured in
 a CUDA graph.  The reference has no counterpart; the nearest is the full-vocabulary KL of
 ``mamba_lite/quant_eval.py:48-68``."""
@@ -15,6 +15,7 @@ import ctypes as C
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -38,6 +39,11 @@ class TokenLogprobs(NamedTuple):
 
 
 # ------------------------------------------------------------------ arguments
+def _refuse_tangent(x: torch.Tensor, what: str) -> None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _check_logits(x: torch.Tensor, what: str) -> None:
     L.require_cuda(x, what)
     L.dtype_code(x.dtype)
@@ -45,6 +51,7 @@ def _check_logits(x: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what}: logits need a last dimension of at least one token, got shape {tuple(x.shape)}")
     if x.shape[-1] > MAX_VOCAB:
         raise ValueError(f"{what}: {x.shape[-1]} tokens, at most {MAX_VOCAB}")
+    _refuse_tangent(x, what)
 
 
 def _check_ids(ids: torch.Tensor, shape, device, what: str, name: str) -> torch.Tensor:
@@ -316,6 +323,8 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.
         raise ValueError(f"{what}: weight is on {weight.device}, hidden on {hidden.device}")
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
+    _refuse_tangent(hidden, what)
+    _refuse_tangent(weight, what)
     lead, (v, k) = hidden.shape[:-1], weight.shape
     if targets is not None:
         targets = _check_ids(targets, lead, hidden.device, what, "targets")

@@ -261,3 +261,21 @@ def test_every_call_is_made_on_the_device_of_its_tensors(monkeypatch):
     assert [c[0] for c in rec.calls] == ["mtp_token_logprobs", "mtp_distill_topk", "mtp_lm_head_logprobs_workspace",
                                          "mtp_lm_head_logprobs"]
     assert all(depth == 1 for _, _, depth in rec.calls)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor that does not require a gradient must not come back without its tangent."""
+    rec = Recorder(monkeypatch)
+    t = torch.zeros(4, dtype=torch.int64)
+    w = torch.randn(9, 16)
+    with torch.autograd.forward_ad.dual_level():
+        x = torch.autograd.forward_ad.make_dual(torch.randn(4, 16), torch.ones(4, 16))
+        dw = torch.autograd.forward_ad.make_dual(w, torch.ones(9, 16))
+        for call in (lambda: P.token_logprobs(x, t), lambda: P.distill_topk_loss(x, t[:, None], torch.zeros(4, 1)),
+                     lambda: P.distill_topk_loss_and_grad(x, t[:, None], torch.zeros(4, 1), torch.ones(4)),
+                     lambda: P.lm_head_logprobs(x, w, t), lambda: P.lm_head_logprobs(torch.randn(4, 16), dw, t)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not rec.calls
+        P.token_logprobs(torch.randn(4, 16), t)  # no dual tensor: as ever
+    assert len(rec.calls) == 1
