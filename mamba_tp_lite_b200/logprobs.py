@@ -5,9 +5,9 @@ taken straight from hidden states and the (tied) lm_head matrix.
 Logits are [..., V] CUDA tensors (float32, bfloat16 or float16) whose rows may be strided
 (``logits[:, :-1]``, a vocabulary whose padding columns are cut off); every statistic and
 per-row result is float32.  ``token_logprobs`` and ``distill_topk_loss`` are
-differentiable with respect to the logits (reverse mode, once).  Calls run on the current stream of the
-logits' device, allocate through torch only and keep nothing, so they can be captured in
-a CUDA graph.  The reference has no counterpart; the nearest is the full-vocabulary KL of
+differentiable with respect to the logits (reverse mode, once).  Calls run on the current
+stream of the logits' device, allocate through torch only and keep nothing, so they can be
+captured in a CUDA graph.  The reference has no counterpart; the nearest is the full-vocabulary KL of
 ``mamba_lite/quant_eval.py:48-68``."""
 from __future__ import annotations
 
@@ -171,9 +171,9 @@ def _logprobs_fwd(x, targets, top_k, temperature, entropy, want_stats):
 
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, targets, top_k, temperature):
+    def forward(ctx, x, targets, top_k, temperature, entropy):
         ctx.set_materialize_grads(False)
-        lp, ent, stats, ids, tlp = _logprobs_fwd(x, targets, top_k, temperature, True, True)
+        lp, ent, stats, ids, tlp = _logprobs_fwd(x, targets, top_k, temperature, entropy, True)
         ctx.save_for_backward(x, targets, stats, ent)
         ctx.temperature = temperature
         if top_k:
@@ -185,8 +185,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def backward(ctx, g, h, *_):
         x, targets, stats, ent = ctx.saved_tensors
         if g is None and h is None:
-            return None, None, None, None
-        return _logprobs_bwd(x, targets, ctx.temperature, stats, ent, g, h), None, None, None
+            return None, None, None, None, None
+        return _logprobs_bwd(x, targets, ctx.temperature, stats, ent, g, h), None, None, None, None
 
 
 def _logprobs_bwd(x, targets, temperature, stats, ent, g, h):
@@ -194,8 +194,7 @@ def _logprobs_bwd(x, targets, temperature, stats, ent, g, h):
     x, outer, inner, ld_outer, ld = _row_layout(x)
     grad, g_ld_outer, g_ld = _grad_like(x, inner, ld_outer, ld)
     _call(x, "mtp_token_logprobs_bwd", x.data_ptr(), L.dtype_code(x.dtype), outer, inner, ld_outer, ld, x.shape[-1],
-          L.ptr(targets), temperature, stats.data_ptr(), ent.data_ptr(), L.ptr(g), L.ptr(h), grad.data_ptr(), g_ld_outer,
-          g_ld)
+          L.ptr(targets), temperature, stats.data_ptr(), L.ptr(ent), L.ptr(g), L.ptr(h), grad.data_ptr(), g_ld_outer, g_ld)
     return grad
 
 
@@ -216,8 +215,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     top_k = _check_top_k(top_k, logits.shape[-1], what)
     temperature = _check_temperature(temperature, what)
     if logits.requires_grad and torch.is_grad_enabled():
-        lp, ent, ids, tlp = _TokenLogprobsFn.apply(logits, targets, top_k, temperature)
-        return TokenLogprobs(lp, ent if entropy else None, ids, tlp)
+        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, top_k, temperature, entropy))
     lp, ent, _, ids, tlp = _logprobs_fwd(logits, targets, top_k, temperature, entropy, False)
     return TokenLogprobs(lp, ent, ids, tlp)
 

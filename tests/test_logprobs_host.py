@@ -279,3 +279,16 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
         assert not rec.calls
         P.token_logprobs(torch.randn(4, 16), t)  # no dual tensor: as ever
     assert len(rec.calls) == 1
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_the_entropy_is_computed_only_where_it_is_asked_for(monkeypatch, requires_grad, entropy):
+    rec = Recorder(monkeypatch)
+    x = torch.randn(4, 16, requires_grad=requires_grad)
+    r = P.token_logprobs(x, torch.zeros(4, dtype=torch.int64), entropy=entropy)
+    assert (r.entropy is not None) == entropy
+    if requires_grad:
+        r.logprob.sum().backward()
+    for name, args, _ in rec.calls:
+        assert (args[10] is not None) == entropy  # where the forward call writes it, and the backward call reads it
