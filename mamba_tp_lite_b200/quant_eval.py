@@ -49,10 +49,11 @@ def topk_kl(ids: torch.Tensor, logprobs: torch.Tensor, q: torch.Tensor) -> torch
 @torch.no_grad()
 def sequence_nll(logits: torch.Tensor, input_ids: torch.Tensor) -> torch.Tensor:
     """Per sequence mean negative log likelihood of input_ids [b, l] under logits [b, l, V] (position i
-    predicts token i + 1; negative ids are padding and do not count); exp of it is the perplexity."""
+    predicts token i + 1; negative ids are padding and do not count); exp of it is the perplexity.  A
+    sequence with no token to predict has 0."""
     targets = input_ids[:, 1:]
     logprob = token_logprobs(logits[:, :-1], targets, entropy=False).logprob
-    return -logprob.sum(dim=1) / (targets >= 0).sum(dim=1)
+    return -logprob.sum(dim=1) / (targets >= 0).sum(dim=1).clamp(min=1)
 
 
 def summarize(per_sequence: dict) -> dict:

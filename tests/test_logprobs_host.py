@@ -292,3 +292,18 @@ def test_the_entropy_is_computed_only_where_it_is_asked_for(monkeypatch, require
         r.logprob.sum().backward()
     for name, args, _ in rec.calls:
         assert (args[10] is not None) == entropy  # where the forward call writes it, and the backward call reads it
+
+
+def test_sequence_nll_of_padded_sequences(monkeypatch):
+    """Partly padded, padded after the first token, and sequences of one token: nothing to predict counts 0."""
+    monkeypatch.setattr(quant_eval, "token_logprobs", lambda x, t, entropy: P.TokenLogprobs(
+        torch.from_numpy(R.token_logprob(x.double().numpy().reshape(-1, x.shape[-1]), t.numpy().reshape(-1))).view(t.shape),
+        None, None, None))
+    g = torch.Generator().manual_seed(0)
+    logits = torch.randn(3, 5, 11, generator=g, dtype=torch.float64)
+    ids = torch.tensor([[1, 2, 3, 4, 5], [6, 7, -1, -1, -1], [8, -1, -1, -1, -1]])
+    lp = torch.log_softmax(logits, -1)
+    want = [-(lp[0, 0, 2] + lp[0, 1, 3] + lp[0, 2, 4] + lp[0, 3, 5]) / 4, -lp[1, 0, 7], torch.tensor(0.0)]
+    got = quant_eval.sequence_nll(logits, ids)
+    np.testing.assert_allclose(got.numpy(), torch.stack([w.double() for w in want]).numpy(), atol=1e-12)
+    assert (quant_eval.sequence_nll(logits[:, :1], ids[:, :1]) == 0).all()
