@@ -829,7 +829,7 @@ __device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a,
   for (int j = 0; j < PER; ++j) {
     const int i = lane + 32 * j;
     const float q = s != 0.f ? e[j] / s : 0.f;
-    bad = bad || q != q || (q != 0.f && id[j] >= a.V);
+    bad = bad || q != q || (t[j] != -INFINITY && id[j] >= a.V);
     if (q != 0.f) neg += q * ((t[j] - m) * a.inv_t - ls);
     te.id[i] = q != 0.f && id[j] < a.V ? (int)id[j] : -1;
     te.q[i] = q;
