@@ -631,14 +631,19 @@ __global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) token_logprobs_kernel(co
 // ----------------------------------------------------------------- gradients
 // out_j = p_j (a + b y_j) with p_j = 2^y_j, y = log2 p; the element `hit` gets `extra` on top.  ENT: b is not 0.
 // A p below 2^-126 still counts where its factor is large: 2^(y + 32) is taken, which is flushed to zero only where p
-// is below the smallest subnormal, and 2^-32 goes into the factor.
+// is below the smallest subnormal, and 2^-32 goes into the factor.  Where the factor is below 2^-29 its product with such
+// a p vanishes anyway, and 2^-32 might push the factor itself out of range: there the lift is 0.
 template <bool ENT> struct Dense {
-  float m, l2, c2;  // largest logit, log2 S, log2 e / T
-  float a, b;       // times 2^-32
-  static constexpr float LIFT = 32.f;
+  float m, l2, c2;  // largest logit, log2 S (less the lift, if not ENT), log2 e / T
+  float a, b, lift;  // a and b times 2^-lift
   __device__ __forceinline__ Dense(float m_, float log_s, float c2_, float a_, float b_)
-      : m(m_), l2(log_s * LOG2E), c2(c2_), a(a_ * 0x1p-32f), b(b_ * 0x1p-32f) {
-    if (!ENT) l2 -= LIFT;
+      : m(m_), l2(log_s * LOG2E), c2(c2_), a(a_), b(b_), lift(0.f) {
+    if (!(fmaxf(fabsf(a), ENT ? -FLOOR_Y * fabsf(b) : 0.f) < 0x1p-30f)) {
+      lift = 32.f;
+      a *= 0x1p-32f;
+      b *= 0x1p-32f;
+    }
+    if (!ENT) l2 -= lift;
   }
   __device__ __forceinline__ F2 two(F2 x) const {
     const F2 y = fma2(add2(x, f2(-m, -m)), f2(c2, c2), f2(-l2, -l2));
@@ -649,7 +654,7 @@ template <bool ENT> struct Dense {
     } else {
       un2(y, y0, y1);
       const F2 f = fma2(f2(fmaxf(y0, FLOOR_Y), fmaxf(y1, FLOOR_Y)), f2(b, b), f2(a, a));
-      un2(add2(y, f2(LIFT, LIFT)), y0, y1);
+      un2(add2(y, f2(lift, lift)), y0, y1);
       return mul2(f2(ex2(y0), ex2(y1)), f);
     }
   }

@@ -4,7 +4,7 @@ import torch
 
 from mamba_tp_lite_b200 import logprobs as P
 from tests.gpu_util import dev
-from tests.test_gpu_logprobs import F32, make
+from tests.test_gpu_logprobs import BF, F32, check_distill, check_grad, make, targets_for, teacher_for
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +21,30 @@ def test_a_used_teacher_entry_past_the_vocabulary_is_reported_however_unlikely()
         if grad is not None:
             assert torch.isnan(grad).all(1).tolist() == [True, False, False, True]
             assert torch.isfinite(grad[1:3]).all()
+
+
+SCALES = [2.0 ** -115, 2.0 ** -100, 2.0 ** -60, 2.0 ** -31, 2.0 ** -29, 2.0 ** 60]
+
+
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,v", [(5, 257), (2500, 130)])
+def test_gradients_of_small_and_large_upstream_gradients(scale, dtype, rows, v):
+    """The gradient is as good relative to a small factor as to a large one."""
+    x = make(rows, v, dtype, 16)
+    t = targets_for(rows, v)
+    g = torch.linspace(0.5, 1.5, rows, device=dev()) * scale
+    h = torch.linspace(-1, 0.9, rows, device=dev()) * scale
+    zero = torch.zeros_like(g)
+    for gg, hh in ((g, h), (g, zero), (zero, h), (g, h / scale), (g / scale, h)):
+        leaf = x.detach().requires_grad_()
+        r = P.token_logprobs(leaf, t)
+        outs = [(r.logprob, gg)] + ([] if hh is zero else [(r.entropy, hh)])
+        (grad,) = torch.autograd.grad([o for o, _ in outs], [leaf], [u for _, u in outs])
+        check_grad(x, t, gg, hh, grad)
+    ids, vals = teacher_for(x, 20)
+    loss, grad = P.distill_topk_loss_and_grad(x, ids, vals, g)
+    check_distill(x, ids, vals, g, loss, grad)
+    leaf = x.detach().requires_grad_()
+    (grad,) = torch.autograd.grad([P.distill_topk_loss(leaf, ids, vals)], [leaf], [g])
+    check_distill(x, ids, vals, g, loss, grad)
