@@ -927,8 +927,7 @@ __global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) distill_kernel(const T *
           qs += te.q[j];
         }
       }
-      const float lp = log_prob(te.x[i], st.m, st.log_s, a.inv_t);
-      if (first) stf(out + id, w * (ex2(lp * LOG2E) - qs));
+      if (first) stf(out + id, d.one(te.x[i]) - w * qs);
     }
   }
 }

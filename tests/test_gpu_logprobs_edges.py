@@ -48,3 +48,18 @@ def test_gradients_of_small_and_large_upstream_gradients(scale, dtype, rows, v):
     leaf = x.detach().requires_grad_()
     (grad,) = torch.autograd.grad([P.distill_topk_loss(leaf, ids, vals)], [leaf], [g])
     check_distill(x, ids, vals, g, loss, grad)
+
+
+@pytest.mark.parametrize("rows", [3, 2500])
+def test_a_teacher_token_that_the_student_all_but_excludes(rows):
+    """q = e^-87 against p = e^-90, below the smallest normal number, under a large weight: p is a twentieth of q."""
+    x = torch.full((rows, 80), -80.0, device=dev())
+    x[:, 5], x[:, 7] = -90.0, 0.0
+    ids = torch.tensor([7, 5], device=dev()).expand(rows, 2)
+    vals = torch.tensor([0.0, -87.0], device=dev()).expand(rows, 2)
+    w = torch.linspace(0.5, 1.5, rows, device=dev()) * 2.0 ** 100
+    loss, grad = P.distill_topk_loss_and_grad(x, ids, vals, w)
+    check_distill(x, ids, vals, w, loss, grad)
+    leaf = x.detach().requires_grad_()
+    (grad,) = torch.autograd.grad([P.distill_topk_loss(leaf, ids, vals)], [leaf], [w])
+    check_distill(x, ids, vals, w, loss, grad)
