@@ -363,13 +363,14 @@ ScorePlan score_plan(int rows, int V) {
   return p;
 }
 
-// Rows of fp32 logits that one pass of the unfused form holds: about 256 MB of them.
+// Rows of fp32 logits that one pass of the unfused form holds: about 256 MB of them, and no more than the grid of the
+// CUDA-core product has places for (65535 tiles of 64 rows).
+int64_t score_ld(int V) { return ((int64_t)V + 7) / 8 * 8; }
 int64_t score_block(int64_t rows, int V) {
-  int64_t b = (256ll << 20) / (4ll * V);
-  b = b < 128 ? 128 : b / 128 * 128;
+  int64_t b = (256ll << 20) / (4 * score_ld(V)) / 128 * 128;
+  b = b < 128 ? 128 : b > 65535 / 2 * 128 ? 65535 / 2 * 128 : b;
   return rows < b ? rows : b;
 }
-int64_t score_ld(int V) { return ((int64_t)V + 7) / 8 * 8; }
 // Behind them 16 bytes for a word that says whether a wait of one of the products has expired.
 int64_t score_block_bytes(int64_t rows, int V) { return score_block(rows, V) * score_ld(V) * 4; }
 
