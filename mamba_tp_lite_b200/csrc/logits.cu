@@ -202,38 +202,46 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, u
   for (int p = 0; p < RING; ++p) fetch_pair(sl, mine, p);
   const int n = sl.n;
   const T *src = sl.mine() + (int64_t)2 * RING * sl.STEP;
-  int slot = 0, in_chunk = 0;
+  int slot = 0, in_chunk = 0, i = 0;
   bool masked = false;
   float chunk = -INFINITY;
-  for (int i = 0; i < n; i += 2) {
-    copy_wait<RING - 1>();
-    uint4 *at = mine + slot * 2 * NT;
-    float2 mx;
-    if (i + 1 == n) mx = accumulate_vec<T, ENT>(st, at[0], c2);
-    else if (ENT && masked) mx = accumulate_pair<T, ENT, true>(st, at[0], at[NT], c2, masked);
-    else mx = accumulate_pair<T, ENT, false>(st, at[0], at[NT], c2, masked);
-    if constexpr (TOP) {
-      if (cm.per == 1) {
-        cm.at[0] = upper<T>(mx.x);
-        if (i + 1 < n) cm.at[CTA] = upper<T>(mx.y);
-        cm.at += 2 * CTA;
-      } else {
-        chunk = max3(chunk, mx.x, mx.y);
-        in_chunk += 2;
-        if (in_chunk == cm.per) {
-          *cm.at = upper<T>(chunk);
-          cm.at += CTA;
-          chunk = -INFINITY;
-          in_chunk = 0;
+  // A thread leaves the first loop at its first masked logit: 777 rows of 50277 fp16 logits, a tenth of them masked, seven
+  // alternatives 29.5 us so, 34 with every group that holds one summed twice.  One loop with both forms in it took 29.0, but
+  // 654 us instead of 643 for 32 x 1023 rows of 50280 bf16 logits, of which none is masked.
+  auto pairs = [&](auto after) {
+    constexpr bool MASKED = decltype(after)::value;
+    while (i < n) {
+      copy_wait<RING - 1>();
+      uint4 *at = mine + slot * 2 * NT;
+      const float2 mx = i + 1 < n ? accumulate_pair<T, ENT, MASKED>(st, at[0], at[NT], c2, masked)
+                                  : accumulate_vec<T, ENT>(st, at[0], c2);
+      if constexpr (TOP) {
+        if (cm.per == 1) {
+          cm.at[0] = upper<T>(mx.x);
+          if (i + 1 < n) cm.at[CTA] = upper<T>(mx.y);
+          cm.at += 2 * CTA;
+        } else {
+          chunk = max3(chunk, mx.x, mx.y);
+          in_chunk += 2;
+          if (in_chunk == cm.per) {
+            *cm.at = upper<T>(chunk);
+            cm.at += CTA;
+            chunk = -INFINITY;
+            in_chunk = 0;
+          }
         }
       }
+      if (i + 2 * RING < n) copy16(at, src);
+      if (i + 2 * RING + 1 < n) copy16(at + NT, src + sl.STEP);
+      copy_commit();
+      src += 2 * sl.STEP;
+      slot = (slot + 1) & (RING - 1);
+      i += 2;
+      if (ENT && !MASKED && masked) break;
     }
-    if (i + 2 * RING < n) copy16(at, src);
-    if (i + 2 * RING + 1 < n) copy16(at + NT, src + sl.STEP);
-    copy_commit();
-    src += 2 * sl.STEP;
-    slot = (slot + 1) & (RING - 1);
-  }
+  };
+  pairs(std::false_type{});
+  if constexpr (ENT) pairs(std::true_type{});  // from the first masked logit on
   if constexpr (TOP) {
     if (in_chunk) *cm.at = upper<T>(chunk);
   }

@@ -4,7 +4,7 @@ import torch
 
 from mamba_tp_lite_b200 import logprobs as P
 from tests.gpu_util import dev
-from tests.test_gpu_logprobs import BF, F32, check_distill, check_grad, make, targets_for, teacher_for
+from tests.test_gpu_logprobs import BF, F16, F32, check_distill, check_forward, check_grad, make, targets_for, teacher_for
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,18 @@ def test_a_teacher_token_that_the_student_all_but_excludes(rows):
     leaf = x.detach().requires_grad_()
     (grad,) = torch.autograd.grad([P.distill_topk_loss(leaf, ids, vals)], [leaf], [w])
     check_distill(x, ids, vals, w, loss, grad)
+
+
+@pytest.mark.parametrize("rows,v", [(6, 50281), (3, 3001), (2500, 1000), (2500, 3001)])
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("which", ["few", "from_the_middle", "up_to_the_middle", "one_lane"])
+def test_masked_logits_that_begin_anywhere_in_a_row(rows, v, dtype, which):
+    """The threads of a warp meet their first masked logit at different times, or never."""
+    x = make(rows, v, dtype, 17)
+    j = torch.arange(v, device=dev())
+    banned = {"few": j % 997 == 5, "from_the_middle": j > v // 2, "up_to_the_middle": j < v // 2,
+              "one_lane": (j // 8) % 32 == 3}[which]
+    x[:, banned] = float("-inf")
+    t = targets_for(rows, v)
+    for k in (0, 5):
+        check_forward(x, t, k)
