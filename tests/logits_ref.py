@@ -132,3 +132,44 @@ def grad_bound(x, grad, mag, eps, tiny, temperature=1.0):
     # an exponential whose argument is lp (|lp| <= 110 where it does not vanish): relative 2 u |lp| + 2^-22
     rel = b + 2.0 ** -22 + 4 * U * (np.minimum(lp, 110) + 2) + entropy_bound(x, temperature)[:, None]
     return mag * rel + np.abs(grad) * eps / 2 + tiny
+
+
+# ------------------------------------------------------------------ hidden states whose products add up exactly
+SUM_GRAIN, SUM_LIMIT = 2.0 ** -11, 2.0 ** 13  # every sum of up to 1024 products is a multiple of one below the other
+
+
+def exact_score_inputs(rows, v, k, seed=0):
+    """(hidden [rows, K], weight [V, K]) in bf16 values, products of which add up without rounding in 24 bits over any 1024
+    (any order) but not over more.  Of 16 positions 15 give 8.5, 960 of them 8160; one gives an odd multiple of 2^-11 for
+    an even token and an even one for an odd token, 64 of them less than 4.  A sum that goes past 2^13 in 24 bits loses an
+    odd multiple's last bit at every step and an even multiple's never, so that the tokens drift apart."""
+    g = np.random.default_rng(seed)
+    h, w = np.ones((rows, k)), np.full((v, k), 8.5)
+    fine = np.arange(k) % 16 == 7
+    h[:, fine] = np.where(g.random((rows, fine.sum())) < 0.5, -1, 1) * 2.0 ** -5
+    w[:, fine] = (2 * g.integers(0, 63, (v, fine.sum())) + (np.arange(v) % 2 == 0)[:, None]) * 2.0 ** -6
+    return h, w
+
+
+def score_accumulators(k):
+    """Positions that one accumulator sums: 64-wide blocks of K in equal numbers, 16 blocks at most."""
+    blocks = -(-k // 64)
+    splits = -(-blocks // 16)
+    return 64 * -(-blocks // splits)
+
+
+def exact_score_bounds(h, w, targets, per_acc=None):
+    """(logits, logprob, its bound, entropy, its bound).  The accumulators (per_acc positions each) are exact; each is
+    added to the ones before it with one rounding, half a step of the sum.  dz is the sum of those.  A log
+    probability moves by at most 2 dz, an entropy by dz sum p |log p + H| to first order, of which 2 dz covers the rest
+    (dz < 2^-8)."""
+    x = h @ w.T
+    dz = np.zeros(len(h))
+    if per_acc:
+        for end in range(2 * per_acc, w.shape[1] + per_acc, per_acc):
+            part = np.abs(h[:, :end] @ w[:, :end].T).max(-1)
+            dz += 2.0 ** np.floor(np.log2(part)) * U
+    lp, ent = log_probs(x), entropy(x)
+    want = token_logprob(x, targets)
+    drift = (np.exp(lp) * np.abs(lp + ent[:, None])).sum(-1)
+    return x, want, logprob_bound(x, want) + 2 * dz, ent, entropy_bound(x) + 2 * dz * drift

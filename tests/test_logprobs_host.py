@@ -307,3 +307,42 @@ def test_sequence_nll_of_padded_sequences(monkeypatch):
     got = quant_eval.sequence_nll(logits, ids)
     np.testing.assert_allclose(got.numpy(), torch.stack([w.double() for w in want]).numpy(), atol=1e-12)
     assert (quant_eval.sequence_nll(logits[:, :1], ids[:, :1]) == 0).all()
+
+
+# ------------------------------------------------------------------ whether a test of scoring can fail
+def _truncated_sum(h, w, step=16):
+    """h . w^T in 24 bits, cut off after every `step` products."""
+    acc = np.zeros((h.shape[0], w.shape[0]))
+    for k in range(0, h.shape[1], step):
+        acc = acc + h[:, k:k + step] @ w[:, k:k + step].T
+        ulp = 2.0 ** (np.floor(np.log2(np.abs(acc))) - 23)
+        acc = np.trunc(acc / ulp) * ulp
+    return acc
+
+
+@pytest.mark.parametrize("rows,v,k", [(6, 777, 1024), (5, 2049, 2048), (4, 1001, 1100), (4, 1001, 2560), (3, 4001, 3000)])
+def test_exact_hidden_states_show_a_loss_of_precision(rows, v, k):
+    """The mistakes that scoring must not make, made here: each goes past the bounds that the GPU is held to."""
+    h, w = R.exact_score_inputs(rows, v, k, k)
+    for a in (h, w):
+        assert torch.equal(torch.from_numpy(a).bfloat16().double(), torch.from_numpy(a))
+    n = R.score_accumulators(k)
+    assert n <= 1024
+    for k0 in range(0, k, n):  # exact in every accumulator: so says the same sum cut off at every step
+        part = h[:, k0:k0 + n] @ w[:, k0:k0 + n].T
+        assert (part < R.SUM_LIMIT).all() and (part % R.SUM_GRAIN == 0).all()
+        assert (_truncated_sum(h[:, k0:k0 + n], w[:, k0:k0 + n]) == part).all()
+    t = np.arange(rows) % v
+    x, lp, lp_bound, ent, ent_bound = R.exact_score_bounds(h, w, t, n if k > n else None)
+
+    def seen(y):
+        return (np.abs(R.token_logprob(y, t) - lp) > lp_bound).all()
+
+    assert not seen(x)
+    assert seen(torch.from_numpy(x).bfloat16().double().numpy())  # logits in bf16
+    gone = x.copy()
+    gone[:, 512:528] = -np.inf
+    assert seen(gone)                                              # sixteen tokens passed over
+    if k > n:
+        assert seen(_truncated_sum(h, w))                          # one accumulator for all of K
+        assert seen(x - h[:, n:n + 16] @ w[:, n:n + 16].T)         # sixteen positions of K passed over
