@@ -205,12 +205,14 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, u
   int slot = 0, in_chunk = 0, i = 0;
   bool masked = false;
   float chunk = -INFINITY;
-  // A thread leaves the first loop at its first masked logit: 777 rows of 50277 fp16 logits, a tenth of them masked, seven
-  // alternatives 29.5 us so, 34 with every group that holds one summed twice.  One loop with both forms in it took 29.0, but
-  // 654 us instead of 643 for 32 x 1023 rows of 50280 bf16 logits, of which none is masked.
-  auto pairs = [&](auto after) {
+  // Masked logits are many or none, as a rule, so a warp looks at its first pairs and then goes through one of two loops;
+  // a thread that meets its first masked logit later changes over by itself.  777 rows of 50277 fp16 logits, a tenth of them
+  // masked, seven alternatives 25.6 us; 29.5 with every thread changing over by itself, 29.0 with both forms in one loop, 34
+  // with every group that holds a masked logit summed twice.  32 x 1023 unmasked rows of 50280 bf16 logits 662 us; 658, 668
+  // and 654 (in another run).
+  auto pairs = [&](auto after, int end) {
     constexpr bool MASKED = decltype(after)::value;
-    while (i < n) {
+    while (i < end) {
       copy_wait<RING - 1>();
       uint4 *at = mine + slot * 2 * NT;
       const float2 mx = i + 1 < n ? accumulate_pair<T, ENT, MASKED>(st, at[0], at[NT], c2, masked)
@@ -240,8 +242,14 @@ __device__ __forceinline__ Stat thread_stats(const Slice<T, GW> &sl, float c2, u
       if (ENT && !MASKED && masked) break;
     }
   };
-  pairs(std::false_type{});
-  if constexpr (ENT) pairs(std::true_type{});  // from the first masked logit on
+  if constexpr (ENT) {
+    pairs(std::false_type{}, min(n, 2));
+    masked = __any_sync(0xffffffffu, masked);
+    if (!masked) pairs(std::false_type{}, n);
+    pairs(std::true_type{}, n);
+  } else {
+    pairs(std::false_type{}, n);
+  }
   if constexpr (TOP) {
     if (in_chunk) *cm.at = upper<T>(chunk);
   }
@@ -572,8 +580,8 @@ __device__ __forceinline__ void top_alternatives(const Slice<T, GW> &sl, Stat st
 
 // ----------------------------------------------------------------- log probabilities
 // Bound by the exponentials at the clocks of a long run under the power cap (16 per cycle and SM, 1.06 a logit: 480 us of
-// the 677 us that 32 x 1023 rows of 50280 bf16 logits take at 1.53 GHz, their issue slots 75% used), by HBM otherwise: the
-// same rows 559 us in isolation, 5.89 TB/s or 0.92 of the measured copy rate.  fp32 rows are HBM-bound: 4096 of 50280
+// the 655 us that 32 x 1023 rows of 50280 bf16 logits take at 1.53 GHz, their issue slots 75% used), by HBM otherwise: the
+// same rows 568 us in isolation, 5.80 TB/s or 0.90 of the measured copy rate.  fp32 rows are HBM-bound: 4096 of 50280
 // 139 us, 0.92.  A ring of 32 KB per CTA and five CTAs per SM were taken: 6 CTAs (spills) 575 us, a ring twice as deep
 // (three CTAs) 11% slower.  Alternatives cost a row its joins and the second look: 2048 fp32 rows 98 us with 64 of them.
 struct FwdArgs {
@@ -863,8 +871,9 @@ __device__ __forceinline__ void read_teacher(const T *row, const DistillArgs &a,
 // The teacher is read by one warp while the row streams in, and its elements of the gradient are written a second time
 // by the CTA that wrote the row, after a barrier, so that the pass over the row does not look for them.
 // Loss and gradient of 8192 rows of 50280 bf16 logits with 64 entries: 324 us against 256 us of HBM traffic (the second
-// reading comes from shared memory and L2), two exponentials a logit, bound by issue slots and by the row's chain of
-// barriers.  Keeping the whole slice in shared memory instead took clusters of two and 355 us.
+// reading comes from shared memory and L2).  Bound by latency: nothing is loaded between a row's two passes (60% of the
+// issue slots used, a warp's stalls are barriers and loads).  Keeping the whole slice in shared memory instead took
+// clusters of two and 355 us.
 template <typename T, int GW, bool GRAD>
 __global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) distill_kernel(const T *__restrict__ logits, Rows rows, DistillArgs a,
                                                          T *__restrict__ grad, Rows grows) {
@@ -942,7 +951,9 @@ __global__ void __launch_bounds__(CTA, GW == 1 ? 4 : 5) distill_kernel(const T *
 
 // How rows are shared out.  A warp takes a row of up to 16 KB where there are rows enough for 16 warps per SM: a CTA's
 // fixed cost a row (its barriers and joins) is several times the work of such a row.  60000 rows of 1000 bf16 logits, loss
-// and gradient: 188 us by warps, 853 us by CTAs.  Else 2^shift CTAs share a row:
+// and gradient with 64 entries: 126 us by warps (189 where tokens are given more than once), 474 by CTAs, against 37 of HBM
+// traffic: the first load, the join and the stores of a row are a chain that only the SM's other warps overlap.  Else 2^shift
+// CTAs share a row:
 //   - until there is one for every SM, each with no fewer vectors than threads: a cluster adds about 2 us of barriers, so
 //     more pays off only where SMs idle (64 rows of 50280 bf16 logits: 10.3 us by 4 CTAs, 12.3 by one; 300 rows: 18.4 by
 //     2, 16.6 by one);
@@ -958,7 +969,7 @@ struct Share {
 inline Share share_rows(int64_t rows, int V, int elem, bool twice, int top_k = 0) {
   const int64_t sms = num_sms(), bytes = (int64_t)V * elem;
   // for its alternatives a warp needs clearly more vectors than alternatives (60000 rows of 1000 bf16 logits, 125 vectors,
-  // 128 alternatives: 1043 us by CTAs, 1948 by warps; 64 alternatives 262 by warps, 574 by CTAs)
+  // 128 alternatives: 1245 us by CTAs, 1671 by warps; 64 alternatives 264 by warps, 569 by CTAs, against 26 of HBM traffic)
   if (bytes <= WARP_ROW && rows >= 16 * sms && bytes / 16 >= top_k + top_k / 4)
     return {true, 0, (unsigned)((rows + Group<1>::ROWS - 1) / Group<1>::ROWS)};
   int shift = 0;

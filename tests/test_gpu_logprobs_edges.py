@@ -78,3 +78,13 @@ def test_masked_logits_that_begin_anywhere_in_a_row(rows, v, dtype, which):
     t = targets_for(rows, v)
     for k in (0, 5):
         check_forward(x, t, k)
+
+
+@pytest.mark.parametrize("rows,v", [(300, 50281), (2500, 1003)])
+def test_masked_rows_give_the_same_bits_every_time(rows, v):
+    x = make(rows, v, BF, 18)
+    x[torch.rand(rows, v, generator=torch.Generator().manual_seed(1)).to(dev()) < 0.003] = float("-inf")
+    t = targets_for(rows, v)
+    want = P.token_logprobs(x, t, top_k=4)
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(P.token_logprobs(x, t, top_k=4), want))
