@@ -363,8 +363,10 @@ int mtp_distill_topk_grad(const void *logits, int dtype, int64_t outer, int64_t 
  * (hidden and weight of dtype MTP_F32 or MTP_BF16), never held as a whole, then logprob, entropy
  * and the top_k alternatives as mtp_token_logprobs.  bf16 operands on 16-byte boundaries with
  * top_k 0 take one tensor-core pass that keeps no logits at all; everything else goes through
- * blocks of about 256 MB of fp32 logits in the workspace.  Where a device wait of either form
- * expires, every log probability (0 for no token excepted) and entropy is NaN.
+ * blocks of about 256 MB of fp32 logits in the workspace, of which the tensor core sums K as a
+ * whole (a logit is up to 8.6e-10 K of itself too small; the pass sums at most 1024 at a time).
+ * Where a device wait of either form expires, every log probability (0 for no token excepted)
+ * and entropy is NaN.
  * workspace: 16-byte aligned device memory of at least the size that
  * mtp_lm_head_logprobs_workspace gives for the same arguments, with nothing in it to start with;
  * calls that overlap on the GPU need one each. */

@@ -10,8 +10,8 @@
 //              tile goes to the workspace, the given token's logit beside it.
 // A second kernel joins a row's tiles.  K is split because the tensor core truncates at every step of its sum: measured
 // against 64 bits, a sum over K is 8.6e-10 K of its value too small (1.8e-6 at K = 2048, which an entropy shows).  Every
-// further split costs 600 cycles a tile, in which the accumulator is read (8192 rows of K = 2048, V = 50280: 1060 us
-// unsplit, 1100 with two splits, 1180 with four, 1364 with eight), so that one sums up to 1024.
+// further split costs a tile 300 to 900 cycles, in which the accumulator is read (8192 rows of K = 2048, V = 50280: 1107 us
+// unsplit, 1124 with two splits, 1186 with four, 1384 with eight), so that one sums up to 1024.
 // The epilogue works on a tile while the tensor core fills the next one's accumulators.
 // Every mbarrier wait is bounded; a CTA that gives up marks its status slot, frees its TMEM and returns, and the second
 // kernel then writes NaN.
@@ -339,8 +339,8 @@ struct ScorePlan {
 };
 
 // Tile width: the multiple of 16 up to 256 that gives the shortest longest CTA, a tile costing its width and 48 columns'
-// time on top.  Measured at V = 50280: 64 rows, K = 768 (one row block) 40.2 us at the chosen 176 against 42.2 at 256;
-// 8192 rows, K = 2048 1073 us at the chosen 256 against 1094 at 240 and 1461 at 192.
+// time on top.  Measured at V = 50280, both kernels, L2 cold: 64 rows, K = 768 (one row block) 32.0 us at the chosen 176
+// against 34.8 at 256; 8192 rows, K = 2048 1124 us at the chosen 256 against 1138 at 240 and 1290 at 192.
 ScorePlan score_plan(int rows, int V) {
   ScorePlan p;
   const int sms = num_sms();

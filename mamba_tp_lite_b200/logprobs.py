@@ -7,8 +7,9 @@ Logits are [..., V] CUDA tensors (float32, bfloat16 or float16) whose rows may b
 per-row result is float32.  ``token_logprobs`` and ``distill_topk_loss`` are
 differentiable with respect to the logits (reverse mode, once).  Calls run on the current
 stream of the logits' device, allocate through torch only and keep nothing, so they can be
-captured in a CUDA graph.  The reference has no counterpart; the nearest is the full-vocabulary KL of
-``mamba_lite/quant_eval.py:48-68``."""
+captured in a CUDA graph.  (As ever in torch, a captured backward pass wants no graph of an
+uncaptured pass over the same leaf alive.)  The reference has no counterpart; the nearest is the
+full-vocabulary KL of ``mamba_lite/quant_eval.py:48-68``."""
 from __future__ import annotations
 
 import ctypes as C
@@ -309,7 +310,12 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.
                      temperature: float = 1.0, entropy: bool = True) -> TokenLogprobs:
     """``token_logprobs`` of the logits hidden [..., K] @ weight [V, K]^T, accumulated in fp32 and never
     held as a whole: [rows, V] is neither rounded to the model's dtype nor written.  float32 or
-    bfloat16, both of one dtype.  No gradient: call it under ``torch.no_grad()``."""
+    bfloat16, both of one dtype.  No gradient: call it under ``torch.no_grad()``.
+
+    bfloat16 on 16-byte boundaries takes one tensor-core pass without ``top_k``.  With it (and
+    otherwise) the logits go through blocks of about 256 MB in fp32, of which the tensor core sums K as
+    a whole, truncating (a logit is up to 8.6e-10 K of itself too small), where the pass sums at most
+    1024 at a time: for wider models the two differ in the last digits."""
     what = "lm_head_logprobs"
     L.require_cuda(hidden, what)
     if hidden.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != hidden.dtype:
