@@ -13,12 +13,12 @@
  * per-tensor-scale mode), and the state scratch of the sequence-chunked scan;
  * the last two grow to the largest size used.  A call that is to be recorded in a
  * CUDA graph therefore needs one call of the same kind before the capture (the
- * package's GraphedStepper runs warm-up steps first); mtp_gemm and the operators on
- * logits do not.  No torch types appear here; the Python package binds this header with
+ * package's GraphedStepper runs warm-up steps first); mtp_gemm, the operators on
+ * logits and those of the 8-bit linear path do not.  No torch types appear here; the Python package binds this header with
  * ctypes.
  *
  * Devices: the library serves one device per process (one rank per process), except
- * mtp_gemm and the operators on logits (any device), the allocation-free reduction scratch, the
+ * mtp_gemm, the operators on logits and the 8-bit linear path (any device), the allocation-free reduction scratch, the
  * reductions' row scratch and the chunked scan's state scratch, which are kept per device; the
  * status word of the fused scan is per process.
  *
@@ -376,6 +376,39 @@ int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, con
                          int dtype, const int64_t *targets, float temperature, float *logprob, float *entropy,
                          int top_k, int64_t *top_ids, float *top_logprobs, void *workspace, int64_t workspace_bytes,
                          void *stream);
+
+/* ---------------------------------------------------------------- 8-bit linear path
+ * Rows of int8 codes with an fp32 scale each: row r stands for codes[r][c] * scale[r].  A row's scale
+ * is max(max |y|, 1e-8) / 127 rounded to fp32 (the formula of tp_utils.py:111), and a code is the
+ * multiple of the scale that is nearest to y (ties to even), -127 to 127, decided as in exact
+ * arithmetic.  (The collectives' quantiser, mtp_quantize_rows_int8, rounds the quotient to fp32
+ * first, as the reference does: about 2 codes in a million are the neighbour.)  A row with a NaN or an
+ * infinity, or whose scale is not finite, has scale NaN and codes 0, so that all that is computed from
+ * it is NaN.  Row r of a matrix is at base + r * ld elements, any alignment of the element type;
+ * rows 0 to 2^31 - 1, cols 1 to 131071 (sums of int8 products stay within int32).  fp32, bf16 or f16
+ * where a dtype is given.  No device memory is allocated and nothing is kept between calls: any
+ * stream, device or graph capture.  The reference has no 8-bit linear layer; the nearest is the
+ * quantiser of its int8 collective (tp_utils.py:103-131). */
+int mtp_quantize_rows(const void *x, int dtype, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes,
+                      float *scale, void *stream);
+/* out[r][c] = codes[r][c] * scale[r], the fp32 product rounded to out_dtype. */
+int mtp_dequantize_rows(const int8_t *codes, int64_t ld_codes, const float *scale, int64_t rows, int cols, void *out,
+                        int out_dtype, int64_t ld_out, void *stream);
+/* The residual's addition, the RMSNorm of model.py:130-135 and the quantiser in one call: h = x + resid in
+ * fp32, rounded to resid_dtype and stored to resid_out (same type; resid_out may be resid itself,
+ * but must not overlap it otherwise, nor x); y = w * h / sqrt(mean(h^2) + eps) with the mean, the root and the products in 64
+ * bits; codes and scale of y.  resid NULL: h = x and resid_out is not written.  eps >= 0. */
+int mtp_rmsnorm_int8(const void *x, int x_dtype, int64_t ld_x, const void *resid, int resid_dtype, int64_t ld_resid,
+                     void *resid_out, int64_t ld_resid_out, int64_t rows, int cols, const void *w, int w_dtype,
+                     float eps, int8_t *codes, int64_t ld_codes, float *scale, void *stream);
+/* out[m][n] = (sum over k of a[m][k] w[n][k]) * a_scale[m] * w_scale[n] (+ bias[n]): the sum exact in
+ * int32, then in fp32 in this order, rounded to out_dtype.  a [M][K] (tokens), w [N][K] (channels),
+ * bias NULL or [N] of bias_dtype.  The same sums whatever kernel the sizes and alignments choose, so
+ * a row's results depend on neither M nor the other rows.  out must not overlap the operands.  Where a device
+ * wait of the tensor-core kernel expires, the results that it did not reach are NaN. */
+int mtp_int8_linear(const int8_t *a, int64_t ld_a, const float *a_scale, int M, int K, const int8_t *w, int64_t ld_w,
+                    const float *w_scale, int N, const void *bias, int bias_dtype, void *out, int out_dtype,
+                    int64_t ld_out, void *stream);
 
 /* ---------------------------------------------------------------- persistent decode
  * One cooperative launch per decode step runs every layer of the model for a batch

@@ -1,0 +1,205 @@
+"""The 8-bit linear path: rows of int8 codes with a scale each (tokens of an activation, output channels of a weight),
+the RMSNorm that writes them together with the residual stream, and the matrix product of two of them.
+
+``MambaLM.quantize_linears`` runs a model's in_proj and out_proj through these; each can be called by itself.  Tensors are
+on CUDA, in float32, bfloat16 or float16, rows may be strided (``xz[:, :es]``); leading dimensions that do not lie on one
+stride are copied.  Calls run on the current stream of their tensors' device, allocate through torch only and keep nothing,
+so they can be captured in a CUDA graph.  No gradient: call them under ``torch.no_grad()``.  The reference has no 8-bit
+linear layer; the nearest is the quantiser of its int8 collective (``mamba_lite/tp_utils.py:103-131``)."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+from .logprobs import _call, _refuse_tangent
+
+__all__ = ["MAX_COLS", "Int8Rows", "quantize_rows", "dequantize_rows", "rms_norm_int8", "add_rms_norm_int8", "int8_linear"]
+
+MAX_COLS = 131071  # of a row: sums of int8 products stay within int32
+MAX_ROWS = (1 << 31) - 1
+
+
+class Int8Rows(NamedTuple):
+    """Rows that stand for ``codes * scale[..., None]``: codes [..., C] int8, scale [...] float32."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+
+
+# ------------------------------------------------------------------ arguments
+def _refuse_grad(what: str, *tensors) -> None:
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
+        _refuse_tangent(t, what)
+
+
+def _check_rows(x: torch.Tensor, what: str, name: str) -> None:
+    L.require_cuda(x, what)
+    L.dtype_code(x.dtype)
+    _check_shape(x, what, name)
+
+
+def _check_shape(x: torch.Tensor, what: str, name: str) -> None:
+    if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_COLS:
+        raise ValueError(f"{what}: {name} needs a last dimension of 1 to {MAX_COLS}, got shape {tuple(x.shape)}")
+    if x.numel() // x.shape[-1] > MAX_ROWS:
+        raise ValueError(f"{what}: {name} has more than {MAX_ROWS} rows")
+
+
+def _check_codes(r: Int8Rows, what: str, name: str) -> None:
+    codes, scale = r
+    L.require_cuda(codes, what)
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} needs int8 codes and float32 scales, got {codes.dtype} and {scale.dtype}")
+    _check_shape(codes, what, name)
+    if scale.shape != codes.shape[:-1]:
+        raise ValueError(f"{what}: {name} has scales of shape {tuple(scale.shape)} for codes of shape {tuple(codes.shape)}")
+    if scale.device != codes.device:
+        raise ValueError(f"{what}: {name} has its scales on {scale.device}, its codes on {codes.device}")
+
+
+def _same_device(t: torch.Tensor, x: torch.Tensor, what: str, name: str) -> None:
+    if t.device != x.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, expected {x.device}")
+
+
+def _as_rows(x: torch.Tensor):
+    """(x as [rows, C] with dense rows, the stride between rows); copied where the leading dimensions have no common stride."""
+    c = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, c)
+    if (x.stride(1) != 1 and c > 1) or (x.shape[0] > 1 and x.stride(0) < c):
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else c)
+
+
+def _extent(x: torch.Tensor):
+    """(first byte of x, the byte after its last)."""
+    at = x.data_ptr()
+    return at, at + (1 + sum((n - 1) * st for n, st in zip(x.shape, x.stride()))) * x.element_size()
+
+
+def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    (x0, x1), (y0, y1) = _extent(x), _extent(y)
+    return x0 < y1 and y0 < x1
+
+
+def _new_rows(x: torch.Tensor):
+    """Uninitialised (codes, scale, stride) for rows like those of x; each row of codes starts on a 16-byte boundary, as the
+    tensor-core product wants it."""
+    lead, c = x.shape[:-1], x.shape[-1]
+    wide = (c + 15) // 16 * 16
+    codes = torch.empty((*lead, wide), device=x.device, dtype=torch.int8)
+    scale = torch.empty(lead, device=x.device, dtype=torch.float32)
+    return (codes if wide == c else codes[..., :c]), scale, wide
+
+
+# ------------------------------------------------------------------ operators
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """int8 rows of x [..., C]: scale = max(max |x|, 1e-8) / 127 in float32, a code is the nearest multiple of it (ties to
+    even), -127 to 127.  A row with a NaN or an infinity has scale NaN and codes 0."""
+    what = "quantize_rows"
+    _check_rows(x, what, "x")
+    _refuse_grad(what, x)
+    codes, scale, ld_codes = _new_rows(x)
+    x, ld = _as_rows(x)
+    _call(x, "mtp_quantize_rows", x.data_ptr(), L.dtype_code(x.dtype), ld, x.shape[0], x.shape[1], codes.data_ptr(), ld_codes,
+          scale.data_ptr())
+    return Int8Rows(codes, scale)
+
+
+def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """What the rows stand for: codes * scale, the float32 product rounded to ``dtype``."""
+    what = "dequantize_rows"
+    _check_codes(rows, what, "rows")
+    code = L.dtype_code(dtype)
+    _refuse_grad(what, rows.scale)
+    out = torch.empty(rows.codes.shape, device=rows.codes.device, dtype=dtype)
+    codes, ld = _as_rows(rows.codes)
+    scale = rows.scale.reshape(-1).contiguous()
+    _call(codes, "mtp_dequantize_rows", codes.data_ptr(), ld, scale.data_ptr(), codes.shape[0], codes.shape[1], out.data_ptr(), code,
+          codes.shape[1])
+    return out
+
+
+def _norm(x, residual, weight, eps, inplace, what):
+    _check_rows(x, what, "x")
+    c = x.shape[-1]
+    if weight.shape != (c,):
+        raise ValueError(f"{what}: weight has shape {tuple(weight.shape)}, expected {(c,)}")
+    _same_device(weight, x, what, "weight")
+    w_code = L.dtype_code(weight.dtype)
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    _refuse_grad(what, x, residual, weight)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    codes, scale, ld_codes = _new_rows(x)
+    h, res_args = None, (None, 0, 0, None, 0)
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
+        _same_device(residual, x, what, "residual")
+        r_code = L.dtype_code(residual.dtype)
+        res, ld_res = _as_rows(residual)
+        if inplace:
+            if res.data_ptr() != residual.data_ptr():
+                raise ValueError(f"{what}: a residual that is updated in place needs rows on one stride")
+            if _overlap(x, residual):
+                raise ValueError(f"{what}: a residual that is updated in place must not share memory with x")
+            h, ld_h = residual, ld_res
+        else:
+            h, ld_h = torch.empty(residual.shape, device=x.device, dtype=residual.dtype), c
+        res_args = (res.data_ptr(), r_code, ld_res, h.data_ptr(), ld_h)
+    x, ld = _as_rows(x)
+    _call(x, "mtp_rmsnorm_int8", x.data_ptr(), L.dtype_code(x.dtype), ld, *res_args, x.shape[0], c, weight.data_ptr(), w_code, eps,
+          codes.data_ptr(), ld_codes, scale.data_ptr())
+    return Int8Rows(codes, scale), h
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> Int8Rows:
+    """``quantize_rows`` of weight * x / sqrt(mean(x^2) + eps) over the last dimension, without the norm in memory; the
+    statistics are held in 64 bits and the norm is not rounded in between."""
+    return _norm(x, None, weight, eps, False, "rms_norm_int8")[0]
+
+
+def add_rms_norm_int8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
+                      inplace: bool = False):
+    """A layer's boundary in one call: (int8 rows of the norm of h, h) with h = x + residual, added in float32 and rounded
+    to the residual's dtype.  ``inplace`` writes h over the residual (its rows on one stride, no two the same memory)."""
+    return _norm(x, residual, weight, eps, inplace, "add_rms_norm_int8")
+
+
+def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, *,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x [..., K] times weight [N, K]^T: (the exact int32 sum of the codes' products) * x's scale * weight's scale (+ bias),
+    in float32 in this order, rounded to ``dtype``; [..., N].  A row's results depend on no other row."""
+    what = "int8_linear"
+    _check_codes(x, what, "x")
+    _check_codes(weight, what, "weight")
+    wc, k = weight.codes, x.codes.shape[-1]
+    if wc.dim() != 2 or wc.shape[1] != k:
+        raise ValueError(f"{what}: x {tuple(x.codes.shape)} and weight {tuple(wc.shape)} do not fit")
+    _same_device(wc, x.codes, what, "weight")
+    code, n = L.dtype_code(dtype), wc.shape[0]
+    b_code = 0
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected {(n,)}")
+        _same_device(bias, x.codes, what, "bias")
+        b_code = L.dtype_code(bias.dtype)
+        bias = bias.contiguous()
+    _refuse_grad(what, x.scale, weight.scale, bias)
+    out = torch.empty((*x.codes.shape[:-1], n), device=wc.device, dtype=dtype)
+    a, ld_a = _as_rows(x.codes)
+    wc, ld_w = _as_rows(wc)
+    a_scale, w_scale = x.scale.reshape(-1).contiguous(), weight.scale.contiguous()
+    _call(a, "mtp_int8_linear", a.data_ptr(), ld_a, a_scale.data_ptr(), a.shape[0], k, wc.data_ptr(), ld_w, w_scale.data_ptr(),
+          n, L.ptr(bias), b_code, out.data_ptr(), code, n)
+    return out
