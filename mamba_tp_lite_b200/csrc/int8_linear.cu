@@ -1,34 +1,12 @@
 // out[M, N] = (a[M, K] . w[N, K]^T) * a_scale[m] * w_scale[n] (+ bias): int8 operands, int32 sums.
-//   int8_simt  64 x 64 tiles, 4 x 4 outputs per thread, byte loads: operands of any alignment.
-#include "common.cuh"
+//   int8_tc.cu  operands on 16-byte boundaries;
+//   int8_simt   64 x 64 tiles, 4 x 4 outputs per thread, byte loads: operands of any alignment.
+#include "int8_linear.cuh"
 
 namespace mtp {
 namespace {
 
-constexpr int MAX_COLS = 131071;
-
-struct Out {
-  void *p;
-  int64_t ld;
-  int dtype;
-  const float *a_scale, *w_scale;
-  const void *bias;
-  int bias_dtype;
-};
-
-__device__ __forceinline__ float ld_bias(const Out &o, int n) {
-  if (o.bias_dtype == MTP_F32) return ((const float *)o.bias)[n];
-  if (o.bias_dtype == MTP_BF16) return __bfloat162float(((const __nv_bfloat16 *)o.bias)[n]);
-  return __half2float(((const __half *)o.bias)[n]);
-}
-
-__device__ __forceinline__ void store_one(const Out &o, int64_t m, int n, int acc) {
-  float v = __fmul_rn(__fmul_rn((float)acc, o.a_scale[m]), o.w_scale[n]);
-  if (o.bias) v = __fadd_rn(v, ld_bias(o, n));
-  if (o.dtype == MTP_F32) ((float *)o.p)[m * o.ld + n] = v;
-  else if (o.dtype == MTP_BF16) ((__nv_bfloat16 *)o.p)[m * o.ld + n] = __float2bfloat16_rn(v);
-  else ((__half *)o.p)[m * o.ld + n] = __float2half_rn(v);
-}
+using namespace i8;
 
 __global__ void __launch_bounds__(256) int8_simt_kernel(const int8_t *__restrict__ a, int64_t ld_a, int M, int K,
                                                         const int8_t *__restrict__ w, int64_t ld_w, int N, int tiles_n,
@@ -74,7 +52,11 @@ __global__ void __launch_bounds__(256) int8_simt_kernel(const int8_t *__restrict
       for (int j = 0; j < 4; ++j) {
         const int64_t m = m0 + ty + 16 * i;
         const int n = n0 + tx + 16 * j;
-        if (m < M && n < N) store_one(o, m, n, acc[i][j]);
+        if (m < M && n < N) {
+          float v = scaled(acc[i][j], o.a_scale[m], o.w_scale[n]);
+          if (o.bias) v = __fadd_rn(v, ld_bias(o, n));
+          store_value(o, m, n, v);
+        }
       }
   }
 }
@@ -96,6 +78,7 @@ extern "C" int mtp_int8_linear(const int8_t *a, int64_t ld_a, const float *a_sca
   MTP_REQUIRE((M == 1 || (ld_a >= K && ld_out >= N)) && (N == 1 || ld_w >= K), "leading dimensions too small");
   cudaStream_t s = (cudaStream_t)stream;
   const Out o{out, ld_out, out_dtype, a_scale, w_scale, bias, bias_dtype};
+  if (tc_eligible(a, ld_a, M, w, ld_w, N)) return linear_tc(a, ld_a, M, K, w, ld_w, N, o, s);
   const int tiles_n = ceil_div(N, 64);
   const int64_t tiles = (int64_t)ceil_div(M, 64) * tiles_n;
   const int grid = (int)(tiles < 148 * 16 ? tiles : 148 * 16);

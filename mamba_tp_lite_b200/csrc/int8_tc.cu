@@ -1,0 +1,491 @@
+// The int8 product on the tensor cores: tcgen05.mma kind::i8, int32 accumulators in tensor memory.
+//
+// Persistent, warp-specialised, one CTA per SM; CG = 2 pairs the CTAs of two SMs on one 256 x bn tile, each with its own 128
+// rows of a and half of the tile's rows of w, so that a row of w is loaded once for 256 rows of a:
+//   warp 0     one lane issues the TMA loads of its CTA (128-byte wide boxes, 128-byte swizzle) into a ring;
+//   warp 1     allocates tensor memory (two accumulators of 128 lanes x 256 columns); in the pair's first CTA one lane issues
+//              tcgen05.mma for both, releases ring slots and signals finished accumulators in both CTAs with tcgen05.commit;
+//   warps 2-9  epilogue, two warps per lane quarter, each on every second block of 128 bytes of output columns: sums to fp32,
+//              times the row's scale (a lane has one row) and the columns' (from shared memory), rounded into a staging block
+//              in the swizzled layout of a TMA store.  It works on one tile while the tensor cores fill the other accumulator.
+// Every wait is bounded; a CTA whose wait expires gives NaN for what it has left, waits (again with a limit) for its copies and
+// products in flight, frees its tensor memory and returns.
+#include "int8_linear.cuh"
+#include "tc_common.cuh"
+
+namespace mtp {
+namespace i8 {
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 128, BK = 128, BN_MAX = 256;  // rows of a per CTA, bytes of K per ring slot, columns per tile
+constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr unsigned long long TIMEOUT_NS = 2000000000ull;
+constexpr int A_BYTES = BM * BK;
+constexpr int CHUNK_BYTES = 32 * 128;  // 32 rows x 128 bytes of output
+
+constexpr int B_BYTES = 128 * BK;  // at most 128 rows of w per CTA: bn = 256 takes a pair
+constexpr int SLOT = A_BYTES + B_BYTES, STAGES = 5;
+constexpr int STAGE_OUT = STAGES * SLOT;                    // the epilogue's blocks, one per warp
+constexpr int COLS = STAGE_OUT + EPI_WARPS * CHUNK_BYTES;   // scales and biases of the columns of two tiles
+constexpr int BARS = COLS + 2 * 2 * BN_MAX * 4;
+constexpr int SMEM_BYTES = BARS + 256 + 1024 /* to align the base */;
+
+struct Params {
+  Out o;
+  int M, N, K;
+  int bn, tiles_m, tiles_n, num_tiles, group_m;
+  int a_rows;    // rows of a box of a
+  int tma_out;   // results by TMA stores
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ void tile_coords(const Params &p, int t, int &mt, int &nt) {
+  const int gsize = p.group_m * p.tiles_n;
+  const int g = t / gsize;
+  const int first_m = g * p.group_m;
+  const int gm = min(p.tiles_m - first_m, p.group_m);
+  const int r = t - g * gsize;
+  mt = first_m + r % gm;
+  nt = r / gm;
+}
+
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y) {
+  if (CG == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                 "l"(tm), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+  else
+    tma_load_2d(dst, tm, bar, x, y);
+}
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+// Arrives at `bar` (of both CTAs of a pair) when the products issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    umma_commit(bar);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+template <typename T> constexpr int PER_WORD = 16 / (int)sizeof(T);  // results in 16 bytes
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int CG, typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+    int8_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmC, const Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn);
+  const uint32_t base = (raw + 1023u) & ~1023u;  // the same in both CTAs of a pair
+  unsigned char *gbase = smem_dyn + (base - raw);
+  const uint32_t bar0 = base + BARS;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t drain_bar = bar0 + 8u * (2 * STAGES + 4);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(gbase + BARS + 8 * (2 * STAGES + 5));
+  volatile int *abort = reinterpret_cast<volatile int *>(gbase + BARS + 8 * (2 * STAGES + 5) + 8);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank = 0;
+  if (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), EPI_WARPS * CG);
+    }
+    mbar_init(drain_bar, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(TMEM_COLS));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(TMEM_COLS));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // both CTAs' barriers are ready
+  tc_fence_after();
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  const uint32_t tmem_base = *tmem_holder;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int b_rows = p.bn / CG;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const uint32_t tx_bytes = (uint32_t)((p.a_rows + b_rows) * BK * CG);
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      for (int t = first; t < p.num_tiles && !*abort; t += step) {
+        int mt, nt;
+        tile_coords(p, t, mt, nt);
+        const int y_a = (mt * CG + (int)rank) * BM, y_b = nt * p.bn + (int)rank * b_rows;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort, TIMEOUT_NS)) break;
+          if (rank == 0) mbar_expect_tx(full_bar(s), tx_bytes);  // both CTAs' bytes count at the first's barrier
+          const uint32_t bar = CG == 2 ? cluster_addr(full_bar(s), 0) : full_bar(s);
+          const uint32_t sa = base + s * SLOT;
+          load_box<CG>(sa, &tmA, bar, kb * BK, y_a);
+          load_box<CG>(sa + A_BYTES, &tmB, bar, kb * BK, y_b);
+          ++issued;
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+      if (*abort && rank == 0) {  // wait (bounded) until the most recent fills have landed
+        const int back = issued < STAGES ? issued : STAGES;
+        for (int i = 0; i < back; ++i) {
+          if (--s < 0) { s = STAGES - 1; ph ^= 1u; }
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(full_bar(s), ph) && globaltimer_ns() - t0 < 100000000ull) {}
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      int s = 0, local = 0;
+      uint32_t ph = 0;
+      bool any = false, ok = true;
+      for (int t = first; ok && t < p.num_tiles && !*abort; t += step, ++local) {
+        const int a = local & 1;
+        const uint32_t use = (uint32_t)(local >> 1);
+        if (!mbar_wait(tempty_bar(a), (use & 1u) ^ 1u, abort, TIMEOUT_NS)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + (uint32_t)(a * BN_MAX);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = base + s * SLOT;
+          const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + A_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)  // 32 bytes along K per instruction; past K both operands are zeros
+            mma<CG>(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), p.idesc, (kb | k) != 0);
+          any = true;
+          commit<CG>(empty_bar(s));
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (ok) commit<CG>(tfull_bar(a));
+      }
+      if (*abort && any) {
+        commit<CG>(drain_bar);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain_bar, 0) && globaltimer_ns() - t0 < 100000000ull) {}
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..9)
+    constexpr int CW = 128 / (int)sizeof(T);  // columns of a block of output
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int et = threadIdx.x - 64;
+    unsigned char *stage = gbase + STAGE_OUT + (warp - 2) * CHUNK_BYTES;
+    float *cols = reinterpret_cast<float *>(gbase + COLS);
+    int local = 0;
+    bool alive = true;
+    for (int t = first; t < p.num_tiles; t += step, ++local) {
+      int mt, nt;
+      tile_coords(p, t, mt, nt);
+      const int a = local & 1;
+      const uint32_t use = (uint32_t)(local >> 1);
+      const int n_tile = nt * p.bn, m0 = (mt * CG + (int)rank) * BM + q * 32;
+      const int m = m0 + lane;
+      const float sa = m < p.M ? p.o.a_scale[m] : 0.f;
+      // the columns' scales and biases: written by all epilogue warps into the buffer that the tile before the last used
+      float *sw = cols + a * 2 * BN_MAX, *sb = sw + BN_MAX;
+      for (int c = et; c < p.bn; c += 32 * EPI_WARPS) {
+        const bool in = n_tile + c < p.N;
+        sw[c] = in ? p.o.w_scale[n_tile + c] : 0.f;
+        sb[c] = in ? ld_bias(p.o, n_tile + c) : 0.f;
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * EPI_WARPS) : "memory");
+      alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, TIMEOUT_NS));
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN_MAX);
+      for (int c0 = half * CW; c0 < p.bn; c0 += 2 * CW) {
+        if (n_tile + c0 >= p.N || m0 >= p.M) break;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();  // the block is free again
+#pragma unroll
+        for (int g = 0; g < CW; g += 32) {
+          int acc[32] = {};
+          if (alive) tmem_ld32(tbase + (uint32_t)(c0 + g), acc);
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 w4 = *reinterpret_cast<const float4 *>(sw + c0 + g + i);
+            v[i] = scaled(acc[i], sa, w4.x);
+            v[i + 1] = scaled(acc[i + 1], sa, w4.y);
+            v[i + 2] = scaled(acc[i + 2], sa, w4.z);
+            v[i + 3] = scaled(acc[i + 3], sa, w4.w);
+          }
+          if (p.o.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 b4 = *reinterpret_cast<const float4 *>(sb + c0 + g + i);
+              v[i] = __fadd_rn(v[i], b4.x);
+              v[i + 1] = __fadd_rn(v[i + 1], b4.y);
+              v[i + 2] = __fadd_rn(v[i + 2], b4.z);
+              v[i + 3] = __fadd_rn(v[i + 3], b4.w);
+            }
+          }
+          if (!alive) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fffffff);
+          }
+          // row `lane` of the block: its eight 16-byte words lie where the 128-byte swizzle has them
+          constexpr int PER = PER_WORD<T>;
+#pragma unroll
+          for (int i = 0; i < 32; i += PER) {
+            const int word = (g + i) / PER;
+            uint4 *at = reinterpret_cast<uint4 *>(stage + lane * 128 + ((word ^ (lane & 7)) << 4));
+            if constexpr (sizeof(T) == 4) {
+              *at = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]),
+                               __float_as_uint(v[i + 3]));
+            } else {
+              *at = make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
+                               pack2<T>(v[i + 6], v[i + 7]));
+            }
+          }
+        }
+        if (p.tma_out) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&tmC),
+                         "r"(smem_u32(stage)), "r"(n_tile + c0), "r"(m0)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {  // rows of any alignment: a row of the block at a time, its columns side by side
+          __syncwarp();
+          const int rows = min(32, p.M - m0), n_in = min(CW, p.N - n_tile - c0);
+          for (int r = 0; r < rows; ++r) {
+            T *out = (T *)p.o.p + (int64_t)(m0 + r) * p.o.ld + n_tile + c0;
+#pragma unroll
+            for (int j = 0; j < CW / 32; ++j) {
+              const int c = j * 32 + lane;
+              const T *from = reinterpret_cast<const T *>(stage + r * 128 + (((c / PER_WORD<T>) ^ (r & 7)) << 4)) + c % PER_WORD<T>;
+              if (c < n_in) out[c] = *from;
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2 && rank != 0)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(tempty_bar(a), 0))
+                       : "memory");
+        else
+          mbar_arrive(tempty_bar(a));
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort) __nanosleep(1000000);  // the other CTA's copies and products in flight
+  if (CG == 2) cluster_sync();       // nothing of the pair is at work in this CTA's memory any more
+  tc_fence_after();
+  if (warp == 1) {
+    if (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+  }
+}
+
+// 2-D map over bytes [rows, cols] with ld bytes between rows; boxes of 128 bytes x box_rows, zeros outside.
+int map_codes(CUtensorMap *tm, const void *ptr, int rows, int cols, int64_t ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MTP_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (rows == 1) ld = (cols + 15) / 16 * 16;  // not used
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MTP_ERR_ARG, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return MTP_OK;
+}
+
+// The same over the results; boxes of 128 bytes x 32 rows.
+int map_out(CUtensorMap *tm, const Out &o, int rows, int cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MTP_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int es = o.dtype == MTP_F32 ? 4 : 2;
+  const int64_t ld = rows == 1 ? ((int64_t)cols * es + 15) / 16 * 16 : o.ld * es;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32u};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = o.dtype == MTP_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : o.dtype == MTP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = fn(tm, type, 2, o.p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MTP_ERR_ARG, "cuTensorMapEncodeTiled (out) failed with code " + std::to_string((int)r));
+  return MTP_OK;
+}
+
+// The kernel's limit of shared memory belongs to the current device.
+template <int CG, typename T> int allow_smem() {
+  static std::atomic<uint64_t> done{0};  // a bit for each device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load() & bit) return MTP_OK;
+  if (cudaFuncSetAttribute(int8_tc_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(MTP_ERR_CUDA, "int8_tc: shared memory");
+  }
+  done.fetch_or(bit);
+  return MTP_OK;
+}
+
+template <int CG, typename T>
+int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tcm, const Params &p, cudaStream_t stream) {
+  int rc = allow_smem<CG, T>();
+  if (rc) return rc;
+  const int places = num_sms() / CG;
+  const int grid = (p.num_tiles < places ? p.num_tiles : places) * CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, int8_tc_kernel<CG, T>, ta, tb, tcm, p);
+  return check_launch("int8_linear");
+}
+
+template <int CG>
+int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int bn,
+        cudaStream_t stream) {
+  Params p{};
+  p.o = o;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.bn = bn;
+  p.tiles_m = ceil_div(M, BM * CG);
+  p.tiles_n = ceil_div(N, bn);
+  p.num_tiles = p.tiles_m * p.tiles_n;
+  p.group_m = 16;
+  p.a_rows = BM;
+  // kind::i8, int32 results, signed operands, both with K innermost
+  p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
+  const size_t es = o.dtype == MTP_F32 ? 4 : 2;
+  p.tma_out = aligned16(o.p) && (M == 1 || ((size_t)o.ld * es) % 16 == 0);
+  CUtensorMap ta, tb, tcm;
+  int rc = map_codes(&ta, a, M, K, ld_a, p.a_rows);
+  if (rc) return rc;
+  rc = map_codes(&tb, w, N, K, ld_w, bn / CG);
+  if (rc) return rc;
+  memset(&tcm, 0, sizeof(tcm));
+  if (p.tma_out) {
+    rc = map_out(&tcm, o, M, N);
+    if (rc) return rc;
+  }
+  if (o.dtype == MTP_F32) return launch<CG, float>(ta, tb, tcm, p, stream);
+  if (o.dtype == MTP_BF16) return launch<CG, __nv_bfloat16>(ta, tb, tcm, p, stream);
+  return launch<CG, __half>(ta, tb, tcm, p, stream);
+}
+
+}  // namespace
+
+bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t ld_w, int N) {
+  return aligned16(a) && aligned16(w) && (M == 1 || ld_a % 16 == 0) && (N == 1 || ld_w % 16 == 0) && M < 0x7ffff000 &&
+         N < 0x7ffff000;
+}
+
+int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
+              cudaStream_t stream) {
+  const int sms = num_sms();
+  if (M > BM && (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN_MAX) * 2 >= sms)
+    return run<2>(a, ld_a, M, K, w, ld_w, N, o, BN_MAX, stream);
+  int bn = 128;
+  while (bn > 64 && (int64_t)ceil_div(M, BM) * ceil_div(N, bn) < sms) bn /= 2;
+  return run<1>(a, ld_a, M, K, w, ld_w, N, o, bn, stream);
+}
+
+}  // namespace i8
+}  // namespace mtp
