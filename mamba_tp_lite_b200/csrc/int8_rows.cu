@@ -1,71 +1,115 @@
 // Rows of int8 codes with a scale each: quantising, reading back, and RMSNorm with the residual's addition and an int8
-// output.  A CTA takes one row: a pass for its statistics, a pass for its codes.
-#include "common.cuh"
+// output.
+//
+// All are bound by HBM.  A row belongs to a team of threads (a warp, or a CTA) that keeps it in registers, so that it is read
+// once: 16 or 32 values a thread, in vectors where rows lie on vector boundaries.  Which of two codes is the nearer is decided as in
+// exact arithmetic without paying for 64 bits at each value: fp32 gives the quotient to 3e-5 of a step, and only a value
+// whose quotient is within 2^-14 of a half (1 in 8000) is looked at again in 64 bits.
+// Rows of more than 16384 values, and rows whose numbers leave fp32's middle range, go through the plain 64-bit loops.
+#include <type_traits>
+#include "int8_linear.cuh"
 
 namespace mtp {
 namespace {
 
-constexpr int THREADS = 256;
-constexpr int MAX_COLS = 131071;  // 127 * 127 * MAX_COLS < 2^31
+using i8::MAX_COLS;
 
-__device__ __forceinline__ double block_reduce(double v, bool sum, double *red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = sum ? v + u : fmax(v, u);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < THREADS / 32; ++i) v = sum ? v + red[i] : fmax(v, red[i]);
-  return v;
-}
+constexpr int E_OF_WARP = 32, E_OF_CTA = 16;  // values of a row that a thread holds
+constexpr int MAX_TEAM = 16384 / E_OF_CTA;
+constexpr int LONG_THREADS = 256;
+constexpr int UNROLL = 4;              // vectors that a thread reads back, their loads in flight together
+constexpr float MAGIC = 12582912.f;    // 1.5 * 2^23: x + MAGIC is x rounded to a whole number, its low byte the int8
+constexpr float BORDER = 0.5f - 1.f / 16384.f;
+constexpr float FLT_TOP = 3.402823466e38f;
+constexpr uint32_t TINY = 0x0d800000u, HUGE_ = 0x71800000u;  // 2^-100, 2^100
+
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 
 // fp32 scale of a row whose largest |y| is amax; NaN for a row with a NaN or an infinity (`bad`).
 __device__ __forceinline__ float scale_of(double amax, bool bad) {
-  const float s = (float)(fmax(amax, 1e-8) / 127.0);
-  return bad || !(s <= 3.402823466e38f) ? __int_as_float(0x7fffffff) : s;
+  const float s = (float)(fmax(amax, 1e-8) * (1.0 / 127.0));
+  return bad || !(s <= FLT_TOP) ? nan_f() : s;
 }
 
-__device__ __forceinline__ int8_t code_of(double y, float s) {
-  return (int8_t)(int)fmin(fmax(rint(y / (double)s), -127.0), 127.0);
+__device__ __forceinline__ int exact_code(double y, float s) { return (int)fmin(fmax(rint(y / (double)s), -127.0), 127.0); }
+
+// Codes of four values p * c, the quotients to fp32's precision: the codes in one word, and the largest distance from a code.
+__device__ __forceinline__ uint32_t codes4(const float *p, float c, float &far) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = fmaf(p[i], c, MAGIC);
+    far = fmaxf(far, fabsf(fmaf(p[i], c, -__fsub_rn(m[i], MAGIC))));
+  }
+  const uint32_t lo = __byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+// The code of a y whose quotient t = y / s (to fp32's precision) lies next to k + 1/2: s (k + 1/2) is exact in 64 bits.
+__device__ __forceinline__ int border_code(double y, float t, float s) {
+  const float k = floorf(t);
+  const double e = ((double)k + 0.5) * (double)s;
+  const int lo = (int)k;
+  return y > e ? lo + 1 : y < e ? lo : lo + (lo & 1);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS) quantize_kernel(const T *__restrict__ x, int64_t ld, int64_t rows, int cols,
-                                                           int8_t *__restrict__ codes, int64_t ld_codes,
-                                                           float *__restrict__ scale) {
-  MTP_PDL_WAIT();
-  MTP_PDL_TRIGGER();
-  __shared__ double red[THREADS / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T *xr = x + r * ld;
-    double amax = 0.0;
-    bool bad = false;
-    for (int c = threadIdx.x; c < cols; c += THREADS) {
-      const float v = fabsf(ldf(xr + c));
-      bad |= !(v <= 3.402823466e38f);
-      amax = fmax(amax, (double)v);
+// ------------------------------------------------------------------ element access
+// N values from p on: one or two vector loads, converted to fp32.
+template <typename T, int N> struct Raw { uint32_t w[sizeof(T) * N / 4]; };
+
+template <typename T, int N>
+__device__ __forceinline__ void load_raw(Raw<T, N> &r, const T *p) {
+  constexpr int W = sizeof(T) * N / 4;
+  if constexpr (W == 2) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    r.w[0] = u.x; r.w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(p + i * 4 / sizeof(T));
+      r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
     }
-    amax = block_reduce(amax, false, red);
-    bad = __syncthreads_or(bad);
-    const float s = scale_of(amax, bad);
-    for (int c = threadIdx.x; c < cols; c += THREADS)
-      codes[r * ld_codes + c] = bad ? 0 : code_of((double)ldf(xr + c), s);
-    if (threadIdx.x == 0) scale[r] = s;
   }
 }
-
-template <typename T>
-__global__ void __launch_bounds__(THREADS) dequantize_kernel(const int8_t *__restrict__ codes, int64_t ld_codes,
-                                                             const float *__restrict__ scale, int64_t rows, int cols,
-                                                             T *__restrict__ out, int64_t ld_out) {
-  MTP_PDL_WAIT();
-  MTP_PDL_TRIGGER();
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += THREADS)
-      stf(out + r * ld_out + c, __fmul_rn((float)codes[r * ld_codes + c], scale[r]));
+template <typename T, int N>
+__device__ __forceinline__ void store_raw(T *p, const Raw<T, N> &r) {
+  constexpr int W = sizeof(T) * N / 4;
+  if constexpr (W == 2) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+      *reinterpret_cast<uint4 *>(p + i * 4 / sizeof(T)) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void to_f32(const Raw<T, N> &r, float *v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      v[i] = __uint_as_float(r.w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    } else {
+      v[i] = __half2float(__ushort_as_half((unsigned short)(r.w[i / 2] >> (16 * (i & 1)))));
+    }
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void from_f32(Raw<T, N> &r, const float *v) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.w[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+        r.w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+        r.w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ float ld_any(const void *p, int dtype, int64_t i) {
@@ -84,49 +128,499 @@ __device__ __forceinline__ float st_any(void *p, int dtype, int64_t i, float v) 
   ((__half *)p)[i] = h;
   return __half2float(h);
 }
+template <typename T> struct Code;
+template <> struct Code<float> { static constexpr int value = MTP_F32; };
+template <> struct Code<__nv_bfloat16> { static constexpr int value = MTP_BF16; };
+template <> struct Code<__half> { static constexpr int value = MTP_F16; };
 
-__global__ void __launch_bounds__(THREADS)
-    rmsnorm_int8_kernel(const void *x, int x_dtype, int64_t ld_x, const void *resid, int r_dtype, int64_t ld_r, void *r_out,
-                        int64_t ld_ro, int64_t rows, int cols, const void *w, int w_dtype, float eps, int8_t *codes,
-                        int64_t ld_codes, float *scale) {
-  MTP_PDL_WAIT();
-  MTP_PDL_TRIGGER();
-  __shared__ double red[THREADS / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    double ss = 0.0;
-    for (int c = threadIdx.x; c < cols; c += THREADS) {
-      float h = ld_any(x, x_dtype, r * ld_x + c);
-      if (resid) h = st_any(r_out, r_dtype, r * ld_ro + c, h + ld_any(resid, r_dtype, r * ld_r + c));
-      ss += (double)h * (double)h;
+// The largest of m, |a| and |b|; NaN if one is.
+__device__ __forceinline__ float max_abs3(float m, float a, float b) {
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return m;
+}
+
+// ------------------------------------------------------------------ teams
+struct Join {
+  double d[32];
+  uint32_t u[32];
+  unsigned long long most;
+};
+
+// A warp or a CTA.  Every thread of the team calls each of these.
+template <bool WARP> struct Team {
+  Join *j;
+  __device__ __forceinline__ int rank() const { return WARP ? threadIdx.x & 31 : threadIdx.x; }
+  __device__ __forceinline__ int size() const { return WARP ? 32 : blockDim.x; }
+  __device__ __forceinline__ void sync() const {
+    if (WARP) __syncwarp();
+    else __syncthreads();
+  }
+  __device__ __forceinline__ uint32_t max_u32(uint32_t v) const {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) j->u[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
+    return __reduce_max_sync(0xffffffffu, lane < n ? j->u[lane] : 0u);
+  }
+  // The sum of s in a fixed order and the largest u.
+  __device__ __forceinline__ void sum_max(double &s, uint32_t &u) const {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    u = __reduce_max_sync(0xffffffffu, u);
+    if (WARP) return;
+    const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (n == 1) return;
+    if (lane == 0) {
+      j->d[threadIdx.x >> 5] = s;
+      j->u[threadIdx.x >> 5] = u;
     }
-    ss = block_reduce(ss, true, red);
-    const double rs = 1.0 / sqrt(ss / cols + (double)eps);
-    // a thread reads back what it has stored itself
-    const void *hp = resid ? r_out : x;
-    const int h_dtype = resid ? r_dtype : x_dtype;
-    const int64_t ld_h = resid ? ld_ro : ld_x;
-    double amax = 0.0;
-    bool bad = false;
-    for (int c = threadIdx.x; c < cols; c += THREADS) {
-      const double y = fabs((double)ld_any(hp, h_dtype, r * ld_h + c) * rs * (double)ld_any(w, w_dtype, c));
-      bad |= !(y <= 1e300);
-      amax = fmax(amax, y);
+    __syncthreads();
+    s = lane < n ? j->d[lane] : 0.0;
+    u = __reduce_max_sync(0xffffffffu, lane < n ? j->u[lane] : 0u);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+  // The largest of values that are not negative; few threads have one above 0.  `most` is 0 before the first call and is not
+  // used twice between barriers.
+  __device__ __forceinline__ double max_rare(double v) const {
+    if (WARP) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+      return v;
     }
-    amax = block_reduce(amax, false, red);
-    float s = scale_of(amax, __syncthreads_or(bad));
-    bad = !(s > 0.f);
-    for (int c = threadIdx.x; c < cols; c += THREADS) {
-      const double y = (double)ld_any(hp, h_dtype, r * ld_h + c) * rs * (double)ld_any(w, w_dtype, c);
-      codes[r * ld_codes + c] = bad ? 0 : code_of(y, s);
+    if (v > 0.0) atomicMax(&j->most, (unsigned long long)__double_as_longlong(v));  // ordered as their bits are
+    __syncthreads();
+    return __longlong_as_double((long long)j->most);
+  }
+  __device__ __forceinline__ double max_all(double v) const {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (WARP) return v;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) j->d[threadIdx.x >> 5] = v;
+    __syncthreads();
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v = fmax(v, j->d[i]);
+    return v;
+  }
+};
+
+// A row in 64 bits throughout: h[c] is read from memory, y = h * rs * w (w NULL: y = h).  For long rows, and for rows whose
+// numbers leave fp32's middle range.
+template <bool WARP>
+__device__ __noinline__ void slow_row(const Team<WARP> &team, const void *h, int h_dtype, const void *w, int w_dtype, double rs,
+                                      int cols, int8_t *codes, float *scale) {
+  double amax = 0.0;
+  uint32_t bad = 0;
+  for (int c = team.rank(); c < cols; c += team.size()) {
+    double y = (double)ld_any(h, h_dtype, c);
+    if (w) y = y * rs * (double)ld_any(w, w_dtype, c);
+    y = fabs(y);
+    bad |= !(y <= 1e300);
+    amax = fmax(amax, y);
+  }
+  amax = team.max_all(amax);
+  team.sync();
+  const float s = scale_of(amax, team.max_u32(bad) != 0);
+  for (int c = team.rank(); c < cols; c += team.size()) {
+    double y = (double)ld_any(h, h_dtype, c);
+    if (w) y = y * rs * (double)ld_any(w, w_dtype, c);
+    codes[c] = (int8_t)(s > 0.f ? exact_code(y, s) : 0);
+  }
+  if (team.rank() == 0) *scale = s;
+}
+
+// Writes the codes of p[] * c for the values a thread holds; value(i, col) gives the 64-bit y of its i-th value.
+template <int VEC, int EACH, typename Y>
+__device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, float s, int8_t *codes, int cols, int rank, int size,
+                                            Y value) {
+  uint32_t q[EACH / 4];
+#pragma unroll
+  for (int g = 0; g < EACH / 4; ++g) {
+    float far = 0.f;
+    q[g] = codes4(p + 4 * g, c, far);
+    if (far > BORDER) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = 4 * g + k;
+        const float m = fmaf(p[i], c, MAGIC), t = __fmul_rn(p[i], c);
+        if (fabsf(fmaf(p[i], c, -__fsub_rn(m, MAGIC))) > BORDER) {
+          const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
+          const uint32_t code = (uint32_t)border_code(value(i, col), t, s) & 0xffu;
+          q[g] = (q[g] & ~(0xffu << (8 * k))) | code << (8 * k);
+        }
+      }
     }
-    if (threadIdx.x == 0) scale[r] = s;
+  }
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int col = i * size + rank;
+      if (col < cols) codes[col] = (int8_t)(q[i / 4] >> (8 * (i & 3)));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) {
+        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(codes + col) = q[v];
+        else *reinterpret_cast<uint2 *>(codes + col) = make_uint2(q[2 * v], q[2 * v + 1]);
+      }
+    }
   }
 }
 
-int grid_for(int64_t rows) { return (int)(rows < 148 * 64 ? rows : 148 * 64); }
+// ------------------------------------------------------------------ quantise
+template <typename T, int VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : MAX_TEAM)
+    quantize_kernel(const T *__restrict__ x, int64_t ld, int64_t rows, int cols, int8_t *__restrict__ codes, int64_t ld_codes,
+                    float *__restrict__ scale) {
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  __shared__ Join join;
+  constexpr int EACH = WARP ? E_OF_WARP : E_OF_CTA;
+  const Team<WARP> team{&join};
+  const int rank = team.rank(), size = team.size();
+  const int64_t r = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (r >= rows) return;
+  const T *xr = x + r * ld;
+  float p[EACH];
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) p[i] = i * size + rank < cols ? ldf(xr + i * size + rank) : 0.f;
+  } else {
+    Raw<T, VEC> raw[EACH / VEC];
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) load_raw(raw[v], xr + col);
+      else raw[v] = Raw<T, VEC>{};
+    }
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) to_f32(raw[v], p + v * VEC);
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < EACH; i += 2) m = max_abs3(m, p[i], p[i + 1]);
+  const uint32_t bits = team.max_u32(__float_as_uint(m));  // as integers: NaN above infinity above all numbers
+  m = __uint_as_float(bits);
+  const float s = bits >= 0x7f800000u ? nan_f() : __fdiv_rn(fmaxf(m, 1e-8f), 127.f);
+  int8_t *out = codes + r * ld_codes;
+  if (!(s > 0.f)) {
+    for (int c = rank; c < cols; c += size) out[c] = 0;
+  } else {
+    const float c = __frcp_rn(s);  // 3.7e-37 at least: a normal number
+    write_codes<VEC>(p, c, s, out, cols, rank, size, [&](int i, int) { return (double)p[i]; });
+  }
+  if (rank == 0) scale[r] = s;
+}
 
+template <typename T>
+__global__ void __launch_bounds__(LONG_THREADS) quantize_long_kernel(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes,
+                                                                     int64_t ld_codes, float *scale) {
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  __shared__ Join join;
+  const Team<false> team{&join};
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    slow_row(team, x + r * ld, Code<T>::value, nullptr, 0, 1.0, cols, codes + r * ld_codes, scale + r);
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ norm
+struct NormArgs {
+  const void *x, *resid;
+  void *r_out;
+  const void *w;
+  int64_t ld_x, ld_r, ld_ro;
+  int64_t rows;
+  int cols, x_dtype, r_dtype, w_dtype;
+  float eps;
+  int8_t *codes;
+  int64_t ld_codes;
+  float *scale;
+  double inv_cols;
+};
+
+template <int VEC> __device__ __forceinline__ void load_weight(const void *w, int dtype, int col, float *v) {
+  if constexpr (VEC == 1) {
+    v[0] = ld_any(w, dtype, col);
+  } else if (dtype == MTP_F32) {
+    Raw<float, VEC> r;
+    load_raw(r, (const float *)w + col);
+    to_f32(r, v);
+  } else if (dtype == MTP_BF16) {
+    Raw<__nv_bfloat16, VEC> r;
+    load_raw(r, (const __nv_bfloat16 *)w + col);
+    to_f32(r, v);
+  } else {
+    Raw<__half, VEC> r;
+    load_raw(r, (const __half *)w + col);
+    to_f32(r, v);
+  }
+}
+
+struct None {};
+
+// TR is the residual's type, or None.  y = h w r with r = 1 / sqrt(mean h^2 + eps); the scale is fp32(max |y| / 127), and the
+// codes are those of (h w) (r / scale).  The sum of squares and r are held in 64 bits; the largest product is found among the
+// fp32 products and then taken exactly (a 48-bit number) from the values whose product rounds to that.
+template <typename TX, typename TR, int VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : MAX_TEAM) norm_kernel(const NormArgs a) {
+  constexpr bool ADD = !std::is_same<TR, None>::value;
+  using TH = typename std::conditional<ADD, TR, TX>::type;  // the stream's type
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  __shared__ Join join;
+  constexpr int EACH = WARP ? E_OF_WARP : E_OF_CTA;
+  const Team<WARP> team{&join};
+  const int rank = team.rank(), size = team.size(), cols = a.cols;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows) return;
+  if (!WARP && threadIdx.x == 0) join.most = 0;  // the first use comes after the barrier of sum_max
+  const TX *xr = (const TX *)a.x + row * a.ld_x;
+  const TR *rr = (const TR *)a.resid + row * a.ld_r;
+  TR *ro = (TR *)a.r_out + row * a.ld_ro;
+  float p[EACH], w[EACH];
+  if constexpr (VEC == 1) {
+    float res[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int c = i * size + rank;
+      p[i] = c < cols ? ldf(xr + c) : 0.f;
+      if constexpr (ADD) res[i] = c < cols ? ldf(rr + c) : 0.f;
+      w[i] = c < cols ? ld_any(a.w, a.w_dtype, c) : 0.f;
+    }
+    if constexpr (ADD) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int c = i * size + rank;
+        p[i] = __fadd_rn(p[i], res[i]);
+        if (c < cols) p[i] = st_any(ro, Code<TR>::value, c, p[i]);
+      }
+    }
+  } else {
+    Raw<TX, VEC> raw[EACH / VEC];
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) load_raw(raw[v], xr + col);
+      else raw[v] = Raw<TX, VEC>{};
+    }
+    if constexpr (ADD) {
+      Raw<TR, VEC> res[EACH / VEC];
+#pragma unroll
+      for (int v = 0; v < EACH / VEC; ++v) {
+        const int col = (v * size + rank) * VEC;
+        if (col < cols) load_raw(res[v], rr + col);
+        else res[v] = Raw<TR, VEC>{};
+      }
+#pragma unroll
+      for (int v = 0; v < EACH / VEC; ++v) {
+        const int col = (v * size + rank) * VEC;
+        float f[VEC], h[VEC];
+        to_f32(raw[v], f);
+        to_f32(res[v], h);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[i] = __fadd_rn(f[i], h[i]);
+        from_f32(res[v], h);
+        to_f32(res[v], p + v * VEC);  // as it is held
+        if (col < cols) store_raw(ro + col, res[v]);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < EACH / VEC; ++v) to_f32(raw[v], p + v * VEC);
+    }
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) {
+        load_weight<VEC>(a.w, a.w_dtype, col, w + v * VEC);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[v * VEC + i] = 0.f;
+      }
+    }
+  }
+  double ss = 0.0, ss2 = 0.0;
+  float top_here = 0.f;
+#pragma unroll
+  for (int i = 0; i < EACH; i += 2) {
+    const double h0 = (double)p[i], h1 = (double)p[i + 1];
+    ss = fma(h0, h0, ss);
+    ss2 = fma(h1, h1, ss2);
+  }
+  ss += ss2;
+#pragma unroll
+  for (int i = 0; i < EACH; i += 2) {
+    p[i] = __fmul_rn(p[i], w[i]);
+    p[i + 1] = __fmul_rn(p[i + 1], w[i + 1]);
+    top_here = max_abs3(top_here, p[i], p[i + 1]);
+  }
+  const uint32_t mine = __float_as_uint(top_here);  // as integers: NaN above infinity above all numbers
+  uint32_t most = mine;
+  team.sum_max(ss, most);
+  const double rs = rsqrt(fma(ss, a.inv_cols, (double)a.eps));
+  const void *hp = ADD ? (const void *)ro : (const void *)xr;  // a thread reads back only what it has stored itself
+  auto h_at = [&](int col) { return (double)ldf((const TH *)hp + col); };
+  int8_t *out = a.codes + row * a.ld_codes;
+  if (most >= TINY && most <= HUGE_ && rs < 1e30) {
+    double top = 0.0;
+    if (mine == most) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        if ((__float_as_uint(p[i]) & 0x7fffffffu) == most) {
+          const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
+          top = fmax(top, fabs(h_at(col) * rs * (double)ld_any(a.w, a.w_dtype, col)));
+        }
+      }
+    }
+    top = team.max_rare(top);
+    const float s = scale_of(top, false);
+    const float c = __fmul_rn((float)rs, __frcp_rn(s));
+    const uint32_t cb = __float_as_uint(c);
+    if (cb >= TINY && cb <= HUGE_) {
+      write_codes<VEC>(p, c, s, out, cols, rank, size,
+                       [&](int, int col) { return h_at(col) * rs * (double)ld_any(a.w, a.w_dtype, col); });
+      if (rank == 0) a.scale[row] = s;
+      return;
+    }
+  }
+  team.sync();  // what other threads of the team have stored of the row
+  slow_row(team, hp, Code<TH>::value, a.w, a.w_dtype, rs, cols, out, a.scale + row);
+}
+
+__global__ void __launch_bounds__(LONG_THREADS) norm_long_kernel(const NormArgs a) {
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  __shared__ Join join;
+  const Team<false> team{&join};
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    double ss = 0.0;
+    uint32_t none = 0;
+    for (int c = threadIdx.x; c < a.cols; c += LONG_THREADS) {
+      float h = ld_any(a.x, a.x_dtype, r * a.ld_x + c);
+      if (a.resid) h = st_any(a.r_out, a.r_dtype, r * a.ld_ro + c, __fadd_rn(h, ld_any(a.resid, a.r_dtype, r * a.ld_r + c)));
+      ss = fma((double)h, (double)h, ss);
+    }
+    team.sum_max(ss, none);
+    const double rs = rsqrt(fma(ss, a.inv_cols, (double)a.eps));
+    const int h_dtype = a.resid ? a.r_dtype : a.x_dtype;
+    const char *h = (const char *)(a.resid ? a.r_out : a.x) + r * (a.resid ? a.ld_ro : a.ld_x) * (h_dtype == MTP_F32 ? 4 : 2);
+    slow_row(team, h, h_dtype, a.w, a.w_dtype, rs, a.cols, a.codes + r * a.ld_codes, a.scale + r);
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ read back
+// A thread takes N codes of a row and writes 16 bytes (N = 1: rows of any alignment).
+template <typename T, int N, typename I>
+__global__ void __launch_bounds__(256) dequantize_kernel(const int8_t *__restrict__ codes, int64_t ld_codes,
+                                                         const float *__restrict__ scale, T *__restrict__ out, int64_t ld_out,
+                                                         I parts, I per_row) {
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+  uint32_t w[UNROLL][N / 4 + (N == 1)];
+  float s[UNROLL];
+  T *to[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const I i = ((I)blockIdx.x * UNROLL + u) * 256 + threadIdx.x;
+    to[u] = nullptr;
+    if (i < parts) {
+      const I r = i / per_row;
+      const int c = (int)(i - r * per_row) * N;
+      const int8_t *from = codes + (int64_t)r * ld_codes + c;
+      to[u] = out + (int64_t)r * ld_out + c;
+      s[u] = scale[r];
+      if constexpr (N == 1) {
+        w[u][0] = (uint8_t)*from;
+      } else if constexpr (N == 4) {
+        w[u][0] = *reinterpret_cast<const uint32_t *>(from);
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(from);
+        w[u][0] = v.x; w[u][1] = v.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    if (!to[u]) continue;
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = __fmul_rn((float)(int8_t)(w[u][k / 4] >> (8 * (k & 3))), s[u]);
+    if constexpr (N == 1) {
+      stf(to[u], v[0]);
+    } else {
+      Raw<T, N> raw;
+      from_f32(raw, v);
+      store_raw(to[u], raw);
+    }
+  }
+}
+
+template <typename T, int N>
+void launch_dequantize(const int8_t *codes, int64_t ld_codes, const float *scale, int64_t rows, int cols, T *out, int64_t ld_out,
+                       cudaStream_t s) {
+  const int64_t per_row = cols / N, parts = rows * per_row;
+  const dim3 grid((unsigned)((parts + 256 * UNROLL - 1) / (256 * UNROLL)));
+  if (parts < 0x7fff0000)
+    launch_pdl(dequantize_kernel<T, N, uint32_t>, grid, dim3(256), 0, s, codes, ld_codes, scale, out, ld_out, (uint32_t)parts,
+               (uint32_t)per_row);
+  else
+    launch_pdl(dequantize_kernel<T, N, int64_t>, grid, dim3(256), 0, s, codes, ld_codes, scale, out, ld_out, parts, per_row);
+}
+
+// ------------------------------------------------------------------ host side
 bool dtype_ok(int d) { return d == MTP_F32 || d == MTP_BF16 || d == MTP_F16; }
 bool rows_ok(int64_t rows, int cols) { return rows >= 0 && rows <= 0x7fffffffll && cols >= 1 && cols <= MAX_COLS; }
+int size_of(int dtype) { return dtype == MTP_F32 ? 4 : 2; }
+
+// Rows from p on, ld elements of es bytes apart, in vectors of n.
+bool on_vectors(const void *p, int64_t ld, int es, int64_t rows, int n) {
+  return aligned(p, es * n < 16 ? es * n : 16) && (rows == 1 || ld * es % (es * n < 16 ? es * n : 16) == 0);
+}
+
+// Threads of a team for rows of cols values, a warp at least.
+int team_of(int cols) { return cols <= 32 * E_OF_WARP ? 32 : ceil_div(cols, E_OF_CTA * 32) * 32; }
+
+template <typename T, int VEC>
+void launch_quantize(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
+                     cudaStream_t s) {
+  const int team = team_of(cols);
+  if (team == 32)
+    launch_pdl(quantize_kernel<T, VEC, true>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, x, ld, rows, cols, codes, ld_codes,
+               scale);
+  else
+    launch_pdl(quantize_kernel<T, VEC, false>, dim3((unsigned)rows), dim3(team), 0, s, x, ld, rows, cols, codes, ld_codes, scale);
+}
+
+template <typename TX, typename TR, int VEC> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
+  const int team = team_of(a.cols);
+  if (team == 32) launch_pdl(norm_kernel<TX, TR, VEC, true>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, s, a);
+  else launch_pdl(norm_kernel<TX, TR, VEC, false>, dim3((unsigned)a.rows), dim3(team), 0, s, a);
+}
+
+template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStream_t s) {
+  constexpr bool ADD = !std::is_same<TR, None>::value;
+  constexpr bool WIDE = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
+  constexpr int VEC = WIDE ? 4 : 8;  // 16 bytes of the wider type
+  const int er = size_of(a.r_dtype);
+  const bool vec = a.cols % VEC == 0 && on_vectors(a.x, a.ld_x, sizeof(TX), a.rows, VEC) &&
+                   on_vectors(a.w, 0, size_of(a.w_dtype), 1, VEC) && on_vectors(a.codes, a.ld_codes, 1, a.rows, VEC) &&
+                   (!ADD || (on_vectors(a.resid, a.ld_r, er, a.rows, VEC) && on_vectors(a.r_out, a.ld_ro, er, a.rows, VEC)));
+  if (vec) launch_norm_team<TX, TR, VEC>(a, s);
+  else launch_norm_team<TX, TR, 1>(a, s);
+}
+
+template <typename TX> bool launch_norm_of(const NormArgs &a, cudaStream_t s) {
+  if (!a.resid) launch_norm<TX, None>(a, s);
+  else if (a.r_dtype == MTP_F32) launch_norm<TX, float>(a, s);
+  else if (!std::is_same<TX, float>::value && a.r_dtype == Code<TX>::value) launch_norm<TX, TX>(a, s);
+  else return false;
+  return true;
+}
 
 }  // namespace
 }  // namespace mtp
@@ -148,10 +642,18 @@ int mtp_quantize_rows(const void *x, int dtype, int64_t ld, int64_t rows, int co
   MTP_REQUIRE(dtype_ok(dtype), "dtype must be F32, BF16 or F16");
   if (rows == 0) return MTP_OK;
   MTP_REQUIRE(x && codes && scale, "null pointer");
-  MTP_REQUIRE((rows == 1 || ld >= cols) && (rows == 1 || ld_codes >= cols), "leading dimensions too small");
+  MTP_REQUIRE(rows == 1 || (ld >= cols && ld_codes >= cols), "leading dimensions too small");
   cudaStream_t s = (cudaStream_t)stream;
-  MTP_DISPATCH_3(dtype, T, launch_pdl(quantize_kernel<T>, dim3(grid_for(rows)), dim3(THREADS), 0, s, (const T *)x, ld, rows,
-                                      cols, codes, ld_codes, scale));
+  MTP_DISPATCH_3(dtype, T, {
+    constexpr int VEC = sizeof(T) == 4 ? 4 : 8;
+    if (cols > MAX_TEAM * E_OF_CTA)
+      launch_pdl(quantize_long_kernel<T>, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s,
+                 (const T *)x, ld, rows, cols, codes, ld_codes, scale);
+    else if (cols % VEC == 0 && on_vectors(x, ld, sizeof(T), rows, VEC) && on_vectors(codes, ld_codes, 1, rows, VEC))
+      launch_quantize<T, VEC>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
+    else
+      launch_quantize<T, 1>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
+  });
   return check_launch("quantize_rows");
 }
 
@@ -163,8 +665,13 @@ int mtp_dequantize_rows(const int8_t *codes, int64_t ld_codes, const float *scal
   MTP_REQUIRE(codes && scale && out, "null pointer");
   MTP_REQUIRE(rows == 1 || (ld_codes >= cols && ld_out >= cols), "leading dimensions too small");
   cudaStream_t s = (cudaStream_t)stream;
-  MTP_DISPATCH_3(out_dtype, T, launch_pdl(dequantize_kernel<T>, dim3(grid_for(rows)), dim3(THREADS), 0, s, codes, ld_codes,
-                                          scale, rows, cols, (T *)out, ld_out));
+  MTP_DISPATCH_3(out_dtype, T, {
+    constexpr int N = 16 / sizeof(T);
+    if (cols % N == 0 && on_vectors(codes, ld_codes, 1, rows, N) && on_vectors(out, ld_out, sizeof(T), rows, N))
+      launch_dequantize<T, N>(codes, ld_codes, scale, rows, cols, (T *)out, ld_out, s);
+    else
+      launch_dequantize<T, 1>(codes, ld_codes, scale, rows, cols, (T *)out, ld_out, s);
+  });
   return check_launch("dequantize_rows");
 }
 
@@ -179,8 +686,12 @@ int mtp_rmsnorm_int8(const void *x, int x_dtype, int64_t ld_x, const void *resid
   MTP_REQUIRE(rows == 1 || (ld_x >= cols && ld_codes >= cols && (!resid || (ld_resid >= cols && ld_resid_out >= cols))),
               "leading dimensions too small");
   cudaStream_t s = (cudaStream_t)stream;
-  launch_pdl(rmsnorm_int8_kernel, dim3(grid_for(rows)), dim3(THREADS), 0, s, x, x_dtype, ld_x, resid, resid_dtype, ld_resid,
-             resid_out, ld_resid_out, rows, cols, w, w_dtype, eps, codes, ld_codes, scale);
+  const NormArgs a{x, resid, resid_out, w, ld_x, ld_resid, ld_resid_out, rows, cols, x_dtype, resid_dtype, w_dtype, eps, codes,
+                   ld_codes, scale, 1.0 / cols};
+  bool done = false;
+  if (cols <= MAX_TEAM * E_OF_CTA) MTP_DISPATCH_3(x_dtype, T, done = launch_norm_of<T>(a, s));
+  if (!done)  // long rows, and a 16-bit stream of another type than x
+    launch_pdl(norm_long_kernel, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s, a);
   return check_launch("rmsnorm_int8");
 }
 
