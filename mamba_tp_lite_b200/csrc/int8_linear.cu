@@ -78,6 +78,7 @@ extern "C" int mtp_int8_linear(const int8_t *a, int64_t ld_a, const float *a_sca
   MTP_REQUIRE((M == 1 || (ld_a >= K && ld_out >= N)) && (N == 1 || ld_w >= K), "leading dimensions too small");
   cudaStream_t s = (cudaStream_t)stream;
   const Out o{out, ld_out, out_dtype, a_scale, w_scale, bias, bias_dtype};
+  if (M <= FEW && tc_eligible(a, ld_a, M, w, ld_w, N)) return linear_few(a, ld_a, M, K, w, ld_w, N, o, s);
   if (tc_eligible(a, ld_a, M, w, ld_w, N)) return linear_tc(a, ld_a, M, K, w, ld_w, N, o, s);
   const int tiles_n = ceil_div(N, 64);
   const int64_t tiles = (int64_t)ceil_div(M, 64) * tiles_n;

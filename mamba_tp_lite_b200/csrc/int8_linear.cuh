@@ -39,5 +39,10 @@ bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t 
 int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
               cudaStream_t stream);
 
+// For few tokens; operands on 16-byte boundaries as above.
+constexpr int FEW = 16;
+int linear_few(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
+               cudaStream_t stream);
+
 }  // namespace i8
 }  // namespace mtp

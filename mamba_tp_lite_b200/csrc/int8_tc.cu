@@ -363,6 +363,184 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
+// ------------------------------------------------------------------ at most 128 tokens
+// One tile of up to 128 tokens x bn channels per cluster, its K split over the cluster's CTAs, so that as many SMs as there
+// are stream w and most of a CTA's copies are in flight at once; each CTA's int32 sums go to its shared memory, and the
+// cluster adds them there (exact in any order).
+constexpr int SPLIT_THREADS = 64 + 32 * EPI_WARPS;  // TMA, MMA and epilogue warps; all of them add
+constexpr int SPLIT_RING = 108 * 1024;  // two CTAs fit an SM: the next call's are set up while this one's work
+constexpr int SPLIT_MAX_STAGES = 24;
+constexpr int SPLIT_SCALES = SPLIT_RING, SPLIT_BARS = SPLIT_SCALES + 3 * 128 * 4;
+constexpr int SPLIT_SMEM = SPLIT_BARS + 512 + 1024;
+
+struct SplitParams {
+  Out o;
+  int M, N, K;
+  int bn, a_rows, stages, slot, split;
+  int vec_out;
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__global__ void __launch_bounds__(SPLIT_THREADS, 1)
+    int8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const SplitParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn);
+  const uint32_t base = (raw + 1023u) & ~1023u;  // the same in all CTAs of a cluster
+  unsigned char *gbase = smem_dyn + (base - raw);
+  const uint32_t bar0 = base + SPLIT_BARS;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (SPLIT_MAX_STAGES + s); };
+  const uint32_t done_bar = bar0 + 8u * (2 * SPLIT_MAX_STAGES);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(gbase + SPLIT_BARS + 8 * (2 * SPLIT_MAX_STAGES + 1));
+  volatile int *abort = reinterpret_cast<volatile int *>(gbase + SPLIT_BARS + 8 * (2 * SPLIT_MAX_STAGES + 1) + 8);
+  const uint32_t abort_at = bar0 + 8u * (2 * SPLIT_MAX_STAGES + 1) + 8u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int n0 = (int)(blockIdx.x / p.split) * p.bn;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int kb0 = (int)((long)num_kb * rank / p.split), kb1 = (int)((long)num_kb * (rank + 1) / p.split);
+
+  MTP_PDL_TRIGGER();
+  if (threadIdx.x == 0) {
+    // w on its way to L2 (where a write of the kernel before would meet it) while that kernel ends
+    for (int kb = kb0; kb < kb1 && kb < kb0 + p.stages; ++kb)
+      asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&tmB), "r"(kb * BK), "r"(n0)
+                   : "memory");
+    for (int s = 0; s < p.stages && s < kb1 - kb0; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_u32(tmem_holder)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  MTP_PDL_WAIT();
+  const uint32_t tmem_base = *tmem_holder;
+  constexpr int LD_PART = 132;  // of a token's sums, in words: 16-byte writes of a warp's rows meet each bank equally often
+  int *part = reinterpret_cast<int *>(gbase);
+  float *scale_w = reinterpret_cast<float *>(gbase + SPLIT_SCALES), *bias_w = scale_w + 128, *scale_a = scale_w + 256;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t tx_bytes = (uint32_t)((p.a_rows + p.bn) * BK);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (kb >= kb0 + p.stages && !mbar_wait(empty_bar(s), ph ^ 1u, abort, TIMEOUT_NS)) break;
+        mbar_expect_tx(full_bar(s), tx_bytes);
+        const uint32_t sa = base + s * p.slot;
+        tma_load_2d(sa, &tmA, full_bar(s), kb * BK, 0);
+        tma_load_2d(sa + p.a_rows * BK, &tmB, full_bar(s), kb * BK, n0);
+        if (++s == p.stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) break;
+        tc_fence_after();
+        const uint32_t sa = base + s * p.slot;
+        const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + p.a_rows * BK);
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k)
+          mma<1>(tmem_base, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), p.idesc, (kb > kb0) || k != 0);
+        commit<1>(empty_bar(s));
+        if (++s == p.stages) { s = 0; ph ^= 1u; }
+      }
+      commit<1>(done_bar);  // after an expired wait for what has been issued
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    if (threadIdx.x - 64 < 128) {  // the scales come while the sums are made
+      const int i = threadIdx.x - 64;
+      const bool in = i < p.bn && n0 + i < p.N;
+      scale_w[i] = in ? p.o.w_scale[n0 + i] : 0.f;
+      bias_w[i] = in ? ld_bias(p.o, n0 + i) : 0.f;
+      scale_a[i] = i < p.M ? p.o.a_scale[i] : 0.f;
+    }
+    const bool alive = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort, TIMEOUT_NS + TIMEOUT_NS / 2));
+    tc_fence_after();
+    if (alive && q * 32 < p.M) {
+      const int m = q * 32 + lane;
+      for (int c = 32 * half; c < p.bn; c += 64) {
+        int r[32];
+        tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+        if (m < p.M) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (c + i < p.bn)
+              *reinterpret_cast<int4 *>(part + m * LD_PART + c + i) = make_int4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  {
+    const int quads = p.bn / 4, total = p.M * quads;
+    bool lost = false;
+    for (int i = 0; i < p.split; ++i) {
+      int v;
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(abort_at, i)));
+      lost |= v != 0;
+    }
+    for (int e = (int)rank * SPLIT_THREADS + threadIdx.x; e < total; e += p.split * SPLIT_THREADS) {
+      const int m = e / quads, c = (e - m * quads) * 4, n = n0 + c;
+      if (n >= p.N) continue;
+      const uint32_t at = base + (uint32_t)(m * LD_PART + c) * 4u;
+      int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+      for (int i = 0; i < p.split; ++i) {
+        const int4 v = ld_cluster(cluster_addr(at, i));
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+      }
+      const float sa = scale_a[m];
+      const int in = min(4, p.N - n);
+      float y[4] = {(float)sum.x, (float)sum.y, (float)sum.z, (float)sum.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = __fmul_rn(__fmul_rn(y[i], sa), scale_w[c + i]);
+        if (p.o.bias) y[i] = __fadd_rn(y[i], bias_w[c + i]);
+        if (lost) y[i] = __int_as_float(0x7fffffff);
+      }
+      if (p.vec_out && in == 4) {
+        const int64_t to = (int64_t)m * p.o.ld + n;
+        if (p.o.dtype == MTP_F32) *reinterpret_cast<float4 *>((float *)p.o.p + to) = make_float4(y[0], y[1], y[2], y[3]);
+        else if (p.o.dtype == MTP_BF16)
+          *reinterpret_cast<uint2 *>((__nv_bfloat16 *)p.o.p + to) = make_uint2(pack2<__nv_bfloat16>(y[0], y[1]), pack2<__nv_bfloat16>(y[2], y[3]));
+        else *reinterpret_cast<uint2 *>((__half *)p.o.p + to) = make_uint2(pack2<__half>(y[0], y[1]), pack2<__half>(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < in) store_value(p.o, m, n + i, y[i]);
+      }
+    }
+  }
+  if (*abort) __nanosleep(1000000);  // copies in flight
+  cluster_sync();                    // no other CTA reads this one's sums any more
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem_base));
+}
+
 // 2-D map over bytes [rows, cols] with ld bytes between rows; boxes of 128 bytes x box_rows, zeros outside.
 int map_codes(CUtensorMap *tm, const void *ptr, int rows, int cols, int64_t ld, int box_rows) {
   EncodeTiledFn fn = encode_fn();
@@ -470,6 +648,77 @@ int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld
   return launch<CG, __half>(ta, tb, tcm, p, stream);
 }
 
+// The kernel's limit of shared memory belongs to the current device.
+int allow_split_smem() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load() & bit) return MTP_OK;
+  if (cudaFuncSetAttribute(int8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SPLIT_SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(MTP_ERR_CUDA, "int8_split: shared memory");
+  }
+  done.fetch_or(bit);
+  return MTP_OK;
+}
+
+int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
+              cudaStream_t stream) {
+  SplitParams p{};
+  p.o = o;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.a_rows = (M + 7) / 8 * 8;
+  const int sms = num_sms(), num_kb = ceil_div(K, BK);
+  // The split with the least time: measured, a call takes 5.3 us and a CTA's bytes at 62 KB/us (64 x 2048 -> 8192 in one, 256
+  // KB: 9.5 us; 64 x 4096 -> 2048 in four, 131 KB: 7.2 us, in one, 524 KB: 12.9), the addition 0.5 us, a further wave 2 us.
+  double best = 1e30;
+  for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
+    int bn = (ceil_div((int64_t)N * split, sms) + 15) / 16 * 16;
+    bn = bn < 32 ? 32 : bn > 128 ? 128 : bn;
+    const int64_t waves = ((int64_t)ceil_div(N, bn) * split + sms - 1) / sms;
+    const double bytes = (double)ceil_div(num_kb, split) * (bn + p.a_rows) * BK;
+    const double cost = (double)waves * bytes + (double)(waves - 1) * 124e3 + (split > 1 ? 31e3 : 0.0);
+    if (cost < best) {
+      best = cost;
+      p.split = split;
+      p.bn = bn;
+    }
+  }
+  p.slot = (p.a_rows + p.bn) * BK;
+  // rows of tokens past a_rows are read by the tensor core from what follows in the slot: the last slot ends 128 rows in
+  p.stages = (SPLIT_RING - (BM - p.a_rows) * BK) / p.slot;
+  if (p.stages > SPLIT_MAX_STAGES) p.stages = SPLIT_MAX_STAGES;
+  p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  const size_t es = o.dtype == MTP_F32 ? 4 : 2;
+  p.vec_out = aligned(o.p, 4 * es) && (M == 1 || o.ld % 4 == 0);
+  CUtensorMap ta, tb;
+  int rc = map_codes(&ta, a, M, K, ld_a, p.a_rows);
+  if (rc) return rc;
+  rc = map_codes(&tb, w, N, K, ld_w, p.bn);
+  if (rc) return rc;
+  rc = allow_split_smem();
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ceil_div(N, p.bn) * p.split);
+  cfg.blockDim = dim3(SPLIT_THREADS);
+  cfg.dynamicSmemBytes = SPLIT_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, int8_split_kernel, ta, tb, p);
+  return check_launch("int8_linear");
+}
+
 }  // namespace
 
 bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t ld_w, int N) {
@@ -480,7 +729,8 @@ bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t 
 int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
               cudaStream_t stream) {
   const int sms = num_sms();
-  if (M > BM && (int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN_MAX) * 2 >= sms)
+  if (M <= BM) return run_split(a, ld_a, M, K, w, ld_w, N, o, stream);
+  if ((int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN_MAX) * 2 >= sms)
     return run<2>(a, ld_a, M, K, w, ld_w, N, o, BN_MAX, stream);
   int bn = 128;
   while (bn > 64 && (int64_t)ceil_div(M, BM) * ceil_div(N, bn) < sms) bn /= 2;

@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .logprobs import _call, _refuse_tangent
@@ -30,30 +31,27 @@ class Int8Rows(NamedTuple):
 # ------------------------------------------------------------------ arguments
 def _refuse_grad(what: str, *tensors) -> None:
     grad = torch.is_grad_enabled()
+    dual = forward_ad._current_level >= 0
     for t in tensors:
         if t is None:
             continue
         if grad and t.requires_grad:
             raise RuntimeError(f"{what} has no gradient; call it under torch.no_grad()")
-        _refuse_tangent(t, what)
-
-
-def _check_rows(x: torch.Tensor, what: str, name: str) -> None:
-    L.require_cuda(x, what)
-    L.dtype_code(x.dtype)
-    _check_shape(x, what, name)
+        if dual:
+            _refuse_tangent(t, what)
 
 
 def _check_shape(x: torch.Tensor, what: str, name: str) -> None:
-    if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_COLS:
-        raise ValueError(f"{what}: {name} needs a last dimension of 1 to {MAX_COLS}, got shape {tuple(x.shape)}")
-    if x.numel() // x.shape[-1] > MAX_ROWS:
+    L.require_cuda(x, what)
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= MAX_COLS:
+        raise ValueError(f"{what}: {name} needs a last dimension of 1 to {MAX_COLS}, got shape {tuple(shape)}")
+    if x.numel() > MAX_ROWS * shape[-1]:
         raise ValueError(f"{what}: {name} has more than {MAX_ROWS} rows")
 
 
 def _check_codes(r: Int8Rows, what: str, name: str) -> None:
     codes, scale = r
-    L.require_cuda(codes, what)
     if codes.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError(f"{what}: {name} needs int8 codes and float32 scales, got {codes.dtype} and {scale.dtype}")
     _check_shape(codes, what, name)
@@ -69,13 +67,21 @@ def _same_device(t: torch.Tensor, x: torch.Tensor, what: str, name: str) -> None
 
 
 def _as_rows(x: torch.Tensor):
-    """(x as [rows, C] with dense rows, the stride between rows); copied where the leading dimensions have no common stride."""
+    """(x as [rows, C] with dense rows, rows, C, the stride between rows); copied where the leading dimensions have no common
+    stride."""
     c = x.shape[-1]
     if x.dim() != 2:
         x = x.reshape(-1, c)
-    if (x.stride(1) != 1 and c > 1) or (x.shape[0] > 1 and x.stride(0) < c):
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else c)
+    rows, (ld, step) = x.shape[0], x.stride()
+    if (step != 1 and c > 1) or (rows > 1 and ld < c):
+        x, ld = x.contiguous(), c
+    return x, rows, c, (ld if rows > 1 else c)
+
+
+def _flat(scale: torch.Tensor) -> torch.Tensor:
+    if scale.dim() != 1:
+        scale = scale.reshape(-1)
+    return scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _extent(x: torch.Tensor):
@@ -92,10 +98,10 @@ def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
 def _new_rows(x: torch.Tensor):
     """Uninitialised (codes, scale, stride) for rows like those of x; each row of codes starts on a 16-byte boundary, as the
     tensor-core product wants it."""
-    lead, c = x.shape[:-1], x.shape[-1]
+    *lead, c = x.shape
     wide = (c + 15) // 16 * 16
-    codes = torch.empty((*lead, wide), device=x.device, dtype=torch.int8)
-    scale = torch.empty(lead, device=x.device, dtype=torch.float32)
+    codes = x.new_empty(*lead, wide, dtype=torch.int8)
+    scale = x.new_empty(lead, dtype=torch.float32)
     return (codes if wide == c else codes[..., :c]), scale, wide
 
 
@@ -104,12 +110,12 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """int8 rows of x [..., C]: scale = max(max |x|, 1e-8) / 127 in float32, a code is the nearest multiple of it (ties to
     even), -127 to 127.  A row with a NaN or an infinity has scale NaN and codes 0."""
     what = "quantize_rows"
-    _check_rows(x, what, "x")
+    _check_shape(x, what, "x")
+    code = L.dtype_code(x.dtype)
     _refuse_grad(what, x)
     codes, scale, ld_codes = _new_rows(x)
-    x, ld = _as_rows(x)
-    _call(x, "mtp_quantize_rows", x.data_ptr(), L.dtype_code(x.dtype), ld, x.shape[0], x.shape[1], codes.data_ptr(), ld_codes,
-          scale.data_ptr())
+    x, rows, c, ld = _as_rows(x)
+    _call(x, "mtp_quantize_rows", x.data_ptr(), code, ld, rows, c, codes.data_ptr(), ld_codes, scale.data_ptr())
     return Int8Rows(codes, scale)
 
 
@@ -117,19 +123,19 @@ def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> torch
     """What the rows stand for: codes * scale, the float32 product rounded to ``dtype``."""
     what = "dequantize_rows"
     _check_codes(rows, what, "rows")
+    codes, scale = rows
     code = L.dtype_code(dtype)
-    _refuse_grad(what, rows.scale)
-    out = torch.empty(rows.codes.shape, device=rows.codes.device, dtype=dtype)
-    codes, ld = _as_rows(rows.codes)
-    scale = rows.scale.reshape(-1).contiguous()
-    _call(codes, "mtp_dequantize_rows", codes.data_ptr(), ld, scale.data_ptr(), codes.shape[0], codes.shape[1], out.data_ptr(), code,
-          codes.shape[1])
+    _refuse_grad(what, scale)
+    out = codes.new_empty(codes.shape, dtype=dtype)
+    codes, n, c, ld = _as_rows(codes)
+    scale = _flat(scale)
+    _call(codes, "mtp_dequantize_rows", codes.data_ptr(), ld, scale.data_ptr(), n, c, out.data_ptr(), code, c)
     return out
 
 
 def _norm(x, residual, weight, eps, inplace, what):
-    _check_rows(x, what, "x")
-    c = x.shape[-1]
+    _check_shape(x, what, "x")
+    x_code, c = L.dtype_code(x.dtype), x.shape[-1]
     if weight.shape != (c,):
         raise ValueError(f"{what}: weight has shape {tuple(weight.shape)}, expected {(c,)}")
     _same_device(weight, x, what, "weight")
@@ -140,14 +146,13 @@ def _norm(x, residual, weight, eps, inplace, what):
     _refuse_grad(what, x, residual, weight)
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    codes, scale, ld_codes = _new_rows(x)
     h, res_args = None, (None, 0, 0, None, 0)
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
         _same_device(residual, x, what, "residual")
         r_code = L.dtype_code(residual.dtype)
-        res, ld_res = _as_rows(residual)
+        res, _, _, ld_res = _as_rows(residual)
         if inplace:
             if res.data_ptr() != residual.data_ptr():
                 raise ValueError(f"{what}: a residual that is updated in place needs rows on one stride")
@@ -155,11 +160,12 @@ def _norm(x, residual, weight, eps, inplace, what):
                 raise ValueError(f"{what}: a residual that is updated in place must not share memory with x")
             h, ld_h = residual, ld_res
         else:
-            h, ld_h = torch.empty(residual.shape, device=x.device, dtype=residual.dtype), c
+            h, ld_h = residual.new_empty(residual.shape), c
         res_args = (res.data_ptr(), r_code, ld_res, h.data_ptr(), ld_h)
-    x, ld = _as_rows(x)
-    _call(x, "mtp_rmsnorm_int8", x.data_ptr(), L.dtype_code(x.dtype), ld, *res_args, x.shape[0], c, weight.data_ptr(), w_code, eps,
-          codes.data_ptr(), ld_codes, scale.data_ptr())
+    codes, scale, ld_codes = _new_rows(x)
+    x, rows, _, ld = _as_rows(x)
+    _call(x, "mtp_rmsnorm_int8", x.data_ptr(), x_code, ld, *res_args, rows, c, weight.data_ptr(), w_code, eps, codes.data_ptr(),
+          ld_codes, scale.data_ptr())
     return Int8Rows(codes, scale), h
 
 
@@ -196,10 +202,10 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
         b_code = L.dtype_code(bias.dtype)
         bias = bias.contiguous()
     _refuse_grad(what, x.scale, weight.scale, bias)
-    out = torch.empty((*x.codes.shape[:-1], n), device=wc.device, dtype=dtype)
-    a, ld_a = _as_rows(x.codes)
-    wc, ld_w = _as_rows(wc)
-    a_scale, w_scale = x.scale.reshape(-1).contiguous(), weight.scale.contiguous()
-    _call(a, "mtp_int8_linear", a.data_ptr(), ld_a, a_scale.data_ptr(), a.shape[0], k, wc.data_ptr(), ld_w, w_scale.data_ptr(),
-          n, L.ptr(bias), b_code, out.data_ptr(), code, n)
+    out = wc.new_empty(*x.codes.shape[:-1], n, dtype=dtype)
+    a, m, _, ld_a = _as_rows(x.codes)
+    wc, _, _, ld_w = _as_rows(wc)
+    a_scale, w_scale = _flat(x.scale), _flat(weight.scale)
+    _call(a, "mtp_int8_linear", a.data_ptr(), ld_a, a_scale.data_ptr(), m, k, wc.data_ptr(), ld_w, w_scale.data_ptr(), n,
+          L.ptr(bias), b_code, out.data_ptr(), code, n)
     return out
