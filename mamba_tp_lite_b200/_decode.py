@@ -38,6 +38,8 @@ def supported(lm) -> str | None:
     if os.environ.get("MTP_DECODE_FUSED", "1") == "0":
         return "disabled by MTP_DECODE_FUSED=0"
     cfg = lm.cfg
+    if lm.layers[0].mixer._int8 is not None:
+        return "int8 linears"
     if lm.embedding.weight.dtype != torch.bfloat16:
         return "model dtype is not bf16"
     if cfg.d_state != 16 or cfg.d_conv != 4:

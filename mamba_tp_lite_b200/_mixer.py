@@ -18,6 +18,10 @@ One mixer forward is this chain of libmtp calls (T = batch x positions):
 
 Activations stay in the model dtype; the residual stream, the reduction
 partials, dt, B, C and the SSM state are fp32.
+
+A dense mixer with int8 linears (``MambaLM.quantize_linears``) takes its in_proj input
+as int8 rows, quantises y in front of out_proj, and hands the out_proj result to
+``add_rms_norm_int8`` in fp32; conv1d, x_proj, dt_proj and the scan are as above.
 """
 from __future__ import annotations
 
@@ -26,6 +30,7 @@ import os
 import torch
 
 from . import _lib as L
+from .int8 import Int8Rows, int8_linear, quantize_rows
 from .tp_utils import KERNEL_MODES, ROW_MODES, comm_for, count_collective
 
 # Optional launch timing for benchmarks: when set to a dict, CUDA events are
@@ -77,6 +82,8 @@ class MixerKernels:
     ``layer_idx``, ``_site_modes`` ({"x_proj": name, "out_proj": name} or None
     for the dense mixer) and ``comm`` (CommCounter) and ``_out_bias()``."""
 
+    _int8 = None  # (in_proj, out_proj) weights as Int8Rows, a scale for each output channel
+
     # ------------------------------------------------------------ helpers
     def _dt(self) -> torch.dtype:
         return self.in_proj.weight.dtype
@@ -89,6 +96,26 @@ class MixerKernels:
                L.dtype_code(a.dtype), L.dtype_code(out.dtype), epi, L.ptr(bias),
                L.dtype_code(bias.dtype) if bias is not None else 0, L.stream_ptr())
         _prof_end(ev, tag, 2.0 * M * N * K)
+
+    def _in_proj(self, xn, tag):
+        """xz = in_proj(xn) in the model dtype; xn [T, D], or its int8 rows for int8 linears."""
+        w, bias, dt_ = self.in_proj.weight, self.in_proj.bias, self._dt()
+        if isinstance(xn, Int8Rows):
+            ev = _prof_begin()
+            xz = int8_linear(xn, self._int8[0], None if bias is None else bias.detach(), dtype=dt_)
+            _prof_end(ev, tag, 2.0 * xz.numel() * w.shape[1])
+            return xz
+        xz = torch.empty(xn.shape[0], 2 * self.es, device=xn.device, dtype=dt_)
+        self._gemm(xn, w, xz, *((L.EPI_BIAS, bias) if bias is not None else (L.EPI_STORE, None)), tag=tag)
+        return xz
+
+    def _out_proj_int8(self, y, tag):
+        """out_proj(y) + bias in fp32 through int8 linears: what is added to the residual stream."""
+        rows, bias = quantize_rows(y), self._out_bias()
+        ev = _prof_begin()
+        out = int8_linear(rows, self._int8[1], None if bias is None else bias.detach(), dtype=torch.float32)
+        _prof_end(ev, tag, 2.0 * out.numel() * y.shape[1])
+        return out
 
     def _check_input(self, x: torch.Tensor, what: str):
         L.require_cuda(x, what)
@@ -202,13 +229,32 @@ class MixerKernels:
         """_prefill_core as a generator: it yields once, after AllReduce #1 has been
         issued, so a driver can interleave the launches of several micro-batches."""
         cfg = self.cfg
+        y, conv_final, ssm_final = yield from self._prefill_mix(self._in_proj(xn, "in_proj"), B, Lq, conv_init, ssm_init,
+                                                                conv_out, ssm_out)
+        partial_o = torch.empty(xn.shape[0], cfg.d_model, device=xn.device, dtype=torch.float32)
+        self._gemm(y, self.out_proj.weight, partial_o, tag="out_proj")
+        self._reduce_out(partial_o, resid, norm_w, eps, normed)
+        return conv_final, ssm_final
+
+    def _prefill_int8(self, rows, B, Lq, conv_init, ssm_init):
+        """rows: int8 rows [T, D] of the block input.  Returns (mixer output fp32 [T, D], conv_final, ssm_final)."""
+        g = self._prefill_mix(self._in_proj(rows, "in_proj"), B, Lq, conv_init, ssm_init)
+        next(g)
+        try:
+            next(g)
+        except StopIteration as done:
+            y, conv_final, ssm_final = done.value
+            return self._out_proj_int8(y, "out_proj"), conv_final, ssm_final
+        raise RuntimeError("prefill stages did not finish")
+
+    def _prefill_mix(self, xz, B, Lq, conv_init, ssm_init, conv_out=None, ssm_out=None):
+        """From in_proj's output xz [T, 2Es] to out_proj's input: (y [T, Es], conv_final, ssm_final), as a generator that
+        yields once, after AllReduce #1 has been issued."""
+        cfg = self.cfg
         es, n, r, k = self.es, cfg.d_state, cfg.dt_rank, cfg.d_conv
-        T = xn.shape[0]
+        T = xz.shape[0]
         dt_ = self._dt()
-        dev = xn.device
-        xz = torch.empty(T, 2 * es, device=dev, dtype=dt_)
-        self._gemm(xn, self.in_proj.weight, xz, *((L.EPI_BIAS, self.in_proj.bias) if self.in_proj.bias is not None
-                                                  else (L.EPI_STORE, None)), tag="in_proj")
+        dev = xz.device
         conv_w = self.conv1d.weight
         conv_b = self.conv1d.bias
         xc = torch.empty(T, es, device=dev, dtype=dt_)
@@ -235,10 +281,7 @@ class MixerKernels:
                    L.ptr(conv_b), L.ptr(conv_init), L.ptr(ssm_init), L.ptr(y), es, L.ptr(conv_final),
                    L.ptr(ssm_final), B, Lq, es, n, r, k, L.stream_ptr())
             _prof_end(ev, "scan", T * (es * 3 * esz + (r + 2 * n) * 4) + B * es * (2 * n * 4 + 2 * (k - 1) * esz))
-            partial_o = torch.empty(T, cfg.d_model, device=dev, dtype=torch.float32)
-            self._gemm(y, self.out_proj.weight, partial_o, tag="out_proj")
-            self._reduce_out(partial_o, resid, norm_w, eps, normed)
-            return conv_final, ssm_final
+            return y, conv_final, ssm_final
         # dt = softplus(dt_proj(dt_low)) in the model dtype, as the reference's dt_proj output
         # (tp_model.py:110-111); the scan widens it to fp32
         dt = torch.empty(T, es, device=dev, dtype=dt_)
@@ -250,27 +293,38 @@ class MixerKernels:
                L.ptr(conv_final), L.ptr(ssm_final), B, Lq, es, n, k, L.dtype_code(dt_), L.stream_ptr())
         # algorithmic bytes: x, z, dt, y in the model dtype, B|C fp32 (+ per-sequence state I/O)
         _prof_end(ev, "scan", T * (es * 4 * esz + 2 * n * 4) + B * es * (2 * n * 4 + 2 * (k - 1) * esz))
-        partial_o = torch.empty(T, cfg.d_model, device=dev, dtype=torch.float32)
-        self._gemm(y, self.out_proj.weight, partial_o, tag="out_proj")
-        self._reduce_out(partial_o, resid, norm_w, eps, normed)
-        return conv_final, ssm_final
+        return y, conv_final, ssm_final
 
     # ------------------------------------------------------------ step core
     def _step_core(self, xn, conv_state, ssm_state, resid, norm_w=None, eps=0.0, normed=None):
         """xn [B, D] (model dtype).  Updates conv_state [B,Es,K-1] and
         ssm_state [B,Es,N] (fp32) in place; adds the output into resid."""
-        cfg = self.cfg
-        es, n, r, k = self.es, cfg.d_state, cfg.dt_rank, cfg.d_conv
-        Bn = xn.shape[0]
-        dt_ = self._dt()
-        dev = xn.device
+        self._check_states(conv_state, ssm_state)
+        y = self._step_mix(self._in_proj(xn, "d_in_proj"), conv_state, ssm_state)
+        partial_o = torch.empty(xn.shape[0], self.cfg.d_model, device=xn.device, dtype=torch.float32)
+        self._gemm(y, self.out_proj.weight, partial_o, tag="d_out_proj")
+        ev = _prof_begin()
+        self._reduce_out(partial_o, resid, norm_w, eps, normed)
+        _prof_end(ev, "d_reduce_out", 0)
+
+    def _step_int8(self, rows, conv_state, ssm_state):
+        """rows: int8 rows [B, D].  Updates the states in place; returns the mixer output fp32 [B, D]."""
+        self._check_states(conv_state, ssm_state)
+        return self._out_proj_int8(self._step_mix(self._in_proj(rows, "d_in_proj"), conv_state, ssm_state), "d_out_proj")
+
+    def _check_states(self, conv_state, ssm_state):
         if ssm_state.dtype != torch.float32:
             raise TypeError("ssm_state must be float32 (allocate the cache with MambaCache.allocate)")
-        if conv_state.dtype != dt_:
-            raise TypeError(f"conv_state dtype {conv_state.dtype} != model dtype {dt_}")
-        xz = torch.empty(Bn, 2 * es, device=dev, dtype=dt_)
-        self._gemm(xn, self.in_proj.weight, xz, *((L.EPI_BIAS, self.in_proj.bias) if self.in_proj.bias is not None
-                                                  else (L.EPI_STORE, None)), tag="d_in_proj")
+        if conv_state.dtype != self._dt():
+            raise TypeError(f"conv_state dtype {conv_state.dtype} != model dtype {self._dt()}")
+
+    def _step_mix(self, xz, conv_state, ssm_state):
+        """From in_proj's output xz [B, 2Es] to out_proj's input y [B, Es]; the states are updated in place."""
+        cfg = self.cfg
+        es, n, r, k = self.es, cfg.d_state, cfg.dt_rank, cfg.d_conv
+        Bn = xz.shape[0]
+        dt_ = self._dt()
+        dev = xz.device
         xc = torch.empty(Bn, es, device=dev, dtype=dt_)
         ev = _prof_begin()
         L.call("mtp_conv1d_silu", L.ptr(xz), 2 * es, L.ptr(self.conv1d.weight), L.ptr(self.conv1d.bias),
@@ -289,11 +343,7 @@ class MixerKernels:
                L.ptr(bc), 2 * n, L.ptr(self.A_log), L.ptr(self.D), L.ptr(self.conv1d.weight), L.ptr(self.conv1d.bias),
                L.ptr(conv_state), L.ptr(ssm_state), L.ptr(y), es, Bn, es, n, r, k, L.dtype_code(dt_), L.stream_ptr())
         _prof_end(ev, "d_step", 0)
-        partial_o = torch.empty(Bn, cfg.d_model, device=dev, dtype=torch.float32)
-        self._gemm(y, self.out_proj.weight, partial_o, tag="d_out_proj")
-        ev = _prof_begin()
-        self._reduce_out(partial_o, resid, norm_w, eps, normed)
-        _prof_end(ev, "d_reduce_out", 0)
+        return y
 
     # ------------------------------------------------------------ reference-shaped API
     def prefill(self, x: torch.Tensor, cache=None):
@@ -302,9 +352,12 @@ class MixerKernels:
         self._check_input(x, "prefill")
         b, l, d = x.shape
         xn = x.reshape(b * l, d).contiguous()
-        resid = torch.zeros(b * l, d, device=x.device, dtype=torch.float32)
         ci = cache.conv_state if cache is not None and cache.conv_state is not None else None
         si = cache.ssm_state.float().contiguous() if cache is not None and cache.ssm_state is not None else None
+        if self._int8 is not None:
+            out, cf, sf = self._prefill_int8(quantize_rows(xn), b, l, ci, si)
+            return out.to(x.dtype).view(b, l, d), cf, sf
+        resid = torch.zeros(b * l, d, device=x.device, dtype=torch.float32)
         cf, sf = self._prefill_core(xn, b, l, ci, si, resid)
         return resid.to(x.dtype).view(b, l, d), cf, sf
 
@@ -317,6 +370,8 @@ class MixerKernels:
         (model.py:249-294 / tp_model.py:137-179)."""
         self._check_input(x_t, "step")
         b, d = x_t.shape
+        if self._int8 is not None:
+            return self._step_int8(quantize_rows(x_t), cache.conv_state, cache.ssm_state).to(x_t.dtype)
         resid = torch.zeros(b, d, device=x_t.device, dtype=torch.float32)
         self._step_core(x_t.contiguous(), cache.conv_state, cache.ssm_state, resid)
         return resid.to(x_t.dtype)

@@ -23,6 +23,7 @@ import torch.nn as nn
 from . import _lib as L
 from ._mixer import MixerKernels
 from .config import MambaConfig
+from .int8 import add_rms_norm_int8, quantize_rows, rms_norm_int8
 
 __all__ = ["MambaConfig", "load_hf_state_dict", "LayerCache", "MambaCache", "RMSNorm", "MambaMixer", "MambaBlock",
            "MambaLM"]
@@ -310,6 +311,25 @@ class _LMKernels:
                  for blk in self.layers)
         c.set_sequence_parallel(ok)
 
+    def _int8_linears(self) -> bool:
+        return self.layers[0].mixer._int8 is not None
+
+    def _layers_int8(self, resid, run):
+        """The layers of a model with int8 linears: ``run(i, rows)`` gives layer i's mixer output (fp32) for its int8 input
+        rows; resid is updated in place.  Returns norm_f(resid) in the model dtype."""
+        eps, last = self.cfg.layer_norm_epsilon, len(self.layers) - 1
+        rows = rms_norm_int8(resid, self.layers[0].norm.weight, eps)
+        for i in range(last + 1):
+            branch = run(i, rows)
+            if i < last:
+                rows, _ = add_rms_norm_int8(branch, resid, self._next_norm_w(i), eps, inplace=True)
+        # the last sum, then norm_f in the model dtype for the lm_head
+        L.call("mtp_reduce_outproj", None, L.RED_FP32, L.ptr(branch), resid.shape[0], resid.shape[1], None, L.ptr(resid), None,
+               float(eps), None, L.F32, L.stream_ptr())
+        normed = torch.empty(resid.shape, device=resid.device, dtype=self._param_dtype())
+        self._norm_into(resid, self.norm_f.weight, normed)
+        return normed
+
     def _forward_prefill(self, input_ids: torch.Tensor, cache=None):
         normed, new_cache = self._forward_hidden(input_ids, cache)
         b, l = input_ids.shape
@@ -320,6 +340,18 @@ class _LMKernels:
         self._sync_sequence_parallel()
         b, l = input_ids.shape
         resid = self._embed(input_ids)
+        if self._int8_linears():
+            new_layers = []
+
+            def run(i, rows):
+                lc = cache.layers[i] if cache is not None else None
+                out, cf, sf = self.layers[i].mixer._prefill_int8(
+                    rows, b, l, lc.conv_state if lc is not None else None,
+                    lc.ssm_state.float().contiguous() if lc is not None else None)
+                new_layers.append(LayerCache(conv_state=cf, ssm_state=sf))
+                return out
+
+            return self._layers_int8(resid, run), MambaCache(new_layers)
         normed = torch.empty(resid.shape, device=resid.device, dtype=self._param_dtype())
         self._norm_into(resid, self.layers[0].norm.weight, normed)
         split = self._overlap_split(b, l)
@@ -383,6 +415,10 @@ class _LMKernels:
             plan.step(binding, ids, normed)
             return self._lm_head(normed).view(b, 1, -1)
         resid = self._embed(input_ids[:, :1])
+        if self._int8_linears():
+            normed = self._layers_int8(resid, lambda i, rows: self.layers[i].mixer._step_int8(
+                rows, cache.layers[i].conv_state, cache.layers[i].ssm_state))
+            return self._lm_head(normed).view(b, 1, -1)
         normed = torch.empty(resid.shape, device=resid.device, dtype=self._param_dtype())
         self._norm_into(resid, self.layers[0].norm.weight, normed)
         eps = self.cfg.layer_norm_epsilon
@@ -454,6 +490,18 @@ class MambaLM(_LMKernels, nn.Module):
         self.embedding = nn.Embedding(cfg.vocab_size, cfg.d_model)
         self.layers = nn.ModuleList([MambaBlock(cfg, i) for i in range(cfg.n_layer)])
         self.norm_f = RMSNorm(cfg.d_model, eps=cfg.layer_norm_epsilon)
+
+    @torch.no_grad()
+    def quantize_linears(self, on: bool = True) -> None:
+        """Runs in_proj and out_proj of every layer in int8 from now on (``int8.py``): weights quantised here, a scale for
+        each output channel; inputs a scale for each token, by the norm that writes them and in front of out_proj.
+        ``prefill``, ``step``, ``score`` and ``generate`` follow; x_proj, dt_proj, the scan and the lm_head stay as they
+        are, and so do the parameters.  Call it again after changing or moving them; ``on=False`` takes it back.  Decode
+        steps then run layer by layer instead of in one launch (capture them with ``GraphedStepper``, which must not
+        outlive a change of this setting)."""
+        for layer in self.layers:
+            m = layer.mixer
+            m._int8 = (quantize_rows(m.in_proj.weight), quantize_rows(m.out_proj.weight)) if on else None
 
     def lm_head(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape

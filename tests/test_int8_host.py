@@ -202,3 +202,22 @@ def test_strides(monkeypatch):
     y = Q.int8_linear(Q.Int8Rows(codes[:, :40], torch.ones(12)[::2]), Q.Int8Rows(codes[:5, 8:], torch.ones(5)))
     args = rec.calls.pop()[1]
     assert args[1] == 48 and args[3:5] == (6, 40) and args[6] == 48 and args[8] == 5 and y.shape == (6, 5)
+
+
+def test_a_model_keeps_its_parameters_and_leaves_the_one_launch_step(monkeypatch):
+    from mamba_tp_lite_b200 import _decode
+    from mamba_tp_lite_b200.config import MambaConfig
+    from mamba_tp_lite_b200.model import MambaLM
+
+    rec = Recorder(monkeypatch)
+    lm = MambaLM(MambaConfig(d_model=64, n_layer=2, vocab_size=64, dt_rank=8)).bfloat16()
+    names = list(lm.state_dict())
+    assert _decode.supported(lm) is None
+    lm.quantize_linears()
+    assert [c[0] for c in rec.calls] == ["mtp_quantize_rows"] * 4 and not any(c[1][0] is None for c in rec.calls)
+    for layer in lm.layers:
+        (i, o), m = layer.mixer._int8, layer.mixer
+        assert i.codes.shape == m.in_proj.weight.shape and o.codes.shape == m.out_proj.weight.shape
+    assert list(lm.state_dict()) == names and _decode.supported(lm) == "int8 linears"
+    lm.quantize_linears(False)
+    assert _decode.supported(lm) is None and all(layer.mixer._int8 is None for layer in lm.layers)
