@@ -14,8 +14,7 @@ namespace {
 
 using i8::MAX_COLS;
 
-constexpr int E_OF_WARP = 32, E_OF_CTA = 16;  // values of a row that a thread holds
-constexpr int MAX_TEAM = 16384 / E_OF_CTA;
+constexpr int MAX_HELD = 16384;        // columns of a row that a CTA holds, 16 or 32 a thread
 constexpr int LONG_THREADS = 256;
 constexpr int UNROLL = 4;              // vectors that a thread reads back, their loads in flight together
 constexpr float MAGIC = 12582912.f;    // 1.5 * 2^23: x + MAGIC is x rounded to a whole number, its low byte the int8
@@ -45,6 +44,30 @@ __device__ __forceinline__ uint32_t codes4(const float *p, float c, float &far) 
   const uint32_t hi = __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
+// Codes of four values x that are held exactly, k being 1 / s to fp32's precision.  x - q s is exact in fp32: a multiple of
+// s's last place, and no more than about s / 2.  So q is the nearest where that is below s / 2, and else the one beside it,
+// or in a tie the even one.  (A tie is no rarity among 16-bit values: half the largest of a row is one.)
+__device__ __forceinline__ uint32_t exact_codes4(const float *x, float k, float s) {
+  float m[4], rem[4], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = fmaf(x[i], k, MAGIC);
+    rem[i] = fmaf(-__fsub_rn(m[i], MAGIC), s, x[i]);
+    far = fmaxf(far, fabsf(rem[i]));
+  }
+  const float half = 0.5f * s;
+  if (far >= half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = fabsf(rem[i]);
+      if (a > half || (a == half && (__float_as_uint(m[i]) & 1))) m[i] += copysignf(1.f, rem[i]);
+    }
+  }
+  const uint32_t lo = __byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
 // The code of a y whose quotient t = y / s (to fp32's precision) lies next to k + 1/2: s (k + 1/2) is exact in 64 bits.
 __device__ __forceinline__ int border_code(double y, float t, float s) {
   const float k = floorf(t);
@@ -230,7 +253,28 @@ __device__ __noinline__ void slow_row(const Team<WARP> &team, const void *h, int
   if (team.rank() == 0) *scale = s;
 }
 
-// Writes the codes of p[] * c for the values a thread holds; value(i, col) gives the 64-bit y of its i-th value.
+// Writes the codes of the values that a thread holds, four to a word.
+template <int VEC, int EACH>
+__device__ __forceinline__ void store_codes(const uint32_t (&q)[EACH / 4], int8_t *codes, int cols, int rank, int size) {
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int col = i * size + rank;
+      if (col < cols) codes[col] = (int8_t)(q[i / 4] >> (8 * (i & 3)));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < EACH / VEC; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) {
+        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(codes + col) = q[v];
+        else *reinterpret_cast<uint2 *>(codes + col) = make_uint2(q[2 * v], q[2 * v + 1]);
+      }
+    }
+  }
+}
+
+// Writes the codes of the products p[] * c that a thread holds; value(i, col) gives the i-th's y in 64 bits.
 template <int VEC, int EACH, typename Y>
 __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, float s, int8_t *codes, int cols, int rank, int size,
                                             Y value) {
@@ -252,33 +296,17 @@ __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, flo
       }
     }
   }
-  if constexpr (VEC == 1) {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int col = i * size + rank;
-      if (col < cols) codes[col] = (int8_t)(q[i / 4] >> (8 * (i & 3)));
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) {
-      const int col = (v * size + rank) * VEC;
-      if (col < cols) {
-        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(codes + col) = q[v];
-        else *reinterpret_cast<uint2 *>(codes + col) = make_uint2(q[2 * v], q[2 * v + 1]);
-      }
-    }
-  }
+  store_codes<VEC, EACH>(q, codes, cols, rank, size);
 }
 
 // ------------------------------------------------------------------ quantise
-template <typename T, int VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : MAX_TEAM)
+template <typename T, int VEC, int EACH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH)
     quantize_kernel(const T *__restrict__ x, int64_t ld, int64_t rows, int cols, int8_t *__restrict__ codes, int64_t ld_codes,
                     float *__restrict__ scale) {
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
   __shared__ Join join;
-  constexpr int EACH = WARP ? E_OF_WARP : E_OF_CTA;
   const Team<WARP> team{&join};
   const int rank = team.rank(), size = team.size();
   const int64_t r = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -309,8 +337,11 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_TEAM)
   if (!(s > 0.f)) {
     for (int c = rank; c < cols; c += size) out[c] = 0;
   } else {
-    const float c = __frcp_rn(s);  // 3.7e-37 at least: a normal number
-    write_codes<VEC>(p, c, s, out, cols, rank, size, [&](int i, int) { return (double)p[i]; });
+    const float k = __frcp_rn(s);  // 3.7e-37 at least: a normal number
+    uint32_t q[EACH / 4];
+#pragma unroll
+    for (int i = 0; i < EACH; i += 4) q[i / 4] = exact_codes4(p + i, k, s);
+    store_codes<VEC, EACH>(q, out, cols, rank, size);
   }
   if (rank == 0) scale[r] = s;
 }
@@ -366,14 +397,13 @@ struct None {};
 // TR is the residual's type, or None.  y = h w r with r = 1 / sqrt(mean h^2 + eps); the scale is fp32(max |y| / 127), and the
 // codes are those of (h w) (r / scale).  The sum of squares and r are held in 64 bits; the largest product is found among the
 // fp32 products and then taken exactly (a 48-bit number) from the values whose product rounds to that.
-template <typename TX, typename TR, int VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : MAX_TEAM) norm_kernel(const NormArgs a) {
+template <typename TX, typename TR, int VEC, int EACH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(const NormArgs a) {
   constexpr bool ADD = !std::is_same<TR, None>::value;
   using TH = typename std::conditional<ADD, TR, TX>::type;  // the stream's type
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
   __shared__ Join join;
-  constexpr int EACH = WARP ? E_OF_WARP : E_OF_CTA;
   const Team<WARP> team{&join};
   const int rank = team.rank(), size = team.size(), cols = a.cols;
   const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -582,24 +612,36 @@ bool on_vectors(const void *p, int64_t ld, int es, int64_t rows, int n) {
   return aligned(p, es * n < 16 ? es * n : 16) && (rows == 1 || ld * es % (es * n < 16 ? es * n : 16) == 0);
 }
 
-// Threads of a team for rows of cols values, a warp at least.
-int team_of(int cols) { return cols <= 32 * E_OF_WARP ? 32 : ceil_div(cols, E_OF_CTA * 32) * 32; }
+// Rows of up to 1024 values go to warps, eight to a CTA (16 values a lane where that is enough: 60000 x 320 bf16 16.6 us, with
+// 32 24.2), longer ones to CTAs of as many threads as hold them.
+template <typename T, int VEC, int EACH, bool WARP>
+void launch_quantize_team(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
+                          cudaStream_t s) {
+  const unsigned grid = (unsigned)(WARP ? (rows + 7) / 8 : rows), threads = WARP ? 256 : ceil_div(cols, EACH * 32) * 32;
+  launch_pdl(quantize_kernel<T, VEC, EACH, WARP>, dim3(grid), dim3(threads), 0, s, x, ld, rows, cols, codes, ld_codes, scale);
+}
 
+// A CTA has 32 values a thread where rows are many (32768 x 4096 bf16: 66.5 us, with 16 74.9), 16 where they are few and a
+// row's own time counts (1 x 4096: 1.6 us, with 32 2.0).
 template <typename T, int VEC>
 void launch_quantize(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
                      cudaStream_t s) {
-  const int team = team_of(cols);
-  if (team == 32)
-    launch_pdl(quantize_kernel<T, VEC, true>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, x, ld, rows, cols, codes, ld_codes,
-               scale);
-  else
-    launch_pdl(quantize_kernel<T, VEC, false>, dim3((unsigned)rows), dim3(team), 0, s, x, ld, rows, cols, codes, ld_codes, scale);
+  if (cols <= 512) launch_quantize_team<T, VEC, 16, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (cols <= 1024) launch_quantize_team<T, VEC, 32, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (rows <= 4 * num_sms()) launch_quantize_team<T, VEC, 16, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else launch_quantize_team<T, VEC, 32, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
 }
 
+template <typename TX, typename TR, int VEC, int EACH, bool WARP> void launch_norm_kernel(const NormArgs &a, cudaStream_t s) {
+  const unsigned grid = (unsigned)(WARP ? (a.rows + 7) / 8 : a.rows), threads = WARP ? 256 : ceil_div(a.cols, EACH * 32) * 32;
+  launch_pdl(norm_kernel<TX, TR, VEC, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
+}
+
+// (A norm's CTA has 16 values a thread at any number of rows: 32768 x 2048 bf16 + fp32 120 us, with 32 160.)
 template <typename TX, typename TR, int VEC> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
-  const int team = team_of(a.cols);
-  if (team == 32) launch_pdl(norm_kernel<TX, TR, VEC, true>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, s, a);
-  else launch_pdl(norm_kernel<TX, TR, VEC, false>, dim3((unsigned)a.rows), dim3(team), 0, s, a);
+  if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, 16, true>(a, s);
+  else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, 32, true>(a, s);
+  else launch_norm_kernel<TX, TR, VEC, 16, false>(a, s);
 }
 
 template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStream_t s) {
@@ -646,7 +688,7 @@ int mtp_quantize_rows(const void *x, int dtype, int64_t ld, int64_t rows, int co
   cudaStream_t s = (cudaStream_t)stream;
   MTP_DISPATCH_3(dtype, T, {
     constexpr int VEC = sizeof(T) == 4 ? 4 : 8;
-    if (cols > MAX_TEAM * E_OF_CTA)
+    if (cols > MAX_HELD)
       launch_pdl(quantize_long_kernel<T>, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s,
                  (const T *)x, ld, rows, cols, codes, ld_codes, scale);
     else if (cols % VEC == 0 && on_vectors(x, ld, sizeof(T), rows, VEC) && on_vectors(codes, ld_codes, 1, rows, VEC))
@@ -689,7 +731,7 @@ int mtp_rmsnorm_int8(const void *x, int x_dtype, int64_t ld_x, const void *resid
   const NormArgs a{x, resid, resid_out, w, ld_x, ld_resid, ld_resid_out, rows, cols, x_dtype, resid_dtype, w_dtype, eps, codes,
                    ld_codes, scale, 1.0 / cols};
   bool done = false;
-  if (cols <= MAX_TEAM * E_OF_CTA) MTP_DISPATCH_3(x_dtype, T, done = launch_norm_of<T>(a, s));
+  if (cols <= MAX_HELD) MTP_DISPATCH_3(x_dtype, T, done = launch_norm_of<T>(a, s));
   if (!done)  // long rows, and a 16-bit stream of another type than x
     launch_pdl(norm_long_kernel, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s, a);
   return check_launch("rmsnorm_int8");
