@@ -37,7 +37,6 @@ struct Params {
   Out o;
   int M, N, K;
   int bn, tiles_m, tiles_n, num_tiles, group_m;
-  int a_rows;    // rows of a box of a
   int tma_out;   // results by TMA stores
   uint32_t idesc;
 };
@@ -178,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      const uint32_t tx_bytes = (uint32_t)((p.a_rows + b_rows) * BK * CG);
+      const uint32_t tx_bytes = (uint32_t)((BM + b_rows) * BK * CG);
       int s = 0, issued = 0;
       uint32_t ph = 0;
       for (int t = first; t < p.num_tiles && !*abort; t += step) {
@@ -628,13 +627,12 @@ int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld
   p.tiles_n = ceil_div(N, bn);
   p.num_tiles = p.tiles_m * p.tiles_n;
   p.group_m = 16;
-  p.a_rows = BM;
   // kind::i8, int32 results, signed operands, both with K innermost
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
   const size_t es = o.dtype == MTP_F32 ? 4 : 2;
   p.tma_out = aligned16(o.p) && (M == 1 || ((size_t)o.ld * es) % 16 == 0);
   CUtensorMap ta, tb, tcm;
-  int rc = map_codes(&ta, a, M, K, ld_a, p.a_rows);
+  int rc = map_codes(&ta, a, M, K, ld_a, BM);
   if (rc) return rc;
   rc = map_codes(&tb, w, N, K, ld_w, bn / CG);
   if (rc) return rc;
@@ -728,13 +726,18 @@ bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t 
 
 int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
               cudaStream_t stream) {
-  const int sms = num_sms();
   if (M <= BM) return run_split(a, ld_a, M, K, w, ld_w, N, o, stream);
-  if ((int64_t)ceil_div(M, 2 * BM) * ceil_div(N, BN_MAX) * 2 >= sms)
-    return run<2>(a, ld_a, M, K, w, ld_w, N, o, BN_MAX, stream);
-  int bn = 128;
-  while (bn > 64 && (int64_t)ceil_div(M, BM) * ceil_div(N, bn) < sms) bn /= 2;
-  return run<1>(a, ld_a, M, K, w, ld_w, N, o, bn, stream);
+  // Of three tiles the one with the least time by what was measured (us): a call's own, then for each round of tiles 0.3 for a
+  // block of K, whatever the tile, and what the epilogue adds.  (512 x 2048 -> 8192: 22.4, 14.1 and 11.7 us; 256 rows: 13.2,
+  // 9.2 and 11.3; 256 x 2048 -> 1024: 7.7, 8.2 and 9.9.)
+  const int sms = num_sms(), num_kb = ceil_div(K, BK);
+  auto time_of = [&](int cg, int bn, double call, double kb, double tile) {
+    const int64_t tiles = (int64_t)ceil_div(M, BM * cg) * ceil_div(N, bn), places = sms / cg;
+    return call + (double)((tiles + places - 1) / places) * (num_kb * kb + tile);
+  };
+  const double t1 = time_of(1, 64, 2.3, 0.287, 0.42), t2 = time_of(1, 128, 2.3, 0.287, 1.1), t3 = time_of(2, 256, 3.4, 0.306, 1.6);
+  if (t3 <= t1 && t3 <= t2) return run<2>(a, ld_a, M, K, w, ld_w, N, o, 256, stream);
+  return run<1>(a, ld_a, M, K, w, ld_w, N, o, t2 <= t1 ? 128 : 64, stream);
 }
 
 }  // namespace i8
