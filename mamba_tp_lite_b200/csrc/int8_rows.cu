@@ -68,6 +68,13 @@ __device__ __forceinline__ uint32_t exact_codes4(const float *x, float k, float 
   return __byte_perm(lo, hi, 0x5410);
 }
 
+// x in 64 bits, converted where it stands: what is rarely needed shall not be kept from an earlier conversion.
+__device__ __forceinline__ double widen(float x) {
+  double d;
+  asm volatile("cvt.f64.f32 %0, %1;" : "=d"(d) : "f"(x));
+  return d;
+}
+
 // The code of a y whose quotient t = y / s (to fp32's precision) lies next to k + 1/2: s (k + 1/2) is exact in 64 bits.
 __device__ __forceinline__ int border_code(double y, float t, float s) {
   const float k = floorf(t);
@@ -398,8 +405,9 @@ struct None {};
 // codes are those of (h w) (r / scale).  The sum of squares and r are held in 64 bits; the largest product is found among the
 // fp32 products and then taken exactly (a 48-bit number) from the values whose product rounds to that.
 template <typename TX, typename TR, int VEC, int EACH, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EACH) norm_kernel(const NormArgs a) {
   constexpr bool ADD = !std::is_same<TR, None>::value;
+  constexpr bool KEEP = EACH == 8;  // few rows: h stays in registers, where else a value of it is read again if need be
   using TH = typename std::conditional<ADD, TR, TX>::type;  // the stream's type
   MTP_PDL_WAIT();
   MTP_PDL_TRIGGER();
@@ -482,6 +490,10 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(cons
     ss2 = fma(h1, h1, ss2);
   }
   ss += ss2;
+  float h[KEEP ? EACH : 1];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (KEEP) h[i] = p[i];
 #pragma unroll
   for (int i = 0; i < EACH; i += 2) {
     p[i] = __fmul_rn(p[i], w[i]);
@@ -493,7 +505,10 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(cons
   team.sum_max(ss, most);
   const double rs = rsqrt(fma(ss, a.inv_cols, (double)a.eps));
   const void *hp = ADD ? (const void *)ro : (const void *)xr;  // a thread reads back only what it has stored itself
-  auto h_at = [&](int col) { return (double)ldf((const TH *)hp + col); };
+  auto y_of = [&](int i, int col) {
+    if constexpr (KEEP) return widen(h[i]) * rs * widen(w[i]);
+    else return (double)ldf((const TH *)hp + col) * rs * (double)ld_any(a.w, a.w_dtype, col);
+  };
   int8_t *out = a.codes + row * a.ld_codes;
   if (most >= TINY && most <= HUGE_ && rs < 1e30) {
     double top = 0.0;
@@ -502,7 +517,7 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(cons
       for (int i = 0; i < EACH; ++i) {
         if ((__float_as_uint(p[i]) & 0x7fffffffu) == most) {
           const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
-          top = fmax(top, fabs(h_at(col) * rs * (double)ld_any(a.w, a.w_dtype, col)));
+          top = fmax(top, fabs(y_of(i, col)));
         }
       }
     }
@@ -511,8 +526,7 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH) norm_kernel(cons
     const float c = __fmul_rn((float)rs, __frcp_rn(s));
     const uint32_t cb = __float_as_uint(c);
     if (cb >= TINY && cb <= HUGE_) {
-      write_codes<VEC>(p, c, s, out, cols, rank, size,
-                       [&](int, int col) { return h_at(col) * rs * (double)ld_any(a.w, a.w_dtype, col); });
+      write_codes<VEC>(p, c, s, out, cols, rank, size, y_of);
       if (rank == 0) a.scale[row] = s;
       return;
     }
@@ -637,9 +651,11 @@ template <typename TX, typename TR, int VEC, int EACH, bool WARP> void launch_no
   launch_pdl(norm_kernel<TX, TR, VEC, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
 }
 
-// (A norm's CTA has 16 values a thread at any number of rows: 32768 x 2048 bf16 + fp32 120 us, with 32 160.)
+// A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 120 us, with 32 160); few rows have CTAs of 8 values a thread
+// whatever their length (1 x 2048: NEW us, with 16 2.9).
 template <typename TX, typename TR, int VEC> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
-  if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, 16, true>(a, s);
+  if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, 8, false>(a, s);
+  else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, 16, true>(a, s);
   else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, 32, true>(a, s);
   else launch_norm_kernel<TX, TR, VEC, 16, false>(a, s);
 }
