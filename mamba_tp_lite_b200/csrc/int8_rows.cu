@@ -90,7 +90,9 @@ template <typename T, int N> struct Raw { uint32_t w[sizeof(T) * N / 4]; };
 template <typename T, int N>
 __device__ __forceinline__ void load_raw(Raw<T, N> &r, const T *p) {
   constexpr int W = sizeof(T) * N / 4;
-  if constexpr (W == 2) {
+  if constexpr (W == 1) {
+    r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+  } else if constexpr (W == 2) {
     const uint2 u = *reinterpret_cast<const uint2 *>(p);
     r.w[0] = u.x; r.w[1] = u.y;
   } else {
@@ -104,7 +106,9 @@ __device__ __forceinline__ void load_raw(Raw<T, N> &r, const T *p) {
 template <typename T, int N>
 __device__ __forceinline__ void store_raw(T *p, const Raw<T, N> &r) {
   constexpr int W = sizeof(T) * N / 4;
-  if constexpr (W == 2) {
+  if constexpr (W == 1) {
+    *reinterpret_cast<uint32_t *>(p) = r.w[0];
+  } else if constexpr (W == 2) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
   } else {
 #pragma unroll
@@ -112,6 +116,60 @@ __device__ __forceinline__ void store_raw(T *p, const Raw<T, N> &r) {
       *reinterpret_cast<uint4 *>(p + i * 4 / sizeof(T)) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
   }
 }
+// N values of a row from column col on, wherever the row begins, zeros from column cols on: the aligned vector that the first
+// of them lies in, and the next one if they reach into it, shifted together.  What is read lies within vectors that hold a value
+// of the row.
+template <typename T, int N>
+__device__ __forceinline__ void load_ragged(Raw<T, N> &r, const T *row, int col, int cols) {
+  constexpr int B = sizeof(T) * N, W = B / 4;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + col), a = at & ~(uintptr_t)(B - 1);
+  const uint32_t s = (uint32_t)(at - a);
+  load_raw(r, reinterpret_cast<const T *>(a));
+  if (s) {
+    Raw<T, N> next{};
+    if (a + B < reinterpret_cast<uintptr_t>(row + cols)) load_raw(next, reinterpret_cast<const T *>(a + B));
+    uint32_t w[2 * W + 1];
+#pragma unroll
+    for (int i = 0; i < W; ++i) { w[i] = r.w[i]; w[W + i] = next.w[i]; }
+    w[2 * W] = 0;
+    if (W == 4 && (s & 8)) {
+#pragma unroll
+      for (int i = 0; i + 2 <= 2 * W; ++i) w[i] = w[i + 2];
+    }
+    if (W >= 2 && (s & 4)) {
+#pragma unroll
+      for (int i = 0; i + 1 <= 2 * W; ++i) w[i] = w[i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (s & 3));
+  }
+  const int n = cols - col;
+  if (n < N) {
+    constexpr int E = 4 / (int)sizeof(T);  // values in a word
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int in = n - i * E;  // of word i
+      if (in <= 0) r.w[i] = 0;
+      else if (in < E) r.w[i] &= (1u << (32 / E * in)) - 1u;
+    }
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void store_ragged(T *row, int col, int cols, const Raw<T, N> &r) {
+  T *to = row + col;
+  const int n = cols - col;
+  if (n >= N && (reinterpret_cast<uintptr_t>(to) & (sizeof(T) * N - 1)) == 0) {
+    store_raw(to, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i >= n) continue;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(to)[i] = r.w[i];
+      else if constexpr (sizeof(T) == 2) reinterpret_cast<unsigned short *>(to)[i] = (unsigned short)(r.w[i / 2] >> (16 * (i & 1)));
+      else to[i] = (T)(r.w[i / 4] >> (8 * (i & 3)));
+    }
+  }
+}
+
 template <typename T, int N> __device__ __forceinline__ void to_f32(const Raw<T, N> &r, float *v) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -260,29 +318,35 @@ __device__ __noinline__ void slow_row(const Team<WARP> &team, const void *h, int
   if (team.rank() == 0) *scale = s;
 }
 
+// The vectors of a row that a thread holds: those at columns (v * size + rank) * VEC.
+template <int VEC, bool RAGGED, int NV, typename T>
+__device__ __forceinline__ void load_row(Raw<T, VEC> (&raw)[NV], const T *row, int cols, int rank, int size) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int col = (v * size + rank) * VEC;
+    if (col >= cols) raw[v] = Raw<T, VEC>{};
+    else if (RAGGED) load_ragged(raw[v], row, col, cols);
+    else load_raw(raw[v], row + col);
+  }
+}
+
 // Writes the codes of the values that a thread holds, four to a word.
-template <int VEC, int EACH>
+template <int VEC, bool RAGGED, int EACH>
 __device__ __forceinline__ void store_codes(const uint32_t (&q)[EACH / 4], int8_t *codes, int cols, int rank, int size) {
-  if constexpr (VEC == 1) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int col = i * size + rank;
-      if (col < cols) codes[col] = (int8_t)(q[i / 4] >> (8 * (i & 3)));
-    }
-  } else {
+  for (int v = 0; v < EACH / VEC; ++v) {
+    const int col = (v * size + rank) * VEC;
+    if (col >= cols) continue;
+    Raw<int8_t, VEC> r;
 #pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) {
-      const int col = (v * size + rank) * VEC;
-      if (col < cols) {
-        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(codes + col) = q[v];
-        else *reinterpret_cast<uint2 *>(codes + col) = make_uint2(q[2 * v], q[2 * v + 1]);
-      }
-    }
+    for (int i = 0; i < VEC / 4; ++i) r.w[i] = q[v * (VEC / 4) + i];
+    if (RAGGED) store_ragged(codes, col, cols, r);
+    else store_raw(codes + col, r);
   }
 }
 
 // Writes the codes of the products p[] * c that a thread holds; value(i, col) gives the i-th's y in 64 bits.
-template <int VEC, int EACH, typename Y>
+template <int VEC, bool RAGGED, int EACH, typename Y>
 __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, float s, int8_t *codes, int cols, int rank, int size,
                                             Y value) {
   uint32_t q[EACH / 4];
@@ -303,11 +367,11 @@ __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, flo
       }
     }
   }
-  store_codes<VEC, EACH>(q, codes, cols, rank, size);
+  store_codes<VEC, RAGGED, EACH>(q, codes, cols, rank, size);
 }
 
 // ------------------------------------------------------------------ quantise
-template <typename T, int VEC, int EACH, bool WARP>
+template <typename T, int VEC, bool RAGGED, int EACH, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH)
     quantize_kernel(const T *__restrict__ x, int64_t ld, int64_t rows, int cols, int8_t *__restrict__ codes, int64_t ld_codes,
                     float *__restrict__ scale) {
@@ -320,20 +384,10 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH)
   if (r >= rows) return;
   const T *xr = x + r * ld;
   float p[EACH];
-  if constexpr (VEC == 1) {
+  Raw<T, VEC> raw[EACH / VEC];
+  load_row<VEC, RAGGED>(raw, xr, cols, rank, size);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) p[i] = i * size + rank < cols ? ldf(xr + i * size + rank) : 0.f;
-  } else {
-    Raw<T, VEC> raw[EACH / VEC];
-#pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) {
-      const int col = (v * size + rank) * VEC;
-      if (col < cols) load_raw(raw[v], xr + col);
-      else raw[v] = Raw<T, VEC>{};
-    }
-#pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) to_f32(raw[v], p + v * VEC);
-  }
+  for (int v = 0; v < EACH / VEC; ++v) to_f32(raw[v], p + v * VEC);
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < EACH; i += 2) m = max_abs3(m, p[i], p[i + 1]);
@@ -348,7 +402,7 @@ __global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH)
     uint32_t q[EACH / 4];
 #pragma unroll
     for (int i = 0; i < EACH; i += 4) q[i / 4] = exact_codes4(p + i, k, s);
-    store_codes<VEC, EACH>(q, out, cols, rank, size);
+    store_codes<VEC, RAGGED, EACH>(q, out, cols, rank, size);
   }
   if (rank == 0) scale[r] = s;
 }
@@ -381,22 +435,18 @@ struct NormArgs {
   double inv_cols;
 };
 
-template <int VEC> __device__ __forceinline__ void load_weight(const void *w, int dtype, int col, float *v) {
-  if constexpr (VEC == 1) {
-    v[0] = ld_any(w, dtype, col);
-  } else if (dtype == MTP_F32) {
-    Raw<float, VEC> r;
-    load_raw(r, (const float *)w + col);
-    to_f32(r, v);
-  } else if (dtype == MTP_BF16) {
-    Raw<__nv_bfloat16, VEC> r;
-    load_raw(r, (const __nv_bfloat16 *)w + col);
-    to_f32(r, v);
-  } else {
-    Raw<__half, VEC> r;
-    load_raw(r, (const __half *)w + col);
-    to_f32(r, v);
-  }
+template <int VEC, bool RAGGED, typename T>
+__device__ __forceinline__ void load_weight_of(const T *w, int col, int cols, float *v) {
+  Raw<T, VEC> r;
+  if (RAGGED) load_ragged(r, w, col, cols);
+  else load_raw(r, w + col);
+  to_f32(r, v);
+}
+template <int VEC, bool RAGGED>
+__device__ __forceinline__ void load_weight(const void *w, int dtype, int col, int cols, float *v) {
+  if (dtype == MTP_F32) load_weight_of<VEC, RAGGED>((const float *)w, col, cols, v);
+  else if (dtype == MTP_BF16) load_weight_of<VEC, RAGGED>((const __nv_bfloat16 *)w, col, cols, v);
+  else load_weight_of<VEC, RAGGED>((const __half *)w, col, cols, v);
 }
 
 struct None {};
@@ -404,7 +454,7 @@ struct None {};
 // TR is the residual's type, or None.  y = h w r with r = 1 / sqrt(mean h^2 + eps); the scale is fp32(max |y| / 127), and the
 // codes are those of (h w) (r / scale).  The sum of squares and r are held in 64 bits; the largest product is found among the
 // fp32 products and then taken exactly (a 48-bit number) from the values whose product rounds to that.
-template <typename TX, typename TR, int VEC, int EACH, bool WARP>
+template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EACH) norm_kernel(const NormArgs a) {
   constexpr bool ADD = !std::is_same<TR, None>::value;
   constexpr bool KEEP = EACH == 8;  // few rows: h stays in registers, where else a value of it is read again if need be
@@ -420,65 +470,40 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
   const TX *xr = (const TX *)a.x + row * a.ld_x;
   const TR *rr = (const TR *)a.resid + row * a.ld_r;
   TR *ro = (TR *)a.r_out + row * a.ld_ro;
+  constexpr int NV = EACH / VEC;
   float p[EACH], w[EACH];
-  if constexpr (VEC == 1) {
-    float res[EACH];
+  Raw<TX, VEC> raw[NV];
+  load_row<VEC, RAGGED>(raw, xr, cols, rank, size);
+  if constexpr (ADD) {
+    Raw<TR, VEC> res[NV];
+    load_row<VEC, RAGGED>(res, rr, cols, rank, size);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int c = i * size + rank;
-      p[i] = c < cols ? ldf(xr + c) : 0.f;
-      if constexpr (ADD) res[i] = c < cols ? ldf(rr + c) : 0.f;
-      w[i] = c < cols ? ld_any(a.w, a.w_dtype, c) : 0.f;
-    }
-    if constexpr (ADD) {
+    for (int v = 0; v < NV; ++v) {
+      const int col = (v * size + rank) * VEC;
+      float f[VEC], h[VEC];
+      to_f32(raw[v], f);
+      to_f32(res[v], h);
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int c = i * size + rank;
-        p[i] = __fadd_rn(p[i], res[i]);
-        if (c < cols) p[i] = st_any(ro, Code<TR>::value, c, p[i]);
+      for (int i = 0; i < VEC; ++i) h[i] = __fadd_rn(f[i], h[i]);
+      from_f32(res[v], h);
+      to_f32(res[v], p + v * VEC);  // as it is held
+      if (col < cols) {
+        if (RAGGED) store_ragged(ro, col, cols, res[v]);
+        else store_raw(ro + col, res[v]);
       }
     }
   } else {
-    Raw<TX, VEC> raw[EACH / VEC];
 #pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) {
-      const int col = (v * size + rank) * VEC;
-      if (col < cols) load_raw(raw[v], xr + col);
-      else raw[v] = Raw<TX, VEC>{};
-    }
-    if constexpr (ADD) {
-      Raw<TR, VEC> res[EACH / VEC];
+    for (int v = 0; v < NV; ++v) to_f32(raw[v], p + v * VEC);
+  }
 #pragma unroll
-      for (int v = 0; v < EACH / VEC; ++v) {
-        const int col = (v * size + rank) * VEC;
-        if (col < cols) load_raw(res[v], rr + col);
-        else res[v] = Raw<TR, VEC>{};
-      }
-#pragma unroll
-      for (int v = 0; v < EACH / VEC; ++v) {
-        const int col = (v * size + rank) * VEC;
-        float f[VEC], h[VEC];
-        to_f32(raw[v], f);
-        to_f32(res[v], h);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) h[i] = __fadd_rn(f[i], h[i]);
-        from_f32(res[v], h);
-        to_f32(res[v], p + v * VEC);  // as it is held
-        if (col < cols) store_raw(ro + col, res[v]);
-      }
+  for (int v = 0; v < NV; ++v) {
+    const int col = (v * size + rank) * VEC;
+    if (col < cols) {
+      load_weight<VEC, RAGGED>(a.w, a.w_dtype, col, cols, w + v * VEC);
     } else {
 #pragma unroll
-      for (int v = 0; v < EACH / VEC; ++v) to_f32(raw[v], p + v * VEC);
-    }
-#pragma unroll
-    for (int v = 0; v < EACH / VEC; ++v) {
-      const int col = (v * size + rank) * VEC;
-      if (col < cols) {
-        load_weight<VEC>(a.w, a.w_dtype, col, w + v * VEC);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) w[v * VEC + i] = 0.f;
-      }
+      for (int i = 0; i < VEC; ++i) w[v * VEC + i] = 0.f;
     }
   }
   double ss = 0.0, ss2 = 0.0;
@@ -526,7 +551,7 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
     const float c = __fmul_rn((float)rs, __frcp_rn(s));
     const uint32_t cb = __float_as_uint(c);
     if (cb >= TINY && cb <= HUGE_) {
-      write_codes<VEC>(p, c, s, out, cols, rank, size, y_of);
+      write_codes<VEC, RAGGED>(p, c, s, out, cols, rank, size, y_of);
       if (rank == 0) a.scale[row] = s;
       return;
     }
@@ -604,6 +629,44 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t *__restric
   }
 }
 
+// Dense results of rows of any alignment: a thread takes N values of them that lie in 16 bytes, of one row or of several.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_dense_kernel(const int8_t *__restrict__ codes, int64_t ld_codes,
+                                                               const float *__restrict__ scale, T *__restrict__ out, int64_t total,
+                                                               int cols) {
+  constexpr int N = 16 / (int)sizeof(T);
+  MTP_PDL_WAIT();
+  MTP_PDL_TRIGGER();
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const int64_t at = (((int64_t)blockIdx.x * UNROLL + u) * 256 + threadIdx.x) * N;
+    if (at >= total) return;
+    int64_t r = at <= 0x7fffffff ? (int64_t)((uint32_t)at / (uint32_t)cols) : at / cols;
+    int c = (int)(at - r * cols);
+    float v[N];
+    if (c + N <= cols) {
+      Raw<int8_t, N> q;
+      load_ragged(q, codes + r * ld_codes, c, cols);
+      const float s = scale[r];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = __fmul_rn((float)(int8_t)(q.w[k / 4] >> (8 * (k & 3))), s);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        v[k] = at + k < total ? __fmul_rn((float)codes[r * ld_codes + c], scale[r]) : 0.f;
+        if (++c == cols) { c = 0; ++r; }
+      }
+    }
+    Raw<T, N> raw;
+    from_f32(raw, v);
+    if (at + N <= total) {
+      store_raw(out + at, raw);
+    } else {
+      for (int k = 0; at + k < total; ++k) stf(out + at + k, v[k]);
+    }
+  }
+}
+
 template <typename T, int N>
 void launch_dequantize(const int8_t *codes, int64_t ld_codes, const float *scale, int64_t rows, int cols, T *out, int64_t ld_out,
                        cudaStream_t s) {
@@ -628,36 +691,36 @@ bool on_vectors(const void *p, int64_t ld, int es, int64_t rows, int n) {
 
 // Rows of up to 1024 values go to warps, eight to a CTA (16 values a lane where that is enough: 60000 x 320 bf16 16.6 us, with
 // 32 24.2), longer ones to CTAs of as many threads as hold them.
-template <typename T, int VEC, int EACH, bool WARP>
+template <typename T, int VEC, bool RAGGED, int EACH, bool WARP>
 void launch_quantize_team(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
                           cudaStream_t s) {
   const unsigned grid = (unsigned)(WARP ? (rows + 7) / 8 : rows), threads = WARP ? 256 : ceil_div(cols, EACH * 32) * 32;
-  launch_pdl(quantize_kernel<T, VEC, EACH, WARP>, dim3(grid), dim3(threads), 0, s, x, ld, rows, cols, codes, ld_codes, scale);
+  launch_pdl(quantize_kernel<T, VEC, RAGGED, EACH, WARP>, dim3(grid), dim3(threads), 0, s, x, ld, rows, cols, codes, ld_codes, scale);
 }
 
 // A CTA has 32 values a thread where rows are many (32768 x 4096 bf16: 66.5 us, with 16 74.9), 16 where they are few and a
 // row's own time counts (1 x 4096: 1.6 us, with 32 2.0).
-template <typename T, int VEC>
+template <typename T, int VEC, bool RAGGED>
 void launch_quantize(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
                      cudaStream_t s) {
-  if (cols <= 512) launch_quantize_team<T, VEC, 16, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
-  else if (cols <= 1024) launch_quantize_team<T, VEC, 32, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
-  else if (rows <= 4 * num_sms()) launch_quantize_team<T, VEC, 16, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
-  else launch_quantize_team<T, VEC, 32, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  if (cols <= 512) launch_quantize_team<T, VEC, RAGGED, 16, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (cols <= 1024) launch_quantize_team<T, VEC, RAGGED, 32, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (rows <= 4 * num_sms()) launch_quantize_team<T, VEC, RAGGED, 16, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else launch_quantize_team<T, VEC, RAGGED, 32, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
 }
 
-template <typename TX, typename TR, int VEC, int EACH, bool WARP> void launch_norm_kernel(const NormArgs &a, cudaStream_t s) {
+template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP> void launch_norm_kernel(const NormArgs &a, cudaStream_t s) {
   const unsigned grid = (unsigned)(WARP ? (a.rows + 7) / 8 : a.rows), threads = WARP ? 256 : ceil_div(a.cols, EACH * 32) * 32;
-  launch_pdl(norm_kernel<TX, TR, VEC, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
+  launch_pdl(norm_kernel<TX, TR, VEC, RAGGED, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
 }
 
 // A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 120 us, with 32 160); few rows have CTAs of 8 values a thread
 // whatever their length (1 x 2048: NEW us, with 16 2.9).
-template <typename TX, typename TR, int VEC> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
-  if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, 8, false>(a, s);
-  else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, 16, true>(a, s);
-  else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, 32, true>(a, s);
-  else launch_norm_kernel<TX, TR, VEC, 16, false>(a, s);
+template <typename TX, typename TR, int VEC, bool RAGGED> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
+  if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, RAGGED, 8, false>(a, s);
+  else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, RAGGED, 16, true>(a, s);
+  else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, RAGGED, 32, true>(a, s);
+  else launch_norm_kernel<TX, TR, VEC, RAGGED, 16, false>(a, s);
 }
 
 template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStream_t s) {
@@ -668,8 +731,8 @@ template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStre
   const bool vec = a.cols % VEC == 0 && on_vectors(a.x, a.ld_x, sizeof(TX), a.rows, VEC) &&
                    on_vectors(a.w, 0, size_of(a.w_dtype), 1, VEC) && on_vectors(a.codes, a.ld_codes, 1, a.rows, VEC) &&
                    (!ADD || (on_vectors(a.resid, a.ld_r, er, a.rows, VEC) && on_vectors(a.r_out, a.ld_ro, er, a.rows, VEC)));
-  if (vec) launch_norm_team<TX, TR, VEC>(a, s);
-  else launch_norm_team<TX, TR, 1>(a, s);
+  if (vec) launch_norm_team<TX, TR, VEC, false>(a, s);
+  else launch_norm_team<TX, TR, VEC, true>(a, s);
 }
 
 template <typename TX> bool launch_norm_of(const NormArgs &a, cudaStream_t s) {
@@ -708,9 +771,9 @@ int mtp_quantize_rows(const void *x, int dtype, int64_t ld, int64_t rows, int co
       launch_pdl(quantize_long_kernel<T>, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s,
                  (const T *)x, ld, rows, cols, codes, ld_codes, scale);
     else if (cols % VEC == 0 && on_vectors(x, ld, sizeof(T), rows, VEC) && on_vectors(codes, ld_codes, 1, rows, VEC))
-      launch_quantize<T, VEC>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
+      launch_quantize<T, VEC, false>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
     else
-      launch_quantize<T, 1>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
+      launch_quantize<T, VEC, true>((const T *)x, ld, rows, cols, codes, ld_codes, scale, s);
   });
   return check_launch("quantize_rows");
 }
@@ -727,6 +790,9 @@ int mtp_dequantize_rows(const int8_t *codes, int64_t ld_codes, const float *scal
     constexpr int N = 16 / sizeof(T);
     if (cols % N == 0 && on_vectors(codes, ld_codes, 1, rows, N) && on_vectors(out, ld_out, sizeof(T), rows, N))
       launch_dequantize<T, N>(codes, ld_codes, scale, rows, cols, (T *)out, ld_out, s);
+    else if (aligned16(out) && (rows == 1 || ld_out == cols))
+      launch_pdl(dequantize_dense_kernel<T>, dim3((unsigned)((rows * cols + 256 * UNROLL * N - 1) / (256 * UNROLL * N))), dim3(256), 0,
+                 s, codes, ld_codes, scale, (T *)out, rows * cols, cols);
     else
       launch_dequantize<T, 1>(codes, ld_codes, scale, rows, cols, (T *)out, ld_out, s);
   });
