@@ -29,9 +29,13 @@ class Int8Rows(NamedTuple):
 
 
 # ------------------------------------------------------------------ arguments
+# A call's time on the host is most of a decode step's small calls, so the common arguments (two dimensions, dense rows) are
+# taken after one row of tests, and everything else, refusals among it, by the functions that name what is wrong.
 def _refuse_grad(what: str, *tensors) -> None:
     grad = torch.is_grad_enabled()
     dual = forward_ad._current_level >= 0
+    if not (grad or dual):
+        return
     for t in tensors:
         if t is None:
             continue
@@ -50,25 +54,21 @@ def _check_shape(x: torch.Tensor, what: str, name: str) -> None:
         raise ValueError(f"{what}: {name} has more than {MAX_ROWS} rows")
 
 
-def _check_codes(r: Int8Rows, what: str, name: str) -> None:
-    codes, scale = r
-    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
-        raise TypeError(f"{what}: {name} needs int8 codes and float32 scales, got {codes.dtype} and {scale.dtype}")
-    _check_shape(codes, what, name)
-    if scale.shape != codes.shape[:-1]:
-        raise ValueError(f"{what}: {name} has scales of shape {tuple(scale.shape)} for codes of shape {tuple(codes.shape)}")
-    if scale.device != codes.device:
-        raise ValueError(f"{what}: {name} has its scales on {scale.device}, its codes on {codes.device}")
-
-
 def _same_device(t: torch.Tensor, x: torch.Tensor, what: str, name: str) -> None:
     if t.device != x.device:
         raise ValueError(f"{what}: {name} is on {t.device}, expected {x.device}")
 
 
-def _as_rows(x: torch.Tensor):
+def _as_rows(x: torch.Tensor, what: str, name: str):
     """(x as [rows, C] with dense rows, rows, C, the stride between rows); copied where the leading dimensions have no common
     stride."""
+    if x.dim() == 2 and x.is_cuda:
+        (rows, c), (ld, step) = x.shape, x.stride()
+        if step == 1 and 1 <= c <= MAX_COLS and 1 < rows <= MAX_ROWS and ld >= c:
+            return x, rows, c, ld
+        if rows == 1 and step == 1 and 1 <= c <= MAX_COLS:
+            return x, 1, c, c
+    _check_shape(x, what, name)
     c = x.shape[-1]
     if x.dim() != 2:
         x = x.reshape(-1, c)
@@ -78,10 +78,19 @@ def _as_rows(x: torch.Tensor):
     return x, rows, c, (ld if rows > 1 else c)
 
 
-def _flat(scale: torch.Tensor) -> torch.Tensor:
+def _as_codes(r: Int8Rows, what: str, name: str):
+    """``_as_rows`` of the codes, with their scales in one dimension."""
+    codes, scale = r
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} needs int8 codes and float32 scales, got {codes.dtype} and {scale.dtype}")
+    rows2 = _as_rows(codes, what, name)
+    if scale.shape != codes.shape[:-1]:
+        raise ValueError(f"{what}: {name} has scales of shape {tuple(scale.shape)} for codes of shape {tuple(codes.shape)}")
+    if scale.device != codes.device:
+        raise ValueError(f"{what}: {name} has its scales on {scale.device}, its codes on {codes.device}")
     if scale.dim() != 1:
         scale = scale.reshape(-1)
-    return scale if scale.is_contiguous() else scale.contiguous()
+    return *rows2, (scale if scale.is_contiguous() else scale.contiguous())
 
 
 def _extent(x: torch.Tensor):
@@ -95,14 +104,21 @@ def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
     return x0 < y1 and y0 < x1
 
 
-def _new_rows(x: torch.Tensor):
+def _new_rows(x: torch.Tensor, rows: int, c: int):
     """Uninitialised (codes, scale, stride) for rows like those of x; each row of codes starts on a 16-byte boundary, as the
     tensor-core product wants it."""
-    *lead, c = x.shape
     wide = (c + 15) // 16 * 16
-    codes = x.new_empty(*lead, wide, dtype=torch.int8)
-    scale = x.new_empty(lead, dtype=torch.float32)
+    if x.dim() == 2:
+        codes, scale = x.new_empty(rows, wide, dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
+    else:
+        lead = x.shape[:-1]
+        codes, scale = x.new_empty(*lead, wide, dtype=torch.int8), x.new_empty(lead, dtype=torch.float32)
     return (codes if wide == c else codes[..., :c]), scale, wide
+
+
+def _new_like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Uninitialised, dense, of x's shape."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
 
 
 # ------------------------------------------------------------------ operators
@@ -110,36 +126,31 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """int8 rows of x [..., C]: scale = max(max |x|, 1e-8) / 127 in float32, a code is the nearest multiple of it (ties to
     even), -127 to 127.  A row with a NaN or an infinity has scale NaN and codes 0."""
     what = "quantize_rows"
-    _check_shape(x, what, "x")
+    x2, rows, c, ld = _as_rows(x, what, "x")
     code = L.dtype_code(x.dtype)
     _refuse_grad(what, x)
-    codes, scale, ld_codes = _new_rows(x)
-    x, rows, c, ld = _as_rows(x)
-    _call(x, "mtp_quantize_rows", x.data_ptr(), code, ld, rows, c, codes.data_ptr(), ld_codes, scale.data_ptr())
+    codes, scale, ld_codes = _new_rows(x, rows, c)
+    _call(x2, "mtp_quantize_rows", x2.data_ptr(), code, ld, rows, c, codes.data_ptr(), ld_codes, scale.data_ptr())
     return Int8Rows(codes, scale)
 
 
 def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """What the rows stand for: codes * scale, the float32 product rounded to ``dtype``."""
     what = "dequantize_rows"
-    _check_codes(rows, what, "rows")
-    codes, scale = rows
+    codes, n, c, ld, scale = _as_codes(rows, what, "rows")
     code = L.dtype_code(dtype)
-    _refuse_grad(what, scale)
-    out = codes.new_empty(codes.shape, dtype=dtype)
-    codes, n, c, ld = _as_rows(codes)
-    scale = _flat(scale)
+    _refuse_grad(what, rows.scale)
+    out = _new_like(rows.codes, dtype)
     _call(codes, "mtp_dequantize_rows", codes.data_ptr(), ld, scale.data_ptr(), n, c, out.data_ptr(), code, c)
     return out
 
 
 def _norm(x, residual, weight, eps, inplace, what):
-    _check_shape(x, what, "x")
-    x_code, c = L.dtype_code(x.dtype), x.shape[-1]
+    x2, rows, c, ld = _as_rows(x, what, "x")
+    x_code, w_code = L.dtype_code(x.dtype), L.dtype_code(weight.dtype)
     if weight.shape != (c,):
         raise ValueError(f"{what}: weight has shape {tuple(weight.shape)}, expected {(c,)}")
     _same_device(weight, x, what, "weight")
-    w_code = L.dtype_code(weight.dtype)
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
@@ -152,7 +163,7 @@ def _norm(x, residual, weight, eps, inplace, what):
             raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
         _same_device(residual, x, what, "residual")
         r_code = L.dtype_code(residual.dtype)
-        res, _, _, ld_res = _as_rows(residual)
+        res, _, _, ld_res = _as_rows(residual, what, "residual")
         if inplace:
             if res.data_ptr() != residual.data_ptr():
                 raise ValueError(f"{what}: a residual that is updated in place needs rows on one stride")
@@ -160,11 +171,10 @@ def _norm(x, residual, weight, eps, inplace, what):
                 raise ValueError(f"{what}: a residual that is updated in place must not share memory with x")
             h, ld_h = residual, ld_res
         else:
-            h, ld_h = residual.new_empty(residual.shape), c
+            h, ld_h = _new_like(residual, residual.dtype), c
         res_args = (res.data_ptr(), r_code, ld_res, h.data_ptr(), ld_h)
-    codes, scale, ld_codes = _new_rows(x)
-    x, rows, _, ld = _as_rows(x)
-    _call(x, "mtp_rmsnorm_int8", x.data_ptr(), x_code, ld, *res_args, rows, c, weight.data_ptr(), w_code, eps, codes.data_ptr(),
+    codes, scale, ld_codes = _new_rows(x, rows, c)
+    _call(x2, "mtp_rmsnorm_int8", x2.data_ptr(), x_code, ld, *res_args, rows, c, weight.data_ptr(), w_code, eps, codes.data_ptr(),
           ld_codes, scale.data_ptr())
     return Int8Rows(codes, scale), h
 
@@ -187,25 +197,20 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
     """x [..., K] times weight [N, K]^T: (the exact int32 sum of the codes' products) * x's scale * weight's scale (+ bias),
     in float32 in this order, rounded to ``dtype``; [..., N].  A row's results depend on no other row."""
     what = "int8_linear"
-    _check_codes(x, what, "x")
-    _check_codes(weight, what, "weight")
-    wc, k = weight.codes, x.codes.shape[-1]
-    if wc.dim() != 2 or wc.shape[1] != k:
-        raise ValueError(f"{what}: x {tuple(x.codes.shape)} and weight {tuple(wc.shape)} do not fit")
-    _same_device(wc, x.codes, what, "weight")
-    code, n = L.dtype_code(dtype), wc.shape[0]
-    b_code = 0
+    a, m, k, ld_a, a_scale = _as_codes(x, what, "x")
+    wc, n, wk, ld_w, w_scale = _as_codes(weight, what, "weight")
+    if wk != k or weight.codes.dim() != 2:
+        raise ValueError(f"{what}: x {tuple(x.codes.shape)} and weight {tuple(weight.codes.shape)} do not fit")
+    _same_device(wc, a, what, "weight")
+    code, b_code = L.dtype_code(dtype), 0
     if bias is not None:
         if bias.shape != (n,):
             raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected {(n,)}")
-        _same_device(bias, x.codes, what, "bias")
+        _same_device(bias, a, what, "bias")
         b_code = L.dtype_code(bias.dtype)
         bias = bias.contiguous()
     _refuse_grad(what, x.scale, weight.scale, bias)
-    out = wc.new_empty(*x.codes.shape[:-1], n, dtype=dtype)
-    a, m, _, ld_a = _as_rows(x.codes)
-    wc, _, _, ld_w = _as_rows(wc)
-    a_scale, w_scale = _flat(x.scale), _flat(weight.scale)
+    out = wc.new_empty(m, n, dtype=dtype) if x.codes.dim() == 2 else wc.new_empty(*x.codes.shape[:-1], n, dtype=dtype)
     _call(a, "mtp_int8_linear", a.data_ptr(), ld_a, a_scale.data_ptr(), m, k, wc.data_ptr(), ld_w, w_scale.data_ptr(), n,
           L.ptr(bias), b_code, out.data_ptr(), code, n)
     return out
