@@ -4,6 +4,8 @@
 // together, and the slices' int32 sums are added in shared memory (exact in any order).  The products go through
 // mma.m16n8k32: 16 channels by 8 tokens.  A lane's 16 bytes of a row are not those that the instruction's layout gives it, but
 // it takes the same ones of w and of the tokens, and the order of k within a sum does not matter.
+// Measured on a B200, L2 cold (us; w at 6550 GB/s): 1 x 2048 -> 8192 5.5 (2.6), 1 x 4096 -> 2048 3.5 (1.3), 16 rows 6.0 and
+// 4.2, 1 x 2048 -> 50280 20.5 (15.7).  About 1 us is the launch, 1.5 the way of one load and of the sums through the CTA.
 #include "int8_linear.cuh"
 
 namespace mtp {

@@ -39,7 +39,8 @@ bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t 
 int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
               cudaStream_t stream);
 
-// For few tokens; operands on 16-byte boundaries as above.
+// For few tokens; operands on 16-byte boundaries as above.  (17 rows x 4096 -> 2048: 9.2 us here in three groups of 8, 6.7 in
+// the tensor-core form; 16 rows 4.2.)
 constexpr int FEW = 16;
 int linear_few(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
                cudaStream_t stream);

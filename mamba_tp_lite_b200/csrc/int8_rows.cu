@@ -1,11 +1,17 @@
 // Rows of int8 codes with a scale each: quantising, reading back, and RMSNorm with the residual's addition and an int8
 // output.
 //
-// All are bound by HBM.  A row belongs to a team of threads (a warp, or a CTA) that keeps it in registers, so that it is read
-// once: 16 or 32 values a thread, in vectors where rows lie on vector boundaries.  Which of two codes is the nearer is decided as in
-// exact arithmetic without paying for 64 bits at each value: fp32 gives the quotient to 3e-5 of a step, and only a value
-// whose quotient is within 2^-14 of a half (1 in 8000) is looked at again in 64 bits.
-// Rows of more than 16384 values, and rows whose numbers leave fp32's middle range, go through the plain 64-bit loops.
+// Bound by HBM, or for a row at a time by latency.  A row belongs to a team of threads (a warp, or a CTA) that keeps it in
+// registers, so that it is read once; vectors of 16 bytes, shifted together from two where rows do not lie on such boundaries.
+// Which of two codes is the nearer is decided as in exact arithmetic without 64 bits for each value: a value held exactly leaves
+// an exact remainder in fp32 (exact_codes4); a norm's quotient is known to 3e-5 of a step in fp32, and only where it is within
+// 2^-14 of a half (1 in 8000) is it taken again in 64 bits (write_codes).  Rows of more than 16384 values, and rows whose
+// numbers leave fp32's middle range, go through 64-bit loops (slow_row).
+//
+// Measured on a B200, L2 cold, beside the bytes at 6550 GB/s (us): quantise 32768 x 4096 bf16 66.3 (61.5), 2560 x 5120 fp32 10.8
+// (10.0), read back 32768 x 4096 bf16 62.6 (61.5); norm 32768 x 2048 bf16 + fp32 stream 120 (113), fp32 + fp32 130 (133), bf16
+// + bf16 97 (72), bf16 alone 80 (31): where few bytes come for each value, a norm is bound by instructions and barriers (26
+// instructions a value, two barriers a row).  Odd widths, 20000 x 1111 bf16: quantise 29 (10), norm with an fp32 stream 106 (37).
 #include <type_traits>
 #include "int8_linear.cuh"
 
@@ -14,7 +20,7 @@ namespace {
 
 using i8::MAX_COLS;
 
-constexpr int MAX_HELD = 16384;        // columns of a row that a CTA holds, 16 or 32 a thread
+constexpr int MAX_HELD = 16384;        // columns of a row that a CTA holds
 constexpr int LONG_THREADS = 256;
 constexpr int UNROLL = 4;              // vectors that a thread reads back, their loads in flight together
 constexpr float MAGIC = 12582912.f;    // 1.5 * 2^23: x + MAGIC is x rounded to a whole number, its low byte the int8
@@ -26,7 +32,7 @@ __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 
 // fp32 scale of a row whose largest |y| is amax; NaN for a row with a NaN or an infinity (`bad`).
 __device__ __forceinline__ float scale_of(double amax, bool bad) {
-  const float s = (float)(fmax(amax, 1e-8) * (1.0 / 127.0));
+  const float s = (float)(fmax(amax, 1e-8) / 127.0);
   return bad || !(s <= FLT_TOP) ? nan_f() : s;
 }
 
@@ -547,8 +553,8 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
       }
     }
     top = team.max_rare(top);
-    const float s = scale_of(top, false);
-    const float c = __fmul_rn((float)rs, __frcp_rn(s));
+    const float s = (float)(fmax(top, 1e-8) * (1.0 / 127.0));
+    const float c = __fmul_rn((float)rs, __frcp_rn(s));  // 0, and so not taken, where s is infinite
     const uint32_t cb = __float_as_uint(c);
     if (cb >= TINY && cb <= HUGE_) {
       write_codes<VEC, RAGGED>(p, c, s, out, cols, rank, size, y_of);
@@ -715,7 +721,7 @@ template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP> v
 }
 
 // A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 120 us, with 32 160); few rows have CTAs of 8 values a thread
-// whatever their length (1 x 2048: NEW us, with 16 2.9).
+// whatever their length (1 x 2048: 2.4 us, with 16 2.9).
 template <typename TX, typename TR, int VEC, bool RAGGED> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
   if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, RAGGED, 8, false>(a, s);
   else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, RAGGED, 16, true>(a, s);

@@ -8,6 +8,11 @@
 //   warps 2-9  epilogue, two warps per lane quarter, each on every second block of 128 bytes of output columns: sums to fp32,
 //              times the row's scale (a lane has one row) and the columns' (from shared memory), rounded into a staging block
 //              in the swizzled layout of a TMA store.  It works on one tile while the tensor cores fill the other accumulator.
+// Bound by the tensor cores and by what feeds them: at full rate the pair's 256 x 256 tile takes 64 bytes a clock and SM from
+// L2, all that a port gives; without the products the copies alone take two thirds of the time.  Measured on a B200 (TOP/s;
+// nominal 4500, 3360 being twice the measured bf16 rate): 32768 x 2048 -> 8192 bf16 378 us, 2900; 32768 x 4096 -> 2048 172 us,
+// 3190; 8192 x 2048 -> 8192 95 us, 2890.  Below K = 1024 the epilogue bounds it: 3.5 us for a tile of a pair, of which the
+// stores 1.2, the reading of tensor memory and the arithmetic 1.1.
 // Every wait is bounded; a CTA whose wait expires gives NaN for what it has left, waits (again with a limit) for its copies and
 // products in flight, frees its tensor memory and returns.
 #include "int8_linear.cuh"
@@ -365,7 +370,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 // ------------------------------------------------------------------ at most 128 tokens
 // One tile of up to 128 tokens x bn channels per cluster, its K split over the cluster's CTAs, so that as many SMs as there
 // are stream w and most of a CTA's copies are in flight at once; each CTA's int32 sums go to its shared memory, and the
-// cluster adds them there (exact in any order).
+// cluster adds them there (exact in any order).  Bound by latency: 64 x 4096 -> 2048 7.2 us (8.4 MB of w: 1.3 us), with K
+// unsplit 12.9; 64 x 2048 -> 8192 8.3 us.
 constexpr int SPLIT_THREADS = 64 + 32 * EPI_WARPS;  // TMA, MMA and epilogue warps; all of them add
 constexpr int SPLIT_RING = 108 * 1024;  // two CTAs fit an SM: the next call's are set up while this one's work
 constexpr int SPLIT_MAX_STAGES = 24;
@@ -661,7 +667,28 @@ int allow_split_smem() {
   return MTP_OK;
 }
 
-int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
+// The split of up to 128 rows with the least time, and that time in us by what was measured: a call takes 5.3, a CTA's bytes
+// come at 62 KB/us (64 x 2048 -> 8192 in one, 256 KB: 9.5; 64 x 4096 -> 2048 in four, 131 KB: 7.2, in one, 524 KB: 12.9), the
+// addition takes 0.5, a further wave 2.
+double plan_split(int M, int N, int K, int &split_of_k, int &columns) {
+  const int sms = num_sms(), num_kb = ceil_div(K, BK), a_rows = (M + 7) / 8 * 8;
+  double best = 1e30;
+  for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
+    int bn = (ceil_div((int64_t)N * split, sms) + 15) / 16 * 16;
+    bn = bn < 32 ? 32 : bn > 128 ? 128 : bn;
+    const int64_t waves = ((int64_t)ceil_div(N, bn) * split + sms - 1) / sms;
+    const double kb = (double)ceil_div(num_kb, split) * (bn + a_rows) * BK / 1e3;
+    const double time = 5.3 + (double)waves * kb / 62.0 + (double)(waves - 1) * 2.0 + (split > 1 ? 0.5 : 0.0);
+    if (time < best) {
+      best = time;
+      split_of_k = split;
+      columns = bn;
+    }
+  }
+  return best;
+}
+
+int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int split, int bn,
               cudaStream_t stream) {
   SplitParams p{};
   p.o = o;
@@ -669,22 +696,8 @@ int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   p.N = N;
   p.K = K;
   p.a_rows = (M + 7) / 8 * 8;
-  const int sms = num_sms(), num_kb = ceil_div(K, BK);
-  // The split with the least time: measured, a call takes 5.3 us and a CTA's bytes at 62 KB/us (64 x 2048 -> 8192 in one, 256
-  // KB: 9.5 us; 64 x 4096 -> 2048 in four, 131 KB: 7.2 us, in one, 524 KB: 12.9), the addition 0.5 us, a further wave 2 us.
-  double best = 1e30;
-  for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
-    int bn = (ceil_div((int64_t)N * split, sms) + 15) / 16 * 16;
-    bn = bn < 32 ? 32 : bn > 128 ? 128 : bn;
-    const int64_t waves = ((int64_t)ceil_div(N, bn) * split + sms - 1) / sms;
-    const double bytes = (double)ceil_div(num_kb, split) * (bn + p.a_rows) * BK;
-    const double cost = (double)waves * bytes + (double)(waves - 1) * 124e3 + (split > 1 ? 31e3 : 0.0);
-    if (cost < best) {
-      best = cost;
-      p.split = split;
-      p.bn = bn;
-    }
-  }
+  p.split = split;
+  p.bn = bn;
   p.slot = (p.a_rows + p.bn) * BK;
   // rows of tokens past a_rows are read by the tensor core from what follows in the slot: the last slot ends 128 rows in
   p.stages = (SPLIT_RING - (BM - p.a_rows) * BK) / p.slot;
@@ -726,7 +739,6 @@ bool tc_eligible(const int8_t *a, int64_t ld_a, int M, const int8_t *w, int64_t 
 
 int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o,
               cudaStream_t stream) {
-  if (M <= BM) return run_split(a, ld_a, M, K, w, ld_w, N, o, stream);
   // Of three tiles the one with the least time by what was measured (us): a call's own, then for each round of tiles 0.3 for a
   // block of K, whatever the tile, and what the epilogue adds.  (512 x 2048 -> 8192: 22.4, 14.1 and 11.7 us; 256 rows: 13.2,
   // 9.2 and 11.3; 256 x 2048 -> 1024: 7.7, 8.2 and 9.9.)
@@ -736,7 +748,14 @@ int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
     return call + (double)((tiles + places - 1) / places) * (num_kb * kb + tile);
   };
   const double t1 = time_of(1, 64, 2.3, 0.287, 0.42), t2 = time_of(1, 128, 2.3, 0.287, 1.1), t3 = time_of(2, 256, 3.4, 0.306, 1.6);
-  if (t3 <= t1 && t3 <= t2) return run<2>(a, ld_a, M, K, w, ld_w, N, o, 256, stream);
+  if (M <= BM) {
+    // Up to 64 rows by split K (32 x 2048 -> 8192: 7.5 us, by tiles of 64 columns 10.7; 64 rows: 8.3 and 8.3); to 128 where
+    // it is the faster (128 x 2048 -> 8192: 10.1 and 8.5; 128 x 4096 -> 2048: 8.6 and 12.1).
+    int split = 1, bn = 128;
+    const double t = plan_split(M, N, K, split, bn);
+    if (M <= 64 || t <= (t1 < t2 ? t1 : t2) + 0.5) return run_split(a, ld_a, M, K, w, ld_w, N, o, split, bn, stream);
+  }
+  if (M > BM && t3 <= t1 && t3 <= t2) return run<2>(a, ld_a, M, K, w, ld_w, N, o, 256, stream);
   return run<1>(a, ld_a, M, K, w, ld_w, N, o, t2 <= t1 ? 128 : 64, stream);
 }
 

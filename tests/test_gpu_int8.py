@@ -1,8 +1,11 @@
 """The 8-bit linear path on the GPU against its definitions in 64 bits (int8_ref.py has the bounds)."""
-import numpy as np
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from mamba_tp_lite_b200 import build as B
 from mamba_tp_lite_b200 import int8 as Q
 from tests import int8_ref as R
 from tests.gpu_util import dev
@@ -246,6 +249,14 @@ def test_linear_of_strided_rows(m, pad, offset):
         check_linear(codes_of(m, k, 1), codes_of(n, k, 2, pad, offset), None, [BF, F32])
 
 
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 40, 128, 129, 700, 2600])
+@pytest.mark.parametrize("n,k", [(70, 1), (130, 15), (64, 17), (100, 100), (1030, 257), (300, 1001), (2100, 2049)])
+def test_what_lies_behind_a_row_is_not_summed(m, n, k):
+    """Rows on 16-byte boundaries, with other codes between them."""
+    pad = -k % 16 or 16
+    check_linear(codes_of(m, k, 1, pad), codes_of(n, k, 2, pad), None, [F32])
+
+
 @pytest.mark.parametrize("m", [1, 3, 16, 40, 128, 300])
 def test_the_largest_sums(m):
     """-128 * -128 over 131071 columns is 2147467264, below 2^31."""
@@ -376,6 +387,32 @@ def test_captured_and_replayed(rows):
             for got, want in zip(out, boundary(*s)):
                 assert torch.equal(got, want)
         assert torch.equal(other[0], outs[1][0])
+
+
+FIRST_CALL = """
+import torch
+from mamba_tp_lite_b200 import int8 as Q
+g = torch.Generator().manual_seed(0)
+x = torch.randn({rows}, 512, generator=g).to(torch.bfloat16).cuda()
+r = torch.randn({rows}, 512, generator=g).cuda()
+w = torch.randn(600, 512, generator=g).cuda()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def run():
+    rows, h = Q.add_rms_norm_int8(x, r, w[0])
+    return Q.int8_linear(rows, Q.quantize_rows(w)), Q.dequantize_rows(rows), h
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+"""
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300, 3000])
+def test_the_first_call_of_a_process_may_be_a_captured_one(rows):
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(rows=rows)], cwd=B.REPO, timeout=300, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_two_streams_at_once():
