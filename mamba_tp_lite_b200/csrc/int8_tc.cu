@@ -749,11 +749,11 @@ int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   };
   const double t1 = time_of(1, 64, 2.3, 0.287, 0.42), t2 = time_of(1, 128, 2.3, 0.287, 1.1), t3 = time_of(2, 256, 3.4, 0.306, 1.6);
   if (M <= BM) {
-    // Up to 64 rows by split K (32 x 2048 -> 8192: 7.5 us, by tiles of 64 columns 10.7; 64 rows: 8.3 and 8.3); to 128 where
-    // it is the faster (128 x 2048 -> 8192: 10.1 and 8.5; 128 x 4096 -> 2048: 8.6 and 12.1).
+    // Below 64 rows by split K (32 x 2048 -> 8192: 7.5 us, by tiles of 64 columns 10.6); from there where it is the faster (64
+    // x 2560 -> 10240: 11.4 and 10.1; 128 x 2048 -> 8192: 10.1 and 8.5; 128 x 4096 -> 2048: 8.6 and 12.1).
     int split = 1, bn = 128;
     const double t = plan_split(M, N, K, split, bn);
-    if (M <= 64 || t <= (t1 < t2 ? t1 : t2) + 0.5) return run_split(a, ld_a, M, K, w, ld_w, N, o, split, bn, stream);
+    if (M < 64 || t <= (t1 < t2 ? t1 : t2) + 0.5) return run_split(a, ld_a, M, K, w, ld_w, N, o, split, bn, stream);
   }
   if (M > BM && t3 <= t1 && t3 <= t2) return run<2>(a, ld_a, M, K, w, ld_w, N, o, 256, stream);
   return run<1>(a, ld_a, M, K, w, ld_w, N, o, t2 <= t1 ? 128 : 64, stream);
