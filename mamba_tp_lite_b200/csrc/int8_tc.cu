@@ -11,8 +11,9 @@
 // Bound by the tensor cores and by what feeds them: at full rate the pair's 256 x 256 tile takes 64 bytes a clock and SM from
 // L2, all that a port gives; without the products the copies alone take two thirds of the time.  Measured on a B200 (TOP/s;
 // nominal 4500, 3360 being twice the measured bf16 rate): 32768 x 2048 -> 8192 bf16 378 us, 2900; 32768 x 4096 -> 2048 172 us,
-// 3190; 8192 x 2048 -> 8192 95 us, 2890.  Below K = 1024 the epilogue bounds it: 3.5 us for a tile of a pair, of which the
-// stores 1.2, the reading of tensor memory and the arithmetic 1.1.
+// 3190; 8192 x 2048 -> 8192 95 us, 2890.  To K = 1024 the epilogue bounds it, 2.6 us for a tile of a pair: 8192 x 1024 ->
+// 16384 109 us (3.5 us a tile and 131 with the arrival at the other CTA's barrier as a release of the cluster's scope, which
+// waits for all stores of its thread, and with divisions for a tile's coordinates).
 // Every wait is bounded; a CTA whose wait expires gives NaN for what it has left, waits (again with a limit) for its copies and
 // products in flight, frees its tensor memory and returns.
 #include "int8_linear.cuh"
@@ -34,8 +35,8 @@ constexpr int CHUNK_BYTES = 32 * 128;  // 32 rows x 128 bytes of output
 constexpr int B_BYTES = 128 * BK;  // at most 128 rows of w per CTA: bn = 256 takes a pair
 constexpr int SLOT = A_BYTES + B_BYTES, STAGES = 5;
 constexpr int STAGE_OUT = STAGES * SLOT;                    // the epilogue's blocks, one per warp
-constexpr int COLS = STAGE_OUT + EPI_WARPS * CHUNK_BYTES;   // scales and biases of the columns of two tiles
-constexpr int BARS = COLS + 2 * 2 * BN_MAX * 4;
+constexpr int COLS = STAGE_OUT + EPI_WARPS * CHUNK_BYTES;   // scales and biases of a warp's columns
+constexpr int BARS = COLS + EPI_WARPS * BN_MAX * 4;
 constexpr int SMEM_BYTES = BARS + 256 + 1024 /* to align the base */;
 
 struct Params {
@@ -44,16 +45,17 @@ struct Params {
   int bn, tiles_m, tiles_n, num_tiles, group_m;
   int tma_out;   // results by TMA stores
   uint32_t idesc;
+  uint64_t div_group, div_m, div_last;  // 2^64 / n, rounded up, for a group's tiles, its rows and the last group's rows
 };
 
+// Tiles in groups of group_m rows of tiles, rows fastest.  Divisions by multiplication: three by the instruction's way took a
+// tile's epilogue 600 cycles.
+__device__ __forceinline__ int div_by(int n, uint64_t m) { return (int)__umul64hi((uint64_t)(uint32_t)n, m); }
 __device__ __forceinline__ void tile_coords(const Params &p, int t, int &mt, int &nt) {
-  const int gsize = p.group_m * p.tiles_n;
-  const int g = t / gsize;
-  const int first_m = g * p.group_m;
-  const int gm = min(p.tiles_m - first_m, p.group_m);
-  const int r = t - g * gsize;
-  mt = first_m + r % gm;
-  nt = r / gm;
+  const int g = div_by(t, p.div_group), r = t - g * p.group_m * p.tiles_n;
+  const int first_m = g * p.group_m, gm = min(p.tiles_m - first_m, p.group_m);
+  nt = gm == 1 ? r : div_by(r, gm == p.group_m ? p.div_m : p.div_last);
+  mt = first_m + r - nt * gm;
 }
 
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
@@ -99,7 +101,8 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     umma_commit(bar);
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
+// 32 columns of a warp's lane quarter; tcgen05.wait::ld comes before they are used.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int *r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
       "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -108,7 +111,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
         "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
         "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 template <typename T> constexpr int PER_WORD = 16 / (int)sizeof(T);  // results in 16 bytes
@@ -247,76 +249,90 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ------------------------------------------------------------ epilogue (warps 2..9)
     constexpr int CW = 128 / (int)sizeof(T);  // columns of a block of output
     const int q = warp & 3, half = (warp - 2) >> 2;
-    const int et = threadIdx.x - 64;
     unsigned char *stage = gbase + STAGE_OUT + (warp - 2) * CHUNK_BYTES;
-    float *cols = reinterpret_cast<float *>(gbase + COLS);
+    // this warp's columns of a tile, block after block: their scales, and after 128 of them their biases
+    float *sw = reinterpret_cast<float *>(gbase + COLS) + (warp - 2) * 256, *sb = sw + 128;
+    constexpr int HELD = 128 / 32;  // of them, a lane's
     int local = 0;
     bool alive = true;
+    // fetched one tile ahead: the scale of this lane's row, and of its columns
+    float next_a = 0.f, next_w[HELD] = {}, next_b[HELD] = {};
+    auto fetch = [&](int t) {
+      if (t >= p.num_tiles) return;
+      int mt, nt;
+      tile_coords(p, t, mt, nt);
+      const int m = (mt * CG + (int)rank) * BM + q * 32 + lane;
+      next_a = m < p.M ? p.o.a_scale[m] : 0.f;
+#pragma unroll
+      for (int j = 0; j < HELD; ++j) {
+        const int i = 32 * j + lane, c = (i / CW * 2 + half) * CW + i % CW, n = nt * p.bn + c;
+        const bool in = c < p.bn && n < p.N;
+        next_w[j] = in ? p.o.w_scale[n] : 0.f;
+        next_b[j] = in ? ld_bias(p.o, n) : 0.f;
+      }
+    };
+    fetch(first);
     for (int t = first; t < p.num_tiles; t += step, ++local) {
       int mt, nt;
       tile_coords(p, t, mt, nt);
       const int a = local & 1;
       const uint32_t use = (uint32_t)(local >> 1);
       const int n_tile = nt * p.bn, m0 = (mt * CG + (int)rank) * BM + q * 32;
-      const int m = m0 + lane;
-      const float sa = m < p.M ? p.o.a_scale[m] : 0.f;
-      // the columns' scales and biases: written by all epilogue warps into the buffer that the tile before the last used
-      float *sw = cols + a * 2 * BN_MAX, *sb = sw + BN_MAX;
-      for (int c = et; c < p.bn; c += 32 * EPI_WARPS) {
-        const bool in = n_tile + c < p.N;
-        sw[c] = in ? p.o.w_scale[n_tile + c] : 0.f;
-        sb[c] = in ? ld_bias(p.o, n_tile + c) : 0.f;
+      const float sa = next_a;
+#pragma unroll
+      for (int j = 0; j < HELD; ++j) {
+        sw[32 * j + lane] = next_w[j];
+        sb[32 * j + lane] = next_b[j];
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(32 * EPI_WARPS) : "memory");
+      __syncwarp();
+      fetch(t + step);
       alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, TIMEOUT_NS));
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN_MAX);
-      for (int c0 = half * CW; c0 < p.bn; c0 += 2 * CW) {
+      int at_col = 0;
+      for (int c0 = half * CW; c0 < p.bn; c0 += 2 * CW, at_col += CW) {
         if (n_tile + c0 >= p.N || m0 >= p.M) break;
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();  // the block is free again
+        int acc[CW] = {};
+        if (alive) {
 #pragma unroll
-        for (int g = 0; g < CW; g += 32) {
-          int acc[32] = {};
-          if (alive) tmem_ld32(tbase + (uint32_t)(c0 + g), acc);
-          float v[32];
+          for (int g = 0; g < CW; g += 32) tmem_ld32(tbase + (uint32_t)(c0 + g), acc + g);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+        uint4 word[8];  // 128 bytes of this lane's row
+        constexpr int PER = PER_WORD<T>;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 w4 = *reinterpret_cast<const float4 *>(sw + c0 + g + i);
-            v[i] = scaled(acc[i], sa, w4.x);
-            v[i + 1] = scaled(acc[i + 1], sa, w4.y);
-            v[i + 2] = scaled(acc[i + 2], sa, w4.z);
-            v[i + 3] = scaled(acc[i + 3], sa, w4.w);
-          }
-          if (p.o.bias) {
+        for (int i = 0; i < CW; i += PER) {
+          float v[PER];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 b4 = *reinterpret_cast<const float4 *>(sb + c0 + g + i);
-              v[i] = __fadd_rn(v[i], b4.x);
-              v[i + 1] = __fadd_rn(v[i + 1], b4.y);
-              v[i + 2] = __fadd_rn(v[i + 2], b4.z);
-              v[i + 3] = __fadd_rn(v[i + 3], b4.w);
+          for (int k = 0; k < PER; k += 4) {
+            const float4 w4 = *reinterpret_cast<const float4 *>(sw + at_col + i + k);
+            v[k] = scaled(acc[i + k], sa, w4.x);
+            v[k + 1] = scaled(acc[i + k + 1], sa, w4.y);
+            v[k + 2] = scaled(acc[i + k + 2], sa, w4.z);
+            v[k + 3] = scaled(acc[i + k + 3], sa, w4.w);
+            if (p.o.bias) {
+              const float4 b4 = *reinterpret_cast<const float4 *>(sb + at_col + i + k);
+              v[k] = __fadd_rn(v[k], b4.x);
+              v[k + 1] = __fadd_rn(v[k + 1], b4.y);
+              v[k + 2] = __fadd_rn(v[k + 2], b4.z);
+              v[k + 3] = __fadd_rn(v[k + 3], b4.w);
             }
           }
           if (!alive) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fffffff);
+            for (int k = 0; k < PER; ++k) v[k] = __int_as_float(0x7fffffff);
           }
-          // row `lane` of the block: its eight 16-byte words lie where the 128-byte swizzle has them
-          constexpr int PER = PER_WORD<T>;
-#pragma unroll
-          for (int i = 0; i < 32; i += PER) {
-            const int word = (g + i) / PER;
-            uint4 *at = reinterpret_cast<uint4 *>(stage + lane * 128 + ((word ^ (lane & 7)) << 4));
-            if constexpr (sizeof(T) == 4) {
-              *at = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]),
-                               __float_as_uint(v[i + 3]));
-            } else {
-              *at = make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
-                               pack2<T>(v[i + 6], v[i + 7]));
-            }
-          }
+          if constexpr (sizeof(T) == 4)
+            word[i / PER] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          else
+            word[i / PER] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();  // the block is free again
+        // row `lane` of the block: its eight 16-byte words lie where the 128-byte swizzle has them
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4 *>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = word[i];
         if (p.tma_out) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -345,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) {
         if (CG == 2 && rank != 0)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(tempty_bar(a), 0))
+          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(tempty_bar(a), 0))
                        : "memory");
         else
           mbar_arrive(tempty_bar(a));
@@ -488,6 +504,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
       for (int c = 32 * half; c < p.bn; c += 64) {
         int r[32];
         tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (m < p.M) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
@@ -633,6 +650,10 @@ int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld
   p.tiles_n = ceil_div(N, bn);
   p.num_tiles = p.tiles_m * p.tiles_n;
   p.group_m = 16;
+  auto inverse = [](int64_t n) { return n > 1 ? ~(uint64_t)0 / (uint64_t)n + 1 : 0; };
+  p.div_group = inverse((int64_t)p.group_m * p.tiles_n);
+  p.div_m = inverse(p.group_m);
+  p.div_last = inverse(p.tiles_m % p.group_m);
   // kind::i8, int32 results, signed operands, both with K innermost
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
   const size_t es = o.dtype == MTP_F32 ? 4 : 2;
