@@ -519,22 +519,29 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   cluster_sync();
   tc_fence_after();
   {
-    const int quads = p.bn / 4, total = p.M * quads;
+    const int quads = p.bn / 4;
     bool lost = false;
     for (int i = 0; i < p.split; ++i) {
       int v;
       asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(abort_at, i)));
       lost |= v != 0;
     }
-    for (int e = (int)rank * SPLIT_THREADS + threadIdx.x; e < total; e += p.split * SPLIT_THREADS) {
-      const int m = e / quads, c = (e - m * quads) * 4, n = n0 + c;
-      if (n >= p.N) continue;
+    // a warp takes a row of sums, or two or four where they are short, of every split-th block of rows
+    const int fold = quads <= 8 ? 2 : quads <= 16 ? 1 : 0, per = 1 << fold;
+    const int c = (lane & (31 >> fold)) * 4, n = n0 + c;
+    for (int m = (((int)rank * (SPLIT_THREADS / 32) + warp) << fold) + (lane >> (5 - fold)); m < p.M;
+         m += p.split * (SPLIT_THREADS / 32) * per) {
+      if (c >= p.bn || n >= p.N) continue;
       const uint32_t at = base + (uint32_t)(m * LD_PART + c) * 4u;
+      int4 part_of[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < p.split) part_of[i] = ld_cluster(cluster_addr(at, i));
       int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 8
-      for (int i = 0; i < p.split; ++i) {
-        const int4 v = ld_cluster(cluster_addr(at, i));
-        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= p.split) continue;
+        sum.x += part_of[i].x; sum.y += part_of[i].y; sum.z += part_of[i].z; sum.w += part_of[i].w;
       }
       const float sa = scale_a[m];
       const int in = min(4, p.N - n);
@@ -559,7 +566,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     }
   }
   if (*abort) __nanosleep(1000000);  // copies in flight
-  cluster_sync();                    // no other CTA reads this one's sums any more
+  // No other CTA reads this one's sums any more.  (Relaxed: nothing written since is read in the cluster; a release would wait
+  // for the results' stores, 0.8 us.)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem_base));
 }
 
