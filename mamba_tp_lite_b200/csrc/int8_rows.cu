@@ -264,7 +264,10 @@ template <bool WARP> struct Team {
     u = __reduce_max_sync(0xffffffffu, u);
     if (WARP) return;
     const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (n == 1) return;
+    if (n == 1) {
+      __syncwarp();  // what one lane has set up for the team
+      return;
+    }
     if (lane == 0) {
       j->d[threadIdx.x >> 5] = s;
       j->u[threadIdx.x >> 5] = u;

@@ -332,6 +332,21 @@ def test_offsets_past_32_bits():
         R.check_rows(q.codes[part], q.scale[part], R.norm(h[part], weight, 1e-5))
 
 
+def test_millions_of_short_rows():
+    rows, k, n = 3_000_001, 16, 24
+    x = rows_of(rows, k, BF, 5)
+    q, h = Q.add_rms_norm_int8(x, x, torch.ones(k, device=dev()), 1e-5)
+    R.check_rows(q.codes, q.scale, R.norm(h, torch.ones(k, device=dev()), 1e-5))
+    r = Q.quantize_rows(x)
+    R.check_rows(r.codes, r.scale, x)
+    assert torch.equal(Q.dequantize_rows(r, BF), (r.codes.float() * r.scale.unsqueeze(-1)).to(BF))
+    w = codes_of(n, k, 2)
+    assert torch.equal(Q.int8_linear(r, w, dtype=F32), R.linear(r.codes, r.scale, w.codes, w.scale, None, F32))
+    odd = Q.Int8Rows(r.codes[:, :13], r.scale)  # off 16-byte boundaries
+    w = codes_of(n, 13, 2)
+    assert torch.equal(Q.int8_linear(odd, w, dtype=BF), R.linear(odd.codes, odd.scale, w.codes, w.scale, None, BF))
+
+
 # ------------------------------------------------------------------ as they are used
 def boundary(x, res, out_w, norm_w, in_w):
     """From a layer's scan output to the next layer's in_proj output."""
