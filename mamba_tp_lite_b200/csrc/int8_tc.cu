@@ -383,11 +383,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// ------------------------------------------------------------------ at most 128 tokens
+// ------------------------------------------------------------------ few tokens
 // One tile of up to 128 tokens x bn channels per cluster, its K split over the cluster's CTAs, so that as many SMs as there
 // are stream w and most of a CTA's copies are in flight at once; each CTA's int32 sums go to its shared memory, and the
-// cluster adds them there (exact in any order).  Bound by latency: 64 x 4096 -> 2048 7.2 us (8.4 MB of w: 1.3 us), with K
-// unsplit 12.9; 64 x 2048 -> 8192 8.3 us.
+// cluster adds them there (exact in any order).  Bound by latency: 64 x 4096 -> 2048 6.5 us (8.4 MB of w: 1.3 us), 32 x 2048 ->
+// 8192 7.1 (16.8 MB: 2.6).
 constexpr int SPLIT_THREADS = 64 + 32 * EPI_WARPS;  // TMA, MMA and epilogue warps; all of them add
 constexpr int SPLIT_RING = 108 * 1024;  // two CTAs fit an SM: the next call's are set up while this one's work
 constexpr int SPLIT_MAX_STAGES = 24;
@@ -397,7 +397,7 @@ constexpr int SPLIT_SMEM = SPLIT_BARS + 512 + 1024;
 struct SplitParams {
   Out o;
   int M, N, K;
-  int bn, a_rows, stages, slot, split;
+  int bn, a_rows, stages, slot, split, tiles_n;
   int vec_out;
   uint32_t idesc;
 };
@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int n0 = (int)(blockIdx.x / p.split) * p.bn;
+  const int tile = (int)(blockIdx.x / p.split), m0 = tile / p.tiles_n * BM, n0 = tile % p.tiles_n * p.bn;
+  const int rows = min(BM, p.M - m0);
   const int num_kb = (p.K + BK - 1) / BK;
   const int kb0 = (int)((long)num_kb * rank / p.split), kb1 = (int)((long)num_kb * (rank + 1) / p.split);
 
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
         if (kb >= kb0 + p.stages && !mbar_wait(empty_bar(s), ph ^ 1u, abort, TIMEOUT_NS)) break;
         mbar_expect_tx(full_bar(s), tx_bytes);
         const uint32_t sa = base + s * p.slot;
-        tma_load_2d(sa, &tmA, full_bar(s), kb * BK, 0);
+        tma_load_2d(sa, &tmA, full_bar(s), kb * BK, m0);
         tma_load_2d(sa + p.a_rows * BK, &tmB, full_bar(s), kb * BK, n0);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
@@ -495,17 +496,17 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
       const bool in = i < p.bn && n0 + i < p.N;
       scale_w[i] = in ? p.o.w_scale[n0 + i] : 0.f;
       bias_w[i] = in ? ld_bias(p.o, n0 + i) : 0.f;
-      scale_a[i] = i < p.M ? p.o.a_scale[i] : 0.f;
+      scale_a[i] = i < rows ? p.o.a_scale[m0 + i] : 0.f;
     }
     const bool alive = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort, TIMEOUT_NS + TIMEOUT_NS / 2));
     tc_fence_after();
-    if (alive && q * 32 < p.M) {
+    if (alive && q * 32 < rows) {
       const int m = q * 32 + lane;
       for (int c = 32 * half; c < p.bn; c += 64) {
         int r[32];
         tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (m < p.M) {
+        if (m < rows) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             if (c + i < p.bn)
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     // a warp takes a row of sums, or two or four where they are short, of every split-th block of rows
     const int fold = quads <= 8 ? 2 : quads <= 16 ? 1 : 0, per = 1 << fold;
     const int c = (lane & (31 >> fold)) * 4, n = n0 + c;
-    for (int m = (((int)rank * (SPLIT_THREADS / 32) + warp) << fold) + (lane >> (5 - fold)); m < p.M;
+    for (int m = (((int)rank * (SPLIT_THREADS / 32) + warp) << fold) + (lane >> (5 - fold)); m < rows;
          m += p.split * (SPLIT_THREADS / 32) * per) {
       if (c >= p.bn || n >= p.N) continue;
       const uint32_t at = base + (uint32_t)(m * LD_PART + c) * 4u;
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
         if (lost) y[i] = __int_as_float(0x7fffffff);
       }
       if (p.vec_out && in == 4) {
-        const int64_t to = (int64_t)m * p.o.ld + n;
+        const int64_t to = (int64_t)(m0 + m) * p.o.ld + n;
         if (p.o.dtype == MTP_F32) *reinterpret_cast<float4 *>((float *)p.o.p + to) = make_float4(y[0], y[1], y[2], y[3]);
         else if (p.o.dtype == MTP_BF16)
           *reinterpret_cast<uint2 *>((__nv_bfloat16 *)p.o.p + to) = make_uint2(pack2<__nv_bfloat16>(y[0], y[1]), pack2<__nv_bfloat16>(y[2], y[3]));
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < in) store_value(p.o, m, n + i, y[i]);
+          if (i < in) store_value(p.o, m0 + m, n + i, y[i]);
       }
     }
   }
@@ -697,18 +698,19 @@ int allow_split_smem() {
   return MTP_OK;
 }
 
-// The split of up to 128 rows with the least time, and that time in us by what was measured: a call takes 5.3, a CTA's bytes
-// come at 62 KB/us (64 x 2048 -> 8192 in one, 256 KB: 9.5; 64 x 4096 -> 2048 in four, 131 KB: 7.2, in one, 524 KB: 12.9), the
-// addition takes 0.5, a further wave 2.
+// The split with the least time, and that time in us by what was measured: a call takes 4.4, a CTA's bytes come at 62 KB/us
+// (64 x 2048 -> 8192 in one, 256 KB: 8.7; 64 x 4096 -> 2048 in four, 131 KB: 6.5, in one, 524 KB: 12.2), the addition takes
+// 0.5, a further wave 2.
 double plan_split(int M, int N, int K, int &split_of_k, int &columns) {
-  const int sms = num_sms(), num_kb = ceil_div(K, BK), a_rows = (M + 7) / 8 * 8;
+  const int sms = num_sms(), num_kb = ceil_div(K, BK), tiles_m = ceil_div(M, BM);
+  const int a_rows = M < BM ? (M + 7) / 8 * 8 : BM;
   double best = 1e30;
   for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
-    int bn = (ceil_div((int64_t)N * split, sms) + 15) / 16 * 16;
+    int bn = (ceil_div((int64_t)N * split * tiles_m, sms) + 15) / 16 * 16;
     bn = bn < 32 ? 32 : bn > 128 ? 128 : bn;
-    const int64_t waves = ((int64_t)ceil_div(N, bn) * split + sms - 1) / sms;
+    const int64_t waves = ((int64_t)ceil_div(N, bn) * tiles_m * split + sms - 1) / sms;
     const double kb = (double)ceil_div(num_kb, split) * (bn + a_rows) * BK / 1e3;
-    const double time = 5.3 + (double)waves * kb / 62.0 + (double)(waves - 1) * 2.0 + (split > 1 ? 0.5 : 0.0);
+    const double time = 4.4 + (double)waves * kb / 62.0 + (double)(waves - 1) * 2.0 + (split > 1 ? 0.5 : 0.0);
     if (time < best) {
       best = time;
       split_of_k = split;
@@ -725,9 +727,10 @@ int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   p.M = M;
   p.N = N;
   p.K = K;
-  p.a_rows = (M + 7) / 8 * 8;
+  p.a_rows = M < BM ? (M + 7) / 8 * 8 : BM;
   p.split = split;
   p.bn = bn;
+  p.tiles_n = ceil_div(N, bn);
   p.slot = (p.a_rows + p.bn) * BK;
   // rows of tokens past a_rows are read by the tensor core from what follows in the slot: the last slot ends 128 rows in
   p.stages = (SPLIT_RING - (BM - p.a_rows) * BK) / p.slot;
@@ -743,7 +746,7 @@ int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   rc = allow_split_smem();
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ceil_div(N, p.bn) * p.split);
+  cfg.gridDim = dim3(ceil_div(M, BM) * p.tiles_n * p.split);
   cfg.blockDim = dim3(SPLIT_THREADS);
   cfg.dynamicSmemBytes = SPLIT_SMEM;
   cfg.stream = stream;
@@ -778,9 +781,9 @@ int linear_tc(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
     return call + (double)((tiles + places - 1) / places) * (num_kb * kb + tile);
   };
   const double t1 = time_of(1, 64, 2.3, 0.287, 0.42), t2 = time_of(1, 128, 2.3, 0.287, 1.1), t3 = time_of(2, 256, 3.4, 0.306, 1.6);
-  if (M <= BM) {
-    // Below 64 rows by split K (32 x 2048 -> 8192: 7.5 us, by tiles of 64 columns 10.6); from there where it is the faster (64
-    // x 2560 -> 10240: 11.4 and 10.1; 128 x 2048 -> 8192: 10.1 and 8.5; 128 x 4096 -> 2048: 8.6 and 12.1).
+  if (M <= 2 * BM) {
+    // Below 64 rows by split K (32 x 2048 -> 8192: 7.1 us, by tiles of 64 columns 10.6); from there where it is the faster (128
+    // x 2048 -> 8192: 9.4 and 8.5; 128 x 4096 -> 2048: 7.7 and 12.1; 160 x 4096 -> 2048: 10.8 and 12.3).
     int split = 1, bn = 128;
     const double t = plan_split(M, N, K, split, bn);
     if (M < 64 || t <= (t1 < t2 ? t1 : t2) + 0.5) return run_split(a, ld_a, M, K, w, ld_w, N, o, split, bn, stream);

@@ -228,7 +228,8 @@ SIZES = [(1, 1, 1), (1, 5, 3), (1, 16, 16), (1, 777, 1001), (1, 2048, 4096), (1,
          (31, 300, 272), (32, 2048, 4096), (33, 8192, 2048), (48, 65, 1040), (64, 2048, 4096), (65, 160, 144), (96, 1024, 512),
          (127, 256, 256), (128, 256, 128), (129, 257, 144), (200, 1000, 1000), (256, 512, 2048), (300, 777, 1008), (333, 777, 1001),
          (513, 2048, 768), (1000, 100, 64), (1025, 640, 16), (2048, 2304, 2560), (4099, 24, 32), (3, 50280, 64),
-         (2500, 4100, 1000), (4099, 3001, 300), (5000, 6400, 128), (20, 10240, 2560), (100, 10240, 2560), (70, 50280, 64), (16, 20000, 2064)]
+         (2500, 4100, 1000), (4099, 3001, 300), (5000, 6400, 128), (20, 10240, 2560), (100, 10240, 2560), (70, 50280, 64), (16, 20000, 2064),
+         (130, 2048, 4096), (255, 1001, 2064), (256, 200, 8192), (192, 70, 20000), (250, 1024, 2048), (256, 2048, 4112)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
