@@ -396,7 +396,7 @@ int mtp_dequantize_rows(const int8_t *codes, int64_t ld_codes, const float *scal
                         int out_dtype, int64_t ld_out, void *stream);
 /* The residual's addition, the RMSNorm of model.py:130-135 and the quantiser in one call: h = x + resid in
  * fp32, rounded to resid_dtype and stored to resid_out (same type; resid_out may be resid itself,
- * but must not overlap it otherwise, nor x); y = w * h / sqrt(mean(h^2) + eps) with the mean, the root and the products in 64
+ * but must not overlap it otherwise, nor x or w); y = w * h / sqrt(mean(h^2) + eps) with the mean, the root and the products in 64
  * bits; codes and scale of y.  resid NULL: h = x and resid_out is not written.  eps >= 0. */
 int mtp_rmsnorm_int8(const void *x, int x_dtype, int64_t ld_x, const void *resid, int resid_dtype, int64_t ld_resid,
                      void *resid_out, int64_t ld_resid_out, int64_t rows, int cols, const void *w, int w_dtype,

@@ -12,6 +12,7 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .logprobs import _call, _refuse_tangent
@@ -95,13 +96,23 @@ def _as_codes(r: Int8Rows, what: str, name: str):
 
 def _extent(x: torch.Tensor):
     """(first byte of x, the byte after its last)."""
-    at = x.data_ptr()
-    return at, at + (1 + sum((n - 1) * st for n, st in zip(x.shape, x.stride()))) * x.element_size()
+    at, n = x.data_ptr(), x.numel()
+    if not x.is_contiguous() and n:
+        n = 1 + sum((size - 1) * st for size, st in zip(x.shape, x.stride()))
+    return at, at + n * x.element_size()
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two tensors (rows as of ``_as_rows``) may share memory."""
     (x0, x1), (y0, y1) = _extent(x), _extent(y)
-    return x0 < y1 and y0 < x1
+    if x1 <= y0 or y1 <= x0:
+        return False
+    if x.dim() == 2 and y.dim() == 2:  # columns beside each other in the same wider rows
+        step = x.stride(0) * x.element_size()
+        if step == y.stride(0) * y.element_size():
+            at, x_row, y_row = (y0 - x0) % max(step, 1), x.shape[1] * x.element_size(), y.shape[1] * y.element_size()
+            return at < x_row or at + y_row > step
+    return True
 
 
 def _new_rows(x: torch.Tensor, rows: int, c: int):
@@ -167,8 +178,9 @@ def _norm(x, residual, weight, eps, inplace, what):
         if inplace:
             if res.data_ptr() != residual.data_ptr():
                 raise ValueError(f"{what}: a residual that is updated in place needs rows on one stride")
-            if _overlap(x, residual):
-                raise ValueError(f"{what}: a residual that is updated in place must not share memory with x")
+            if _overlap(x, residual) or _overlap(weight, residual):
+                raise ValueError(f"{what}: a residual that is updated in place must not share memory with x or weight")
+            increment_version(residual)  # a backward pass that has kept it shall see that it changed
             h, ld_h = residual, ld_res
         else:
             h, ld_h = _new_like(residual, residual.dtype), c

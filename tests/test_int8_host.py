@@ -69,7 +69,7 @@ def test_arguments(monkeypatch):
     rec = Recorder(monkeypatch)
     x, w = rows(), torch.ones(16)
     r = Q.Int8Rows(*plain(x.double()))
-    far = torch.empty(16, device="meta")
+    far, wide = torch.empty(16, device="meta"), torch.randn(5, 32)
     refused = [
         (TypeError, "dtype", lambda: Q.quantize_rows(x.double())),
         (TypeError, "dtype", lambda: Q.quantize_rows(x.to(torch.int32))),
@@ -97,6 +97,9 @@ def test_arguments(monkeypatch):
         (ValueError, "one stride", lambda: Q.add_rms_norm_int8(x.view(2, 2, 16), rows(6, 16).view(2, 3, 16)[:, 1:], w, inplace=True)),
         (ValueError, "share memory", lambda: Q.add_rms_norm_int8(x, x, w, inplace=True)),
         (ValueError, "share memory", lambda: Q.add_rms_norm_int8(x[:3], x[1:], w, inplace=True)),
+        (ValueError, "share memory", lambda: Q.add_rms_norm_int8(rows(), x, x[3], inplace=True)),
+        (ValueError, "share memory", lambda: Q.add_rms_norm_int8(wide[:, :16], wide[:, 15:31], w, inplace=True)),
+        (ValueError, "share memory", lambda: Q.add_rms_norm_int8(wide[1:, :16], wide.as_strided((4, 16), (32, 1), 24), w, inplace=True)),
         (ValueError, "do not fit", lambda: Q.int8_linear(r, Q.Int8Rows(r.codes[:, :15], r.scale))),
         (ValueError, "do not fit", lambda: Q.int8_linear(r, Q.Int8Rows(r.codes[0], r.scale[0]))),
         (ValueError, "weight is on", lambda: Q.int8_linear(r, Q.Int8Rows(torch.empty(4, 16, device="meta", dtype=torch.int8),
@@ -110,6 +113,25 @@ def test_arguments(monkeypatch):
         with pytest.raises(error, match=text):
             call()
     assert not rec.calls
+
+
+def test_in_place_beside_x_and_weight_in_one_buffer(monkeypatch):
+    rec = Recorder(monkeypatch)
+    wide, w = torch.randn(4, 48), torch.randn(32)
+    for x, res, weight in [(wide[:, :16], wide[:, 16:32], w[:16]), (wide[:, 32:], wide[:, :16], w[16:]), (wide[:2, :16], wide[2:, :16], w[:16]),
+                           (wide[:0, :16], wide[:0, :16], w[:16])]:
+        assert Q.add_rms_norm_int8(x, res, weight, inplace=True)[1] is res
+    assert len(rec.calls) == 4
+
+
+def test_in_place_is_seen_by_a_backward_pass(monkeypatch):
+    Recorder(monkeypatch)
+    res, scale = rows(), torch.ones(16, requires_grad=True)
+    y = res * scale  # keeps res
+    with torch.no_grad():
+        Q.add_rms_norm_int8(rows(), res, torch.ones(16), inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
 
 
 def test_gradients_are_refused(monkeypatch):
