@@ -429,7 +429,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   const int num_kb = (p.K + BK - 1) / BK;
   const int kb0 = (int)((long)num_kb * rank / p.split), kb1 = (int)((long)num_kb * (rank + 1) / p.split);
 
-  MTP_PDL_TRIGGER();
   if (threadIdx.x == 0) {
     // w on its way to L2 (where a write of the kernel before would meet it) while that kernel ends
     for (int kb = kb0; kb < kb1 && kb < kb0 + p.stages; ++kb)
@@ -450,6 +449,8 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Not before the tensor memory is there: a next kernel's CTA that took it first, and waits for this kernel, would end both.
+  MTP_PDL_TRIGGER();
   MTP_PDL_WAIT();
   const uint32_t tmem_base = *tmem_holder;
   constexpr int LD_PART = 132;  // of a token's sums, in words: 16-byte writes of a warp's rows meet each bank equally often
