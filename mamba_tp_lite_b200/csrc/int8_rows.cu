@@ -9,9 +9,9 @@
 // numbers leave fp32's middle range, go through 64-bit loops (slow_row).
 //
 // Measured on a B200, L2 cold, beside the bytes at 6550 GB/s (us): quantise 32768 x 4096 bf16 66.3 (61.5), 2560 x 5120 fp32 10.8
-// (10.0), read back 32768 x 4096 bf16 62.6 (61.5); norm 32768 x 2048 bf16 + fp32 stream 120 (113), fp32 + fp32 130 (133), bf16
-// + bf16 97 (72), bf16 alone 80 (31): where few bytes come for each value, a norm is bound by instructions and barriers (26
-// instructions a value, two barriers a row).  Odd widths, 20000 x 1111 bf16: quantise 29 (10), norm with an fp32 stream 106 (37).
+// (10.0), read back 32768 x 4096 bf16 62.6 (61.5); norm 32768 x 2048 bf16 + fp32 stream 113 (113), fp32 + fp32 130 (133), bf16
+// + bf16 82 (72), bf16 alone 68 (31): where few bytes come for each value, a norm is bound by its instructions (25 a value, issued
+// in 74% of the cycles).  Odd widths, 20000 x 1111 bf16: quantise 29 (10), norm with an fp32 stream 89 (37).
 #include <type_traits>
 #include "int8_linear.cuh"
 
@@ -354,11 +354,13 @@ __device__ __forceinline__ void store_codes(const uint32_t (&q)[EACH / 4], int8_
   }
 }
 
-// Writes the codes of the products p[] * c that a thread holds; value(i, col) gives the i-th's y in 64 bits.
-template <int VEC, bool RAGGED, int EACH, typename Y>
+// Writes the codes of the products p[] * c that a thread holds; value(i, col) gives the i-th's y in 64 bits.  INLINE: where it
+// takes its values from registers, each border stands on its own; else they are met in a loop after the words are written, which
+// keeps the kernel's code short (32768 x 1024 bf16 alone 38 us, each on its own 46).
+template <int VEC, bool RAGGED, int EACH, bool INLINE, typename Y>
 __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, float s, int8_t *codes, int cols, int rank, int size,
                                             Y value) {
-  uint32_t q[EACH / 4];
+  uint32_t q[EACH / 4], near[(EACH + 31) / 32] = {};
 #pragma unroll
   for (int g = 0; g < EACH / 4; ++g) {
     float far = 0.f;
@@ -367,16 +369,31 @@ __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, flo
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = 4 * g + k;
-        const float m = fmaf(p[i], c, MAGIC), t = __fmul_rn(p[i], c);
+        const float m = fmaf(p[i], c, MAGIC);
         if (fabsf(fmaf(p[i], c, -__fsub_rn(m, MAGIC))) > BORDER) {
-          const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
-          const uint32_t code = (uint32_t)border_code(value(i, col), t, s) & 0xffu;
-          q[g] = (q[g] & ~(0xffu << (8 * k))) | code << (8 * k);
+          if (INLINE) {
+            const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
+            const uint32_t code = (uint32_t)border_code(value(i, col), __fmul_rn(p[i], c), s) & 0xffu;
+            q[g] = (q[g] & ~(0xffu << (8 * k))) | code << (8 * k);
+          } else {
+            near[i / 32] |= 1u << (i & 31);
+          }
         }
       }
     }
   }
   store_codes<VEC, RAGGED, EACH>(q, codes, cols, rank, size);
+  if (!INLINE) {
+#pragma unroll
+    for (int j = 0; j < (EACH + 31) / 32; ++j) {
+#pragma unroll 1
+      for (uint32_t left = near[j]; left; left &= left - 1) {
+        const int i = 32 * j + __ffs(left) - 1, col = ((i / VEC) * size + rank) * VEC + i % VEC;
+        const double y = value(i, col);
+        codes[col] = (int8_t)border_code(y, (float)(y / (double)s), s);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ quantise
@@ -505,16 +522,19 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
 #pragma unroll
     for (int v = 0; v < NV; ++v) to_f32(raw[v], p + v * VEC);
   }
+  auto weights = [&] {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int col = (v * size + rank) * VEC;
-    if (col < cols) {
-      load_weight<VEC, RAGGED>(a.w, a.w_dtype, col, cols, w + v * VEC);
-    } else {
+    for (int v = 0; v < NV; ++v) {
+      const int col = (v * size + rank) * VEC;
+      if (col < cols) {
+        load_weight<VEC, RAGGED>(a.w, a.w_dtype, col, cols, w + v * VEC);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) w[v * VEC + i] = 0.f;
+        for (int i = 0; i < VEC; ++i) w[v * VEC + i] = 0.f;
+      }
     }
-  }
+  };
+  if (!RAGGED) weights();  // ragged rows have the registers of their shifts to themselves first (20000 x 1111 bf16 + fp32: 88 us, else 98)
   double ss = 0.0, ss2 = 0.0;
   float top_here = 0.f;
 #pragma unroll
@@ -524,6 +544,7 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
     ss2 = fma(h1, h1, ss2);
   }
   ss += ss2;
+  if (RAGGED) weights();
   float h[KEEP ? EACH : 1];
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
@@ -546,11 +567,23 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
   int8_t *out = a.codes + row * a.ld_codes;
   if (most >= TINY && most <= HUGE_ && rs < 1e30) {
     double top = 0.0;
+    uint32_t at_top[(EACH + 31) / 32] = {};
     if (mine == most) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         if ((__float_as_uint(p[i]) & 0x7fffffffu) == most) {
           const int col = ((i / VEC) * size + rank) * VEC + i % VEC;
+          if (KEEP) top = fmax(top, fabs(y_of(i, col)));
+          else at_top[i / 32] |= 1u << (i & 31);
+        }
+      }
+    }
+    if (!KEEP) {
+#pragma unroll
+      for (int j = 0; j < (EACH + 31) / 32; ++j) {
+#pragma unroll 1
+        for (uint32_t left = at_top[j]; left; left &= left - 1) {
+          const int i = 32 * j + __ffs(left) - 1, col = ((i / VEC) * size + rank) * VEC + i % VEC;
           top = fmax(top, fabs(y_of(i, col)));
         }
       }
@@ -560,7 +593,7 @@ __global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EAC
     const float c = __fmul_rn((float)rs, __frcp_rn(s));  // 0, and so not taken, where s is infinite
     const uint32_t cb = __float_as_uint(c);
     if (cb >= TINY && cb <= HUGE_) {
-      write_codes<VEC, RAGGED>(p, c, s, out, cols, rank, size, y_of);
+      write_codes<VEC, RAGGED, EACH, KEEP>(p, c, s, out, cols, rank, size, y_of);
       if (rank == 0) a.scale[row] = s;
       return;
     }
@@ -723,13 +756,14 @@ template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP> v
   launch_pdl(norm_kernel<TX, TR, VEC, RAGGED, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
 }
 
-// A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 120 us, with 32 160); few rows have CTAs of 8 values a thread
-// whatever their length (1 x 2048: 2.4 us, with 16 2.9).
+// A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 113 us, with 32 135), 32 where x and the stream are of 16 bits and
+// take few registers (bf16 alone: 68 us, with 16 75; 8192 x 5120: 45 and 57), though not for ragged rows (20000 x 1111: 45 us, with
+// 32 68); few rows have CTAs of 8 values a thread whatever their length (1 x 2048: 2.4 us, with 16 2.9).
 template <typename TX, typename TR, int VEC, bool RAGGED> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
   if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, RAGGED, 8, false>(a, s);
   else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, RAGGED, 16, true>(a, s);
   else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, RAGGED, 32, true>(a, s);
-  else launch_norm_kernel<TX, TR, VEC, RAGGED, 16, false>(a, s);
+  else launch_norm_kernel<TX, TR, VEC, RAGGED, VEC == 8 && !RAGGED ? 32 : 16, false>(a, s);
 }
 
 template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStream_t s) {

@@ -119,6 +119,25 @@ def test_add_norm(rows, cols, x_type, r_type):
     assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scale, q.scale)
 
 
+# many rows: codes next to a border, and rows whose largest product stands in several places
+@pytest.mark.parametrize("cols", [500, 1000, 1001, 1200, 2048, 2051, 5120])
+@pytest.mark.parametrize("x_type,r_type", [(F32, F32), (BF, F32), (BF, BF), (F16, F32), (F16, F16), (F32, None), (BF, None), (F16, None)])
+def test_norm_of_many_rows(cols, x_type, r_type):
+    x = rows_of(700, cols, x_type, cols)
+    x[:, 7::97] = x[:, 7:8]
+    w = 1 + 0.3 * torch.randn(cols, generator=gen(3), device=dev())
+    w[7::97] = 40.0
+    for weight in (w, w.to(BF)):
+        if r_type is None:
+            q, h = Q.rms_norm_int8(x, weight, 1e-5), x
+        else:
+            res = rows_of(700, cols, r_type, cols + 1)
+            res[:, 7::97] = res[:, 7:8]
+            q, h = Q.add_rms_norm_int8(x, res, weight, 1e-5)
+            assert torch.equal(h, R.add(x, res))
+        R.check_rows(q.codes, q.scale, R.norm(h, weight, 1e-5))
+
+
 @pytest.mark.parametrize("rows,cols", SHAPES)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_norm_without_a_residual(rows, cols, dtype):
