@@ -398,7 +398,7 @@ __device__ __forceinline__ void write_codes(const float (&p)[EACH], float c, flo
 
 // ------------------------------------------------------------------ quantise
 template <typename T, int VEC, bool RAGGED, int EACH, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : MAX_HELD / EACH)
+__global__ void __launch_bounds__(WARP ? 256 : (MAX_HELD / EACH + 31) / 32 * 32)
     quantize_kernel(const T *__restrict__ x, int64_t ld, int64_t rows, int cols, int8_t *__restrict__ codes, int64_t ld_codes,
                     float *__restrict__ scale) {
   MTP_PDL_WAIT();
@@ -481,7 +481,7 @@ struct None {};
 // codes are those of (h w) (r / scale).  The sum of squares and r are held in 64 bits; the largest product is found among the
 // fp32 products and then taken exactly (a 48-bit number) from the values whose product rounds to that.
 template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : MAX_HELD / EACH) norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : EACH == 8 ? 1024 : (MAX_HELD / EACH + 31) / 32 * 32) norm_kernel(const NormArgs a) {
   constexpr bool ADD = !std::is_same<TR, None>::value;
   constexpr bool KEEP = EACH == 8;  // few rows: h stays in registers, where else a value of it is read again if need be
   using TH = typename std::conditional<ADD, TR, TX>::type;  // the stream's type
@@ -731,8 +731,9 @@ bool on_vectors(const void *p, int64_t ld, int es, int64_t rows, int n) {
   return aligned(p, es * n < 16 ? es * n : 16) && (rows == 1 || ld * es % (es * n < 16 ? es * n : 16) == 0);
 }
 
-// Rows of up to 1024 values go to warps, eight to a CTA (16 values a lane where that is enough: 60000 x 320 bf16 16.6 us, with
-// 32 24.2), longer ones to CTAs of as many threads as hold them.
+// Rows of up to 1024 values go to warps, eight to a CTA, with 16, 24 or 32 values a lane (60000 x 320 bf16 16.6 us, with 32 24.2; 32768
+// x 768 14.1, with 32 16.0), many rows to 1536 with 48 (32768 x 1536 bf16 27.5 us, by CTAs 36.5; though not ragged ones: 1335 fp32
+// 94 and 78), longer ones to CTAs of as many threads as hold them.
 template <typename T, int VEC, bool RAGGED, int EACH, bool WARP>
 void launch_quantize_team(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
                           cudaStream_t s) {
@@ -746,8 +747,10 @@ template <typename T, int VEC, bool RAGGED>
 void launch_quantize(const T *x, int64_t ld, int64_t rows, int cols, int8_t *codes, int64_t ld_codes, float *scale,
                      cudaStream_t s) {
   if (cols <= 512) launch_quantize_team<T, VEC, RAGGED, 16, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (cols <= 768) launch_quantize_team<T, VEC, RAGGED, 24, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
   else if (cols <= 1024) launch_quantize_team<T, VEC, RAGGED, 32, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
   else if (rows <= 4 * num_sms()) launch_quantize_team<T, VEC, RAGGED, 16, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
+  else if (cols <= 1536 && !RAGGED) launch_quantize_team<T, VEC, false, 48, true>(x, ld, rows, cols, codes, ld_codes, scale, s);
   else launch_quantize_team<T, VEC, RAGGED, 32, false>(x, ld, rows, cols, codes, ld_codes, scale, s);
 }
 
@@ -756,14 +759,18 @@ template <typename TX, typename TR, int VEC, bool RAGGED, int EACH, bool WARP> v
   launch_pdl(norm_kernel<TX, TR, VEC, RAGGED, EACH, WARP>, dim3(grid), dim3(threads), 0, s, a);
 }
 
-// A norm's CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 113 us, with 32 135), 32 where x and the stream are of 16 bits and
-// take few registers (bf16 alone: 68 us, with 16 75; 8192 x 5120: 45 and 57), though not for ragged rows (20000 x 1111: 45 us, with
-// 32 68); few rows have CTAs of 8 values a thread whatever their length (1 x 2048: 2.4 us, with 16 2.9).
+// A norm's rows of up to 768 values go to warps (60000 x 768 fp32: 92 us, by CTAs 95), longer ones to CTAs (32768 x 1024 fp32: 69 us,
+// by warps 74; ragged, 1001: 128 and 209).  A CTA has 16 values a thread (32768 x 2048 bf16 + fp32: 113 us, with 32 135), but where x
+// and the stream are of 16 bits and take few registers 24 or 32, whichever leaves fewer without a value (bf16 alone: 68 us, with 16
+// 75; 1536 columns: 54, with 32 66), though not for ragged rows (20000 x 1111: 45 us, with 32 68).  Few rows have CTAs of 8 values a
+// thread whatever their length (1 x 2048: 2.4 us, with 16 2.9).
 template <typename TX, typename TR, int VEC, bool RAGGED> void launch_norm_team(const NormArgs &a, cudaStream_t s) {
   if (a.rows <= 4 * num_sms() && a.cols <= MAX_HELD / 2) launch_norm_kernel<TX, TR, VEC, RAGGED, 8, false>(a, s);
   else if (a.cols <= 512) launch_norm_kernel<TX, TR, VEC, RAGGED, 16, true>(a, s);
-  else if (a.cols <= 1024) launch_norm_kernel<TX, TR, VEC, RAGGED, 32, true>(a, s);
-  else launch_norm_kernel<TX, TR, VEC, RAGGED, VEC == 8 && !RAGGED ? 32 : 16, false>(a, s);
+  else if (a.cols <= 768) launch_norm_kernel<TX, TR, VEC, RAGGED, 24, true>(a, s);
+  else if constexpr (VEC == 4 || RAGGED) launch_norm_kernel<TX, TR, VEC, RAGGED, 16, false>(a, s);
+  else if (ceil_div(a.cols, 768) * 768 < ceil_div(a.cols, 1024) * 1024) launch_norm_kernel<TX, TR, VEC, RAGGED, 24, false>(a, s);
+  else launch_norm_kernel<TX, TR, VEC, RAGGED, 32, false>(a, s);
 }
 
 template <typename TX, typename TR> void launch_norm(const NormArgs &a, cudaStream_t s) {

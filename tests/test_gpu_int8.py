@@ -119,8 +119,19 @@ def test_add_norm(rows, cols, x_type, r_type):
     assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scale, q.scale)
 
 
+@pytest.mark.parametrize("cols", [500, 701, 768, 769, 1000, 1024, 1025, 1200, 1335, 1536, 1537, 2048, 5120])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_many_rows(cols, dtype):
+    x = rows_of(700, cols, dtype, cols)
+    x[0::5] *= x[0::5].abs().amax(-1, keepdim=True).reciprocal() * 127  # steps of 1: ties
+    x[0::5] = (x[0::5] * 2).round() / 2
+    q = Q.quantize_rows(x)
+    R.check_rows(q.codes, q.scale, x)
+    assert torch.equal(q.codes[0::5].double(), (x[0::5].double() / q.scale[0::5].double().unsqueeze(-1)).round().clamp(-127, 127))
+
+
 # many rows: codes next to a border, and rows whose largest product stands in several places
-@pytest.mark.parametrize("cols", [500, 1000, 1001, 1200, 2048, 2051, 5120])
+@pytest.mark.parametrize("cols", [500, 701, 768, 1000, 1001, 1200, 1536, 2048, 2051, 5120])
 @pytest.mark.parametrize("x_type,r_type", [(F32, F32), (BF, F32), (BF, BF), (F16, F32), (F16, F16), (F32, None), (BF, None), (F16, None)])
 def test_norm_of_many_rows(cols, x_type, r_type):
     x = rows_of(700, cols, x_type, cols)
