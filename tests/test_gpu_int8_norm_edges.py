@@ -32,3 +32,44 @@ def test_a_weight_at_every_offset(rows, cols, x_type, residual):
             R.check_rows(q.codes, q.scale, R.norm(h, w, 1e-5))
             own = call(w.clone())
             assert torch.equal(q.codes, own.codes) and torch.equal(q.scale, own.scale)
+
+
+# fp16 pairs (their bits) and an fp32 weight: the largest |y| of a row of such a pair and zeros is 127 t and one unit in the last
+# place of a 64-bit number, t the middle between two fp32 numbers, where the product with 1 / 127 rounds otherwise than the quotient
+BORDERS = {2: [("0x1.69880cp+6", -20296, -24234), ("0x1.697b8cp+6", -18826, 6391), ("0x1.69b676p+6", -19865, 6046),
+               ("0x1.698af4p+6", 14871, -22293)],
+           1024: [("0x1.ff75d2p+1", 17027, -20864), ("0x1.ff9404p+1", 15872, 8631), ("0x1.ffdd62p+1", 15897, -26133)],
+           2048: [("0x1.69f292p+1", -16580, 11752)]}
+
+
+@pytest.mark.parametrize("cols,weight,h0,h1", [(c, *b) for c in BORDERS for b in BORDERS[c]])
+def test_a_scale_is_the_quotient_rounded_once(cols, weight, h0, h1):
+    """max |y| / 127 in 64 bits, then to fp32, next to the middle between two fp32 numbers, in every form of the kernel.  The
+    kernel's operations are followed one by one: the sum of two fp16 squares and its product with a power of two are exact."""
+    w = torch.zeros(cols, device=dev())
+    w[0] = float.fromhex(weight)
+    x = torch.zeros(1, cols, device=dev(), dtype=F16)
+    x[0, :2] = torch.tensor([h0, h1], dtype=torch.int16).view(F16).to(dev())
+    d = x[0, :2].double()
+    y = (d[0] * torch.rsqrt(d.square().sum() * (1.0 / cols) + float(torch.tensor(1e-5))) * w[0].double()).abs()
+    by = torch.full_like(y, 127.0)
+    want = (y / by).float()
+    assert want != (y * (1.0 / by)).float()  # the row is one of those
+    for rows in (1, 700):
+        x, zero = x[:1].repeat(rows, 1), torch.zeros(rows, cols, device=dev())
+        for q in [Q.rms_norm_int8(x, w, 1e-5), Q.rms_norm_int8(x.float(), w, 1e-5)] + [
+                Q.add_rms_norm_int8(x.to(x_type), zero.to(r_type), w, 1e-5)[0]
+                for x_type, r_type in [(F16, F16), (F16, F32), (F32, F32), (F32, F16)]]:
+            assert (q.scale == want).all()
+
+
+@pytest.mark.parametrize("cols", [40, 1024, 2051, 5120, 16400])
+def test_scales_are_quotients_rounded_once(cols):
+    """Rows of +-1 and eps 0: |y| is the weight.  (An fp32 number / 127 is never next to the middle between two others: the
+    order of a sum does not matter.)"""
+    g = gen(cols)
+    x = (torch.rand(900, cols, generator=g, device=dev()) < 0.5) * 2.0 - 1
+    w = torch.rand(cols, generator=g, device=dev()) + 0.5
+    want = (w.double().amax() / torch.full((), 127.0, device=dev(), dtype=torch.float64)).float()
+    for t in (F32, BF):
+        assert (Q.rms_norm_int8(x.to(t), w, 0.0).scale == want).all()
