@@ -103,7 +103,7 @@ def _extent(x: torch.Tensor):
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
-    """Whether two tensors (rows as of ``_as_rows``) may share memory."""
+    """Whether two tensors may share memory; of rows (two dimensions) on the same stride it is told exactly."""
     (x0, x1), (y0, y1) = _extent(x), _extent(y)
     if x1 <= y0 or y1 <= x0:
         return False
@@ -178,7 +178,7 @@ def _norm(x, residual, weight, eps, inplace, what):
         if inplace:
             if res.data_ptr() != residual.data_ptr():
                 raise ValueError(f"{what}: a residual that is updated in place needs rows on one stride")
-            if _overlap(x, residual) or _overlap(weight, residual):
+            if _overlap(x2, res) or _overlap(weight, residual):
                 raise ValueError(f"{what}: a residual that is updated in place must not share memory with x or weight")
             increment_version(residual)  # a backward pass that has kept it shall see that it changed
             h, ld_h = residual, ld_res

@@ -73,3 +73,14 @@ def test_scales_are_quotients_rounded_once(cols):
     want = (w.double().amax() / torch.full((), 127.0, device=dev(), dtype=torch.float64)).float()
     for t in (F32, BF):
         assert (Q.rms_norm_int8(x.to(t), w, 0.0).scale == want).all()
+
+
+@pytest.mark.parametrize("b,l,d", [(2, 5, 96), (3, 70, 33)])
+def test_in_place_beside_x_in_three_dimensions(b, l, d):
+    buf = rows_of(b * l, 2 * d, BF, 7).reshape(b, l, 2 * d).clone()
+    x, res = buf[:, :, :d], buf[:, :, d:]
+    kept, want = x.clone(), R.add(x, res)
+    w = 1 + 0.3 * torch.randn(d, generator=gen(3), device=dev())
+    q, h = Q.add_rms_norm_int8(x, res, w, 1e-5, inplace=True)
+    assert h is res and torch.equal(res, want) and torch.equal(x, kept)
+    R.check_rows(q.codes.reshape(-1, d), q.scale.reshape(-1), R.norm(want, w, 1e-5).reshape(-1, d))
