@@ -26,6 +26,7 @@ as int8 rows, quantises y in front of out_proj, and hands the out_proj result to
 from __future__ import annotations
 
 import os
+import weakref
 
 import torch
 
@@ -75,6 +76,37 @@ def _prof_end(start, name, work):
     PROFILE.setdefault(name, []).append((start, e, work))
 
 
+def _nothing():
+    return None
+
+
+class Watched:
+    """A weight that int8 rows were made from, so that a later change is noticed: in place (``load_state_dict``, an optimiser;
+    not through ``.data`` or of an inference tensor, which torch does not count), by another tensor in its place, or by a
+    move to another device or type.  A deep or pickled copy watches the weight that was copied with it."""
+
+    __slots__ = ("weight", "at", "version")
+
+    def __init__(self, w):
+        self.weight, self.at = weakref.ref(w), w.data_ptr()
+        self.version = None if w.is_inference() else w._version
+
+    def changed(self, w) -> bool:
+        if w is None or self.weight() is not w or w.data_ptr() != self.at:
+            return True
+        return self.version is not None and w._version != self.version
+
+    def __getstate__(self):
+        w = self.weight()
+        return (None if self.changed(w) else w,)
+
+    def __setstate__(self, state):
+        if state[0] is None:
+            self.weight, self.at, self.version = _nothing, 0, None
+        else:
+            self.__init__(state[0])
+
+
 class MixerKernels:
     """Mixin holding the kernel calls.  Expects the reference's parameter
     layout on ``self`` (in_proj, conv1d, x_proj, dt_proj, A_log, D, out_proj)
@@ -83,8 +115,26 @@ class MixerKernels:
     for the dense mixer) and ``comm`` (CommCounter) and ``_out_bias()``."""
 
     _int8 = None  # (in_proj, out_proj) weights as Int8Rows, a scale for each output channel
+    _int8_of = None  # what they were made from: a Watched for each that is a parameter, else None
 
     # ------------------------------------------------------------ helpers
+    def _set_int8(self, on: bool) -> None:
+        rows = (quantize_rows(self.in_proj.weight), quantize_rows(self.out_proj.weight)) if on else None
+        of = tuple(None if w is None else Watched(w) for w in self._int8_parameters()) if on else None
+        self._int8, self._int8_of = rows, of
+
+    def _int8_parameters(self):
+        modules = self._modules  # past nn.Module's look-up, which would be most of a check
+        return modules["in_proj"]._parameters.get("weight"), modules["out_proj"]._parameters.get("weight")
+
+    def _check_int8(self) -> None:
+        if self._int8_of is None:
+            return
+        (i, o), (w_i, w_o) = self._int8_of, self._int8_parameters()
+        if i is not None and i.changed(w_i) or o is not None and o.changed(w_o):
+            raise RuntimeError(f"layer {self.layer_idx}: the weights of in_proj or out_proj have changed or moved since "
+                               "quantize_linears(); call it again")
+
     def _dt(self) -> torch.dtype:
         return self.in_proj.weight.dtype
 
@@ -355,6 +405,7 @@ class MixerKernels:
         ci = cache.conv_state if cache is not None and cache.conv_state is not None else None
         si = cache.ssm_state.float().contiguous() if cache is not None and cache.ssm_state is not None else None
         if self._int8 is not None:
+            self._check_int8()
             out, cf, sf = self._prefill_int8(quantize_rows(xn), b, l, ci, si)
             return out.to(x.dtype).view(b, l, d), cf, sf
         resid = torch.zeros(b * l, d, device=x.device, dtype=torch.float32)
@@ -371,6 +422,7 @@ class MixerKernels:
         self._check_input(x_t, "step")
         b, d = x_t.shape
         if self._int8 is not None:
+            self._check_int8()
             return self._step_int8(quantize_rows(x_t), cache.conv_state, cache.ssm_state).to(x_t.dtype)
         resid = torch.zeros(b, d, device=x_t.device, dtype=torch.float32)
         self._step_core(x_t.contiguous(), cache.conv_state, cache.ssm_state, resid)

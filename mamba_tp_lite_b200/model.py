@@ -23,7 +23,7 @@ import torch.nn as nn
 from . import _lib as L
 from ._mixer import MixerKernels
 from .config import MambaConfig
-from .int8 import add_rms_norm_int8, quantize_rows, rms_norm_int8
+from .int8 import add_rms_norm_int8, rms_norm_int8
 
 __all__ = ["MambaConfig", "load_hf_state_dict", "LayerCache", "MambaCache", "RMSNorm", "MambaMixer", "MambaBlock",
            "MambaLM"]
@@ -312,7 +312,11 @@ class _LMKernels:
         c.set_sequence_parallel(ok)
 
     def _int8_linears(self) -> bool:
-        return self.layers[0].mixer._int8 is not None
+        if self.layers[0].mixer._int8 is None:
+            return False
+        for layer in self.layers._modules.values():  # all of them before the first layer of a step changes the cache
+            layer._modules["mixer"]._check_int8()
+        return True
 
     def _layers_int8(self, resid, run):
         """The layers of a model with int8 linears: ``run(i, rows)`` gives layer i's mixer output (fp32) for its int8 input
@@ -496,12 +500,12 @@ class MambaLM(_LMKernels, nn.Module):
         """Runs in_proj and out_proj of every layer in int8 from now on (``int8.py``): weights quantised here, a scale for
         each output channel; inputs a scale for each token, by the norm that writes them and in front of out_proj.
         ``prefill``, ``step``, ``score`` and ``generate`` follow; x_proj, dt_proj, the scan and the lm_head stay as they
-        are, and so do the parameters.  Call it again after changing or moving them; ``on=False`` takes it back.  Decode
-        steps then run layer by layer instead of in one launch (capture them with ``GraphedStepper``, which must not
-        outlive a change of this setting)."""
+        are, and so do the parameters (in_proj and out_proj take half as much memory again).  Call it again after changing or
+        moving them: a pass refuses weights that have changed since, but for changes through ``.data``, which torch does not
+        count.  ``on=False`` takes it back.  Decode steps then run layer by layer instead of in one launch (capture them with
+        ``GraphedStepper``, which must not outlive a change of this setting)."""
         for layer in self.layers:
-            m = layer.mixer
-            m._int8 = (quantize_rows(m.in_proj.weight), quantize_rows(m.out_proj.weight)) if on else None
+            layer.mixer._set_int8(on)
 
     def lm_head(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
