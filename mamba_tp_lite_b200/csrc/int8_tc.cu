@@ -43,7 +43,7 @@ struct Params {
   Out o;
   int M, N, K;
   int bn, tiles_m, tiles_n, num_tiles, group_m;
-  int tma_out;   // results by TMA stores
+  int tma_cols;  // blocks of results that end by this column go by TMA stores
   uint32_t idesc;
   uint64_t div_group, div_m, div_last;  // 2^64 / n, rounded up, for a group's tiles, its rows and the last group's rows
 };
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<uint4 *>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = word[i];
-        if (p.tma_out) {
+        if (n_tile + c0 + CW <= p.tma_cols) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                          : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else {  // rows of any alignment: a row of the block at a time, its columns side by side
+        } else {  // rows of any alignment, and the end of a row: a row of the block at a time, its columns side by side
           __syncwarp();
           const int rows = min(32, p.M - m0), n_in = min(CW, p.N - n_tile - c0);
           for (int r = 0; r < rows; ++r) {
@@ -668,14 +668,15 @@ int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld
   // kind::i8, int32 results, signed operands, both with K innermost
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
   const size_t es = o.dtype == MTP_F32 ? 4 : 2;
-  p.tma_out = aligned16(o.p) && (M == 1 || ((size_t)o.ld * es) % 16 == 0);
+  // a TMA store writes whole words of 16 bytes, past the end of a row that ends inside one
+  if (aligned16(o.p) && (M == 1 || ((size_t)o.ld * es) % 16 == 0)) p.tma_cols = N * es % 16 == 0 ? 0x7fffffff : N;
   CUtensorMap ta, tb, tcm;
   int rc = map_codes(&ta, a, M, K, ld_a, BM);
   if (rc) return rc;
   rc = map_codes(&tb, w, N, K, ld_w, bn / CG);
   if (rc) return rc;
   memset(&tcm, 0, sizeof(tcm));
-  if (p.tma_out) {
+  if (p.tma_cols) {
     rc = map_out(&tcm, o, M, N);
     if (rc) return rc;
   }
