@@ -9,7 +9,8 @@ namespace mtp {
 
 bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda, int ldb);
 int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype,
-            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired = nullptr);
+            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired = nullptr,
+            bool to_ldc = false);
 
 struct EpiArgs {
   void *C;

@@ -522,8 +522,9 @@ bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda
          ldb >= K;
 }
 
+// to_ldc: what lies between N and ldc in C's rows may be written.
 int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype,
-            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired) {
+            int epi, const void *bias, int bias_dtype, cudaStream_t stream, int *expired, bool to_ldc) {
   using namespace tc;
   MTP_REQUIRE(gemm_tc_eligible(A, B, M, N, K, lda, ldb),
               "tcgen05 GEMM needs 16-byte aligned A/B, K >= 8 and lda, ldb multiples of 8");
@@ -562,7 +563,8 @@ int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda,
     const char *e = getenv("MTP_GEMM_TMA_STORE");
     return !(e && e[0] == '0');
   }();
-  p.tma_store = tma_store_on && p.vec_ok && N >= 16 && M >= 32;
+  // a TMA store writes whole words of 16 bytes, past the end of a row that ends inside one
+  p.tma_store = tma_store_on && p.vec_ok && N >= 16 && M >= 32 && (to_ldc || N * cb % 16 == 0);
   memset(&tcm, 0, sizeof(tcm));
   if (p.tma_store) {
     rc = make_tmap_c(&tcm, C, M, N, ldc, c_dtype);

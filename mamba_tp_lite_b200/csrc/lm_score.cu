@@ -24,7 +24,7 @@ namespace mtp {
 bool gemm_tc_eligible(const void *A, const void *B, int M, int N, int K, int lda, int ldb);
 bool gemm_on_tensor_cores(const void *A, const void *B, int M, int N, int K, int lda, int ldb, int ab_dtype);
 int gemm_tc(const void *A, const void *B, void *C, int M, int N, int K, int lda, int ldb, int ldc, int c_dtype, int epi,
-            const void *bias, int bias_dtype, cudaStream_t stream, int *expired);
+            const void *bias, int bias_dtype, cudaStream_t stream, int *expired, bool to_ldc);
 int launch_token_logprobs(const void *logits, int dtype, int64_t outer, int64_t inner, int64_t ld_outer, int64_t ld, int V,
                           const int64_t *targets, float temperature, float *logprob, float *entropy, float *stats, int top_k,
                           int64_t *top_ids, float *top_logprobs, const int *expired, cudaStream_t stream);
@@ -476,7 +476,7 @@ int mtp_lm_head_logprobs(const void *hidden, int ld_hidden, int rows, int K, con
     const char *h = (const char *)hidden + (size_t)r0 * ld_hidden * es;
     int rc = gemm_on_tensor_cores(h, weight, n, V, K, ld_hidden, ld_weight, dtype)
                  ? gemm_tc(h, weight, workspace, n, V, K, ld_hidden, ld_weight, (int)ld, MTP_F32, MTP_EPI_STORE, nullptr, 0,
-                           st, expired)
+                           st, expired, true)
                  : mtp_gemm(h, weight, workspace, n, V, K, ld_hidden, ld_weight, (int)ld, dtype, MTP_F32, MTP_EPI_STORE,
                             nullptr, 0, stream);
     if (rc) return rc;

@@ -31,3 +31,22 @@ def test_int8_product(m, k, n, pad):
         assert torch.equal(out, R.linear(a.codes, a.scale, w.codes, w.scale, bias, t))
         out.fill_(7.0)
         assert (held == 7.0).all()
+
+
+@pytest.mark.parametrize("m,k", [(3, 64), (20, 64), (33, 512), (130, 2048), (700, 256)])
+@pytest.mark.parametrize("n", [1, 16, 100, 257, 700, 1031, 4099, 4100, 4102])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_bf16_product(m, k, n, pad):
+    """Whole numbers: the sums are exact in fp32, in any order."""
+    g = torch.Generator(device=dev()).manual_seed(k)
+    a, w = (torch.randint(-4, 5, (r, k), generator=g, device=dev()).to(torch.bfloat16) for r in (m, n))
+    bias = (torch.arange(n, device=dev()) % 7).to(F32)
+    want = a.double() @ w.double().T
+    for t in (F32, torch.bfloat16):
+        for epi, b in ((L.EPI_STORE, None), (L.EPI_BIAS, bias)):
+            held, out = guarded(m, n, pad, t)
+            L.call("mtp_gemm", L.ptr(a), L.ptr(w), L.ptr(out), m, n, k, k, k, held.stride(0), L.BF16, L.dtype_code(t), epi, L.ptr(b),
+                   L.F32, L.stream_ptr())
+            assert torch.equal(out, (want if b is None else want + b.double()).to(t))
+            out.fill_(7.0)
+            assert (held == 7.0).all()
