@@ -14,8 +14,9 @@
 // 3190; 8192 x 2048 -> 8192 95 us, 2890.  To K = 1024 the epilogue bounds it, 2.6 us for a tile of a pair: 8192 x 1024 ->
 // 16384 109 us (3.5 us a tile and 131 with the arrival at the other CTA's barrier as a release of the cluster's scope, which
 // waits for all stores of its thread, and with divisions for a tile's coordinates).
-// Every wait is bounded; a CTA whose wait expires gives NaN for what it has left, waits (again with a limit) for its copies and
-// products in flight, frees its tensor memory and returns.
+// Every wait is bounded.  Where one expires, the CTA gives NaN for what it has left (the split-K form: for all results of its
+// cluster), and when all its warps are through waits, again with a limit, for its copies and products in flight, frees its
+// tensor memory and returns.
 #include "int8_linear.cuh"
 #include "tc_common.cuh"
 
@@ -45,6 +46,7 @@ struct Params {
   int bn, tiles_m, tiles_n, num_tiles, group_m;
   int tma_cols;  // blocks of results that end by this column go by TMA stores
   uint32_t idesc;
+  unsigned long long timeout_ns;
   uint64_t div_group, div_m, div_last;  // 2^64 / n, rounded up, for a group's tiles, its rows and the last group's rows
 };
 
@@ -111,6 +113,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int *r) {
         "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
         "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+}
+
+// After an expired wait, by the thread that has issued them: until the last fills of a ring have landed (100 ms at most), s being
+// the slot that would be next and ph its parity.
+template <typename Bar>
+__device__ __forceinline__ void drain_fills(Bar full_bar, int slots, int issued, int s, uint32_t ph) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (int i = 0; i < issued && i < slots; ++i) {
+    if (--s < 0) { s = slots - 1; ph ^= 1u; }
+    while (!mbar_try_wait(full_bar(s), ph) && globaltimer_ns() - t0 < 100000000ull) {}
+  }
+}
+// The same for the products that a commit to `bar` (its first phase) follows.
+__device__ __forceinline__ void drain_products(uint32_t bar) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, 0) && globaltimer_ns() - t0 < 100000000ull) {}
 }
 
 template <typename T> constexpr int PER_WORD = 16 / (int)sizeof(T);  // results in 16 bytes
@@ -180,19 +198,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem_base = *tmem_holder;
   const int num_kb = (p.K + BK - 1) / BK;
   const int b_rows = p.bn / CG;
+  // of the threads that issue copies and products: the ring's next slot, its parity, and how many (whether any) were issued
+  int s = 0, issued = 0;
+  uint32_t ph = 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
       const uint32_t tx_bytes = (uint32_t)((BM + b_rows) * BK * CG);
-      int s = 0, issued = 0;
-      uint32_t ph = 0;
       for (int t = first; t < p.num_tiles && !*abort; t += step) {
         int mt, nt;
         tile_coords(p, t, mt, nt);
         const int y_a = (mt * CG + (int)rank) * BM, y_b = nt * p.bn + (int)rank * b_rows;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort, TIMEOUT_NS)) break;
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort, p.timeout_ns)) break;
           if (rank == 0) mbar_expect_tx(full_bar(s), tx_bytes);  // both CTAs' bytes count at the first's barrier
           const uint32_t bar = CG == 2 ? cluster_addr(full_bar(s), 0) : full_bar(s);
           const uint32_t sa = base + s * SLOT;
@@ -202,46 +221,32 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
       }
-      if (*abort && rank == 0) {  // wait (bounded) until the most recent fills have landed
-        const int back = issued < STAGES ? issued : STAGES;
-        for (int i = 0; i < back; ++i) {
-          if (--s < 0) { s = STAGES - 1; ph ^= 1u; }
-          const unsigned long long t0 = globaltimer_ns();
-          while (!mbar_try_wait(full_bar(s), ph) && globaltimer_ns() - t0 < 100000000ull) {}
-        }
-      }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      int s = 0, local = 0;
-      uint32_t ph = 0;
-      bool any = false, ok = true;
+      int local = 0;
+      bool ok = true;
       for (int t = first; ok && t < p.num_tiles && !*abort; t += step, ++local) {
         const int a = local & 1;
         const uint32_t use = (uint32_t)(local >> 1);
-        if (!mbar_wait(tempty_bar(a), (use & 1u) ^ 1u, abort, TIMEOUT_NS)) break;
+        if (!mbar_wait(tempty_bar(a), (use & 1u) ^ 1u, abort, p.timeout_ns)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(a * BN_MAX);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), ph, abort, p.timeout_ns)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = base + s * SLOT;
           const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + A_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)  // 32 bytes along K per instruction; past K both operands are zeros
             mma<CG>(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), p.idesc, (kb | k) != 0);
-          any = true;
+          issued = 1;
           commit<CG>(empty_bar(s));
           if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
         if (ok) commit<CG>(tfull_bar(a));
-      }
-      if (*abort && any) {
-        commit<CG>(drain_bar);
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain_bar, 0) && globaltimer_ns() - t0 < 100000000ull) {}
       }
     }
     __syncwarp();
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
       fetch(t + step);
-      alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, TIMEOUT_NS));
+      alive = __all_sync(0xffffffffu, alive && mbar_wait(tfull_bar(a), use & 1u, abort, p.timeout_ns));
       tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN_MAX);
       int at_col = 0;
@@ -372,8 +377,19 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (*abort) __nanosleep(1000000);  // the other CTA's copies and products in flight
-  if (CG == 2) cluster_sync();       // nothing of the pair is at work in this CTA's memory any more
+  if (*abort) {
+    if (threadIdx.x == 0 && rank == 0) drain_fills(full_bar, STAGES, issued, s, ph);
+    if (threadIdx.x == 0 && rank != 0) {  // its copies count at the first CTA's barriers; they take some microseconds
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {}
+    }
+    if (threadIdx.x == 32 && issued) {
+      commit<CG>(drain_bar);
+      drain_products(drain_bar);
+    }
+    __syncthreads();
+  }
+  if (CG == 2) cluster_sync();  // nothing of the pair is at work in this CTA's memory any more
   tc_fence_after();
   if (warp == 1) {
     if (CG == 2)
@@ -400,6 +416,7 @@ struct SplitParams {
   int bn, a_rows, stages, slot, split, tiles_n;
   int vec_out;
   uint32_t idesc;
+  unsigned long long timeout_ns;
 };
 
 __device__ __forceinline__ int4 ld_cluster(uint32_t addr) {
@@ -455,29 +472,28 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   const uint32_t tmem_base = *tmem_holder;
   constexpr int LD_PART = 132;  // of a token's sums, in words: 16-byte writes of a warp's rows meet each bank equally often
   int *part = reinterpret_cast<int *>(gbase);
+  int s = 0, issued = 0;  // of the threads that issue copies and products: the ring's next slot, its parity, fills issued
+  uint32_t ph = 0;
   float *scale_w = reinterpret_cast<float *>(gbase + SPLIT_SCALES), *bias_w = scale_w + 128, *scale_a = scale_w + 256;
 
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t tx_bytes = (uint32_t)((p.a_rows + p.bn) * BK);
-      int s = 0;
-      uint32_t ph = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (kb >= kb0 + p.stages && !mbar_wait(empty_bar(s), ph ^ 1u, abort, TIMEOUT_NS)) break;
+        if (kb >= kb0 + p.stages && !mbar_wait(empty_bar(s), ph ^ 1u, abort, p.timeout_ns)) break;
         mbar_expect_tx(full_bar(s), tx_bytes);
         const uint32_t sa = base + s * p.slot;
         tma_load_2d(sa, &tmA, full_bar(s), kb * BK, m0);
         tma_load_2d(sa + p.a_rows * BK, &tmB, full_bar(s), kb * BK, n0);
+        ++issued;
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(full_bar(s), ph, abort, TIMEOUT_NS)) break;
+        if (!mbar_wait(full_bar(s), ph, abort, p.timeout_ns)) break;
         tc_fence_after();
         const uint32_t sa = base + s * p.slot;
         const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + p.a_rows * BK);
@@ -499,7 +515,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
       bias_w[i] = in ? ld_bias(p.o, n0 + i) : 0.f;
       scale_a[i] = i < rows ? p.o.a_scale[m0 + i] : 0.f;
     }
-    const bool alive = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort, TIMEOUT_NS + TIMEOUT_NS / 2));
+    const bool alive = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort, p.timeout_ns + p.timeout_ns / 2));
     tc_fence_after();
     if (alive && q * 32 < rows) {
       const int m = q * 32 + lane;
@@ -567,7 +583,11 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
       }
     }
   }
-  if (*abort) __nanosleep(1000000);  // copies in flight
+  if (*abort) {
+    if (threadIdx.x == 0) drain_fills(full_bar, p.stages, issued, s, ph);
+    if (threadIdx.x == 32) drain_products(done_bar);
+    __syncwarp();
+  }
   // No other CTA reads this one's sums any more.  (Relaxed: nothing written since is read in the cluster; a release would wait
   // for the results' stores, 0.8 us.)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
@@ -648,9 +668,7 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tcm,
   return check_launch("int8_linear");
 }
 
-template <int CG>
-int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int bn,
-        cudaStream_t stream) {
+template <int CG> Params tile_params(int M, int K, int N, const Out &o, int bn) {
   Params p{};
   p.o = o;
   p.M = M;
@@ -670,6 +688,14 @@ int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld
   const size_t es = o.dtype == MTP_F32 ? 4 : 2;
   // a TMA store writes whole words of 16 bytes, past the end of a row that ends inside one
   if (aligned16(o.p) && (M == 1 || ((size_t)o.ld * es) % 16 == 0)) p.tma_cols = N * es % 16 == 0 ? 0x7fffffff : N;
+  p.timeout_ns = TIMEOUT_NS;
+  return p;
+}
+
+template <int CG>
+int run(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int bn,
+        cudaStream_t stream) {
+  const Params p = tile_params<CG>(M, K, N, o, bn);
   CUtensorMap ta, tb, tcm;
   int rc = map_codes(&ta, a, M, K, ld_a, BM);
   if (rc) return rc;
@@ -722,8 +748,7 @@ double plan_split(int M, int N, int K, int &split_of_k, int &columns) {
   return best;
 }
 
-int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int split, int bn,
-              cudaStream_t stream) {
+SplitParams split_params(int M, int K, int N, const Out &o, int split, int bn) {
   SplitParams p{};
   p.o = o;
   p.M = M;
@@ -740,15 +765,15 @@ int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
   const size_t es = o.dtype == MTP_F32 ? 4 : 2;
   p.vec_out = aligned(o.p, 4 * es) && (M == 1 || o.ld % 4 == 0);
-  CUtensorMap ta, tb;
-  int rc = map_codes(&ta, a, M, K, ld_a, p.a_rows);
-  if (rc) return rc;
-  rc = map_codes(&tb, w, N, K, ld_w, p.bn);
-  if (rc) return rc;
-  rc = allow_split_smem();
+  p.timeout_ns = TIMEOUT_NS;
+  return p;
+}
+
+int launch_split(const CUtensorMap &ta, const CUtensorMap &tb, const SplitParams &p, cudaStream_t stream) {
+  int rc = allow_split_smem();
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ceil_div(M, BM) * p.tiles_n * p.split);
+  cfg.gridDim = dim3(ceil_div(p.M, BM) * p.tiles_n * p.split);
   cfg.blockDim = dim3(SPLIT_THREADS);
   cfg.dynamicSmemBytes = SPLIT_SMEM;
   cfg.stream = stream;
@@ -763,6 +788,17 @@ int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int6
   cfg.numAttrs = 2;
   cudaLaunchKernelEx(&cfg, int8_split_kernel, ta, tb, p);
   return check_launch("int8_linear");
+}
+
+int run_split(const int8_t *a, int64_t ld_a, int M, int K, const int8_t *w, int64_t ld_w, int N, const Out &o, int split, int bn,
+              cudaStream_t stream) {
+  const SplitParams p = split_params(M, K, N, o, split, bn);
+  CUtensorMap ta, tb;
+  int rc = map_codes(&ta, a, M, K, ld_a, p.a_rows);
+  if (rc) return rc;
+  rc = map_codes(&tb, w, N, K, ld_w, p.bn);
+  if (rc) return rc;
+  return launch_split(ta, tb, p, stream);
 }
 
 }  // namespace
