@@ -1,7 +1,8 @@
-"""The norm with int8 output where its forms could part."""
+"""The norm with int8 output where its forms could part, and what lies around its results and around rows that are read back."""
 import pytest
 import torch
 
+from mamba_tp_lite_b200 import _lib as L
 from mamba_tp_lite_b200 import int8 as Q
 from tests import int8_ref as R
 from tests.gpu_util import dev
@@ -73,6 +74,61 @@ def test_scales_are_quotients_rounded_once(cols):
     want = (w.double().amax() / torch.full((), 127.0, device=dev(), dtype=torch.float64)).float()
     for t in (F32, BF):
         assert (Q.rms_norm_int8(x.to(t), w, 0.0).scale == want).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 96), (3, 101), (3, 4096), (700, 500), (700, 701), (700, 1111), (700, 2048), (3, 16400)])
+@pytest.mark.parametrize("x_type,r_type", [(BF, F32), (F32, F32), (BF, BF), (F16, F16), (F32, BF), (BF, None), (F32, None)])
+@pytest.mark.parametrize("left,right", [(0, 0), (16, 16), (3, 6)])
+def test_what_lies_around_a_norm_s_outputs_stays(rows, cols, x_type, r_type, left, right):
+    """Codes, scales and the stream inside wider and longer buffers, through the C entry point; also in place."""
+    x = rows_of(rows, cols, x_type, cols, left, right)
+    w = (1 + 0.3 * torch.randn(cols, generator=gen(3), device=dev()))
+    wide = left + cols + right
+    inside = (slice(2, 2 + rows), slice(left, left + cols))
+
+    def guarded(dtype, value):
+        return torch.full((rows + 4, wide), value, device=dev(), dtype=dtype)
+
+    for inplace in ((False, True) if r_type else (False,)):
+        codes, scale = guarded(torch.int8, 77), torch.full((rows + 4,), 7.0, device=dev())
+        res_args, h, own = (None, 0, 0, None, 0), x, None
+        if r_type:
+            res = rows_of(rows, cols, r_type, cols + 1)
+            own = guarded(r_type, 7.0)
+            if inplace:
+                own[inside] = res
+                given = own[inside]
+            else:
+                given = res
+            res_args = (given.data_ptr(), L.dtype_code(r_type), given.stride(0), own[inside].data_ptr(), wide)
+            h = R.add(x, res)
+        L.call("mtp_rmsnorm_int8", x.data_ptr(), L.dtype_code(x_type), x.stride(0), *res_args, rows, cols, w.data_ptr(), L.F32, 1e-5,
+               codes[inside].data_ptr(), wide, scale[2:].data_ptr(), L.stream_ptr())
+        R.check_rows(codes[inside], scale[2:2 + rows], R.norm(h, w, 1e-5))
+        if own is not None:
+            assert torch.equal(own[inside], h)
+            own[inside] = 7.0
+            assert (own == 7.0).all()
+        codes[inside], scale[2:2 + rows] = 77, 7.0
+        assert (codes == 77).all() and (scale == 7.0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 8), (5, 13), (33, 100), (300, 1111), (40, 4096)])
+@pytest.mark.parametrize("out", [F32, BF, F16])
+@pytest.mark.parametrize("left,right", [(0, 8), (8, 8), (16, 0), (1, 0), (3, 6)])
+def test_what_lies_around_rows_that_are_read_back_stays(rows, cols, out, left, right):
+    """Results inside wider rows, on a vector's boundary and off it, through the C entry point."""
+    codes = torch.randint(-127, 128, (rows, cols + 16), generator=gen(cols), device=dev()).to(torch.int8)
+    scale = torch.rand(rows, generator=gen(rows), device=dev()) + 0.1
+    held = torch.full((rows + 4, left + cols + right), 7.0, device=dev(), dtype=out)
+    inside = held[2:2 + rows, left:left + cols]
+    for at in (0, 8, 5):
+        part = codes[:, at:at + cols]
+        L.call("mtp_dequantize_rows", part.data_ptr(), cols + 16, scale.data_ptr(), rows, cols, inside.data_ptr(), L.dtype_code(out),
+               held.stride(0), L.stream_ptr())
+        assert torch.equal(inside, (part.float() * scale[:, None]).to(out))
+        inside.fill_(7.0)
+        assert (held == 7.0).all()
 
 
 @pytest.mark.parametrize("b,l,d", [(2, 5, 96), (3, 70, 33)])
