@@ -26,7 +26,6 @@ as int8 rows, quantises y in front of out_proj, and hands the out_proj result to
 from __future__ import annotations
 
 import os
-import weakref
 
 import torch
 
@@ -76,10 +75,6 @@ def _prof_end(start, name, work):
     PROFILE.setdefault(name, []).append((start, e, work))
 
 
-def _nothing():
-    return None
-
-
 class Watched:
     """A weight that int8 rows were made from, so that a later change is noticed: in place (``load_state_dict``, an optimiser;
     not through ``.data`` or of an inference tensor, which torch does not count), by another tensor in its place, or by a
@@ -88,21 +83,21 @@ class Watched:
     __slots__ = ("weight", "at", "version")
 
     def __init__(self, w):
-        self.weight, self.at = weakref.ref(w), w.data_ptr()
+        # held, and not by a weak reference, which torch.utils.swap_tensors refuses
+        self.weight, self.at = w, w.data_ptr()
         self.version = None if w.is_inference() else w._version
 
     def changed(self, w) -> bool:
-        if w is None or self.weight() is not w or w.data_ptr() != self.at:
+        if w is None or self.weight is not w or w.data_ptr() != self.at:
             return True
         return self.version is not None and w._version != self.version
 
     def __getstate__(self):
-        w = self.weight()
-        return (None if self.changed(w) else w,)
+        return (None if self.changed(self.weight) else self.weight,)
 
     def __setstate__(self, state):
         if state[0] is None:
-            self.weight, self.at, self.version = _nothing, 0, None
+            self.weight, self.at, self.version = None, 0, None
         else:
             self.__init__(state[0])
 

@@ -93,6 +93,18 @@ def in_place(lm):
         lm.layers[1].mixer.in_proj.weight[3, 5] += 1
 
 
+def swapped(change):
+    """The same where torch puts the new tensors into the old Python objects."""
+    def run(lm):
+        torch.__future__.set_swap_module_params_on_conversion(True)
+        try:
+            change(lm)
+        finally:
+            torch.__future__.set_swap_module_params_on_conversion(False)
+
+    return run
+
+
 def a_training_step(lm):
     for p in lm.parameters():
         p.grad = torch.ones_like(p)
@@ -100,7 +112,8 @@ def a_training_step(lm):
 
 
 CHANGES = [lambda lm: lm.load_state_dict(double(lm)), lambda lm: lm.load_state_dict(double(lm), assign=True), a_new_parameter, a_new_linear,
-           in_place, a_training_step, lambda lm: lm.float(), lambda lm: lm.to("meta")]
+           in_place, a_training_step, lambda lm: lm.float(), lambda lm: lm.to("meta"), swapped(lambda lm: lm.load_state_dict(double(lm))),
+           swapped(lambda lm: lm.float())]
 
 
 @pytest.mark.parametrize("change", range(len(CHANGES)))
