@@ -2,7 +2,7 @@
 //   int8_few.cu  up to 16 rows, operands on 16-byte boundaries;
 //   int8_tc.cu   more rows, operands on 16-byte boundaries;
 //   int8_simt    here: 64 x 64 tiles, 4 x 4 outputs per thread, byte loads: operands of any alignment (333 x 1001 -> 777 with
-//                rows of 1001 bytes: 41 us; quantize_rows puts rows on 16-byte boundaries, 6.6 us).
+//                rows of 1001 bytes: 59 us; quantize_rows puts rows on 16-byte boundaries, 6.6 us).
 #include "int8_linear.cuh"
 
 namespace mtp {

@@ -32,7 +32,7 @@ __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 
 // a / 127 rounded to nearest, by a product with 1 / 127 and a correction from its remainder (P. Markstein, IBM J. Res. Dev. 34,
 // 1990: with 1 / b rounded to nearest and q within a unit in the last place, fma(a - q b, 1 / b, q) is the rounded quotient).
-// With a division the norm is slower (32768 x 2048 bf16 alone: 74 us, 84), with the product alone a scale in 10^11 is
+// With a division the norm is slower (32768 x 2048 bf16 alone: 70 us, 80), with the product alone a scale in 10^11 is
 // another fp32 number.
 __device__ __forceinline__ double over_127(double a) {
   constexpr double k = 1.0 / 127.0;
@@ -476,7 +476,7 @@ template <int VEC, bool RAGGED, typename T>
 __device__ __forceinline__ void load_weight_of(const T *w, int col, int cols, float *v) {
   if constexpr (RAGGED && sizeof(T) * VEC > 16) {
     // 8 fp32 weights beside 16-bit rows: 32 bytes, more than load_ragged shifts together.  As two vectors where the weight lies on
-    // 16-byte boundaries, as an allocation does (20000 x 1111 fp16 + fp16: 78 us), else one by one (92).
+    // 16-byte boundaries, as an allocation does (20000 x 1111 fp16 + fp16: 74 us), else one by one (88).
     if ((reinterpret_cast<uintptr_t>(w) & 15) == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
@@ -894,7 +894,7 @@ int mtp_rmsnorm_int8(const void *x, int x_dtype, int64_t ld_x, const void *resid
                    ld_codes, scale, 1.0 / cols};
   bool done = false;
   if (cols <= MAX_HELD) MTP_DISPATCH_3(x_dtype, T, done = launch_norm_of<T>(a, s));
-  if (!done)  // long rows, and a 16-bit stream of another type than x
+  if (!done)  // long rows, and every 16-bit stream of another type than x, fp32 x with a 16-bit stream among them (598 us for 32768 x 2048)
     launch_pdl(norm_long_kernel, dim3((unsigned)(rows < 148 * 8 ? rows : 148 * 8)), dim3(LONG_THREADS), 0, s, a);
   return check_launch("rmsnorm_int8");
 }
